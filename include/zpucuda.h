@@ -55,7 +55,9 @@ enum {
  * takes all nine.  BOOL is one byte, 0 or 1. */
 enum {
     ZPUCUDA_F64 = 0, ZPUCUDA_F32 = 1, ZPUCUDA_F16 = 2, ZPUCUDA_I64 = 3, ZPUCUDA_I32 = 4,
-    ZPUCUDA_I16 = 5, ZPUCUDA_I8 = 6, ZPUCUDA_U8 = 7, ZPUCUDA_BOOL = 8
+    ZPUCUDA_I16 = 5, ZPUCUDA_I8 = 6, ZPUCUDA_U8 = 7, ZPUCUDA_BOOL = 8,
+    /* Not one of zpu's types: the language-model head takes it beside F32 and F16. */
+    ZPUCUDA_BF16 = 9
 };
 
 /* prims.AXIS_NONE (src/zpu/prims.zig:169). */
@@ -449,6 +451,100 @@ int zpucuda_mlp_trace_read(zpucuda_mlp *h, float *ms, int n);
  * second GPU. */
 int zpucuda_debug_peer_reduce(const float *d_inbox, int world, int64_t n, float *d_out, const uint64_t *d_flags,
                               uint64_t epoch, uint32_t spin_limit, uint32_t *d_err, void *stream);
+
+/* ------------------------------------------------------ language-model head */
+/* The operators around a language model's output projection: the norm before
+ * it, the loss that trains it against a larger model, the product in 8-bit
+ * integers that serves it, and the choice of the next token.  zpu has the
+ * norm as a composition of its prims (nn layer norm, pinned by the oracle);
+ * the others have no counterpart in the reference.
+ *  - Activations and logits are [rows, n] of F32, F16 or BF16 with unit stride
+ *    along the row and any row pitch (ld*, in elements, >= the row's length)
+ *    and any alignment that fits their elements; rows may be 0.  Sums are held
+ *    in f32 or wider and each result is rounded to its type once.
+ *  - Calls are asynchronous on `stream` and, with no wait in them, may be
+ *    captured in a CUDA graph.  Results do not depend on the run: the same
+ *    inputs give the same bits.
+ *
+ * layer_norm: y = (x - mean) * rstd * gamma + beta over each row, rstd =
+ *   1 / sqrt(mean((x - mean)^2) + eps).  gamma / beta: [cols] of type wtype, or
+ *   NULL for 1 / 0.  mean / rstd: [rows] f32 for the gradient, or NULL.
+ *   y may be x (same pitch).
+ * layer_norm_grad: dx, dgamma (sum over rows of dy * xhat) and dbeta (sum of
+ *   dy), dgamma / dbeta of type wtype; a NULL output is not computed.  dx may
+ *   be dy or x (same pitch). */
+int zpucuda_layer_norm(int dtype, const void *d_x, int64_t ldx, int wtype, const void *d_gamma, const void *d_beta,
+                       void *d_y, int64_t ldy, float *d_mean, float *d_rstd, int64_t rows, int64_t cols, double eps,
+                       void *stream);
+int zpucuda_layer_norm_grad(int dtype, const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx,
+                            const float *d_mean, const float *d_rstd, int wtype, const void *d_gamma, void *d_dx,
+                            int64_t lddx, void *d_dgamma, void *d_dbeta, int64_t rows, int64_t cols, void *stream);
+/* Distillation from a teacher's `top` highest logits (at most 1024 a row):
+ * teacher [rows, top] of type ttype at the vocabulary indices [rows, top] of
+ * type itype (I32 or I64; -1: no entry).  With z = logits / temperature, q =
+ * softmax(z) over the vocabulary and p = softmax(teacher / temperature) over
+ * the listed entries:
+ *   loss = weight * temperature^2 * sum p (log p - log q)           [rows] f32
+ *   dlogits = temperature * weight * dloss * (q - p)        (p 0 where unlisted)
+ * weight, dloss: [rows] f32 or NULL for 1.  A row whose weight is 0, whose
+ * entries are all -1 or all have a teacher logit of -inf, or (gradient) whose
+ * dloss is 0, gives exactly 0 whatever its logits hold.  Another index outside
+ * [0, vocab) makes its row's loss and gradient NaN.  An index that is listed
+ * twice has the sum of its entries.
+ *   distill_loss: the loss, and (unless NULL) lse = log sum exp z, 0 where the
+ *     loss is not computed.
+ *   distill_grad: the gradient, from that lse.
+ *   distill_value_and_grad: both, from one reading of the logits.
+ * dlogits has the logits' type and may be the logits (same pitch). */
+int zpucuda_distill_loss(int dtype, const void *d_logits, int64_t ld, int ttype, const void *d_teacher, int64_t ldt,
+                         int itype, const void *d_indices, int64_t ldi, const float *d_weight, double temperature,
+                         float *d_loss, float *d_lse, int64_t rows, int64_t vocab, int64_t top, void *stream);
+int zpucuda_distill_grad(int dtype, const void *d_logits, int64_t ld, int ttype, const void *d_teacher, int64_t ldt,
+                         int itype, const void *d_indices, int64_t ldi, const float *d_weight, double temperature,
+                         const float *d_lse, const float *d_dloss, void *d_dlogits, int64_t ldd, int64_t rows,
+                         int64_t vocab, int64_t top, void *stream);
+int zpucuda_distill_value_and_grad(int dtype, const void *d_logits, int64_t ld, int ttype, const void *d_teacher,
+                                   int64_t ldt, int itype, const void *d_indices, int64_t ldi, const float *d_weight,
+                                   double temperature, const float *d_dloss, float *d_loss, void *d_dlogits,
+                                   int64_t ldd, int64_t rows, int64_t vocab, int64_t top, void *stream);
+/* The linear layer in 8-bit integers.
+ *   int8_quantize: q [rows, cols] and scale [rows] with scale = max |x| / 127 and
+ *     q = round(x / scale) (half to even); a row of zeros has scale 0, a row with
+ *     a NaN or an infinity has scale NaN and q = 0.
+ *   int8_matmul: out[m, n] = (sum over k of a[m, k] * b[n, k]) * sa[m] * sb[n]
+ *     + bias[n] (NULL: 0), the sum exact in 32-bit integers (k <= 131071,
+ *     otherwise NotSupported), out of type dtype.  a: [m, k] with a scale per row
+ *     (token), b: [n, k] with a scale per row (output channel).
+ *   int8_linear: y = x w^T with x [rows, inner] quantised by row on the way:
+ *     int8_quantize and int8_matmul in one call.  work: device memory of
+ *     zpucuda_int8_linear_work(rows, inner) bytes, 16-byte aligned, that no other
+ *     work in flight uses.
+ * The product reads a and b fastest where their addresses and pitches are
+ * multiples of 16. */
+int zpucuda_int8_quantize(int dtype, const void *d_x, int64_t ldx, int8_t *d_q, int64_t ldq, float *d_scale,
+                          int64_t rows, int64_t cols, void *stream);
+int zpucuda_int8_matmul(const int8_t *d_a, int64_t lda, const float *d_sa, const int8_t *d_b, int64_t ldb,
+                        const float *d_sb, const float *d_bias, int dtype, void *d_out, int64_t ldo, int64_t m,
+                        int64_t n, int64_t k, void *stream);
+int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d_w, int64_t ldw, const float *d_sw,
+                        const float *d_bias, void *d_y, int64_t ldy, int64_t rows, int64_t cols, int64_t inner,
+                        void *d_work, int64_t work_bytes, void *stream);
+int64_t zpucuda_int8_linear_work(int64_t rows, int64_t inner);
+/* Chooses a token of each row of logits [rows, vocab] (vocab <= 2^22) from one
+ * given uniform number in [0, 1) a row (utype F32 or F64).  Tokens are ranked by
+ * falling logit, equal ones by rising index; a token's weight is the whole number
+ * floor(2^40 exp((x - max x) / temperature)).  Kept are the top_k first ranks (<= 0:
+ * all), of those the shortest run of first ranks that holds ceil(top_p * their
+ * weight) (>= 1: all), of those the tokens of weight at least ceil(min_p * 2^40).
+ * The token is the first index whose running sum of kept weights exceeds
+ * floor(uniform * their sum): whole numbers throughout, so the choice does not
+ * depend on how the work is split.  A temperature that is not above 0 takes the
+ * first rank.  logprob (or NULL): the token's log probability among the kept.
+ * NaN and -inf logits are never chosen; a row of nothing else gives token -1 and
+ * -inf.  temperature, top_k, top_p, min_p: [rows] each, or NULL for 1, 0, 1, 0. */
+int zpucuda_sample(int dtype, const void *d_logits, int64_t ld, int utype, const void *d_uniform,
+                   const float *d_temperature, const int32_t *d_top_k, const float *d_top_p, const float *d_min_p,
+                   int64_t *d_token, float *d_logprob, int64_t rows, int64_t vocab, void *stream);
 
 /* ------------------------------------------------- allocation-free variant */
 /* No counterpart in the reference: an addition for callers that cannot

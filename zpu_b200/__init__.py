@@ -11,7 +11,8 @@ from ._capi import (AXIS_NONE, DT_BOOL, DT_I64, F32, F64, PRIM, Blob, Step, Tens
                     exported_names, lib)
 
 __all__ = ["lib", "check", "ZpuCudaError", "Plan", "gemm", "matmul", "matmul_shape", "stream_of",
-           "launch_count", "AXIS_NONE", "F32", "F64", "PRIM"]
+           "launch_count", "AXIS_NONE", "F32", "F64", "PRIM", "layer_norm", "layer_norm_grad", "distill_loss",
+           "distill_grad", "distill_value_and_grad", "quantize_rows", "int8_matmul", "Int8Linear", "sample"]
 
 
 CUDA_STREAM_LEGACY = 0x1  # cudaStreamLegacy
@@ -279,3 +280,7 @@ def _fill_value(v, vid, dt, shape, depth=0):
     for i, s in enumerate(shape):
         v.dims[i] = s
     v.batch_depth = depth
+
+
+from .head import (Int8Linear, distill_grad, distill_loss, distill_value_and_grad, int8_matmul,  # noqa: E402
+                   layer_norm, layer_norm_grad, quantize_rows, sample)

@@ -15,6 +15,7 @@ MAX_RANK = 8
 AXIS_NONE = -2
 F64, F32 = 0, 1
 DT_I64 = 3  # zpu DType.i64: argmax / argmin results
+DT_BF16 = 9  # not one of zpu's types: the language-model head only
 DT_BOOL = 8  # zpu DType.bool (one byte): predicates, any / all
 # residency states of a buffer (zpucuda_buf_residency)
 RES_DEVICE, RES_HOST, RES_BOTH = 1, 2, 3
@@ -156,6 +157,18 @@ SIGNATURES = {
     "zpucuda_mlp_exchange_mode": (I32, [P]),
     "zpucuda_mlp_trace": (I32, [P, I32]),
     "zpucuda_mlp_trace_read": (I32, [P, P, I32]),
+    "zpucuda_layer_norm": (I32, [I32, P, I64, I32, P, P, P, I64, P, P, I64, I64, C.c_double, P]),
+    "zpucuda_layer_norm_grad": (I32, [I32, P, I64, P, I64, P, P, I32, P, P, I64, P, P, I64, I64, P]),
+    "zpucuda_distill_loss": (I32, [I32, P, I64, I32, P, I64, I32, P, I64, P, C.c_double, P, P, I64, I64, I64, P]),
+    "zpucuda_distill_grad": (I32, [I32, P, I64, I32, P, I64, I32, P, I64, P, C.c_double, P, P, P, I64, I64, I64, I64,
+                                   P]),
+    "zpucuda_distill_value_and_grad": (I32, [I32, P, I64, I32, P, I64, I32, P, I64, P, C.c_double, P, P, P, I64, I64,
+                                             I64, I64, P]),
+    "zpucuda_int8_quantize": (I32, [I32, P, I64, P, I64, P, I64, I64, P]),
+    "zpucuda_int8_matmul": (I32, [P, I64, P, P, I64, P, P, I32, P, I64, I64, I64, I64, P]),
+    "zpucuda_int8_linear": (I32, [I32, P, I64, P, I64, P, P, P, I64, I64, I64, I64, P, I64, P]),
+    "zpucuda_int8_linear_work": (I64, [I64, I64]),
+    "zpucuda_sample": (I32, [I32, P, I64, I32, P, P, P, P, P, P, P, I64, I64, P]),
     "zpucuda_debug_peer_reduce": (I32, [P, I32, I64, P, P, U64, C.c_uint32, P, P]),
 }
 

@@ -1,0 +1,320 @@
+"""A language model's output head on the device (zpucuda_layer_norm,
+zpucuda_distill_*, zpucuda_int8_* and zpucuda_sample).
+
+The operators around the output projection: layer norm and its gradient, the
+distillation loss from a teacher's top logits and its gradient, the linear
+layer in 8-bit integers, and the choice of the next token.  Activations and
+logits are [rows, n] CUDA tensors of float32, float16 or bfloat16, contiguous
+along the row and with any row pitch (a slice of a wider tensor is read in
+place); results are new tensors unless `out` names one.  With `stream`, the
+call runs on that torch stream and its new tensors belong to it.
+"""
+from . import _capi
+from ._capi import check, lib
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _stream(stream):
+    from . import stream_of
+    return stream_of(stream)
+
+
+def _refuse(status, text):
+    raise _capi.ZpuCudaError(status, text)
+
+
+def _code(name, t):
+    torch = _torch()
+    if t.dtype == torch.float32:
+        return _capi.F32
+    if t.dtype == torch.float16:
+        return 2
+    if t.dtype == torch.bfloat16:
+        return _capi.DT_BF16
+    _refuse(9, "%s: dtype %s is not float32, float16 or bfloat16" % (name, t.dtype))
+
+
+def _matrix(name, t, like=None, shape=None):
+    """Checks a [rows, n] argument; its row pitch in elements."""
+    if t.dim() != 2:
+        _refuse(5, "%s: %d axes, [rows, n] is wanted" % (name, t.dim()))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        _refuse(2, "%s: shape %s, %s is wanted" % (name, tuple(t.shape), tuple(shape)))
+    _device(name, t, like)
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        _refuse(7, "%s: its rows are not contiguous" % name)
+    # torch leaves the stride of an axis of one (or no) row arbitrary
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if ld < t.shape[1]:
+        _refuse(7, "%s: its rows overlap" % name)
+    return ld
+
+
+def _device(name, t, like=None):
+    if not t.is_cuda or (like is not None and t.device != like.device):
+        _refuse(12, "%s is on %s" % (name, t.device if like is None or not t.is_cuda
+                                     else "%s, not %s" % (t.device, like.device)))
+
+
+def _vector(name, t, n, like, dtype=None):
+    """Checks an optional [n] argument; its address."""
+    if t is None:
+        return None
+    if tuple(t.shape) != (n,):
+        _refuse(2, "%s: shape %s, (%d,) is wanted" % (name, tuple(t.shape), n))
+    if dtype is not None and t.dtype != dtype:
+        _refuse(3, "%s: dtype %s, %s is wanted" % (name, t.dtype, dtype))
+    _device(name, t, like)
+    if n > 1 and t.stride(0) != 1:
+        _refuse(7, "%s is not contiguous" % name)
+    return t.data_ptr()
+
+
+def _output(name, out, like, shape=None, dtype=None):
+    """`out`, checked, or a new tensor; and its row pitch."""
+    shape = tuple(like.shape) if shape is None else shape
+    dtype = like.dtype if dtype is None else dtype
+    if out is None:
+        return _torch().empty(shape, dtype=dtype, device=like.device), shape[1]
+    if out.dtype != dtype:
+        _refuse(3, "%s: dtype %s, %s is wanted" % (name, out.dtype, dtype))
+    return out, _matrix(name, out, like, shape)
+
+
+def _on(stream):
+    """New tensors of the block belong to the stream that the call runs on."""
+    if stream is None:
+        import contextlib
+        return contextlib.nullcontext()
+    return _torch().cuda.stream(stream)
+
+
+# ------------------------------------------------------------- layer norm
+def _weights(x, gamma, beta):
+    cols = x.shape[1]
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        _refuse(3, "gamma is %s, beta is %s" % (gamma.dtype, beta.dtype))
+    g, b = _vector("gamma", gamma, cols, x), _vector("beta", beta, cols, x)
+    some = gamma if gamma is not None else beta
+    return (_capi.F32 if some is None else _code("gamma / beta", some)), g, b
+
+
+def layer_norm(x, gamma=None, beta=None, eps=1e-5, out=None, stats=False, stream=None):
+    """(x - mean) / sqrt(var + eps) * gamma + beta over each row of x.  With
+    `stats` also the rows' mean and 1 / sqrt(var + eps) (float32), which
+    layer_norm_grad takes.  `out` may be x."""
+    torch = _torch()
+    ldx, code = _matrix("x", x), _code("x", x)
+    wt, g, b = _weights(x, gamma, beta)
+    rows, cols = x.shape
+    with _on(stream):
+        y, ldy = _output("out", out, x)
+        mean = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
+        rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
+    check(lib().zpucuda_layer_norm(code, x.data_ptr(), ldx, wt, g, b, y.data_ptr(), ldy,
+                                   mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None,
+                                   rows, cols, eps, _stream(stream)))
+    return (y, mean, rstd) if stats else y
+
+
+def layer_norm_grad(dy, x, mean, rstd, gamma=None, out=None, stream=None):
+    """(dx, dgamma, dbeta) of layer_norm for the output's gradient dy: dx like
+    x (in `out`, which may be dy or x), dgamma and dbeta like gamma (float32
+    without one)."""
+    torch = _torch()
+    ldx, code = _matrix("x", x), _code("x", x)
+    if dy.dtype != x.dtype:
+        _refuse(3, "dy is %s, x is %s" % (dy.dtype, x.dtype))
+    lddy = _matrix("dy", dy, x, x.shape)
+    rows, cols = x.shape
+    m = _vector("mean", mean, rows, x, torch.float32)
+    r = _vector("rstd", rstd, rows, x, torch.float32)
+    wt, g, _ = _weights(x, gamma, None)
+    with _on(stream):
+        dx, lddx = _output("out", out, x)
+        dgamma = torch.empty(cols, dtype=gamma.dtype if gamma is not None else torch.float32, device=x.device)
+        dbeta = torch.empty_like(dgamma)
+    check(lib().zpucuda_layer_norm_grad(code, dy.data_ptr(), lddy, x.data_ptr(), ldx, m, r, wt, g, dx.data_ptr(), lddx,
+                                        dgamma.data_ptr(), dbeta.data_ptr(), rows, cols, _stream(stream)))
+    return dx, dgamma, dbeta
+
+
+# ------------------------------------------------------------- distillation
+def _distill_args(logits, teacher, indices, weight):
+    torch = _torch()
+    ld, code = _matrix("logits", logits), _code("logits", logits)
+    rows, vocab = logits.shape
+    if teacher.dim() != 2 or teacher.shape[0] != rows:
+        _refuse(2, "teacher: shape %s, [%d, top] is wanted" % (tuple(teacher.shape), rows))
+    if indices.dtype not in (torch.int32, torch.int64):
+        _refuse(9, "indices: dtype %s is not int32 or int64" % indices.dtype)
+    ldt = _matrix("teacher", teacher, logits)
+    ldi = _matrix("indices", indices, logits, teacher.shape)
+    w = _vector("weight", weight, rows, logits, torch.float32)
+    head = (code, logits.data_ptr(), ld, _code("teacher", teacher), teacher.data_ptr(), ldt,
+            4 if indices.dtype == torch.int32 else _capi.DT_I64, indices.data_ptr(), ldi, w)
+    return head, (rows, vocab, teacher.shape[1])
+
+
+def distill_loss(logits, teacher, indices, temperature=1.0, weight=None, stream=None):
+    """(loss, lse): weight * T^2 * KL(teacher's listed softmax || student's
+    softmax) of each row at temperature T, and log sum exp(logits / T).
+    teacher: the teacher's top logits [rows, top] at the vocabulary `indices`
+    (int32 / int64; -1: no entry).  A row with weight 0 or no entry gives 0."""
+    torch = _torch()
+    head, dims = _distill_args(logits, teacher, indices, weight)
+    with _on(stream):
+        loss = torch.empty(dims[0], dtype=torch.float32, device=logits.device)
+        lse = torch.empty_like(loss)
+    check(lib().zpucuda_distill_loss(*head, temperature, loss.data_ptr(), lse.data_ptr(), *dims, _stream(stream)))
+    return loss, lse
+
+
+def distill_grad(logits, teacher, indices, lse, dloss=None, temperature=1.0, weight=None, out=None, stream=None):
+    """The gradient of sum(dloss * loss) with regard to the logits, from
+    distill_loss's lse.  `out` may be the logits."""
+    torch = _torch()
+    head, dims = _distill_args(logits, teacher, indices, weight)
+    l = _vector("lse", lse, dims[0], logits, torch.float32)
+    d = _vector("dloss", dloss, dims[0], logits, torch.float32)
+    with _on(stream):
+        g, ldg = _output("out", out, logits)
+    check(lib().zpucuda_distill_grad(*head, temperature, l, d, g.data_ptr(), ldg, *dims, _stream(stream)))
+    return g
+
+
+def distill_value_and_grad(logits, teacher, indices, dloss=None, temperature=1.0, weight=None, out=None, stream=None):
+    """(loss, dlogits): distill_loss and distill_grad from one reading of the
+    logits.  `out` may be the logits."""
+    torch = _torch()
+    head, dims = _distill_args(logits, teacher, indices, weight)
+    d = _vector("dloss", dloss, dims[0], logits, torch.float32)
+    with _on(stream):
+        loss = torch.empty(dims[0], dtype=torch.float32, device=logits.device)
+        g, ldg = _output("out", out, logits)
+    check(lib().zpucuda_distill_value_and_grad(*head, temperature, d, loss.data_ptr(), g.data_ptr(), ldg, *dims,
+                                               _stream(stream)))
+    return loss, g
+
+
+# ------------------------------------------------------------- 8-bit integers
+def quantize_rows(x, stream=None):
+    """(q, scale): int8 rows and their float32 scales, scale = max |row| / 127."""
+    torch = _torch()
+    ldx, code = _matrix("x", x), _code("x", x)
+    rows, cols = x.shape
+    with _on(stream):
+        # a row pitch of a multiple of 16 bytes, as the product reads best
+        q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :cols]
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    check(lib().zpucuda_int8_quantize(code, x.data_ptr(), ldx, q.data_ptr(), _matrix("q", q), scale.data_ptr(),
+                                      rows, cols, _stream(stream)))
+    return q, scale
+
+
+def _int8(name, t, like=None):
+    if t.dtype != _torch().int8:
+        _refuse(3, "%s: dtype %s, int8 is wanted" % (name, t.dtype))
+    return _matrix(name, t, like)
+
+
+def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=None, out=None, stream=None):
+    """(a @ b.T) * a_scale[:, None] * b_scale + bias for int8 a [m, k] and b
+    [n, k] with float32 scales per row, summed exactly; float32 unless `dtype`
+    or `out` says otherwise."""
+    torch = _torch()
+    lda, ldb = _int8("a", a), _int8("b", b, a)
+    m, k = a.shape
+    n = b.shape[0]
+    if b.shape[1] != k:
+        _refuse(2, "a is %s, b is %s" % (tuple(a.shape), tuple(b.shape)))
+    sa = _vector("a_scale", a_scale, m, a, torch.float32)
+    sb = _vector("b_scale", b_scale, n, a, torch.float32)
+    bi = _vector("bias", bias, n, a, torch.float32)
+    if dtype is None:
+        dtype = out.dtype if out is not None else torch.float32
+    with _on(stream):
+        y, ldy = _output("out", out, a, (m, n), dtype)
+    check(lib().zpucuda_int8_matmul(a.data_ptr(), lda, sa, b.data_ptr(), ldb, sb, bi, _code("out", y), y.data_ptr(),
+                                    ldy, m, n, k, _stream(stream)))
+    return y
+
+
+class Int8Linear:
+    """y = x @ weight.T + bias with int8 weights [cols, inner] and a float32
+    scale per output channel, x quantised by row as it comes.  Made from
+    quantised weights, or by Int8Linear.from_float.  Weights at a row pitch of
+    a multiple of 16 bytes are kept as they are, others copied to one."""
+
+    def __init__(self, weight, scale, bias=None):
+        torch = _torch()
+        _int8("weight", weight)
+        cols, inner = weight.shape
+        _vector("scale", scale, cols, weight, torch.float32)
+        _vector("bias", bias, cols, weight, torch.float32)
+        self._ld = weight.stride(0) if cols > 1 else (inner + 15) // 16 * 16
+        if self._ld % 16 or weight.data_ptr() % 16:
+            self._ld = (inner + 15) // 16 * 16
+            kept = torch.empty((cols, self._ld), dtype=torch.int8, device=weight.device)[:, :inner]
+            weight = kept.copy_(weight)
+        self.weight, self.scale, self.bias = weight, scale, bias
+
+    @classmethod
+    def from_float(cls, weight, bias=None, stream=None):
+        """From float32 / float16 / bfloat16 weights [cols, inner]."""
+        with _on(stream):
+            return cls(*quantize_rows(weight, stream), bias)
+
+    def __call__(self, x, out=None, stream=None):
+        torch = _torch()
+        ldx, code = _matrix("x", x, self.weight), _code("x", x)
+        rows, inner = x.shape
+        cols = self.weight.shape[0]
+        if inner != self.weight.shape[1]:
+            _refuse(2, "x is %s, the weight %s" % (tuple(x.shape), tuple(self.weight.shape)))
+        with _on(stream):
+            y, ldy = _output("out", out, x, (rows, cols))
+            work = torch.empty(lib().zpucuda_int8_linear_work(rows, inner), dtype=torch.uint8, device=x.device)
+        check(lib().zpucuda_int8_linear(code, x.data_ptr(), ldx, self.weight.data_ptr(), self._ld,
+                                        self.scale.data_ptr(), None if self.bias is None else self.bias.data_ptr(),
+                                        y.data_ptr(), ldy, rows, cols, inner, work.data_ptr(), work.numel(),
+                                        _stream(stream)))
+        return y
+
+
+# ------------------------------------------------------------- the next token
+def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
+    """(token, logprob): a token (int64) of each row of logits, drawn with the
+    given uniform numbers (float32 / float64 in [0, 1)), and its log
+    probability among the tokens kept.  temperature (float32; <= 0: the
+    likeliest token), top_k (int32; <= 0: all), top_p (float32; >= 1: all) and
+    min_p (float32; <= 0: all) are [rows] tensors, or plain numbers for every
+    row.  NaN and -inf logits are never drawn; a row of nothing else gives -1."""
+    torch = _torch()
+    ld, code = _matrix("logits", logits), _code("logits", logits)
+    rows, vocab = logits.shape
+    if uniform.dtype not in (torch.float32, torch.float64):
+        _refuse(9, "uniform: dtype %s is not float32 or float64" % uniform.dtype)
+    u = _vector("uniform", uniform, rows, logits)
+    keep = []
+
+    def each(name, v, dtype):
+        if v is None:
+            return None
+        if not hasattr(v, "data_ptr"):
+            v = torch.full((rows,), v, dtype=dtype, device=logits.device)
+            keep.append(v)
+        return _vector(name, v, rows, logits, dtype)
+
+    with _on(stream):
+        rules = (each("temperature", temperature, torch.float32), each("top_k", top_k, torch.int32),
+                 each("top_p", top_p, torch.float32), each("min_p", min_p, torch.float32))
+        token = torch.empty(rows, dtype=torch.int64, device=logits.device)
+        logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    check(lib().zpucuda_sample(code, logits.data_ptr(), ld, 0 if uniform.dtype == torch.float64 else 1, u, *rules,
+                               token.data_ptr(), logprob.data_ptr(), rows, vocab, _stream(stream)))
+    return token, logprob
