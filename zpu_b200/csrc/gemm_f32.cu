@@ -68,6 +68,7 @@
 #include <mutex>
 
 #include "gemm.cuh"
+#include "int8.cuh"
 #include "region.cuh"
 
 namespace zc {
@@ -1755,6 +1756,10 @@ extern "C" int zpucuda_check_device(void) {
     unsigned int e = 0;
     cudaError_t r = cudaMemcpyFromSymbol(&e, zc::g_gemm_error, sizeof e);
     if (r != cudaSuccess) return zc::cuda_fail(r, "cudaMemcpyFromSymbol(device error word)");
+    if (!e) {
+        const int st = zc::int8_device_error(&e);
+        if (st) return st;
+    }
     if (e) return zc::set_error(ZPUCUDA_ERR_TIMEOUT, "a device-side bounded wait ran out in a GEMM kernel");
     return ZPUCUDA_OK;
 }
