@@ -31,25 +31,104 @@ __device__ __forceinline__ float result(int sum, float sa, float sb, const float
     return bias ? __fadd_rn(v, b) : v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(NT) quantize_kernel(const T *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale,
-                                                      int64_t cols) {
-    __shared__ float sm[NT / 32];
-    const int64_t row = blockIdx.x;
-    const T *xr = x + row * ldx;
-    float m = 0.0f;
-    for (int64_t c = threadIdx.x; c < cols; c += NT) m = max_nan(m, fabsf(to_f(xr[c])));
-    m = warp_max_nan(m);
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
-    __syncthreads();
-    m = sm[0];
-    for (int w = 1; w < NT / 32; w++) m = max_nan(m, sm[w]);
-    const float s = isfinite(m) ? m / 127.0f : NAN;
-    for (int64_t c = threadIdx.x; c < cols; c += NT) {
-        const float v = fminf(fmaxf(rintf(to_f(xr[c]) / s), -127.0f), 127.0f);
-        q[row * ldq + c] = s > 0.0f ? (int8_t)(int)v : (int8_t)0;
+// rint(x / s) of n values as bytes, s > 0 and r = 1 / s rounded.  Adding 1.5 * 2^23
+// rounds to a whole number (half to even) and leaves it in the low bits.  x * r is
+// off by less than 127 * 2^-22 from x / s, so only a product that close to a tie
+// needs the division (about one value in 10^4).
+template <int N, typename T>
+__device__ __forceinline__ void quantize_n(const T (&x)[N], float s, float r, int8_t (&q)[N]) {
+    constexpr float magic = 12582912.0f;
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float t = __fmul_rn(to_f(x[i]), r), u = __fadd_rn(t, magic);
+        near |= fabsf(__fsub_rn(t, __fsub_rn(u, magic))) > 0.4999f;
+        q[i] = (int8_t)__float_as_int(u);
     }
-    if (threadIdx.x == 0) scale[row] = s;
+    if (near)
+#pragma unroll
+        for (int i = 0; i < N; i++) q[i] = (int8_t)__float_as_int(__fadd_rn(to_f(x[i]) / s, magic));
+}
+
+// The same by its definition, for any scale (0 and NaN give 0).
+__device__ __forceinline__ int8_t slow_quantized(float x, float s) {
+    return s > 0.0f ? (int8_t)(int)fminf(fmaxf(rintf(x / s), -127.0f), 127.0f) : (int8_t)0;
+}
+
+// TPR threads hold a row in registers, V elements at a time (V > 1: 16-byte
+// loads), NV times each; rows that this does not hold are read twice (NV = 0).
+// One pass over HBM: 4096 x 8192 bf16 (100 MB moved) takes @Q4096@ us.
+template <typename T, int V, int TPR, int NV>
+__global__ void __launch_bounds__(TPR < NT ? NT : TPR)
+    quantize_kernel(const T *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int64_t rows, int64_t cols) {
+    constexpr int BLOCK = TPR < NT ? NT : TPR;
+    __shared__ float sm[BLOCK / 32];
+    struct alignas(V * sizeof(T)) Vec {
+        T e[V];
+    };
+    struct alignas(V) Out {
+        int8_t e[V];
+    };
+    const int64_t row = (int64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
+    const int t = threadIdx.x % TPR;
+    const bool in = row < rows;
+    const T *xr = x + (in ? row : 0) * ldx;
+    const int64_t n = cols / V, rest = n * V;  // whole vectors; the last cols % V elements are thread 0's
+    Vec v[NV ? NV : 1];
+    float m = 0.0f;
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            if (in && t + j * TPR < n) v[j] = ((const Vec *)xr)[t + j * TPR];
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            if (in && t + j * TPR < n)
+#pragma unroll
+                for (int e = 0; e < V; e++) m = max_nan(m, fabsf(to_f(v[j].e[e])));
+    } else if (in) {
+        for (int64_t i = t; i < n; i += TPR) {
+            v[0] = ((const Vec *)xr)[i];
+#pragma unroll
+            for (int e = 0; e < V; e++) m = max_nan(m, fabsf(to_f(v[0].e[e])));
+        }
+    }
+    if (V > 1 && in && t == 0)
+        for (int64_t c = rest; c < cols; c++) m = max_nan(m, fabsf(to_f(xr[c])));
+    m = warp_max_nan(m);
+    if (TPR > 32) {
+        if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
+        __syncthreads();
+        const int w0 = threadIdx.x / TPR * (TPR / 32);
+        m = sm[w0];
+#pragma unroll
+        for (int w = 1; w < TPR / 32; w++) m = max_nan(m, sm[w0 + w]);
+    }
+    if (!in) return;
+    const float s = isfinite(m) ? m / 127.0f : NAN, r = 1.0f / s;
+    const bool ok = s > 0.0f && isfinite(r);  // r overflows for a scale below 2^-128: divide
+    int8_t *qr = q + row * ldq;
+    auto put = [&](const Vec &w, int64_t i) {
+        Out o;
+        if (ok) {
+            quantize_n(w.e, s, r, o.e);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) o.e[e] = slow_quantized(to_f(w.e[e]), s);
+        }
+        ((Out *)qr)[i] = o;
+    };
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            if (t + j * TPR < n) put(v[j], t + j * TPR);
+    } else {
+        for (int64_t i = t; i < n; i += TPR) put(((const Vec *)xr)[i], i);
+    }
+    if (t == 0) {
+        if (V > 1)
+            for (int64_t c = rest; c < cols; c++) qr[c] = slow_quantized(to_f(xr[c]), s);
+        scale[row] = s;
+    }
 }
 
 // A 64 x 64 tile of the product per block, 64 bytes of the inner axis at a
@@ -84,6 +163,224 @@ __global__ void __launch_bounds__(NT) int8_matmul_kernel(const int8_t *a, int64_
         }
 }
 
+// The product of a few tokens: the weights' bytes are all that counts, so each is
+// loaded once, 16 bytes a lane, four loads in flight (64 KiB an SM).  A warp keeps the same
+// 512-byte chunks (at most CPW) of the inner axis for all its channels, so its
+// lanes hold the tokens' values of those bytes in registers: a load costs four
+// multiply-adds a token and one sum over the warp, which goes to the block's
+// whole-number sums.  X is int8 (with its scales), or one of the head's types,
+// which each block quantises for itself while its first weights are on their
+// way: one launch for a token's whole linear layer.
+constexpr int GV_WARPS = 16, GV_LOADS = 4, GV_CHANNELS = 512;
+
+// 16 neighbouring values of a token's row from c on as 32-bit numbers, 0 past k.
+template <typename X>
+__device__ __forceinline__ void load16(const X *x, int c, int k, bool vec, float (&f)[16]) {
+    if (vec && c + 16 <= k) {
+        struct alignas(16) Vec {
+            X e[16 / sizeof(X)];
+        };
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(X); j++) {
+            const Vec v = ((const Vec *)(x + c))[j];
+#pragma unroll
+            for (int e = 0; e < 16 / (int)sizeof(X); e++) f[j * (16 / sizeof(X)) + e] = to_f(v.e[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; e++) f[e] = c + e < k ? to_f(x[c + e]) : 0.0f;
+    }
+}
+
+template <int M, int CPW, typename X, typename T>
+__global__ void __launch_bounds__(GV_WARPS * 32, 2)
+    int8_vec_kernel(const X *x, int64_t ldx, const float *sx, const int8_t *w, int64_t ldw, const float *sw,
+                    const float *bias, T *out, int64_t ldo, int m, int64_t n, int k, int per, int cw) {
+    __shared__ int sums[GV_CHANNELS * M];
+    __shared__ float red[M][GV_WARPS], scale[M];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+    // warp = (group of channels, place on the inner axis); its chunk j is at byte (place + cw j) 512 + 16 lane
+    const int groups = nw / cw, place = warp % cw, group = warp / cw;
+    constexpr int U = GV_LOADS / CPW;  // channels in flight
+    uint32_t xq[M][CPW][4];
+    int rest[CPW];  // bytes of the row from the lane's place on
+#pragma unroll
+    for (int j = 0; j < CPW; j++) rest[j] = k - (place + cw * j) * 512 - lane * 16;
+
+    bool first = true;
+    for (int64_t c0 = (int64_t)blockIdx.x * per; c0 < n; c0 += (int64_t)gridDim.x * per) {
+        const int nch = (int)(n - c0 < per ? n - c0 : per);
+        const int whole = c0 + nch == n ? nch - 1 : nch;  // channels whose row is not the last
+        int next = group;                                 // the next channel to be loaded
+        const int8_t *fp = w + (c0 + group) * ldw + place * 512 + lane * 16;
+        uint4 buf[U][CPW];
+        auto fetch = [&](uint4 (&v)[CPW]) {
+#pragma unroll
+            for (int j = 0; j < CPW; j++) {
+                // 16 bytes that begin inside a row end inside its pitch (a multiple of 16); what lies past k
+                // meets zeros.  Only the last channel's row may end with the memory: its part is added below.
+                v[j] = make_uint4(0, 0, 0, 0);
+                if (next < (rest[j] < 16 ? whole : nch) && rest[j] > 0)
+                    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(v[j].x), "=r"(v[j].y), "=r"(v[j].z), "=r"(v[j].w)
+                                 : "l"(fp + cw * j * 512));
+            }
+            next += groups;
+            fp += groups * ldw;
+        };
+#pragma unroll
+        for (int u = 0; u < U; u++) fetch(buf[u]);
+        for (int i = threadIdx.x; i < M * nch; i += blockDim.x) sums[i] = 0;
+        if (first) {  // the tokens, while the first weights are on their way
+            first = false;
+            if constexpr (sizeof(X) == 1) {
+#pragma unroll
+                for (int r = 0; r < M; r++)
+#pragma unroll
+                    for (int j = 0; j < CPW; j++) {
+                        const int c = (place + cw * j) * 512 + lane * 16;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            uint32_t q = 0;
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (r < m && c + 4 * e + i < k) q |= (uint32_t)(uint8_t)x[r * ldx + c + 4 * e + i] << (8 * i);
+                            xq[r][j][e] = q;
+                        }
+                    }
+                if (threadIdx.x < m) scale[threadIdx.x] = sx[threadIdx.x];
+            } else {
+                const bool vec = ((uintptr_t)x & 15) == 0 && ldx * (int64_t)sizeof(X) % 16 == 0;
+                float f[16];
+#pragma unroll
+                for (int r = 0; r < M; r++) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < CPW; j++) {
+                        if (r >= m) break;
+                        load16(x + r * ldx, (place + cw * j) * 512 + lane * 16, k, vec, f);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) top = max_nan(top, fabsf(f[e]));
+                    }
+                    top = warp_max_nan(top);
+                    if (lane == 0) red[r][warp] = top;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int r = 0; r < M; r++) {
+                    const float t = warp_max_nan(red[r][lane % nw]);
+                    const float s = isfinite(t) ? t / 127.0f : NAN, inv = 1.0f / s;
+                    const bool ok = s > 0.0f && isfinite(inv);
+#pragma unroll
+                    for (int j = 0; j < CPW; j++) {
+                        alignas(4) int8_t q[16] = {};
+                        if (r < m) {
+                            load16(x + r * ldx, (place + cw * j) * 512 + lane * 16, k, vec, f);
+                            if (ok) {
+                                quantize_n(f, s, inv, q);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 16; e++) q[e] = slow_quantized(f[e], s);
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) xq[r][j][e] = ((const uint32_t *)q)[e];
+                    }
+                    if (threadIdx.x == 0) scale[r] = s;
+                }
+            }
+        }
+        __syncthreads();
+        for (int c = group; c < nch; c += groups * U) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int ch = c + u * groups;
+                if (ch < nch) {
+                    int acc[M] = {};
+#pragma unroll
+                    for (int j = 0; j < CPW; j++)
+#pragma unroll
+                        for (int r = 0; r < M; r++) {
+                            acc[r] = __dp4a((int)buf[u][j].x, (int)xq[r][j][0], acc[r]);
+                            acc[r] = __dp4a((int)buf[u][j].y, (int)xq[r][j][1], acc[r]);
+                            acc[r] = __dp4a((int)buf[u][j].z, (int)xq[r][j][2], acc[r]);
+                            acc[r] = __dp4a((int)buf[u][j].w, (int)xq[r][j][3], acc[r]);
+                        }
+                    fetch(buf[u]);
+#pragma unroll
+                    for (int r = 0; r < M; r++) {
+                        const int t = __reduce_add_sync(0xffffffffu, acc[r]);
+                        if (lane == 0) atomicAdd(&sums[ch * M + r], t);
+                    }
+                }
+            }
+        }
+        if (whole < nch && group == 0) {  // the end of the last row, byte by byte
+#pragma unroll
+            for (int j = 0; j < CPW; j++) {
+                if (rest[j] <= 0 || rest[j] >= 16) continue;
+                const int8_t *p = w + (n - 1) * ldw + (k - rest[j]);
+                for (int r = 0; r < m; r++) {
+                    int t = 0;
+#pragma unroll
+                    for (int i = 0; i < 15; i++) {
+                        int8_t q = 0;
+#pragma unroll
+                        for (int rr = 0; rr < M; rr++)
+                            if (rr == r) q = (int8_t)(xq[rr][j][i >> 2] >> (8 * (i & 3)));
+                        if (i < rest[j]) t += (int)p[i] * (int)q;
+                    }
+                    atomicAdd(&sums[whole * M + r], t);
+                }
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < nch * m; i += blockDim.x) {
+            const int c = i % nch, r = i / nch;
+            out[r * ldo + c0 + c] = from_f<T>(result(sums[c * M + r], scale[r], sw[c0 + c], bias, bias ? bias[c0 + c] : 0.0f));
+        }
+        __syncthreads();  // the sums have been read
+    }
+}
+
+// Whether the kernel above takes m tokens of k values: their values of a warp's
+// chunks fit its registers.
+int vec_rows(int64_t m) { return m <= 2 ? (int)m : 4; }
+int vec_chunks(int64_t k) {
+    const int64_t c = (k + 512 * GV_WARPS - 1) / (512 * GV_WARPS);
+    return c <= 2 ? (int)c : c <= 4 ? 4 : 0;
+}
+bool takes_vec(const int8_t *w, int64_t ldw, int64_t m, int64_t k) {
+    return m >= 1 && m <= 4 && k > 0 && aligned_to(w, 16) && ldw % 16 == 0 && vec_chunks(k) &&
+           vec_rows(m) * vec_chunks(k) <= 4;
+}
+
+template <int M, int CPW, typename X, typename T>
+int launch_vec(const X *x, int64_t ldx, const float *sx, const int8_t *w, int64_t ldw, const float *sw, const float *bias,
+               T *out, int64_t ldo, int64_t m, int64_t n, int64_t k, cudaStream_t s) {
+    const int chunks = (int)((k + 511) / 512), cw = (chunks + CPW - 1) / CPW, groups = GV_WARPS / cw;
+    int64_t per = (n + 2 * num_sms() - 1) / (2 * num_sms());
+    if (per > GV_CHANNELS) per = GV_CHANNELS;
+    int64_t blocks = (n + per - 1) / per;
+    if (blocks > 2 * num_sms()) blocks = 2 * num_sms();
+    int8_vec_kernel<M, CPW, X, T><<<(unsigned)blocks, cw * groups * 32, 0, s>>>(x, ldx, sx, w, ldw, sw, bias, out, ldo, (int)m,
+                                                                               n, (int)k, (int)per, cw);
+    ZC_LAUNCHED("int8_vec_kernel");
+    return ZPUCUDA_OK;
+}
+template <typename X, typename T>
+int product_vec(const X *x, int64_t ldx, const float *sx, const int8_t *w, int64_t ldw, const float *sw, const float *bias,
+                T *out, int64_t ldo, int64_t m, int64_t n, int64_t k, cudaStream_t s) {
+    switch (vec_rows(m) * 8 + vec_chunks(k)) {
+    case 8 + 1: return launch_vec<1, 1, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
+    case 8 + 2: return launch_vec<1, 2, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
+    case 8 + 4: return launch_vec<1, 4, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
+    case 16 + 1: return launch_vec<2, 1, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
+    case 16 + 2: return launch_vec<2, 2, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
+    default: return launch_vec<4, 1, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
+    }
+}
+
 // A product on the tensor cores: D[p, q] = sum over k of P[p, k] * Q[q, k] in
 // tiles of 128 x BN, for operands that a tensor map can describe (addresses
 // and row pitches multiples of 16 bytes).  P is a and Q is b, or (SWAP) P is b
@@ -92,21 +389,21 @@ __global__ void __launch_bounds__(NT) int8_matmul_kernel(const int8_t *a, int64_
 //
 // One CTA per SM walks tiles; warp 0 loads 128-byte slices of both operands by
 // TMA into a ring of stages, one lane of warp 1 issues tcgen05.mma (kind::i8,
-// exact 32-bit sums in TMEM), warps 2-5 turn a finished tile into the result
+// exact 32-bit sums in TMEM), warps 2-9 turn a finished tile into the result
 // while the next one is summed into the other TMEM buffer.  With few tiles the
-// inner axis is split over a cluster, whose CTAs hand their sums to the first
-// through shared memory (whole numbers: the split does not change the result).
-constexpr int TC_THREADS = 192;
+// inner axis is split over a cluster, whose CTAs add up each other's sums through
+// shared memory (whole numbers: the split does not change the result).
+constexpr int TC_THREADS = 320;  // producer, issuer, eight storing warps
 constexpr int TC_STAGE_A = 128 * 128;
 template <int BN>
 struct TcTile {
     static constexpr int STAGE = TC_STAGE_A + BN * 128;
     static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
     static constexpr int COLS = 2 * BN < 32 ? 32 : 2 * BN;  // two sums in TMEM
-    static constexpr int PART = 128 * (BN + 1) * 4;         // a split's sums, rows padded against bank conflicts
-    static constexpr int XPOSE = 4 * 32 * 33 * 4;           // 32 x 32 results of each of the four storing warps
-    static constexpr int SMEM = STAGES * STAGE + XPOSE + 1024;
-    static_assert(SMEM <= 227 * 1024 && (BN == 256 || PART <= STAGES * STAGE), "shared memory");
+    static constexpr int PART = BN * 132 * 4;               // a split's sums, one Q row after another
+    static constexpr int TURN = 8 * 32 * 64;                // 32 rows of 64 bytes of each storing warp
+    static constexpr int SMEM = STAGES * STAGE + TURN + 1024;
+    static_assert(SMEM + 16 * BN + 512 <= 227 * 1024 && (BN == 256 || PART <= STAGES * STAGE), "shared memory");
 };
 
 struct TcArgs {
@@ -139,6 +436,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full[TT::STAGES], empty[TT::STAGES], tfull[2], tfree[2];
     __shared__ uint32_t tmem_base;
+    __shared__ float sq[2][BN], bq[2][BN];  // the Q side's scales and biases, of this tile and the next
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ntiles = A.tiles_p * A.tiles_q;
     const int split = A.splits > 1 ? (int)cluster_rank() : 0;
@@ -158,7 +456,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         for (int b = 0; b < 2; b++) {
             tc::mb_init(&tfull[b], 1);
-            tc::mb_init(&tfree[b], 128);
+            tc::mb_init(&tfree[b], 256);
         }
         tc::mb_init_fence();
     }
@@ -218,70 +516,93 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             }
         }
     } else {
-        const int q4 = warp & 3;  // the quarter of the TMEM lanes that this warp may read
+        // warp w reads the quarter w % 4 of the TMEM lanes, and one half of the columns
+        constexpr int HALF = BN >= 32 ? BN / 2 : BN;
+        const int q4 = warp & 3, half = (warp - 2) >> 2;
         const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+        const bool idle = half * HALF >= BN;
         T *out = (T *)A.out;
-        float *turn = (float *)(smem + TT::STAGES * TT::STAGE) + q4 * 32 * 33;
-        const bool vec = !SWAP && ((uintptr_t)out & 15) == 0 && (A.ldo * (int64_t)sizeof(T)) % 16 == 0;
+        uint8_t *turn = smem + TT::STAGES * TT::STAGE + (warp - 2) * 2048;
+        const bool vec = ((uintptr_t)out & 15) == 0 && (A.ldo * (int64_t)sizeof(T)) % 16 == 0;
         int n = 0;
         for (int t = blockIdx.x; t < ntiles; t += gridDim.x, n++) {
             int tp, tq;
             place(t, &tp, &tq);
             const int buf = n & 1;
-            if (!tc::mb_wait(&tfull[buf], (n >> 1) & 1, &g_int8_error)) break;
-            __syncwarp();
+            const int64_t p = (int64_t)tp * 128 + q4 * 32 + lane;
+            float sp = 0.0f, bp = 0.0f;
+            if (A.splits == 1) {  // the scales, while the sums are being made
+                for (int i = threadIdx.x - 64; i < BN; i += 256) {
+                    const int64_t q = (int64_t)tq * BN + i;
+                    const bool in = q < (SWAP ? A.tokens : A.channels);
+                    sq[buf][i] = in ? (SWAP ? A.sa[q] : A.sb[q]) : 0.0f;
+                    if (!SWAP) bq[buf][i] = in && A.bias ? A.bias[q] : 0.0f;
+                }
+                if (p < (SWAP ? A.channels : A.tokens)) sp = SWAP ? A.sb[p] : A.sa[p];
+                if (SWAP && A.bias && p < A.channels) bp = A.bias[p];
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+            }
+            const bool ok = tc::mb_wait(&tfull[buf], (n >> 1) & 1, &g_int8_error);
+            if (!__all_sync(0xffffffffu, ok)) break;
             tc::fence_after();
-            if (A.splits > 1) {  // this split's sums, for the first CTA of the cluster (one tile per cluster)
-                int *part = (int *)smem + (q4 * 32 + lane) * (BN + 1);
-                for (int c = 0; c < BN; c += 16) {
+            if (A.splits > 1) {  // this split's sums, for the whole cluster (one tile per cluster)
+                int *part = (int *)smem + q4 * 32 + lane;
+                for (int c = half * HALF; !idle && c < half * HALF + HALF; c += 16) {
                     int v[16];
                     tc::tmem_ld16(tmem + lanes + (uint32_t)(buf * BN + c), v);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) part[c + i] = v[i];
+                    for (int i = 0; i < 16; i++) part[(c + i) * 132] = v[i];
                 }
                 break;
             }
-            const int64_t p = (int64_t)tp * 128 + q4 * 32 + lane;
-            const float sp = SWAP ? (p < A.channels ? A.sb[p] : 0.0f) : (p < A.tokens ? A.sa[p] : 0.0f);
-            const float bp = SWAP && A.bias && p < A.channels ? A.bias[p] : 0.0f;
-#pragma unroll 1
-            for (int c = 0; c < BN; c += 16) {
-                int v[16];
-                __syncwarp();
-                tc::tmem_ld16(tmem + lanes + (uint32_t)(buf * BN + c), v);
-                const int64_t q0 = (int64_t)tq * BN + c;
-                if constexpr (SWAP) {  // a lane is a channel: 32 neighbours of one token's row per store
+            if constexpr (SWAP) {  // a lane is a channel: 32 neighbours of one token's row per store
+                for (int c = half * HALF; !idle && c < half * HALF + HALF; c += 16) {
+                    int v[16];
+                    __syncwarp();
+                    tc::tmem_ld16(tmem + lanes + (uint32_t)(buf * BN + c), v);
+                    const int64_t q0 = (int64_t)tq * BN + c;
 #pragma unroll
                     for (int i = 0; i < 16; i++)
                         if (q0 + i < A.tokens && p < A.channels)
-                            out[(q0 + i) * A.ldo + p] = from_f<T>(result(v[i], A.sa[q0 + i], sp, A.bias, bp));
-                } else {
-                    float y[16];
+                            out[(q0 + i) * A.ldo + p] = from_f<T>(result(v[i], sq[buf][c + i], sp, A.bias, bp));
+                }
+            } else {
+                // 32 rows of 64 bytes turned in shared memory (16-byte piece u of row r at
+                // u ^ (r / 2 % 4)), so that a store writes 64 bytes of each of eight rows
+                constexpr int W = 64 / sizeof(T), E = 16 / sizeof(T);
+#pragma unroll 1
+                for (int c = half * HALF; c < half * HALF + HALF; c += W) {
+                    __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int64_t q = q0 + i < A.channels ? q0 + i : A.channels - 1;
-                        y[i] = result(v[i], sp, A.sb[q], A.bias, A.bias ? A.bias[q] : 0.0f);
+                    for (int h = 0; h < W; h += 16) {
+                        int v[16];
+                        tc::tmem_ld16(tmem + lanes + (uint32_t)(buf * BN + c + h), v);
+                        alignas(16) T w[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            w[i] = from_f<T>(result(v[i], sp, sq[buf][c + h + i], A.bias, bq[buf][c + h + i]));
+#pragma unroll
+                        for (int u = 0; u < 16 / E; u++)
+                            *(uint4 *)(turn + lane * 64 + (((h / E + u) ^ (lane >> 1 & 3)) * 16)) = ((const uint4 *)w)[u];
                     }
-                    if (vec && q0 + 16 <= A.channels) {
-                        if (p < A.tokens) {
-                            alignas(16) T w[16];
+                    __syncwarp();
+                    const int64_t q0 = (int64_t)tq * BN + c, p0 = (int64_t)tp * 128 + q4 * 32;
+                    if (vec && q0 + W <= A.channels) {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) w[i] = from_f<T>(y[i]);
-#pragma unroll
-                            for (int i = 0; i < (int)sizeof(w) / 16; i++)
-                                ((uint4 *)(out + p * A.ldo + q0))[i] = ((const uint4 *)w)[i];
+                        for (int r = 0; r < 32; r += 8) {
+                            const int rr = r + (lane >> 2), u = lane & 3;
+                            if (p0 + rr < A.tokens)
+                                *(uint4 *)(out + (p0 + rr) * A.ldo + q0 + u * E) =
+                                    *(const uint4 *)(turn + rr * 64 + ((u ^ (rr >> 1 & 3)) * 16));
                         }
-                    } else {  // turned in shared memory: 16 neighbours of each of two rows per store
-                        __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < 16; i++) turn[lane * 33 + i] = y[i];
-                        __syncwarp();
-#pragma unroll
-                        for (int r = 0; r < 32; r += 2) {
-                            const int rr = r + (lane >> 4);
-                            const int64_t row = (int64_t)tp * 128 + q4 * 32 + rr, q = q0 + (lane & 15);
-                            if (row < A.tokens && q < A.channels) out[row * A.ldo + q] = from_f<T>(turn[rr * 33 + (lane & 15)]);
-                        }
+                    } else {
+                        const int rows = (int)(A.tokens - p0 < 32 ? A.tokens - p0 : 32);
+                        constexpr int R = 32 / W;  // rows of a store
+                        const int j = lane % W;
+                        if (q0 + j < A.channels)
+                            for (int r = lane / W; r < rows; r += R)
+                                out[(p0 + r) * A.ldo + q0 + j] =
+                                    *(const T *)(turn + r * 64 + (((j / E) ^ (r >> 1 & 3)) * 16) + (j % E) * sizeof(T));
                     }
                 }
             }
@@ -293,20 +614,30 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     if (A.splits > 1) {
         // all sums are in place (the stages' loads have all been read by then)
         cluster_sync();
-        if (split == 0) {
-            int tp, tq;
-            place(blockIdx.x, &tp, &tq);
-            T *out = (T *)A.out;
-            for (int i = threadIdx.x; i < 128 * BN; i += TC_THREADS) {
-                // neighbouring threads hold neighbouring channels
-                const int pr = SWAP ? i & 127 : i / BN, qc = SWAP ? i >> 7 : i % BN;
-                int sum = ((const int *)smem)[pr * (BN + 1) + qc];
-                for (int r = 1; r < A.splits; r++) sum += ((const int *)cluster_map(smem, r))[pr * (BN + 1) + qc];
-                const int64_t p = (int64_t)tp * 128 + pr, q = (int64_t)tq * BN + qc;
-                const int64_t token = SWAP ? q : p, ch = SWAP ? p : q;
-                if (token < A.tokens && ch < A.channels)
-                    out[token * A.ldo + ch] = from_f<T>(result(sum, A.sa[token], A.sb[ch], A.bias, A.bias ? A.bias[ch] : 0.0f));
+        // each CTA adds up its share: four neighbouring channels of a token a thread
+        int tp, tq;
+        place(blockIdx.x, &tp, &tq);
+        T *out = (T *)A.out;
+        const int share = (BN + A.splits - 1) / A.splits, first = split * share, end = min(BN, first + share);
+        for (int i = threadIdx.x; i < (end - first) * 32; i += TC_THREADS) {
+            const int qc = first + (i >> 5), at = qc * 132 + (i & 31) * 4;
+            const int64_t token = (int64_t)tq * BN + qc, ch = (int64_t)tp * 128 + (i & 31) * 4;
+            if (token >= A.tokens || ch >= A.channels) continue;
+            int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 8
+            for (int r = 0; r < A.splits; r++) {
+                const int4 v = *(const int4 *)((const int *)cluster_map(smem, r) + at);
+                sum.x += v.x;
+                sum.y += v.y;
+                sum.z += v.z;
+                sum.w += v.w;
             }
+            const int y[4] = {sum.x, sum.y, sum.z, sum.w};
+            const float sa = A.sa[token];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (ch + e < A.channels)
+                    out[token * A.ldo + ch + e] = from_f<T>(result(y[e], sa, A.sb[ch + e], A.bias, A.bias ? A.bias[ch + e] : 0.0f));
         }
         cluster_sync();  // the others' shared memory stays until it has been read
     }
@@ -373,9 +704,13 @@ int product_tc(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, i
     *done = false;
     // a tensor map's rows: at most 2^31, its coordinates 32 bits
     if (!aligned_to(a, 16) || !aligned_to(b, 16) || lda % 16 || ldb % 16 || k == 0) return ZPUCUDA_OK;
-    // few tokens: weights along the 128 rows, the tokens in the narrowest tile that holds them
-    const bool swap = m <= 128;
-    const int bn = !swap ? 256 : m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+    // few tokens: weights along the 128 rows, the tokens in the narrowest tile that holds them; so too where
+    // the tiles fill less than half of the SMs and the inner axis will be split
+    const bool swap = m <= 128 || (m + 127) / 128 * ((n + 127) / 128) * 2 <= num_sms();
+    // wide tiles read half as much per product; narrow ones where they fill the SMs' last wave better
+    const auto waves = [&](int w) { return ((m + 127) / 128 * ((n + w - 1) / w) + num_sms() - 1) / num_sms(); };
+    const int wide = 2 * waves(256) <= waves(128) ? 256 : 128;
+    const int bn = !swap ? wide : m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
     TcArgs A = {sa, sb, bias, out, ldo, m, n};
     const int64_t P = swap ? n : m, Q = swap ? m : n;
     A.tiles_p = (int)((P + 127) / 128);
@@ -385,31 +720,52 @@ int product_tc(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, i
     // split the inner axis while the tiles leave most SMs idle, with at least four slices left to each
     int64_t splits = 1;
     const int64_t tiles = (int64_t)A.tiles_p * A.tiles_q;
-    while (bn <= 128 && splits < 8 && tiles * splits * 2 <= num_sms() && A.kt / (splits * 2) >= 4) splits *= 2;
+    while (swap && splits < 8 && tiles * splits * 2 <= num_sms() && A.kt / (splits * 2) >= 4) splits *= 2;
     A.kt_split = (int)((A.kt + splits - 1) / splits);
     A.splits = (A.kt + A.kt_split - 1) / A.kt_split;  // no split without a slice
     CUtensorMap mp, mq;
     if (!make_map(&mp, swap ? b : a, k, P, swap ? ldb : lda, 128) || !make_map(&mq, swap ? a : b, k, Q, swap ? lda : ldb, bn))
         return ZPUCUDA_OK;
     *done = true;
-    if (!swap) return launch_tc<256, false, T>(mp, mq, A, s);
+    if (!swap) return bn == 256 ? launch_tc<256, false, T>(mp, mq, A, s) : launch_tc<128, false, T>(mp, mq, A, s);
     if (bn == 16) return launch_tc<16, true, T>(mp, mq, A, s);
     if (bn == 32) return launch_tc<32, true, T>(mp, mq, A, s);
     if (bn == 64) return launch_tc<64, true, T>(mp, mq, A, s);
     return launch_tc<128, true, T>(mp, mq, A, s);
 }
 
+template <typename T, int V>
+int launch_quantize(const T *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int64_t rows, int64_t cols,
+                    cudaStream_t s) {
+    constexpr int NV = V > 1 ? 4 : 16;
+    const int64_t n = cols / V;
+    const unsigned few = (unsigned)((rows + NT / 32 - 1) / (NT / 32)), all = (unsigned)rows;
+    // a warp a row while it holds the row, then 256 and 1024 threads
+    if (n <= 32 * NV) quantize_kernel<T, V, 32, NV><<<few, NT, 0, s>>>(x, ldx, q, ldq, scale, rows, cols);
+    else if (n <= NT * NV) quantize_kernel<T, V, NT, NV><<<all, NT, 0, s>>>(x, ldx, q, ldq, scale, rows, cols);
+    else if (n <= 1024 * NV) quantize_kernel<T, V, 1024, NV><<<all, 1024, 0, s>>>(x, ldx, q, ldq, scale, rows, cols);
+    else quantize_kernel<T, V, 1024, 0><<<all, 1024, 0, s>>>(x, ldx, q, ldq, scale, rows, cols);
+    ZC_LAUNCHED("quantize_kernel");
+    return ZPUCUDA_OK;
+}
+
 int quantize(int dtype, const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int64_t rows, int64_t cols,
              cudaStream_t s) {
     if (rows == 0) return ZPUCUDA_OK;
-    ZC_HEAD_TYPE(dtype, T, quantize_kernel<T><<<(unsigned)rows, NT, 0, s>>>((const T *)x, ldx, q, ldq, scale, cols));
-    ZC_LAUNCHED("quantize_kernel");
-    return ZPUCUDA_OK;
+    const int V = 16 / elem_bytes(dtype);
+    const bool vec = aligned_to(x, 16) && ldx % V == 0 && aligned_to(q, V) && ldq % V == 0;
+    ZC_HEAD_TYPE(dtype, T, {
+        constexpr int W = 16 / sizeof(T);
+        return vec ? launch_quantize<T, W>((const T *)x, ldx, q, ldq, scale, rows, cols, s)
+                   : launch_quantize<T, 1>((const T *)x, ldx, q, ldq, scale, rows, cols, s);
+    });
 }
 
 int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb, const float *sb,
             const float *bias, int dtype, void *out, int64_t ldo, int64_t m, int64_t n, int64_t k, cudaStream_t s) {
     if (m == 0 || n == 0) return ZPUCUDA_OK;
+    if (takes_vec(b, ldb, m, k))
+        ZC_HEAD_TYPE(dtype, T, return (product_vec<int8_t, T>(a, lda, sa, b, ldb, sb, bias, (T *)out, ldo, m, n, k, s)));
     bool done = false;
     ZC_HEAD_TYPE(dtype, T, ZC_TRY(product_tc<T>(a, lda, sa, b, ldb, sb, bias, (T *)out, ldo, m, n, k, s, &done)));
     if (done) return ZPUCUDA_OK;
@@ -469,6 +825,9 @@ int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d
     if (!d_work || work_bytes < zpucuda_int8_linear_work(rows, inner) || !aligned_to(d_work, 16))
         return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "int8_linear: work: null, too small or not 16-byte aligned");
     cudaStream_t s = resolve_stream(stream);
+    if (takes_vec(d_w, ldw, rows, inner))
+        ZC_HEAD_TYPE(dtype, T, return (product_vec<T, T>((const T *)d_x, ldx, nullptr, d_w, ldw, d_sw, d_bias, (T *)d_y,
+                                                         ldy, rows, cols, inner, s)));
     const int64_t ldq = (inner + 15) / 16 * 16;
     int8_t *q = (int8_t *)d_work;
     float *scale = (float *)(q + rows * ldq);
