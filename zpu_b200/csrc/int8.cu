@@ -163,104 +163,109 @@ __global__ void __launch_bounds__(NT) int8_matmul_kernel(const int8_t *a, int64_
         }
 }
 
-// The product of a few tokens: the weights' bytes are all that counts, so each is
-// loaded once, 16 bytes a lane, four loads in flight (64 KiB an SM).  A warp keeps the same
-// 512-byte chunks (at most CPW) of the inner axis for all its channels, so its
-// lanes hold the tokens' values of those bytes in registers: a load costs four
-// multiply-adds a token and one sum over the warp, which goes to the block's
-// whole-number sums.  X is int8 (with its scales), or one of the head's types,
-// which each block quantises for itself while its first weights are on their
-// way: one launch for a token's whole linear layer.
-constexpr int GV_WARPS = 16, GV_LOADS = 4, GV_CHANNELS = 512;
+// The product of one or two tokens: the weights' bytes are all that counts, so
+// they are streamed once, by bulk copies into shared memory: 16 warps with a ring
+// of two 4 KiB slots each keep 128 KiB an SM in flight, and the first of them are
+// on their way before the tokens are even read (loads into registers: 18.5 us
+// where this takes 15.1, 16384 x 4096).  X is int8 (with its scales), or
+// one of the head's types, which each block quantises for itself: one launch
+// for a token's whole linear layer.  A unit is a slot's worth: several short
+// rows, or a piece of a long one; a block's units are dealt out evenly to its
+// warps, and what a warp has of a channel goes to the block's whole-number sums.
+constexpr int GV_WARPS = 16, GV_SLOTS = 2, GV_SLOT = 4096, GV_ROWS = 8, GV_CHANNELS = 512;
+constexpr int GV_RING = GV_WARPS * GV_SLOTS * GV_SLOT, GV_X = 64 * 1024;  // shared memory: weights, tokens
 
-// 16 neighbouring values of a token's row from c on as 32-bit numbers, 0 past k.
-template <typename X>
-__device__ __forceinline__ void load16(const X *x, int c, int k, bool vec, float (&f)[16]) {
-    if (vec && c + 16 <= k) {
-        struct alignas(16) Vec {
-            X e[16 / sizeof(X)];
-        };
-#pragma unroll
-        for (int j = 0; j < (int)sizeof(X); j++) {
-            const Vec v = ((const Vec *)(x + c))[j];
-#pragma unroll
-            for (int e = 0; e < 16 / (int)sizeof(X); e++) f[j * (16 / sizeof(X)) + e] = to_f(v.e[e]);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++) f[e] = c + e < k ? to_f(x[c + e]) : 0.0f;
-    }
-}
+struct VecArgs {
+    const int8_t *w;
+    const float *sx, *sw, *bias;
+    int64_t ldx, ldw, ldo, n;
+    int m, k, per;       // tokens, values, channels of a block's round
+    int seg, segs, rows; // bytes of a piece, pieces of a row, rows of a unit (1 where a row has several pieces)
+};
 
-template <int M, int CPW, typename X, typename T>
-__global__ void __launch_bounds__(GV_WARPS * 32, 2)
-    int8_vec_kernel(const X *x, int64_t ldx, const float *sx, const int8_t *w, int64_t ldw, const float *sw,
-                    const float *bias, T *out, int64_t ldo, int m, int64_t n, int k, int per, int cw) {
+template <int M, typename X, typename T>
+__global__ void __launch_bounds__(GV_WARPS * 32, 1) int8_vec_kernel(const X *x, T *out, const VecArgs A) {
+    extern __shared__ __align__(128) uint8_t vec_smem[];
     __shared__ int sums[GV_CHANNELS * M];
     __shared__ float red[M][GV_WARPS], scale[M];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-    // warp = (group of channels, place on the inner axis); its chunk j is at byte (place + cw j) 512 + 16 lane
-    const int groups = nw / cw, place = warp % cw, group = warp / cw;
-    constexpr int U = GV_LOADS / CPW;  // channels in flight
-    uint32_t xq[M][CPW][4];
-    int rest[CPW];  // bytes of the row from the lane's place on
-#pragma unroll
-    for (int j = 0; j < CPW; j++) rest[j] = k - (place + cw * j) * 512 - lane * 16;
+    __shared__ uint64_t full[GV_WARPS][GV_SLOTS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k = A.k;
+    uint8_t *ring = vec_smem + warp * (GV_SLOTS * GV_SLOT);
+    int8_t *xs = (int8_t *)vec_smem + GV_RING;
+    const int pitch = (k + 511) / 512 * 512;  // of the tokens' rows, zeros past k
+    if (lane == 0) {
+        for (int i = 0; i < GV_SLOTS; i++) tc::mb_init(&full[warp][i], 1);
+        tc::mb_init_fence();
+    }
+    __syncwarp();
 
-    bool first = true;
-    for (int64_t c0 = (int64_t)blockIdx.x * per; c0 < n; c0 += (int64_t)gridDim.x * per) {
-        const int nch = (int)(n - c0 < per ? n - c0 : per);
-        const int whole = c0 + nch == n ? nch - 1 : nch;  // channels whose row is not the last
-        int next = group;                                 // the next channel to be loaded
-        const int8_t *fp = w + (c0 + group) * ldw + place * 512 + lane * 16;
-        uint4 buf[U][CPW];
-        auto fetch = [&](uint4 (&v)[CPW]) {
-#pragma unroll
-            for (int j = 0; j < CPW; j++) {
-                // 16 bytes that begin inside a row end inside its pitch (a multiple of 16); what lies past k
-                // meets zeros.  Only the last channel's row may end with the memory: its part is added below.
-                v[j] = make_uint4(0, 0, 0, 0);
-                if (next < (rest[j] < 16 ? whole : nch) && rest[j] > 0)
-                    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(v[j].x), "=r"(v[j].y), "=r"(v[j].z), "=r"(v[j].w)
-                                 : "l"(fp + cw * j * 512));
+    bool first = true, ok = true;
+    int issued = 0, used = 0;  // this warp's units, over all rounds
+    for (int64_t c0 = (int64_t)blockIdx.x * A.per; c0 < A.n; c0 += (int64_t)gridDim.x * A.per) {
+        const int nch = (int)(A.n - c0 < A.per ? A.n - c0 : A.per);
+        const int units = (nch + A.rows - 1) / A.rows * A.segs;
+        const int u0 = (int)((int64_t)units * warp / GV_WARPS), u1 = (int)((int64_t)units * (warp + 1) / GV_WARPS);
+        int next = u0;
+        auto issue = [&]() {  // lane 0: unit `next` into its slot
+            const int slot = issued % GV_SLOTS, piece = next % A.segs, ch = next / A.segs * A.rows;
+            const int rows = min(A.rows, nch - ch), at = piece * A.seg, rest = k - at;
+            uint8_t *dst = ring + slot * GV_SLOT;
+            const int8_t *src = A.w + (c0 + ch) * A.ldw + at;
+            // 16 bytes that begin inside a row end inside its pitch (a multiple of 16), and what lies past k meets
+            // zeros; the last row may end with the memory, so its last bytes come one by one
+            const int size = min(A.seg, (rest + 15) & ~15);
+            const bool last = c0 + ch + rows == A.n && (rest & 15) && rest < A.seg;
+            const int lsize = last ? rest & ~15 : size;
+            if (last)
+                for (int b = lsize; b < rest; b++) dst[(rows - 1) * A.seg + b] = (uint8_t)src[(rows - 1) * A.ldw + b];
+            tc::mb_expect_tx(&full[warp][slot], (uint32_t)(size * (rows - 1) + lsize));
+            for (int r = 0; r < rows; r++) {
+                const int n = r == rows - 1 ? lsize : size;
+                if (n)
+                    asm volatile(
+                        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                            tc::su32(dst + r * A.seg)),
+                        "l"(src + r * A.ldw), "r"(n), "r"(tc::su32(&full[warp][slot]))
+                        : "memory");
             }
-            next += groups;
-            fp += groups * ldw;
+            next++;
+            issued++;
         };
-#pragma unroll
-        for (int u = 0; u < U; u++) fetch(buf[u]);
-        for (int i = threadIdx.x; i < M * nch; i += blockDim.x) sums[i] = 0;
+        if (lane == 0)
+            while (ok && next < u1 && issued - used < GV_SLOTS) issue();
+        for (int i = threadIdx.x; i < M * nch; i += GV_WARPS * 32) sums[i] = 0;
         if (first) {  // the tokens, while the first weights are on their way
             first = false;
+            for (int i = threadIdx.x; i < M * pitch / 16; i += GV_WARPS * 32) ((uint4 *)xs)[i] = make_uint4(0, 0, 0, 0);
             if constexpr (sizeof(X) == 1) {
-#pragma unroll
-                for (int r = 0; r < M; r++)
-#pragma unroll
-                    for (int j = 0; j < CPW; j++) {
-                        const int c = (place + cw * j) * 512 + lane * 16;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            uint32_t q = 0;
-#pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                if (r < m && c + 4 * e + i < k) q |= (uint32_t)(uint8_t)x[r * ldx + c + 4 * e + i] << (8 * i);
-                            xq[r][j][e] = q;
-                        }
-                    }
-                if (threadIdx.x < m) scale[threadIdx.x] = sx[threadIdx.x];
+                __syncthreads();
+                for (int r = 0; r < A.m; r++) {
+                    const int n = ((uintptr_t)x & 15) == 0 && A.ldx % 16 == 0 ? k / 16 : 0;
+                    for (int i = threadIdx.x; i < n; i += GV_WARPS * 32)
+                        ((uint4 *)(xs + r * pitch))[i] = ((const uint4 *)(x + r * A.ldx))[i];
+                    for (int c = n * 16 + threadIdx.x; c < k; c += GV_WARPS * 32) xs[r * pitch + c] = x[r * A.ldx + c];
+                }
+                if (threadIdx.x < A.m) scale[threadIdx.x] = A.sx[threadIdx.x];
             } else {
-                const bool vec = ((uintptr_t)x & 15) == 0 && ldx * (int64_t)sizeof(X) % 16 == 0;
-                float f[16];
+                constexpr int V = 16 / sizeof(X);
+                struct alignas(16) Vec {
+                    X e[V];
+                };
+                struct alignas(V) Out {
+                    int8_t e[V];
+                };
+                const int n = ((uintptr_t)x & 15) == 0 && A.ldx % V == 0 ? k / V : 0;  // whole vectors
 #pragma unroll
                 for (int r = 0; r < M; r++) {
                     float top = 0.0f;
+                    if (r < A.m) {
+                        const X *xr = x + r * A.ldx;
+                        for (int i = threadIdx.x; i < n; i += GV_WARPS * 32) {
+                            const Vec v = ((const Vec *)xr)[i];
 #pragma unroll
-                    for (int j = 0; j < CPW; j++) {
-                        if (r >= m) break;
-                        load16(x + r * ldx, (place + cw * j) * 512 + lane * 16, k, vec, f);
-#pragma unroll
-                        for (int e = 0; e < 16; e++) top = max_nan(top, fabsf(f[e]));
+                            for (int e = 0; e < V; e++) top = max_nan(top, fabsf(to_f(v.e[e])));
+                        }
+                        for (int c = n * V + threadIdx.x; c < k; c += GV_WARPS * 32) top = max_nan(top, fabsf(to_f(xr[c])));
                     }
                     top = warp_max_nan(top);
                     if (lane == 0) red[r][warp] = top;
@@ -268,117 +273,144 @@ __global__ void __launch_bounds__(GV_WARPS * 32, 2)
                 __syncthreads();
 #pragma unroll
                 for (int r = 0; r < M; r++) {
-                    const float t = warp_max_nan(red[r][lane % nw]);
+                    if (r >= A.m) break;
+                    const X *xr = x + r * A.ldx;
+                    const float t = warp_max_nan(red[r][lane % GV_WARPS]);
                     const float s = isfinite(t) ? t / 127.0f : NAN, inv = 1.0f / s;
-                    const bool ok = s > 0.0f && isfinite(inv);
+                    const bool quick = s > 0.0f && isfinite(inv);
+                    for (int i = threadIdx.x; i < n; i += GV_WARPS * 32) {
+                        const Vec v = ((const Vec *)xr)[i];
+                        Out o;
+                        if (quick) {
+                            quantize_n(v.e, s, inv, o.e);
+                        } else {
 #pragma unroll
-                    for (int j = 0; j < CPW; j++) {
-                        alignas(4) int8_t q[16] = {};
-                        if (r < m) {
-                            load16(x + r * ldx, (place + cw * j) * 512 + lane * 16, k, vec, f);
-                            if (ok) {
-                                quantize_n(f, s, inv, q);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 16; e++) q[e] = slow_quantized(f[e], s);
-                            }
+                            for (int e = 0; e < V; e++) o.e[e] = slow_quantized(to_f(v.e[e]), s);
                         }
-#pragma unroll
-                        for (int e = 0; e < 4; e++) xq[r][j][e] = ((const uint32_t *)q)[e];
+                        ((Out *)(xs + r * pitch))[i] = o;
                     }
+                    for (int c = n * V + threadIdx.x; c < k; c += GV_WARPS * 32) xs[r * pitch + c] = slow_quantized(to_f(xr[c]), s);
                     if (threadIdx.x == 0) scale[r] = s;
                 }
             }
         }
         __syncthreads();
-        for (int c = group; c < nch; c += groups * U) {
+
+        int acc[M] = {};
+        for (int u = u0; u < u1; u++) {
+            const int slot = used % GV_SLOTS, piece = u % A.segs, ch = u / A.segs * A.rows;
+            if (!__all_sync(0xffffffffu, ok && tc::mb_wait(&full[warp][slot], (used / GV_SLOTS) & 1, &g_int8_error))) {
+                ok = false;
+                break;
+            }
+            const uint8_t *src = ring + slot * GV_SLOT;
+            const int rows = min(A.rows, nch - ch), size = min(A.seg, k - piece * A.seg);
+            const int8_t *xp = xs + piece * A.seg + lane * 16;
+            auto step = [&](int (&sum)[M], const uint8_t *row, const int4 (&y)[M]) {
+                const int4 v = *(const int4 *)(row + lane * 16);
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int ch = c + u * groups;
-                if (ch < nch) {
-                    int acc[M] = {};
+                for (int t = 0; t < M; t++) {
+                    sum[t] = __dp4a(v.x, y[t].x, sum[t]);
+                    sum[t] = __dp4a(v.y, y[t].y, sum[t]);
+                    sum[t] = __dp4a(v.z, y[t].z, sum[t]);
+                    sum[t] = __dp4a(v.w, y[t].w, sum[t]);
+                }
+            };
+            auto token = [&](int4 (&y)[M], int at) {
 #pragma unroll
-                    for (int j = 0; j < CPW; j++)
+                for (int t = 0; t < M; t++) y[t] = *(const int4 *)(xp + t * pitch + at);
+            };
+            auto flush = [&](int (&sum)[M], int c) {
 #pragma unroll
-                        for (int r = 0; r < M; r++) {
-                            acc[r] = __dp4a((int)buf[u][j].x, (int)xq[r][j][0], acc[r]);
-                            acc[r] = __dp4a((int)buf[u][j].y, (int)xq[r][j][1], acc[r]);
-                            acc[r] = __dp4a((int)buf[u][j].z, (int)xq[r][j][2], acc[r]);
-                            acc[r] = __dp4a((int)buf[u][j].w, (int)xq[r][j][3], acc[r]);
+                for (int t = 0; t < M; t++) {
+                    const int s = __reduce_add_sync(0xffffffffu, sum[t]);
+                    if (lane == 0) atomicAdd(&sums[c * M + t], s);
+                    sum[t] = 0;
+                }
+            };
+            int4 y[M];
+            if (A.rows == 1) {  // a piece of one row, in steps that do not wait for one another's loads
+                int at = 0;
+                for (; at + 2048 <= size; at += 2048)
+#pragma unroll
+                    for (int i = 0; i < 2048; i += 512) {
+                        token(y, at + i);
+                        step(acc, src + at + i, y);
+                    }
+                for (; at < size; at += 512)
+                    if (at + lane * 16 < size) {
+                        token(y, at);
+                        step(acc, src + at, y);
+                    }
+                __syncwarp();
+                if (piece == A.segs - 1 || u == u1 - 1) flush(acc, ch);  // all that this warp has of the channel
+            } else {  // four short rows at a time (those past `rows` come to nothing)
+                for (int r = 0; r < rows; r += 4) {
+                    int sum[4][M] = {};
+                    for (int at = 0; at < size; at += 512)
+                        if (at + lane * 16 < size) {
+                            token(y, at);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) step(sum[i], src + (r + i) * A.seg + at, y);
                         }
-                    fetch(buf[u]);
+                    __syncwarp();
 #pragma unroll
-                    for (int r = 0; r < M; r++) {
-                        const int t = __reduce_add_sync(0xffffffffu, acc[r]);
-                        if (lane == 0) atomicAdd(&sums[ch * M + r], t);
-                    }
+                    for (int i = 0; i < 4; i++)
+                        if (r + i < rows) flush(sum[i], ch + r + i);
                 }
             }
-        }
-        if (whole < nch && group == 0) {  // the end of the last row, byte by byte
-#pragma unroll
-            for (int j = 0; j < CPW; j++) {
-                if (rest[j] <= 0 || rest[j] >= 16) continue;
-                const int8_t *p = w + (n - 1) * ldw + (k - rest[j]);
-                for (int r = 0; r < m; r++) {
-                    int t = 0;
-#pragma unroll
-                    for (int i = 0; i < 15; i++) {
-                        int8_t q = 0;
-#pragma unroll
-                        for (int rr = 0; rr < M; rr++)
-                            if (rr == r) q = (int8_t)(xq[rr][j][i >> 2] >> (8 * (i & 3)));
-                        if (i < rest[j]) t += (int)p[i] * (int)q;
-                    }
-                    atomicAdd(&sums[whole * M + r], t);
-                }
-            }
+            __syncwarp();  // the slot has been read
+            used++;
+            if (lane == 0 && next < u1) issue();
+            issued = __shfl_sync(0xffffffffu, issued, 0);
+            next = __shfl_sync(0xffffffffu, next, 0);
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < nch * m; i += blockDim.x) {
+        for (int i = threadIdx.x; i < nch * A.m; i += GV_WARPS * 32) {
             const int c = i % nch, r = i / nch;
-            out[r * ldo + c0 + c] = from_f<T>(result(sums[c * M + r], scale[r], sw[c0 + c], bias, bias ? bias[c0 + c] : 0.0f));
+            out[r * A.ldo + c0 + c] =
+                from_f<T>(result(sums[c * M + r], scale[r], A.sw[c0 + c], A.bias, A.bias ? A.bias[c0 + c] : 0.0f));
         }
         __syncthreads();  // the sums have been read
     }
+    if (!ok && lane == 0)  // give up only once the copies in flight have landed
+        for (int i = used; i < issued; i++) tc::mb_wait(&full[warp][i % GV_SLOTS], (i / GV_SLOTS) & 1, &g_int8_error);
 }
 
-// Whether the kernel above takes m tokens of k values: their values of a warp's
-// chunks fit its registers.
-int vec_rows(int64_t m) { return m <= 2 ? (int)m : 4; }
-int vec_chunks(int64_t k) {
-    const int64_t c = (k + 512 * GV_WARPS - 1) / (512 * GV_WARPS);
-    return c <= 2 ? (int)c : c <= 4 ? 4 : 0;
-}
+// Whether the kernel above takes m tokens of k values: they fit its shared memory.
+// (Four tokens took 25 us, on the tensor cores 18.)
 bool takes_vec(const int8_t *w, int64_t ldw, int64_t m, int64_t k) {
-    return m >= 1 && m <= 4 && k > 0 && aligned_to(w, 16) && ldw % 16 == 0 && vec_chunks(k) &&
-           vec_rows(m) * vec_chunks(k) <= 4;
+    return m >= 1 && m <= 2 && k > 0 && aligned_to(w, 16) && ldw % 16 == 0 && m * ((k + 511) / 512 * 512) <= GV_X;
 }
 
-template <int M, int CPW, typename X, typename T>
-int launch_vec(const X *x, int64_t ldx, const float *sx, const int8_t *w, int64_t ldw, const float *sw, const float *bias,
-               T *out, int64_t ldo, int64_t m, int64_t n, int64_t k, cudaStream_t s) {
-    const int chunks = (int)((k + 511) / 512), cw = (chunks + CPW - 1) / CPW, groups = GV_WARPS / cw;
-    int64_t per = (n + 2 * num_sms() - 1) / (2 * num_sms());
+template <int M, typename X, typename T>
+int launch_vec(const X *x, T *out, VecArgs A, cudaStream_t s) {
+    auto f = int8_vec_kernel<M, X, T>;
+    static bool attr[64] = {false};
+    const int dev = current_device();
+    if (dev < 0 || dev >= 64 || !attr[dev]) {
+        ZC_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, GV_RING + GV_X));
+        if (dev >= 0 && dev < 64) attr[dev] = true;
+    }
+    A.seg = A.k >= GV_SLOT ? GV_SLOT : (A.k + 15) / 16 * 16;
+    A.segs = (A.k + A.seg - 1) / A.seg;
+    A.rows = A.segs > 1 ? 1 : GV_SLOT / A.seg < GV_ROWS ? GV_SLOT / A.seg : GV_ROWS;
+    int64_t per = (A.n + num_sms() - 1) / num_sms();
     if (per > GV_CHANNELS) per = GV_CHANNELS;
-    int64_t blocks = (n + per - 1) / per;
-    if (blocks > 2 * num_sms()) blocks = 2 * num_sms();
-    int8_vec_kernel<M, CPW, X, T><<<(unsigned)blocks, cw * groups * 32, 0, s>>>(x, ldx, sx, w, ldw, sw, bias, out, ldo, (int)m,
-                                                                               n, (int)k, (int)per, cw);
+    A.per = (int)per;
+    // fewer rows a unit while a block has fewer units than warps
+    while (A.rows > 1 && (per + A.rows - 1) / A.rows < GV_WARPS) A.rows--;
+    const int64_t blocks = (A.n + per - 1) / per;
+    const size_t smem = GV_RING + (size_t)M * ((A.k + 511) / 512 * 512);
+    f<<<(unsigned)(blocks < num_sms() ? blocks : num_sms()), GV_WARPS * 32, smem, s>>>(x, out, A);
     ZC_LAUNCHED("int8_vec_kernel");
     return ZPUCUDA_OK;
 }
 template <typename X, typename T>
 int product_vec(const X *x, int64_t ldx, const float *sx, const int8_t *w, int64_t ldw, const float *sw, const float *bias,
                 T *out, int64_t ldo, int64_t m, int64_t n, int64_t k, cudaStream_t s) {
-    switch (vec_rows(m) * 8 + vec_chunks(k)) {
-    case 8 + 1: return launch_vec<1, 1, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
-    case 8 + 2: return launch_vec<1, 2, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
-    case 8 + 4: return launch_vec<1, 4, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
-    case 16 + 1: return launch_vec<2, 1, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
-    case 16 + 2: return launch_vec<2, 2, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
-    default: return launch_vec<4, 1, X, T>(x, ldx, sx, w, ldw, sw, bias, out, ldo, m, n, k, s);
-    }
+    const VecArgs A = {w, sx, sw, bias, ldx, ldw, ldo, n, (int)m, (int)k};
+    return m == 1 ? launch_vec<1>(x, out, A, s) : launch_vec<2>(x, out, A, s);
 }
 
 // A product on the tensor cores: D[p, q] = sum over k of P[p, k] * Q[q, k] in
