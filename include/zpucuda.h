@@ -472,13 +472,17 @@ int zpucuda_debug_peer_reduce(const float *d_inbox, int world, int64_t n, float 
  *   y may be x (same pitch).
  * layer_norm_grad: dx, dgamma (sum over rows of dy * xhat) and dbeta (sum of
  *   dy), dgamma / dbeta of type wtype; a NULL output is not computed.  dx may
- *   be dy or x (same pitch). */
+ *   be dy or x (same pitch).  work: device memory of
+ *   zpucuda_layer_norm_grad_work(rows, cols) bytes, 16-byte aligned, that no
+ *   other work in flight uses (not needed without dgamma and dbeta). */
 int zpucuda_layer_norm(int dtype, const void *d_x, int64_t ldx, int wtype, const void *d_gamma, const void *d_beta,
                        void *d_y, int64_t ldy, float *d_mean, float *d_rstd, int64_t rows, int64_t cols, double eps,
                        void *stream);
 int zpucuda_layer_norm_grad(int dtype, const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx,
                             const float *d_mean, const float *d_rstd, int wtype, const void *d_gamma, void *d_dx,
-                            int64_t lddx, void *d_dgamma, void *d_dbeta, int64_t rows, int64_t cols, void *stream);
+                            int64_t lddx, void *d_dgamma, void *d_dbeta, int64_t rows, int64_t cols, void *d_work,
+                            int64_t work_bytes, void *stream);
+int64_t zpucuda_layer_norm_grad_work(int64_t rows, int64_t cols);
 /* Distillation from a teacher's `top` highest logits (at most 1024 a row):
  * teacher [rows, top] of type ttype at the vocabulary indices [rows, top] of
  * type itype (I32 or I64; -1: no entry).  With z = logits / temperature, q =

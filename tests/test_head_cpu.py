@@ -23,9 +23,9 @@ def call(L, name, order, good, **bad):
 
 NORM = "dt x ldx wt gamma beta y ldy mean rstd rows cols eps stream"
 NORM_OK = dict(dt=F32, x=A, ldx=8, wt=F32, gamma=A, beta=A, y=A, ldy=8, mean=A, rstd=A, rows=0, cols=8, eps=1e-5, stream=1)
-NORM_GRAD = "dt dy lddy x ldx mean rstd wt gamma dx lddx dgamma dbeta rows cols stream"
+NORM_GRAD = "dt dy lddy x ldx mean rstd wt gamma dx lddx dgamma dbeta rows cols work nwork stream"
 NORM_GRAD_OK = dict(dt=F32, dy=A, lddy=8, x=A, ldx=8, mean=A, rstd=A, wt=F32, gamma=A, dx=A, lddx=8, dgamma=None,
-                    dbeta=None, rows=0, cols=8, stream=1)
+                    dbeta=None, rows=0, cols=8, work=None, nwork=0, stream=1)
 TEACH = "dt x ld tt teacher ldt it index ldi weight T "
 TEACH_OK = dict(dt=F32, x=A, ld=8, tt=F32, teacher=A, ldt=4, it=I64, index=A, ldi=4, weight=None, T=2.0, loss=A, lse=A,
                 dloss=None, d=A, ldd=8, rows=0, vocab=8, top=4, stream=1)
@@ -54,7 +54,9 @@ CASES = [
     ("zpucuda_layer_norm_grad", NORM_GRAD, NORM_GRAD_OK, [
         (dict(dt=F64), NOT_SUPPORTED, "dy: the type"), (dict(lddy=7), OUT_OF_SHAPE, "dy"),
         (dict(lddx=0), OUT_OF_SHAPE, "dx"), (dict(rows=1, mean=None), INVALID, "mean"),
-        (dict(rows=1, rstd=None), INVALID, "rstd"), (dict(rows=1, x=None), INVALID, "x: null")]),
+        (dict(rows=1, rstd=None), INVALID, "rstd"), (dict(rows=1, x=None), INVALID, "x: null"),
+        (dict(rows=1, dgamma=A), INVALID, "work"), (dict(rows=1, dgamma=A, work=A, nwork=63), INVALID, "work"),
+        (dict(rows=1, dbeta=A, work=A + 4, nwork=1 << 20), INVALID, "work")]),
     ("zpucuda_distill_loss", LOSS, TEACH_OK, [
         (dict(T=0.0), INVALID, "temperature"), (dict(T=float("inf")), INVALID, "temperature"),
         (dict(T=float("nan")), INVALID, "temperature"), (dict(T=-1.0), INVALID, "temperature"),

@@ -158,7 +158,8 @@ SIGNATURES = {
     "zpucuda_mlp_trace": (I32, [P, I32]),
     "zpucuda_mlp_trace_read": (I32, [P, P, I32]),
     "zpucuda_layer_norm": (I32, [I32, P, I64, I32, P, P, P, I64, P, P, I64, I64, C.c_double, P]),
-    "zpucuda_layer_norm_grad": (I32, [I32, P, I64, P, I64, P, P, I32, P, P, I64, P, P, I64, I64, P]),
+    "zpucuda_layer_norm_grad": (I32, [I32, P, I64, P, I64, P, P, I32, P, P, I64, P, P, I64, I64, P, I64, P]),
+    "zpucuda_layer_norm_grad_work": (I64, [I64, I64]),
     "zpucuda_distill_loss": (I32, [I32, P, I64, I32, P, I64, I32, P, I64, P, C.c_double, P, P, I64, I64, I64, P]),
     "zpucuda_distill_grad": (I32, [I32, P, I64, I32, P, I64, I32, P, I64, P, C.c_double, P, P, P, I64, I64, I64, I64,
                                    P]),

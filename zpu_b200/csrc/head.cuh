@@ -8,6 +8,8 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace zc {
@@ -55,6 +57,133 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
+}
+
+// ---- rows in pieces of 16 bytes
+// Piece i of a row holds its elements i * N .. i * N + N - 1 (N = 16 / the
+// element's size), wherever the row starts: an address that is no multiple of
+// 16 costs a second load and some shifts, not another order of a sum, so a
+// result does not depend on the alignment.  Nothing outside the row is touched.
+
+template <typename T>
+constexpr int kPiece = 16 / (int)sizeof(T);
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4 &q, float (&f)[kPiece<T>]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                f[2 * i] = __uint_as_float(w[i] << 16);
+                f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            } else {
+                const __half2 h = *(const __half2 *)&w[i];
+                f[2 * i] = __low2float(h);
+                f[2 * i + 1] = __high2float(h);
+            }
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float (&f)[kPiece<T>]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            w[i] = __float_as_uint(f[i]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *(const uint32_t *)&h;
+        } else {
+            const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *(const uint32_t *)&h;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Bytes s .. s + 15 of the 32 bytes lo, hi (0 <= s < 16).
+__device__ __forceinline__ uint4 bytes_from(const uint4 &lo, const uint4 &hi, uint32_t s) {
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int i = 0; i < 6; i++) w[i] = (s & 8) ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; i++) w[i] = (s & 4) ? w[i + 1] : w[i];
+    const uint32_t b = (s & 3) * 8;
+    return make_uint4(__funnelshift_r(w[0], w[1], b), __funnelshift_r(w[1], w[2], b), __funnelshift_r(w[2], w[3], b),
+                      __funnelshift_r(w[3], w[4], b));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t raw_bits(T x) {
+    if constexpr (sizeof(T) == 4) return *(const uint32_t *)&x;
+    else return *(const uint16_t *)&x;
+}
+
+// Piece i of the row (its elements past n are 0).
+template <typename T>
+__device__ __forceinline__ uint4 load_piece(const T *row, int64_t i, int64_t n) {
+    constexpr int N = kPiece<T>;
+    const T *p = row + i * N;
+    const uint32_t s = (uint32_t)(uintptr_t)p & 15;
+    if ((i + 1) * N <= n) {
+        if (s == 0) return *(const uint4 *)p;
+        const uint4 *q = (const uint4 *)((uintptr_t)p & ~(uintptr_t)15);
+        if (i > 0 && (const T *)(q + 2) <= row + n) return bytes_from(q[0], q[1], s);
+    }
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (i * N + e < n) w[e * (int)sizeof(T) / 4] |= raw_bits(p[e]) << (e * (int)sizeof(T) % 4 * 8);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_elements(T *p, const uint4 &q, int from, int to) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < kPiece<T>; e++)
+        if (e >= from && e < to) {
+            if constexpr (sizeof(T) == 4) ((uint32_t *)p)[e] = w[e];
+            else ((uint16_t *)p)[e] = (uint16_t)(w[e / 2] >> (e % 2 * 16));
+        }
+}
+
+// Stores piece i of the row (its elements below n), for a whole warp at a time:
+// lane l has piece i0 + l, and those past the row's end store nothing.  Where the
+// row starts off a 16-byte boundary, each lane stores the 16 aligned bytes that
+// hold its neighbour's end and its own beginning.
+template <typename T>
+__device__ __forceinline__ void store_piece(T *row, int64_t i, int64_t n, const uint4 &v) {
+    constexpr int N = kPiece<T>;
+    T *p = row + i * N;
+    const uint32_t s = (uint32_t)(uintptr_t)p & 15;
+    const int64_t rest = n - i * N;
+    const int have = rest >= N ? N : rest > 0 ? (int)rest : 0;  // elements of this piece
+    if (s == 0) {
+        if (have == N) *(uint4 *)p = v;
+        else store_elements(p, v, 0, have);
+        return;
+    }
+    uint4 before;
+    before.x = __shfl_up_sync(0xffffffffu, v.x, 1);
+    before.y = __shfl_up_sync(0xffffffffu, v.y, 1);
+    before.z = __shfl_up_sync(0xffffffffu, v.z, 1);
+    before.w = __shfl_up_sync(0xffffffffu, v.w, 1);
+    const int lane = threadIdx.x & 31;
+    const int head = (int)(16 - s) / (int)sizeof(T);  // elements up to the boundary
+    if (lane > 0 && have >= head) {
+        *(uint4 *)((uintptr_t)p & ~(uintptr_t)15) = bytes_from(before, v, 16 - s);
+    } else {
+        // the neighbour's end, unless it is another warp's, and what there is of the beginning
+        if (lane > 0 && rest + N > head) store_elements(p - N, before, head, rest + N < N ? (int)rest + N : N);
+        store_elements(p, v, 0, have < head ? have : head);
+    }
+    if (lane == 31) store_elements(p, v, head, have);
 }
 
 // Calls F<type> for one of the head's element types.

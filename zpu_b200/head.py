@@ -138,8 +138,10 @@ def layer_norm_grad(dy, x, mean, rstd, gamma=None, out=None, stream=None):
         dx, lddx = _output("out", out, x)
         dgamma = torch.empty(cols, dtype=gamma.dtype if gamma is not None else torch.float32, device=x.device)
         dbeta = torch.empty_like(dgamma)
+        work = torch.empty(lib().zpucuda_layer_norm_grad_work(rows, cols), dtype=torch.uint8, device=x.device)
     check(lib().zpucuda_layer_norm_grad(code, dy.data_ptr(), lddy, x.data_ptr(), ldx, m, r, wt, g, dx.data_ptr(), lddx,
-                                        dgamma.data_ptr(), dbeta.data_ptr(), rows, cols, _stream(stream)))
+                                        dgamma.data_ptr(), dbeta.data_ptr(), rows, cols, work.data_ptr(), work.numel(),
+                                        _stream(stream)))
     return dx, dgamma, dbeta
 
 
