@@ -186,6 +186,61 @@ __device__ __forceinline__ void store_piece(T *row, int64_t i, int64_t n, const 
     if (lane == 31) store_elements(p, v, head, have);
 }
 
+// A ring of D rows' pieces in shared memory, filled by asynchronous copies: a warp
+// has its lanes' pieces t + j * TPR (j < NV) of ROWS rows (tensors) a slot, and no
+// other warp reads them.  Bytes in flight cost no registers this way.
+template <typename T, int TPR, int NV, int ROWS, int D>
+struct RowRing {
+    static constexpr int kWarp = D * ROWS * NV * 33;  // uint4 a warp: 32 lanes' 16 bytes, and the next 16
+    uint4 *base;
+    int lane, t;
+
+    __device__ __forceinline__ RowRing(uint4 *smem, int t_)
+        : base(smem + (threadIdx.x >> 5) * kWarp), lane(threadIdx.x & 31), t(t_) {}
+    __device__ __forceinline__ uint4 *at(int slot, int r, int j) const { return base + ((slot * ROWS + r) * NV + j) * 33; }
+
+    static __device__ __forceinline__ void copy(uint4 *dst, const uint8_t *src, int size) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)),
+                     "l"(src), "r"(size)
+                     : "memory");
+    }
+    // The aligned 16 bytes that hold the row's pieces, clipped at its end.  Before its
+    // beginning lie the bytes of the row before it, except (`first`) at the matrix's.
+    __device__ __forceinline__ void issue(int slot, int r, const T *row, int64_t n, bool first) const {
+        const uint32_t s = (uint32_t)(uintptr_t)row & 15;
+        const uint8_t *from = (const uint8_t *)row - s;
+        const int64_t end = s + n * (int64_t)sizeof(T);
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int64_t b = (int64_t)(t + j * TPR) * 16;
+            if (b >= end) continue;
+            uint4 *dst = at(slot, r, j);
+            if (first && s && b == 0) {
+                T *e = (T *)(dst + lane);
+                for (int i = (int)(s / sizeof(T)); i < kPiece<T> && i * (int)sizeof(T) < end; i++) e[i] = row[i - (int)(s / sizeof(T))];
+            } else {
+                copy(dst + lane, from + b, end - b < 16 ? (int)(end - b) : 16);
+            }
+            if (s && lane == 31 && b + 16 < end) copy(dst + 32, from + b + 16, end - b < 32 ? (int)(end - b) - 16 : 16);
+        }
+    }
+    static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    // Until all but the last D - 1 groups have landed, for the whole warp.
+    static __device__ __forceinline__ void wait() {
+        asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+        __syncwarp();
+    }
+    // Piece t + j * TPR, 0 past the row's end.
+    __device__ __forceinline__ uint4 read(int slot, int r, int j, const T *row, int64_t n) const {
+        const uint32_t s = (uint32_t)(uintptr_t)row & 15;
+        const int64_t b = (int64_t)(t + j * TPR) * 16, end = s + n * (int64_t)sizeof(T);
+        const uint4 *src = at(slot, r, j) + lane, none = make_uint4(0, 0, 0, 0);
+        const uint4 lo = b < end ? src[0] : none;
+        if (s == 0) return lo;
+        return bytes_from(lo, b + 16 < end ? src[1] : none, s);
+    }
+};
+
 // Calls F<type> for one of the head's element types.
 #define ZC_HEAD_TYPE(dt, T, ...)                                   \
     do {                                                           \

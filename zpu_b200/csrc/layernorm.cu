@@ -17,7 +17,8 @@ namespace {
 
 constexpr int NT = 256;
 constexpr int kPerThread = 16;  // columns that a thread of the one-pass gradient holds
-constexpr int kMaxParts = 2;    // blocks an SM of the gradient
+constexpr int kMaxCluster = 8;  // blocks of a cluster of it
+constexpr int64_t kMaxOnePass = 512 * kPerThread * kMaxCluster;
 
 // The weights of piece i of a row (N from column i * N on, `have` of them), as
 // f32; `dflt` without any.
@@ -80,36 +81,20 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2 *sm, int bar
 
 // ------------------------------------------------------------------ forward
 
-// TPR threads a row, NV pieces a thread.  NV = 0: rows too long for registers,
-// read three times (from L2 after the first).
-template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR < NT ? NT : TPR)
-    ln_kernel(const T *x, int64_t ldx, int wt, const void *gamma, const void *beta, T *y, int64_t ldy, float *mean,
-              float *rstd, int64_t rows, int64_t cols, float eps) {
-    constexpr int BLOCK = TPR < NT ? NT : TPR, N = kPiece<T>;
-    __shared__ float2 sm[2][BLOCK / 32];
-    const int64_t row = (int64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
-    if (row >= rows) return;  // a whole warp; with TPR > 32 a block has one row
-    const int t = threadIdx.x % TPR;
-    const T *xr = x + row * ldx;
-    T *yr = y + row * ldy;
-    const int64_t n = (cols + N - 1) / N;
-    const float inv = 1.0f / (float)cols;
-    uint4 v[NV ? NV : 1];
-    if constexpr (NV > 0) {
-#pragma unroll
-        for (int j = 0; j < NV; j++)
-            v[j] = t + j * TPR < n ? load_piece(xr, t + j * TPR, cols) : make_uint4(0, 0, 0, 0);
-    }
-    // a thread's part of the three passes, over its pieces
+// A thread's part of the forward pass over its pieces of a row.
+template <typename T>
+struct Row {
+    static constexpr int N = kPiece<T>;
+    int64_t cols;
     float s = 0.0f, d1 = 0.0f, d2 = 0.0f, mu, rest, rs;
-    auto sum = [&](const uint4 &in) {  // what is past the row's end is 0
+
+    __device__ __forceinline__ void sum(const uint4 &in) {  // what is past the row's end is 0
         float a[N];
         unpack<T>(in, a);
 #pragma unroll
         for (int e = 0; e < N; e++) s += a[e];
-    };
-    auto spread = [&](const uint4 &in, int64_t i) {
+    }
+    __device__ __forceinline__ void spread(const uint4 &in, int64_t i) {
         float a[N];
         unpack<T>(in, a);
         const int have = in_row<N>(i, cols);
@@ -119,9 +104,17 @@ __global__ void __launch_bounds__(TPR < NT ? NT : TPR)
             d1 += d;
             d2 += d * d;
         }
-    };
-    auto put = [&](const uint4 &in, int64_t i) {  // a whole warp's pieces
-        float a[N], g[N], b[N];
+    }
+    // The mean of what the rounded mean leaves is taken off again: rows far
+    // from zero keep the digits that a 32-bit mean alone would cost them.
+    __device__ __forceinline__ void finish(float2 q, float inv, float eps) {
+        rest = q.x * inv;
+        float var = q.y * inv - rest * rest;
+        var = var < 0.0f ? 0.0f : var;  // NaN stays
+        rs = 1.0f / sqrtf(var + eps);
+    }
+    __device__ __forceinline__ void put(const uint4 &in, int64_t i, T *y, int wt, const void *gamma, const void *beta) {
+        float a[N], g[N], b[N];  // a whole warp's pieces
         unpack<T>(in, a);
         const int have = in_row<N>(i, cols);
         load_w<N>(gamma, wt, i, have, 1.0f, g);
@@ -129,180 +122,254 @@ __global__ void __launch_bounds__(TPR < NT ? NT : TPR)
 #pragma unroll
         for (int e = 0; e < N; e++) a[e] = ((a[e] - mu) - rest) * rs * g[e] + b[e];
         __syncwarp();
-        store_piece(yr, i, cols, pack<T>(a));
-    };
-    if constexpr (NV > 0) {
+        store_piece(y, i, cols, pack<T>(a));
+    }
+};
+
+// TPR threads a row, NV pieces a thread; a block walks rows, D of them on their
+// way to shared memory while one is worked on.
+template <typename T, int TPR, int NV, int D>
+__global__ void __launch_bounds__(TPR < NT ? NT : TPR)
+    ln_kernel(const T *x, int64_t ldx, int wt, const void *gamma, const void *beta, T *y, int64_t ldy, float *mean,
+              float *rstd, int64_t rows, int64_t cols, float eps) {
+    constexpr int BLOCK = TPR < NT ? NT : TPR, GROUPS = BLOCK / TPR;
+    extern __shared__ uint4 ring_smem[];
+    __shared__ float2 sm[2][2][BLOCK / 32];
+    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    const RowRing<T, TPR, NV, 1, D> ring(ring_smem, t);
+    const int64_t step = (int64_t)gridDim.x * GROUPS;
+    int64_t row = (int64_t)blockIdx.x * GROUPS + group;
+    const float inv = 1.0f / (float)cols;
 #pragma unroll
-        for (int j = 0; j < NV; j++) sum(v[j]);
-    } else {
-        for (int64_t i = t; i < n; i += TPR) sum(load_piece(xr, i, cols));
+    for (int d = 0; d < D; d++) {
+        if (row + d * step < rows) ring.issue(d, 0, x + (row + d * step) * ldx, cols, row + d * step == 0);
+        ring.commit();
     }
-    mu = row_sum2<TPR>(s, 0.0f, sm[0], 0).x * inv;
-    // The mean of what the rounded mean leaves is taken off again: rows far
-    // from zero keep the digits that a 32-bit mean alone would cost them.
-    if constexpr (NV > 0) {
+    int slot = 0;
+    for (int odd = 0; row < rows; row += step, odd ^= 1) {
+        ring.wait();
+        uint4 v[NV];
 #pragma unroll
-        for (int j = 0; j < NV; j++) spread(v[j], t + j * TPR);
-    } else {
-        for (int64_t i = t; i < n; i += TPR) spread(load_piece(xr, i, cols), i);
-    }
-    const float2 q = row_sum2<TPR>(d1, d2, sm[1], 0);
-    rest = q.x * inv;
-    float var = q.y * inv - rest * rest;
-    var = var < 0.0f ? 0.0f : var;  // NaN stays
-    rs = 1.0f / sqrtf(var + eps);
-    if constexpr (NV > 0) {
+        for (int j = 0; j < NV; j++) v[j] = ring.read(slot, 0, j, x + row * ldx, cols);
+        __syncwarp();
+        if (row + D * step < rows) ring.issue(slot, 0, x + (row + D * step) * ldx, cols, false);
+        ring.commit();
+        slot = slot + 1 == D ? 0 : slot + 1;
+        Row<T> R = {cols};
 #pragma unroll
-        for (int j = 0; j < NV; j++) put(v[j], t + j * TPR);
-    } else {
-        for (int64_t i = t; i - (t & 31) < n; i += TPR) put(i < n ? load_piece(xr, i, cols) : make_uint4(0, 0, 0, 0), i);
+        for (int j = 0; j < NV; j++) R.sum(v[j]);
+        R.mu = row_sum2<TPR>(R.s, 0.0f, sm[odd][0], 0).x * inv;
+#pragma unroll
+        for (int j = 0; j < NV; j++) R.spread(v[j], t + j * TPR);
+        R.finish(row_sum2<TPR>(R.d1, R.d2, sm[odd][1], 0), inv, eps);
+#pragma unroll
+        for (int j = 0; j < NV; j++) R.put(v[j], t + j * TPR, y + row * ldy, wt, gamma, beta);
+        if (t == 0) {
+            if (mean) mean[row] = R.mu + R.rest;
+            if (rstd) rstd[row] = R.rs;
+        }
     }
-    if (t == 0) {
-        if (mean) mean[row] = mu + rest;
-        if (rstd) rstd[row] = rs;
+}
+
+// Rows too long for the above: read three times, from L2 after the first.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+    ln_long_kernel(const T *x, int64_t ldx, int wt, const void *gamma, const void *beta, T *y, int64_t ldy, float *mean,
+                   float *rstd, int64_t cols, float eps) {
+    __shared__ float2 sm[2][32];
+    const int64_t row = blockIdx.x, n = (cols + kPiece<T> - 1) / kPiece<T>;
+    const T *xr = x + row * ldx;
+    const float inv = 1.0f / (float)cols;
+    Row<T> R = {cols};
+    for (int64_t i = threadIdx.x; i < n; i += 1024) R.sum(load_piece(xr, i, cols));
+    R.mu = row_sum2<1024>(R.s, 0.0f, sm[0], 0).x * inv;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) R.spread(load_piece(xr, i, cols), i);
+    R.finish(row_sum2<1024>(R.d1, R.d2, sm[1], 0), inv, eps);
+    for (int64_t i = threadIdx.x; i - (threadIdx.x & 31) < n; i += 1024)
+        R.put(i < n ? load_piece(xr, i, cols) : make_uint4(0, 0, 0, 0), i, y + row * ldy, wt, gamma, beta);
+    if (threadIdx.x == 0) {
+        if (mean) mean[row] = R.mu + R.rest;
+        if (rstd) rstd[row] = R.rs;
     }
+}
+
+// Blocks of f that an SM holds at once (looked up once a device), after allowing it `smem`.
+template <typename F>
+int blocks_per_sm(F f, int block, size_t smem, int *cache) {
+    const int dev = current_device();
+    if (dev >= 0 && dev < 64 && cache[dev]) return cache[dev];
+    int n = 0;
+    if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, f, block, smem) != cudaSuccess || n < 1)
+        return 0;
+    if (dev >= 0 && dev < 64) cache[dev] = n;
+    return n;
+}
+
+template <typename T, int TPR, int NV, int D>
+int launch_ln_ring(const T *x, int64_t ldx, int wt, const void *gamma, const void *beta, T *y, int64_t ldy, float *mean,
+                   float *rstd, int64_t rows, int64_t cols, float eps, cudaStream_t s) {
+    constexpr int BLOCK = TPR < NT ? NT : TPR, GROUPS = BLOCK / TPR;
+    auto f = ln_kernel<T, TPR, NV, D>;
+    const size_t smem = (size_t)(BLOCK / 32) * RowRing<T, TPR, NV, 1, D>::kWarp * 16;
+    static int cache[64] = {0};
+    const int per = blocks_per_sm(f, BLOCK, smem, cache);
+    if (!per) return cuda_fail(cudaGetLastError(), "layer_norm: occupancy");
+    const int64_t want = (rows + GROUPS - 1) / GROUPS, most = (int64_t)per * num_sms();
+    f<<<(unsigned)(want < most ? want : most), BLOCK, smem, s>>>(x, ldx, wt, gamma, beta, y, ldy, mean, rstd, rows, cols, eps);
+    ZC_LAUNCHED("ln_kernel");
+    return ZPUCUDA_OK;
 }
 
 template <typename T>
 int launch_ln(const T *x, int64_t ldx, int wt, const void *gamma, const void *beta, T *y, int64_t ldy, float *mean,
               float *rstd, int64_t rows, int64_t cols, float eps, cudaStream_t s) {
     const int64_t n = (cols + kPiece<T> - 1) / kPiece<T>;
-    const unsigned few = (unsigned)((rows + NT / 32 - 1) / (NT / 32)), all = (unsigned)rows;
-#define LN(TPR, NV)                                                                                         \
-    ln_kernel<T, TPR, NV><<<TPR == 32 ? few : all, TPR < NT ? NT : TPR, 0, s>>>(x, ldx, wt, gamma, beta, y, \
-                                                                               ldy, mean, rstd, rows, cols, eps)
+#define LN(TPR, NV, D) return launch_ln_ring<T, TPR, NV, D>(x, ldx, wt, gamma, beta, y, ldy, mean, rstd, rows, cols, eps, s)
     // a warp holds 128 pieces, 256 threads 1024, 1024 threads 4096
-    if (n <= 32) LN(32, 1);
-    else if (n <= 64) LN(32, 2);
-    else if (n <= 128) LN(32, 4);
-    else if (n <= 256) LN(256, 1);
-    else if (n <= 512) LN(256, 2);
-    else if (n <= 1024) LN(256, 4);
-    else if (n <= 2048) LN(1024, 2);
-    else if (n <= 4096) LN(1024, 4);
-    else LN(1024, 0);
+    if (n <= 32) LN(32, 1, 4);
+    if (n <= 64) LN(32, 2, 4);
+    if (n <= 128) LN(32, 4, 3);
+    if (n <= 256) LN(256, 1, 4);
+    if (n <= 512) LN(256, 2, 4);
+    if (n <= 1024) LN(256, 4, 3);
+    if (n <= 2048) LN(1024, 2, 3);
+    if (n <= 4096) LN(1024, 4, 2);
 #undef LN
-    ZC_LAUNCHED("ln_kernel");
+    ln_long_kernel<T><<<(unsigned)rows, 1024, 0, s>>>(x, ldx, wt, gamma, beta, y, ldy, mean, rstd, cols, eps);
+    ZC_LAUNCHED("ln_long_kernel");
     return ZPUCUDA_OK;
 }
 
 // ----------------------------------------------------------------- backward
 
 // One pass: TPR threads a row, BLOCK / TPR rows of a block at a time, NV pieces a
-// thread.  The next row's loads are in flight while this one is reduced and
-// written.  parts: [gridDim.x][2][cols] sums, or null.  1024 threads (64
-// registers each) keep the sums in shared memory, every thread its own.
-template <typename T, int TPR, int NV, int BLOCK>
+// thread; D rows are on their way to shared memory while one is worked on.  A row
+// that a block does not hold is split over a cluster (CLUSTER), whose blocks tell
+// one another their parts of its two sums.  parts: a row of [2][cols] sums for
+// each block (cluster), or null.
+template <typename T, int TPR, int NV, int BLOCK, int D, bool CLUSTER>
 __global__ void __launch_bounds__(BLOCK)
     ln_grad_kernel(const T *dy, int64_t lddy, const T *x, int64_t ldx, const float *mean, const float *rstd, int wt,
                    const void *gamma, T *dx, int64_t lddx, float *parts, int64_t rows, int64_t cols) {
-    constexpr int GROUPS = BLOCK / TPR, N = kPiece<T>;
-    constexpr bool SHARED = BLOCK == 1024;
-    __shared__ float2 sm[2][BLOCK / 32];
-    extern __shared__ __align__(16) float comb[];  // [2][pitch], to add up the groups, or SHARED
-    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, bar = 1 + (TPR > 32 ? group : 0);
-    const int64_t n = (cols + N - 1) / N, pitch = n * N;
-    const float inv = 1.0f / (float)cols;
-    constexpr int K = SHARED ? 1 : NV;
-    float gs[K][N], ag[K][N] = {}, ab[K][N] = {};
-    auto weights = [&](int j, float (&w)[N]) { load_w<N>(gamma, wt, t + j * TPR, in_row<N>(t + j * TPR, cols), 1.0f, w); };
-    if constexpr (SHARED) {
-        for (int64_t c = threadIdx.x; c < 2 * pitch; c += BLOCK) comb[c] = 0.0f;
-        __syncthreads();
-    } else {
-#pragma unroll
-        for (int j = 0; j < NV; j++) weights(j, gs[j]);
+    constexpr int GROUPS = BLOCK / TPR, N = kPiece<T>, PITCH = TPR * NV * N;
+    __shared__ float2 sm[2][BLOCK / 32], peers[2][kMaxCluster];
+    extern __shared__ uint4 grad_smem[];
+    uint32_t rank = 0, size = 1;
+    if constexpr (CLUSTER) {
+        asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
     }
-    uint4 vx[NV], vd[NV], px[NV], pd[NV];
-    float mu = 0.0f, rs = 0.0f, pmu = 0.0f, prs = 0.0f;
-    auto load = [&](int64_t row) {
-        if (row >= rows) return;
-        pmu = mean[row];
-        prs = rstd[row];
+    const int group = threadIdx.x / TPR, bar = 1 + (TPR > 32 ? group : 0);
+    const int t = threadIdx.x % TPR, p0 = t + (int)rank * TPR * NV;  // in the block's part of a row, in the row
+    const int64_t n = (cols + N - 1) / N;
+    const float inv = 1.0f / (float)cols;
+    float g[NV][N], ag[NV][N] = {}, ab[NV][N] = {};
 #pragma unroll
-        for (int j = 0; j < NV; j++)
-            if (t + j * TPR < n) {
-                px[j] = load_piece(x + row * ldx, t + j * TPR, cols);
-                pd[j] = load_piece(dy + row * lddy, t + j * TPR, cols);
-            }
+    for (int j = 0; j < NV; j++) load_w<N>(gamma, wt, p0 + j * TPR, in_row<N>(p0 + j * TPR, cols), 1.0f, g[j]);
+    const RowRing<T, TPR, NV, 2, D> ring(grad_smem, p0);
+    const int64_t step = (int64_t)(gridDim.x / size) * GROUPS;
+    int64_t row = (int64_t)(blockIdx.x / size) * GROUPS + group;
+    auto issue = [&](int slot, int64_t r) {
+        if (r < rows) {
+            ring.issue(slot, 0, x + r * ldx, cols, r == 0);
+            ring.issue(slot, 1, dy + r * lddy, cols, r == 0);
+        }
+        ring.commit();
     };
-    const int64_t step = (int64_t)gridDim.x * GROUPS;
-    int64_t row = (int64_t)blockIdx.x * GROUPS + group;
-    load(row);
+#pragma unroll
+    for (int d = 0; d < D; d++) issue(d, row + d * step);
+    int slot = 0;
     for (int odd = 0; row < rows; row += step, odd ^= 1) {
-        mu = pmu;
-        rs = prs;
+        const float mu = mean[row], rs = rstd[row];
+        ring.wait();
+        uint4 vx[NV], vd[NV];
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            vx[j] = px[j];
-            vd[j] = pd[j];
+            vx[j] = ring.read(slot, 0, j, x + row * ldx, cols);
+            vd[j] = ring.read(slot, 1, j, dy + row * lddy, cols);
         }
-        load(row + step);
+        __syncwarp();
+        issue(slot, row + D * step);
+        slot = slot + 1 == D ? 0 : slot + 1;
         float a = 0.0f, b = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; j++) {  // past the row's end dy is 0, and all that follows from it
-            if (t + j * TPR >= n) continue;
-            float fx[N], fd[N], w[N];
+            if (p0 + j * TPR >= n) continue;
+            float fx[N], fd[N];
             unpack<T>(vx[j], fx);
             unpack<T>(vd[j], fd);
-            if constexpr (SHARED) weights(j, w);
-            float *sg = comb + (t + j * TPR) * N, *sb = sg + pitch;
 #pragma unroll
             for (int e = 0; e < N; e++) {
-                const float xh = (fx[e] - mu) * rs, d = fd[e];
-                const float gd = d * (SHARED ? w[e] : gs[SHARED ? 0 : j][e]);
+                const float xh = (fx[e] - mu) * rs, d = fd[e], gd = d * g[j][e];
                 a += gd;
                 b += gd * xh;
-                if constexpr (SHARED) {
-                    sg[e] += d * xh;
-                    sb[e] += d;
-                } else {
-                    ag[j][e] += d * xh;
-                    ab[j][e] += d;
-                }
+                ag[j][e] += d * xh;
+                ab[j][e] += d;
             }
         }
         if (!dx) continue;
         // two buffers: a thread that is a row ahead does not overwrite what another still reads
-        const float2 q = row_sum2<TPR>(a, b, sm[odd] + group * (TPR / 32), bar);
+        float2 q = row_sum2<TPR>(a, b, sm[odd] + group * (TPR / 32), bar);
+        if constexpr (CLUSTER) {
+            if (threadIdx.x < size) {
+                uint32_t there;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                             : "=r"(there)
+                             : "r"((uint32_t)__cvta_generic_to_shared(&peers[odd][rank])), "r"(threadIdx.x));
+                asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(q.x), "f"(q.y) : "memory");
+            }
+            __syncwarp();
+            asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            q = make_float2(0.0f, 0.0f);
+            for (uint32_t r = 0; r < size; r++) {
+                q.x += peers[odd][r].x;
+                q.y += peers[odd][r].y;
+            }
+        }
         const float ma = q.x * inv, mb = q.y * inv;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            float fx[N], fd[N], w[N];
+            float fx[N], fd[N];
             unpack<T>(vx[j], fx);
             unpack<T>(vd[j], fd);
-            if constexpr (SHARED) weights(j, w);
 #pragma unroll
             for (int e = 0; e < N; e++) {
                 const float xh = (fx[e] - mu) * rs;
-                fx[e] = rs * (fd[e] * (SHARED ? w[e] : gs[SHARED ? 0 : j][e]) - ma - xh * mb);
+                fx[e] = rs * (fd[e] * g[j][e] - ma - xh * mb);
             }
             __syncwarp();
-            store_piece(dx + row * lddx, t + j * TPR, cols, pack<T>(fx));
+            store_piece(dx + row * lddx, p0 + j * TPR, cols, pack<T>(fx));
         }
+    }
+    // no block ends while another may still write to its shared memory
+    if constexpr (CLUSTER) {
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     if (!parts) return;
-    float *out = parts + (int64_t)blockIdx.x * 2 * cols;
-    if constexpr (!SHARED) {  // the groups add up in their order
-        for (int k = 0; k < GROUPS; k++) {
-            __syncthreads();
-            if (group == k)
+    // the groups add up in their order, in the ring's place
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    float *comb = (float *)grad_smem;  // [2][PITCH]
+    for (int k = 0; k < GROUPS; k++) {
+        __syncthreads();
+        if (group == k)
 #pragma unroll
-                for (int j = 0; j < NV; j++) {
-                    if (t + j * TPR >= n) continue;
-                    float *sg = comb + (t + j * TPR) * N, *sb = sg + pitch;
+            for (int j = 0; j < NV; j++) {
+                float *sg = comb + (t + j * TPR) * N, *sb = sg + PITCH;
 #pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        sg[e] = k ? sg[e] + ag[j][e] : ag[j][e];
-                        sb[e] = k ? sb[e] + ab[j][e] : ab[j][e];
-                    }
+                for (int e = 0; e < N; e++) {
+                    sg[e] = k ? sg[e] + ag[j][e] : ag[j][e];
+                    sb[e] = k ? sb[e] + ab[j][e] : ab[j][e];
                 }
-        }
+            }
     }
     __syncthreads();
-    for (int64_t c = threadIdx.x; c < cols; c += BLOCK) {
+    const int64_t c0 = (int64_t)rank * PITCH, m = cols - c0 < PITCH ? cols - c0 : PITCH;
+    float *out = parts + (int64_t)(blockIdx.x / size) * 2 * cols + c0;
+    for (int64_t c = threadIdx.x; c < m; c += BLOCK) {
         out[c] = comb[c];
-        out[cols + c] = comb[pitch + c];
+        out[cols + c] = comb[PITCH + c];
     }
 }
 
@@ -392,36 +459,44 @@ int launch_grad_long(const T *dy, int64_t lddy, const T *x, int64_t ldx, const f
     return ZPUCUDA_OK;
 }
 
-// Threads a row and rows a block of the one-pass gradient.
+// Threads a row, rows a block, blocks a row and rows of sums of the one-pass gradient.
 struct GradShape {
-    int tpr, groups, blocks;
+    int tpr, groups, cluster, parts;
 };
 GradShape grad_shape(int64_t rows, int64_t cols) {
     GradShape g;
-    g.tpr = cols <= 32 * kPerThread ? 32 : cols <= 256 * kPerThread ? 256 : cols <= 512 * kPerThread ? 512 : 1024;
-    const int block = g.tpr == 32 ? 256 : g.tpr <= 512 ? 512 : 1024;
-    g.groups = block / g.tpr;
-    const int64_t want = (rows + g.groups - 1) / g.groups, most = (int64_t)num_sms() * (g.tpr == 32 ? kMaxParts : 1);
-    g.blocks = (int)(want < most ? want : most);
+    g.tpr = cols <= 32 * kPerThread ? 32 : cols <= 256 * kPerThread ? 256 : 512;
+    g.groups = (g.tpr == 32 ? 256 : 512) / g.tpr;
+    g.cluster = (int)((cols + (int64_t)g.tpr * kPerThread - 1) / ((int64_t)g.tpr * kPerThread));
+    const int64_t want = (rows + g.groups - 1) / g.groups, most = (int64_t)num_sms() * (g.tpr == 32 ? 2 : 1) / g.cluster;
+    g.parts = (int)(want < most ? want : most);
     return g;
 }
 
-template <typename T, int TPR, int NV, int BLOCK>
+template <typename T, int TPR, int NV, int BLOCK, int D, bool CLUSTER = false>
 int launch_grad(const GradShape &g, const T *dy, int64_t lddy, const T *x, int64_t ldx, const float *mean,
                 const float *rstd, int wt, const void *gamma, T *dx, int64_t lddx, float *parts, int64_t rows,
                 int64_t cols, cudaStream_t s) {
-    auto f = ln_grad_kernel<T, TPR, NV, BLOCK>;
-    const size_t smem = (size_t)((cols + kPiece<T> - 1) / kPiece<T> * kPiece<T>) * 8;
-    if (smem > 40 * 1024) {  // at most 128 KiB
-        static bool attr[64] = {false};
-        const int dev = current_device();
-        if (dev < 0 || dev >= 64 || !attr[dev]) {
-            ZC_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, TPR * kPerThread * 8));
-            if (dev >= 0 && dev < 64) attr[dev] = true;
-        }
-    }
-    f<<<g.blocks, BLOCK, smem, s>>>(dy, lddy, x, ldx, mean, rstd, wt, gamma, dx, lddx, parts, rows, cols);
-    ZC_LAUNCHED("ln_grad_kernel");
+    auto f = ln_grad_kernel<T, TPR, NV, BLOCK, D, CLUSTER>;
+    // the ring, in whose place the sums are added up at the end
+    constexpr size_t ring = (size_t)(BLOCK / 32) * RowRing<T, TPR, NV, 2, D>::kWarp * 16, sums = (size_t)TPR * NV * kPiece<T> * 8;
+    constexpr size_t smem = ring > sums ? ring : sums;
+    static_assert(smem <= 226 * 1024, "shared memory");
+    static int cache[64] = {0};
+    if (!blocks_per_sm(f, BLOCK, smem, cache)) return cuda_fail(cudaGetLastError(), "layer_norm_grad: occupancy");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(g.parts * g.cluster));
+    cfg.blockDim = dim3(BLOCK);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)g.cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = CLUSTER ? 1 : 0;
+    ZC_CUDA(cudaLaunchKernelEx(&cfg, f, dy, lddy, x, ldx, mean, rstd, wt, gamma, dx, lddx, parts, rows, cols));
+    count_launch();
     return ZPUCUDA_OK;
 }
 
@@ -429,20 +504,19 @@ template <typename T>
 int launch_grad_for(const GradShape &g, const T *dy, int64_t lddy, const T *x, int64_t ldx, const float *mean,
                     const float *rstd, int wt, const void *gamma, T *dx, int64_t lddx, float *parts, int64_t rows,
                     int64_t cols, cudaStream_t s) {
-#define GRAD(TPR, NV, BLOCK) \
-    return launch_grad<T, TPR, NV, BLOCK>(g, dy, lddy, x, ldx, mean, rstd, wt, gamma, dx, lddx, parts, rows, cols, s)
-    constexpr int NV = kPerThread / kPiece<T>;
+    constexpr int NV = kPerThread / kPiece<T>, D = NV > 2 ? 2 : 4;
     const bool half = cols * 2 <= (int64_t)g.tpr * kPerThread;  // half of the columns a thread
+#define GRAD(...) return launch_grad<T, __VA_ARGS__>(g, dy, lddy, x, ldx, mean, rstd, wt, gamma, dx, lddx, parts, rows, cols, s)
     if (g.tpr == 32) {
-        if (half) GRAD(32, NV / 2, 256);
-        GRAD(32, NV, 256);
+        if (half) GRAD(32, NV / 2, 256, 4);
+        GRAD(32, NV, 256, 4);
     }
     if (g.tpr == 256) {
-        if (half) GRAD(256, NV / 2, 512);
-        GRAD(256, NV, 512);
+        if (half) GRAD(256, NV / 2, 512, 4);
+        GRAD(256, NV, 512, D);
     }
-    if (g.tpr == 512) GRAD(512, NV, 512);
-    GRAD(1024, NV, 1024);
+    if (g.cluster == 1) GRAD(512, NV, 512, D);
+    GRAD(512, NV, 512, D, true);
 #undef GRAD
 }
 
@@ -471,8 +545,8 @@ int zpucuda_layer_norm(int dtype, const void *d_x, int64_t ldx, int wtype, const
 }
 
 int64_t zpucuda_layer_norm_grad_work(int64_t rows, int64_t cols) {
-    if (rows < 0 || cols < 1 || cols > 1024 * kPerThread) return 0;
-    return (int64_t)grad_shape(rows, cols).blocks * 2 * cols * (int64_t)sizeof(float);
+    if (rows < 0 || cols < 1 || cols > kMaxOnePass) return 0;
+    return (int64_t)grad_shape(rows, cols).parts * 2 * cols * (int64_t)sizeof(float);
 }
 
 int zpucuda_layer_norm_grad(int dtype, const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx,
@@ -495,7 +569,7 @@ int zpucuda_layer_norm_grad(int dtype, const void *d_dy, int64_t lddy, const voi
     if (need > 0 && (!d_work || work_bytes < need || !aligned_to(d_work, 16)))
         return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "layer_norm_grad: work: null, too small or not 16-byte aligned");
     cudaStream_t s = resolve_stream(stream);
-    if (cols > 1024 * kPerThread)
+    if (cols > kMaxOnePass)
         ZC_HEAD_TYPE(dtype, T,
                      return launch_grad_long<T>((const T *)d_dy, lddy, (const T *)d_x, ldx, d_mean, d_rstd, wtype, d_gamma,
                                                 (T *)d_dx, lddx, d_dgamma, d_dbeta, rows, cols, s));
@@ -506,7 +580,7 @@ int zpucuda_layer_norm_grad(int dtype, const void *d_dy, int64_t lddy, const voi
                                                d_gamma, (T *)d_dx, lddx, sums ? (float *)d_work : nullptr, rows, cols, s)));
     }
     if (sums) {
-        ln_parts_kernel<<<(unsigned)((2 * cols + 31) / 32), 512, 0, s>>>((const float *)d_work, rows > 0 ? g.blocks : 0, wtype,
+        ln_parts_kernel<<<(unsigned)((2 * cols + 31) / 32), 512, 0, s>>>((const float *)d_work, rows > 0 ? g.parts : 0, wtype,
                                                                         d_dgamma, d_dbeta, cols);
         ZC_LAUNCHED("ln_parts_kernel");
     }
