@@ -68,6 +68,35 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 template <typename T>
 constexpr int kPiece = 16 / (int)sizeof(T);
 
+// Two f32 values in one register pair: sm_100 adds and multiplies both with one
+// instruction, each rounded as by itself.
+struct f32x2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ f32x2 make2(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ f32x2 make2(float x) { return make2(x, x); }
+__device__ __forceinline__ float lo2(f32x2 a) { return __uint_as_float((uint32_t)a.v); }
+__device__ __forceinline__ float hi2(f32x2 a) { return __uint_as_float((uint32_t)(a.v >> 32)); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
 template <typename T>
 __device__ __forceinline__ void unpack(const uint4 &q, float (&f)[kPiece<T>]) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -104,6 +133,24 @@ __device__ __forceinline__ uint4 pack(const float (&f)[kPiece<T>]) {
         }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack2(const uint4 &q, f32x2 (&f)[kPiece<T> / 2]) {
+    float x[kPiece<T>];
+    unpack<T>(q, x);
+#pragma unroll
+    for (int i = 0; i < kPiece<T> / 2; i++) f[i] = make2(x[2 * i], x[2 * i + 1]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack2(const f32x2 (&f)[kPiece<T> / 2]) {
+    float x[kPiece<T>];
+#pragma unroll
+    for (int i = 0; i < kPiece<T> / 2; i++) {
+        x[2 * i] = lo2(f[i]);
+        x[2 * i + 1] = hi2(f[i]);
+    }
+    return pack<T>(x);
 }
 
 // Bytes s .. s + 15 of the 32 bytes lo, hi (0 <= s < 16).
@@ -188,8 +235,9 @@ __device__ __forceinline__ void store_piece(T *row, int64_t i, int64_t n, const 
 
 // A ring of D rows' pieces in shared memory, filled by asynchronous copies: a warp
 // has its lanes' pieces t + j * TPR (j < NV) of ROWS rows (tensors) a slot, and no
-// other warp reads them.  Bytes in flight cost no registers this way.
-template <typename T, int TPR, int NV, int ROWS, int D>
+// other warp reads them.  Bytes in flight cost no registers this way.  EVEN: rows
+// start on 16-byte boundaries and hold whole pieces.
+template <typename T, int TPR, int NV, int ROWS, int D, bool EVEN>
 struct RowRing {
     static constexpr int kWarp = D * ROWS * NV * 33;  // uint4 a warp: 32 lanes' 16 bytes, and the next 16
     uint4 *base;
@@ -207,7 +255,7 @@ struct RowRing {
     // The aligned 16 bytes that hold the row's pieces, clipped at its end.  Before its
     // beginning lie the bytes of the row before it, except (`first`) at the matrix's.
     __device__ __forceinline__ void issue(int slot, int r, const T *row, int64_t n, bool first) const {
-        const uint32_t s = (uint32_t)(uintptr_t)row & 15;
+        const uint32_t s = EVEN ? 0 : (uint32_t)(uintptr_t)row & 15;
         const uint8_t *from = (const uint8_t *)row - s;
         const int64_t end = s + n * (int64_t)sizeof(T);
 #pragma unroll
@@ -215,6 +263,10 @@ struct RowRing {
             const int64_t b = (int64_t)(t + j * TPR) * 16;
             if (b >= end) continue;
             uint4 *dst = at(slot, r, j);
+            if constexpr (EVEN) {
+                copy(dst + lane, from + b, 16);
+                continue;
+            }
             if (first && s && b == 0) {
                 T *e = (T *)(dst + lane);
                 for (int i = (int)(s / sizeof(T)); i < kPiece<T> && i * (int)sizeof(T) < end; i++) e[i] = row[i - (int)(s / sizeof(T))];
@@ -232,11 +284,11 @@ struct RowRing {
     }
     // Piece t + j * TPR, 0 past the row's end.
     __device__ __forceinline__ uint4 read(int slot, int r, int j, const T *row, int64_t n) const {
-        const uint32_t s = (uint32_t)(uintptr_t)row & 15;
+        const uint32_t s = EVEN ? 0 : (uint32_t)(uintptr_t)row & 15;
         const int64_t b = (int64_t)(t + j * TPR) * 16, end = s + n * (int64_t)sizeof(T);
         const uint4 *src = at(slot, r, j) + lane, none = make_uint4(0, 0, 0, 0);
         const uint4 lo = b < end ? src[0] : none;
-        if (s == 0) return lo;
+        if (EVEN || s == 0) return lo;
         return bytes_from(lo, b + 16 < end ? src[1] : none, s);
     }
 };

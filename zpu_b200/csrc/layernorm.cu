@@ -16,7 +16,7 @@ namespace zc {
 namespace {
 
 constexpr int NT = 256;
-constexpr int kPerThread = 16;  // columns that a thread of the one-pass gradient holds
+constexpr int kPerThread = 16;  // columns of a row that a thread holds
 constexpr int kMaxCluster = 8;  // blocks of a cluster of it
 constexpr int64_t kMaxOnePass = 512 * kPerThread * kMaxCluster;
 
@@ -59,84 +59,88 @@ __device__ __forceinline__ int in_row(int64_t i, int64_t cols) {
 }
 
 // Sums of two values over the TPR threads of a row; every thread gets both.
-// sm: TPR / 32 entries of the row's own; barrier `bar` is the row's own.
+// sm: 2 * TPR / 32 floats of the row's own; barrier `bar` is the row's own.
 template <int TPR>
-__device__ __forceinline__ float2 row_sum2(float a, float b, float2 *sm, int bar) {
+__device__ __forceinline__ float2 row_sum2(float a, float b, float *sm, int bar) {
+    const int lane = threadIdx.x & 31;
+    const bool up = lane & 16;  // the lower lanes go on with a, the upper ones with b
+    float v = (up ? b : a) + __shfl_xor_sync(0xffffffffu, up ? a : b, 16);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
-    if (TPR == 32) return make_float2(a, b);
-    if ((threadIdx.x & 31) == 0) sm[(threadIdx.x % TPR) >> 5] = make_float2(a, b);
-    asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(TPR) : "memory");
-    float2 t = make_float2(0.0f, 0.0f);
+    for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (TPR > 32) {
+        constexpr int W = TPR / 32;
+        if ((lane & 15) == 0) sm[((threadIdx.x % TPR) >> 5) + (up ? W : 0)] = v;
+        asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(TPR) : "memory");
+        if constexpr (W == 32) {
+            float p = sm[lane], q = sm[32 + lane];
+            v = (up ? q : p) + __shfl_xor_sync(0xffffffffu, up ? p : q, 16);
 #pragma unroll
-    for (int w = 0; w < TPR / 32; w++) {
-        t.x += sm[w].x;
-        t.y += sm[w].y;
+            for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        } else {
+            v = sm[(lane & (W - 1)) + (up ? W : 0)];
+#pragma unroll
+            for (int o = W / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        }
     }
-    return t;
+    return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
 }
 
 // ------------------------------------------------------------------ forward
 
-// A thread's part of the forward pass over its pieces of a row.
-template <typename T>
-struct Row {
-    static constexpr int N = kPiece<T>;
-    int64_t cols;
-    float s = 0.0f, d1 = 0.0f, d2 = 0.0f, mu, rest, rs;
+// The weights of a piece in pairs.
+template <int N>
+__device__ __forceinline__ void load_w2(const void *p, int wt, int64_t i, int have, float dflt, f32x2 (&f)[N / 2]) {
+    float w[N];
+    load_w<N>(p, wt, i, have, dflt, w);
+#pragma unroll
+    for (int e = 0; e < N / 2; e++) f[e] = make2(w[2 * e], w[2 * e + 1]);
+}
 
-    __device__ __forceinline__ void sum(const uint4 &in) {  // what is past the row's end is 0
-        float a[N];
-        unpack<T>(in, a);
+// What a thread does with its pieces of a row, forward.  The mean of what the
+// rounded mean leaves (`rest`) is taken off again: rows far from zero keep the
+// digits that a 32-bit mean alone would cost them.
+template <typename T>
+struct Fwd {
+    static constexpr int N = kPiece<T>, H = N / 2;
+    static __device__ __forceinline__ void sum(const f32x2 (&a)[H], f32x2 &s) {  // what is past the row's end is 0
 #pragma unroll
-        for (int e = 0; e < N; e++) s += a[e];
+        for (int e = 0; e < H; e++) s = add2(s, a[e]);
     }
-    __device__ __forceinline__ void spread(const uint4 &in, int64_t i) {
-        float a[N];
-        unpack<T>(in, a);
-        const int have = in_row<N>(i, cols);
+    static __device__ __forceinline__ void spread(f32x2 (&a)[H], int have, float mu, f32x2 &d1, f32x2 &d2) {
 #pragma unroll
-        for (int e = 0; e < N; e++) {
-            const float d = e < have ? a[e] - mu : 0.0f;
-            d1 += d;
-            d2 += d * d;
+        for (int e = 0; e < H; e++) {
+            a[e] = add2(a[e], make2(-mu));
+            if (2 * e + 1 >= have) a[e] = make2(2 * e < have ? lo2(a[e]) : 0.0f, 0.0f);
+            d1 = add2(d1, a[e]);
+            d2 = fma2(a[e], a[e], d2);
         }
     }
-    // The mean of what the rounded mean leaves is taken off again: rows far
-    // from zero keep the digits that a 32-bit mean alone would cost them.
-    __device__ __forceinline__ void finish(float2 q, float inv, float eps) {
-        rest = q.x * inv;
+    // (mean - mu, 1 / deviation) from the sums of d and d^2.
+    static __device__ __forceinline__ float2 finish(float2 q, float inv, float eps) {
+        const float rest = q.x * inv;
         float var = q.y * inv - rest * rest;
         var = var < 0.0f ? 0.0f : var;  // NaN stays
-        rs = 1.0f / sqrtf(var + eps);
+        return make_float2(rest, 1.0f / sqrtf(var + eps));
     }
-    __device__ __forceinline__ void put(const uint4 &in, int64_t i, T *y, int wt, const void *gamma, const void *beta) {
-        float a[N], g[N], b[N];  // a whole warp's pieces
-        unpack<T>(in, a);
-        const int have = in_row<N>(i, cols);
-        load_w<N>(gamma, wt, i, have, 1.0f, g);
-        load_w<N>(beta, wt, i, have, 0.0f, b);
+    static __device__ __forceinline__ uint4 out(const f32x2 (&a)[H], float2 f, const f32x2 (&g)[H], const f32x2 (&b)[H]) {
+        f32x2 y[H];
 #pragma unroll
-        for (int e = 0; e < N; e++) a[e] = ((a[e] - mu) - rest) * rs * g[e] + b[e];
-        __syncwarp();
-        store_piece(y, i, cols, pack<T>(a));
+        for (int e = 0; e < H; e++) y[e] = fma2(mul2(add2(a[e], make2(-f.x)), make2(f.y)), g[e], b[e]);
+        return pack2<T>(y);
     }
 };
 
-// TPR threads a row, NV pieces a thread; a block walks rows, D of them on their
-// way to shared memory while one is worked on.
-template <typename T, int TPR, int NV, int D>
+// TPR threads a row, NV pieces a thread, whose weights it keeps in registers; a
+// block walks rows, D of them on their way to shared memory while one is worked on.
+template <typename T, int TPR, int NV, int D, bool EVEN>
 __global__ void __launch_bounds__(TPR < NT ? NT : TPR)
     ln_kernel(const T *x, int64_t ldx, int wt, const void *gamma, const void *beta, T *y, int64_t ldy, float *mean,
               float *rstd, int64_t rows, int64_t cols, float eps) {
-    constexpr int BLOCK = TPR < NT ? NT : TPR, GROUPS = BLOCK / TPR;
+    constexpr int BLOCK = TPR < NT ? NT : TPR, GROUPS = BLOCK / TPR, N = kPiece<T>;
     extern __shared__ uint4 ring_smem[];
-    __shared__ float2 sm[2][2][BLOCK / 32];
-    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
-    const RowRing<T, TPR, NV, 1, D> ring(ring_smem, t);
+    __shared__ float sm[2][2][BLOCK / 16];
+    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, bar = 1 + (TPR > 32 ? group : 0);
+    const RowRing<T, TPR, NV, 1, D, EVEN> ring(ring_smem, t);
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     int64_t row = (int64_t)blockIdx.x * GROUPS + group;
     const float inv = 1.0f / (float)cols;
@@ -145,28 +149,46 @@ __global__ void __launch_bounds__(TPR < NT ? NT : TPR)
         if (row + d * step < rows) ring.issue(d, 0, x + (row + d * step) * ldx, cols, row + d * step == 0);
         ring.commit();
     }
+    f32x2 g[NV][N / 2], b[NV][N / 2];
+    int have[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        have[j] = EVEN ? ((int64_t)(t + j * TPR) * N < cols ? N : 0) : in_row<N>(t + j * TPR, cols);
+        load_w2<N>(gamma, wt, t + j * TPR, have[j], 1.0f, g[j]);
+        load_w2<N>(beta, wt, t + j * TPR, have[j], 0.0f, b[j]);
+    }
     int slot = 0;
     for (int odd = 0; row < rows; row += step, odd ^= 1) {
         ring.wait();
-        uint4 v[NV];
+        f32x2 v[NV][N / 2], s = make2(0.0f), d1 = s, d2 = s;
 #pragma unroll
-        for (int j = 0; j < NV; j++) v[j] = ring.read(slot, 0, j, x + row * ldx, cols);
+        for (int j = 0; j < NV; j++) {
+            unpack2<T>(ring.read(slot, 0, j, x + row * ldx, cols), v[j]);
+            Fwd<T>::sum(v[j], s);
+        }
         __syncwarp();
         if (row + D * step < rows) ring.issue(slot, 0, x + (row + D * step) * ldx, cols, false);
         ring.commit();
         slot = slot + 1 == D ? 0 : slot + 1;
-        Row<T> R = {cols};
+        const float mu = row_sum2<TPR>(lo2(s) + hi2(s), 0.0f, sm[odd][0] + group * (TPR / 16), bar).x * inv;
 #pragma unroll
-        for (int j = 0; j < NV; j++) R.sum(v[j]);
-        R.mu = row_sum2<TPR>(R.s, 0.0f, sm[odd][0], 0).x * inv;
+        for (int j = 0; j < NV; j++)
+            if (!EVEN || have[j]) Fwd<T>::spread(v[j], EVEN ? N : have[j], mu, d1, d2);
+        const float2 f = Fwd<T>::finish(row_sum2<TPR>(lo2(d1) + hi2(d1), lo2(d2) + hi2(d2), sm[odd][1] + group * (TPR / 16), bar), inv, eps);
 #pragma unroll
-        for (int j = 0; j < NV; j++) R.spread(v[j], t + j * TPR);
-        R.finish(row_sum2<TPR>(R.d1, R.d2, sm[odd][1], 0), inv, eps);
-#pragma unroll
-        for (int j = 0; j < NV; j++) R.put(v[j], t + j * TPR, y + row * ldy, wt, gamma, beta);
+        for (int j = 0; j < NV; j++) {
+            T *yr = y + row * ldy;
+            if constexpr (EVEN) {
+                if (have[j]) *(uint4 *)(yr + (t + j * TPR) * N) = Fwd<T>::out(v[j], f, g[j], b[j]);
+            } else {
+                const uint4 o = Fwd<T>::out(v[j], f, g[j], b[j]);
+                __syncwarp();
+                store_piece(yr, t + j * TPR, cols, o);
+            }
+        }
         if (t == 0) {
-            if (mean) mean[row] = R.mu + R.rest;
-            if (rstd) rstd[row] = R.rs;
+            if (mean) mean[row] = mu + f.x;
+            if (rstd) rstd[row] = f.y;
         }
     }
 }
@@ -176,20 +198,36 @@ template <typename T>
 __global__ void __launch_bounds__(1024)
     ln_long_kernel(const T *x, int64_t ldx, int wt, const void *gamma, const void *beta, T *y, int64_t ldy, float *mean,
                    float *rstd, int64_t cols, float eps) {
-    __shared__ float2 sm[2][32];
-    const int64_t row = blockIdx.x, n = (cols + kPiece<T> - 1) / kPiece<T>;
+    constexpr int N = kPiece<T>;
+    __shared__ float sm[2][64];
+    const int64_t row = blockIdx.x, n = (cols + N - 1) / N;
     const T *xr = x + row * ldx;
     const float inv = 1.0f / (float)cols;
-    Row<T> R = {cols};
-    for (int64_t i = threadIdx.x; i < n; i += 1024) R.sum(load_piece(xr, i, cols));
-    R.mu = row_sum2<1024>(R.s, 0.0f, sm[0], 0).x * inv;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) R.spread(load_piece(xr, i, cols), i);
-    R.finish(row_sum2<1024>(R.d1, R.d2, sm[1], 0), inv, eps);
-    for (int64_t i = threadIdx.x; i - (threadIdx.x & 31) < n; i += 1024)
-        R.put(i < n ? load_piece(xr, i, cols) : make_uint4(0, 0, 0, 0), i, y + row * ldy, wt, gamma, beta);
+    f32x2 v[N / 2], s = make2(0.0f), d1 = s, d2 = s;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        unpack2<T>(load_piece(xr, i, cols), v);
+        Fwd<T>::sum(v, s);
+    }
+    const float mu = row_sum2<1024>(lo2(s) + hi2(s), 0.0f, sm[0], 1).x * inv;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        unpack2<T>(load_piece(xr, i, cols), v);
+        Fwd<T>::spread(v, in_row<N>(i, cols), mu, d1, d2);
+    }
+    const float2 f = Fwd<T>::finish(row_sum2<1024>(lo2(d1) + hi2(d1), lo2(d2) + hi2(d2), sm[1], 1), inv, eps);
+    for (int64_t i = threadIdx.x; i - (threadIdx.x & 31) < n; i += 1024) {
+        f32x2 none = make2(0.0f), unused = none;
+        unpack2<T>(i < n ? load_piece(xr, i, cols) : make_uint4(0, 0, 0, 0), v);
+        Fwd<T>::spread(v, in_row<N>(i, cols), mu, none, unused);
+        f32x2 g[N / 2], b[N / 2];
+        load_w2<N>(gamma, wt, i, in_row<N>(i, cols), 1.0f, g);
+        load_w2<N>(beta, wt, i, in_row<N>(i, cols), 0.0f, b);
+        const uint4 o = Fwd<T>::out(v, f, g, b);
+        __syncwarp();
+        store_piece(y + row * ldy, i, cols, o);
+    }
     if (threadIdx.x == 0) {
-        if (mean) mean[row] = R.mu + R.rest;
-        if (rstd) rstd[row] = R.rs;
+        if (mean) mean[row] = mu + f.x;
+        if (rstd) rstd[row] = f.y;
     }
 }
 
@@ -206,12 +244,18 @@ int blocks_per_sm(F f, int block, size_t smem, int *cache) {
     return n;
 }
 
-template <typename T, int TPR, int NV, int D>
+// Whether rows of cols elements at pitches of ld start on 16-byte boundaries and hold whole pieces.
+template <typename T>
+bool even_rows(const void *p, int64_t ld, int64_t rows, int64_t cols) {
+    return cols % kPiece<T> == 0 && aligned_to(p, 16) && (rows <= 1 || ld % kPiece<T> == 0);
+}
+
+template <typename T, int TPR, int NV, int D, bool EVEN>
 int launch_ln_ring(const T *x, int64_t ldx, int wt, const void *gamma, const void *beta, T *y, int64_t ldy, float *mean,
                    float *rstd, int64_t rows, int64_t cols, float eps, cudaStream_t s) {
     constexpr int BLOCK = TPR < NT ? NT : TPR, GROUPS = BLOCK / TPR;
-    auto f = ln_kernel<T, TPR, NV, D>;
-    const size_t smem = (size_t)(BLOCK / 32) * RowRing<T, TPR, NV, 1, D>::kWarp * 16;
+    auto f = ln_kernel<T, TPR, NV, D, EVEN>;
+    const size_t smem = (size_t)(BLOCK / 32) * RowRing<T, TPR, NV, 1, D, EVEN>::kWarp * 16;
     static int cache[64] = {0};
     const int per = blocks_per_sm(f, BLOCK, smem, cache);
     if (!per) return cuda_fail(cudaGetLastError(), "layer_norm: occupancy");
@@ -225,16 +269,19 @@ template <typename T>
 int launch_ln(const T *x, int64_t ldx, int wt, const void *gamma, const void *beta, T *y, int64_t ldy, float *mean,
               float *rstd, int64_t rows, int64_t cols, float eps, cudaStream_t s) {
     const int64_t n = (cols + kPiece<T> - 1) / kPiece<T>;
-#define LN(TPR, NV, D) return launch_ln_ring<T, TPR, NV, D>(x, ldx, wt, gamma, beta, y, ldy, mean, rstd, rows, cols, eps, s)
-    // a warp holds 128 pieces, 256 threads 1024, 1024 threads 4096
-    if (n <= 32) LN(32, 1, 4);
-    if (n <= 64) LN(32, 2, 4);
-    if (n <= 128) LN(32, 4, 3);
-    if (n <= 256) LN(256, 1, 4);
-    if (n <= 512) LN(256, 2, 4);
-    if (n <= 1024) LN(256, 4, 3);
-    if (n <= 2048) LN(1024, 2, 3);
-    if (n <= 4096) LN(1024, 4, 2);
+    const bool even = even_rows<T>(x, ldx, rows, cols) && even_rows<T>(y, ldy, rows, cols);
+#define LN(...)                                                                                                              \
+    return even ? launch_ln_ring<T, __VA_ARGS__, true>(x, ldx, wt, gamma, beta, y, ldy, mean, rstd, rows, cols, eps, s)      \
+                : launch_ln_ring<T, __VA_ARGS__, false>(x, ldx, wt, gamma, beta, y, ldy, mean, rstd, rows, cols, eps, s)
+    // sixteen columns a thread at most (32-bit: four pieces; 16-bit: two)
+    constexpr int NV = kPerThread / kPiece<T>;
+    if (n <= 32 * NV / 2) LN(32, NV / 2, 4);
+    if (n <= 32 * NV) LN(32, NV, 4);
+    if (n <= 128 * NV / 2) LN(128, NV / 2, 4);
+    if (n <= 128 * NV) LN(128, NV, 4);
+    if (n <= 512 * NV / 2) LN(512, NV / 2, 4);
+    if (n <= 512 * NV) LN(512, NV, 3);
+    if (n <= 1024 * NV) LN(1024, NV, 2);
 #undef LN
     ln_long_kernel<T><<<(unsigned)rows, 1024, 0, s>>>(x, ldx, wt, gamma, beta, y, ldy, mean, rstd, cols, eps);
     ZC_LAUNCHED("ln_long_kernel");
@@ -248,12 +295,13 @@ int launch_ln(const T *x, int64_t ldx, int wt, const void *gamma, const void *be
 // that a block does not hold is split over a cluster (CLUSTER), whose blocks tell
 // one another their parts of its two sums.  parts: a row of [2][cols] sums for
 // each block (cluster), or null.
-template <typename T, int TPR, int NV, int BLOCK, int D, bool CLUSTER>
+template <typename T, int TPR, int NV, int BLOCK, int D, bool CLUSTER, bool EVEN>
 __global__ void __launch_bounds__(BLOCK)
     ln_grad_kernel(const T *dy, int64_t lddy, const T *x, int64_t ldx, const float *mean, const float *rstd, int wt,
                    const void *gamma, T *dx, int64_t lddx, float *parts, int64_t rows, int64_t cols) {
     constexpr int GROUPS = BLOCK / TPR, N = kPiece<T>, PITCH = TPR * NV * N;
-    __shared__ float2 sm[2][BLOCK / 32], peers[2][kMaxCluster];
+    __shared__ float2 peers[2][kMaxCluster];
+    __shared__ float sm[2][BLOCK / 16];
     extern __shared__ uint4 grad_smem[];
     uint32_t rank = 0, size = 1;
     if constexpr (CLUSTER) {
@@ -264,10 +312,14 @@ __global__ void __launch_bounds__(BLOCK)
     const int t = threadIdx.x % TPR, p0 = t + (int)rank * TPR * NV;  // in the block's part of a row, in the row
     const int64_t n = (cols + N - 1) / N;
     const float inv = 1.0f / (float)cols;
-    float g[NV][N], ag[NV][N] = {}, ab[NV][N] = {};
+    f32x2 g[NV][N / 2], ag[NV][N / 2], ab[NV][N / 2];
 #pragma unroll
-    for (int j = 0; j < NV; j++) load_w<N>(gamma, wt, p0 + j * TPR, in_row<N>(p0 + j * TPR, cols), 1.0f, g[j]);
-    const RowRing<T, TPR, NV, 2, D> ring(grad_smem, p0);
+    for (int j = 0; j < NV; j++) {
+        load_w2<N>(gamma, wt, p0 + j * TPR, in_row<N>(p0 + j * TPR, cols), 1.0f, g[j]);
+#pragma unroll
+        for (int e = 0; e < N / 2; e++) ag[j][e] = ab[j][e] = make2(0.0f);
+    }
+    const RowRing<T, TPR, NV, 2, D, EVEN> ring(grad_smem, p0);
     const int64_t step = (int64_t)(gridDim.x / size) * GROUPS;
     int64_t row = (int64_t)(blockIdx.x / size) * GROUPS + group;
     auto issue = [&](int slot, int64_t r) {
@@ -280,37 +332,41 @@ __global__ void __launch_bounds__(BLOCK)
 #pragma unroll
     for (int d = 0; d < D; d++) issue(d, row + d * step);
     int slot = 0;
+    float next_mu = 0.0f, next_rs = 0.0f;
+    if (row < rows) {
+        next_mu = mean[row];
+        next_rs = rstd[row];
+    }
     for (int odd = 0; row < rows; row += step, odd ^= 1) {
-        const float mu = mean[row], rs = rstd[row];
+        const float mu = next_mu, rs = next_rs;
+        if (row + step < rows) {
+            next_mu = mean[row + step];
+            next_rs = rstd[row + step];
+        }
         ring.wait();
-        uint4 vx[NV], vd[NV];
+        // xhat and dy * gamma; past the row's end dy is 0, and all that follows from it
+        f32x2 xh[NV][N / 2], gd[NV][N / 2], a = make2(0.0f), b = a;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            vx[j] = ring.read(slot, 0, j, x + row * ldx, cols);
-            vd[j] = ring.read(slot, 1, j, dy + row * lddy, cols);
+            f32x2 d[N / 2];
+            unpack2<T>(ring.read(slot, 0, j, x + row * ldx, cols), xh[j]);
+            unpack2<T>(ring.read(slot, 1, j, dy + row * lddy, cols), d);
+#pragma unroll
+            for (int e = 0; e < N / 2; e++) {
+                xh[j][e] = mul2(add2(xh[j][e], make2(-mu)), make2(rs));
+                gd[j][e] = mul2(d[e], g[j][e]);
+                a = add2(a, gd[j][e]);
+                b = fma2(gd[j][e], xh[j][e], b);
+                ag[j][e] = fma2(d[e], xh[j][e], ag[j][e]);
+                ab[j][e] = add2(ab[j][e], d[e]);
+            }
         }
         __syncwarp();
         issue(slot, row + D * step);
         slot = slot + 1 == D ? 0 : slot + 1;
-        float a = 0.0f, b = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NV; j++) {  // past the row's end dy is 0, and all that follows from it
-            if (p0 + j * TPR >= n) continue;
-            float fx[N], fd[N];
-            unpack<T>(vx[j], fx);
-            unpack<T>(vd[j], fd);
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const float xh = (fx[e] - mu) * rs, d = fd[e], gd = d * g[j][e];
-                a += gd;
-                b += gd * xh;
-                ag[j][e] += d * xh;
-                ab[j][e] += d;
-            }
-        }
         if (!dx) continue;
         // two buffers: a thread that is a row ahead does not overwrite what another still reads
-        float2 q = row_sum2<TPR>(a, b, sm[odd] + group * (TPR / 32), bar);
+        float2 q = row_sum2<TPR>(lo2(a) + hi2(a), lo2(b) + hi2(b), sm[odd] + group * (TPR / 16), bar);
         if constexpr (CLUSTER) {
             if (threadIdx.x < size) {
                 uint32_t there;
@@ -327,19 +383,18 @@ __global__ void __launch_bounds__(BLOCK)
                 q.y += peers[odd][r].y;
             }
         }
-        const float ma = q.x * inv, mb = q.y * inv;
+        const f32x2 m = make2(-rs * (q.x * inv)), k = make2(-rs * (q.y * inv)), r2 = make2(rs);
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            float fx[N], fd[N];
-            unpack<T>(vx[j], fx);
-            unpack<T>(vd[j], fd);
 #pragma unroll
-            for (int e = 0; e < N; e++) {
-                const float xh = (fx[e] - mu) * rs;
-                fx[e] = rs * (fd[e] * g[j][e] - ma - xh * mb);
+            for (int e = 0; e < N / 2; e++) xh[j][e] = fma2(xh[j][e], k, fma2(gd[j][e], r2, m));
+            T *o = dx + row * lddx;
+            if constexpr (EVEN) {
+                if (p0 + j * TPR < n) *(uint4 *)(o + (int64_t)(p0 + j * TPR) * N) = pack2<T>(xh[j]);
+            } else {
+                __syncwarp();
+                store_piece(o, p0 + j * TPR, cols, pack2<T>(xh[j]));
             }
-            __syncwarp();
-            store_piece(dx + row * lddx, p0 + j * TPR, cols, pack<T>(fx));
         }
     }
     // no block ends while another may still write to its shared memory
@@ -359,8 +414,9 @@ __global__ void __launch_bounds__(BLOCK)
                 float *sg = comb + (t + j * TPR) * N, *sb = sg + PITCH;
 #pragma unroll
                 for (int e = 0; e < N; e++) {
-                    sg[e] = k ? sg[e] + ag[j][e] : ag[j][e];
-                    sb[e] = k ? sb[e] + ab[j][e] : ab[j][e];
+                    const float u = e & 1 ? hi2(ag[j][e / 2]) : lo2(ag[j][e / 2]), v = e & 1 ? hi2(ab[j][e / 2]) : lo2(ab[j][e / 2]);
+                    sg[e] = k ? sg[e] + u : u;
+                    sb[e] = k ? sb[e] + v : v;
                 }
             }
     }
@@ -381,8 +437,18 @@ __global__ void __launch_bounds__(512) ln_parts_kernel(const float *parts, int n
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;  // of 2 * cols
     float s = 0.0f;
-    if (c < 2 * cols)
-        for (int i = w; i < nparts; i += 16) s += parts[(int64_t)i * 2 * cols + c];
+    if (c < 2 * cols) {
+        const float *p = parts + c;
+        int i = w;
+        for (; i + 64 < nparts; i += 80) {  // five loads in flight
+            float v[5];
+#pragma unroll
+            for (int u = 0; u < 5; u++) v[u] = p[(int64_t)(i + 16 * u) * 2 * cols];
+#pragma unroll
+            for (int u = 0; u < 5; u++) s += v[u];
+        }
+        for (; i < nparts; i += 16) s += p[(int64_t)i * 2 * cols];
+    }
     sm[w][lane] = s;
     __syncthreads();
     if (w == 0 && c < 2 * cols) {
@@ -399,7 +465,7 @@ template <typename T>
 __global__ void __launch_bounds__(1024) ln_dx_kernel(const T *dy, int64_t lddy, const T *x, int64_t ldx,
                                                      const float *mean, const float *rstd, int wt, const void *gamma,
                                                      T *dx, int64_t lddx, int64_t cols) {
-    __shared__ float2 sm[32];
+    __shared__ float sm[64];
     const int64_t row = blockIdx.x;
     const T *xr = x + row * ldx, *dr = dy + row * lddy;
     T *o = dx + row * lddx;
@@ -410,7 +476,7 @@ __global__ void __launch_bounds__(1024) ln_dx_kernel(const T *dy, int64_t lddy, 
         a += g;
         b += g * ((to_f(xr[c]) - mu) * rs);
     }
-    const float2 t = row_sum2<1024>(a, b, sm, 0);
+    const float2 t = row_sum2<1024>(a, b, sm, 1);
     const float ma = t.x / (float)cols, mb = t.y / (float)cols;
     for (int64_t c = threadIdx.x; c < cols; c += 1024) {
         const float g = to_f(dr[c]) * (gamma ? load_f(gamma, wt, c) : 1.0f);
@@ -473,13 +539,13 @@ GradShape grad_shape(int64_t rows, int64_t cols) {
     return g;
 }
 
-template <typename T, int TPR, int NV, int BLOCK, int D, bool CLUSTER = false>
+template <typename T, int TPR, int NV, int BLOCK, int D, bool CLUSTER, bool EVEN>
 int launch_grad(const GradShape &g, const T *dy, int64_t lddy, const T *x, int64_t ldx, const float *mean,
                 const float *rstd, int wt, const void *gamma, T *dx, int64_t lddx, float *parts, int64_t rows,
                 int64_t cols, cudaStream_t s) {
-    auto f = ln_grad_kernel<T, TPR, NV, BLOCK, D, CLUSTER>;
+    auto f = ln_grad_kernel<T, TPR, NV, BLOCK, D, CLUSTER, EVEN>;
     // the ring, in whose place the sums are added up at the end
-    constexpr size_t ring = (size_t)(BLOCK / 32) * RowRing<T, TPR, NV, 2, D>::kWarp * 16, sums = (size_t)TPR * NV * kPiece<T> * 8;
+    constexpr size_t ring = (size_t)(BLOCK / 32) * RowRing<T, TPR, NV, 2, D, EVEN>::kWarp * 16, sums = (size_t)TPR * NV * kPiece<T> * 8;
     constexpr size_t smem = ring > sums ? ring : sums;
     static_assert(smem <= 226 * 1024, "shared memory");
     static int cache[64] = {0};
@@ -506,16 +572,19 @@ int launch_grad_for(const GradShape &g, const T *dy, int64_t lddy, const T *x, i
                     int64_t cols, cudaStream_t s) {
     constexpr int NV = kPerThread / kPiece<T>, D = NV > 2 ? 2 : 4;
     const bool half = cols * 2 <= (int64_t)g.tpr * kPerThread;  // half of the columns a thread
-#define GRAD(...) return launch_grad<T, __VA_ARGS__>(g, dy, lddy, x, ldx, mean, rstd, wt, gamma, dx, lddx, parts, rows, cols, s)
+    const bool even = even_rows<T>(x, ldx, rows, cols) && even_rows<T>(dy, lddy, rows, cols) && even_rows<T>(dx, lddx, rows, cols);
+#define GRAD(...)                                                                                                                     \
+    return even ? launch_grad<T, __VA_ARGS__, true>(g, dy, lddy, x, ldx, mean, rstd, wt, gamma, dx, lddx, parts, rows, cols, s)       \
+                : launch_grad<T, __VA_ARGS__, false>(g, dy, lddy, x, ldx, mean, rstd, wt, gamma, dx, lddx, parts, rows, cols, s)
     if (g.tpr == 32) {
-        if (half) GRAD(32, NV / 2, 256, 4);
-        GRAD(32, NV, 256, 4);
+        if (half) GRAD(32, NV / 2, 256, 4, false);
+        GRAD(32, NV, 256, 4, false);
     }
     if (g.tpr == 256) {
-        if (half) GRAD(256, NV / 2, 512, 4);
-        GRAD(256, NV, 512, D);
+        if (half) GRAD(256, NV / 2, 512, 4, false);
+        GRAD(256, NV, 512, D, false);
     }
-    if (g.cluster == 1) GRAD(512, NV, 512, D);
+    if (g.cluster == 1) GRAD(512, NV, 512, D, false);
     GRAD(512, NV, 512, D, true);
 #undef GRAD
 }
