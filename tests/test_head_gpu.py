@@ -294,6 +294,15 @@ def test_distill(zc, rows, vocab, top, t):
     check_distill(zc, student, teacher, index, 0.7, None, None)
 
 
+@pytest.mark.parametrize("t,rows,vocab", [("f32", 2, 450001), ("bf16", 1, 900003), ("f16", 3, 262145), ("f32", 3, 131073),
+                                          ("bf16", 700, 513), ("f16", 1200, 100), ("f32", 400, 9001)])
+def test_distill_by_the_size_of_a_row(zc, rows, vocab, t):
+    """Rows in one block, in clusters of each size, and beyond what a cluster holds."""
+    g = gen(21)
+    student, teacher, index = teach(g, rows, vocab, 12, t)
+    check_distill(zc, strided(student, 1, 0), teacher, index, 2.0, None, torch.rand(rows, generator=g, device="cuda"))
+
+
 @pytest.mark.parametrize("t", list(TYPES))
 @pytest.mark.parametrize("pitch,shift", [(1, 0), (8, 8), (5, 3)])
 @pytest.mark.parametrize("vocab", [1001, 4096, 40007])

@@ -8,13 +8,33 @@
 // listed, or all of them -inf), with weight 0 or (gradient) c = 0 gives 0
 // and its logits are not read.  Any other index outside [0, vocab) makes its
 // row NaN.
+// HBM bounds it, with the exponential unit close behind (two exponentials an
+// element where both loss and gradient are wanted): a row is copied once into
+// the shared memory of a cluster of blocks, a slice each, where its maximum, sum
+// and gradient are computed; slices are small enough (64 KiB) that several
+// blocks of an SM overlap one another's copies and arithmetic.  A slice is
+// counted in aligned 16-byte granules of memory, so an odd vocabulary costs two
+// partial granules a row and nothing else.
 #include "head.cuh"
+#include "tcgen05.cuh"
+#include "waits.cuh"
 
 namespace zc {
+
+static __device__ unsigned int g_distill_error;
+
+int distill_device_error(unsigned int *e) {
+    ZC_CUDA(cudaMemcpyFromSymbol(e, g_distill_error, sizeof *e));
+    return ZPUCUDA_OK;
+}
+
 namespace {
 
 constexpr int NT = 256;
 constexpr int kMaxTop = 1024;
+constexpr int kMaxCluster = 8;
+constexpr int kSlice = 64 * 1024, kMaxSlice = 200 * 1024;  // bytes: wanted, possible
+constexpr int kCopies = 4;                                 // of a slice, each waited for by itself
 
 struct Args {
     const void *teacher, *indices;
@@ -53,8 +73,302 @@ __device__ __forceinline__ float block_sum(float v, float *sm) {
     return v;
 }
 
+// 2^x (error 2^-22 of the result; -inf gives 0).
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// The elements of a granule outside [from, to) replaced by -inf.
+template <typename T>
+__device__ __forceinline__ uint4 keep_elements(const uint4 &q, int from, int to) {
+    float f[kPiece<T>];
+    unpack<T>(q, f);
+#pragma unroll
+    for (int e = 0; e < kPiece<T>; e++)
+        if (e < from || e >= to) f[e] = -INFINITY;
+    return pack<T>(f);  // exact: the values come from that type
+}
+
+// exp2 arguments of a granule relative to `ref`.  16-bit logits take one
+// multiply-add (k = log2(e) / T, its rounding is far below theirs); 32-bit ones
+// form z - ref first, so that the error stays relative to the distance.
+template <typename T>
+struct Scale {
+    f32x2 k, off, log2e;
+    __device__ __forceinline__ Scale(float inv_t, float ref) {
+        if constexpr (sizeof(T) == 4) {
+            k = make2(inv_t);
+            off = make2(-ref);
+            log2e = make2(1.4426950408889634f);
+        } else {
+            k = make2(inv_t * 1.4426950408889634f);
+            off = make2(-ref * 1.4426950408889634f);
+        }
+    }
+    __device__ __forceinline__ f32x2 arg(f32x2 x) const {
+        const f32x2 d = fma2(x, k, off);
+        if constexpr (sizeof(T) == 4) return mul2(d, log2e);
+        else return d;
+    }
+};
+
+// What the blocks of a row tell one another.
+template <int WARPS>
+struct Shares {
+    float2 part[kMaxCluster][WARPS];  // each warp's maximum of z and its sum of e^(z - maximum)
+    float pz[kMaxCluster];            // each block's sum of p z over the listed entries in its slice
+};
+
+template <typename T, bool LOSS, bool GRAD, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+    distill_kernel(const T *logits, int64_t ld, T *out, int64_t ldo, const Args A) {
+    constexpr int N = kPiece<T>, WARPS = THREADS / 32;
+    extern __shared__ __align__(128) uint4 slice_smem[];
+    __shared__ uint64_t full[kCopies];
+    __shared__ Shares<WARPS> sh;
+    __shared__ float red[2][WARPS];
+    __shared__ float sp[kMaxTop];
+    __shared__ int si[kMaxTop];
+    uint32_t rank, size;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+    const int64_t row = blockIdx.x / size;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const T *x = logits + row * ld;
+    T *o = GRAD ? out + row * ldo : nullptr;
+    // the row's granules g: elements g * N - skew + e
+    const int skew = (int)(((uintptr_t)x & 15) / sizeof(T));
+    const int64_t granules = (skew + A.vocab + N - 1) / N;
+    const int64_t g0 = granules * rank / size, g1 = granules * (rank + 1) / size;
+    const int n = (int)(g1 - g0);
+    const float inv_t = 1.0f / A.T;
+
+    const float w = A.weight ? A.weight[row] : 1.0f;
+    const float c = GRAD ? A.T * (w * (A.dloss ? A.dloss[row] : 1.0f)) : 0.0f;
+    const bool want_loss = LOSS && w != 0.0f, want_grad = GRAD && c != 0.0f, want = want_loss || want_grad;
+    auto whole = [&](int64_t g) { return g * N >= skew && (g + 1) * N <= skew + A.vocab; };
+
+    // the slice's whole granules by bulk copies, the others element by element
+    const int per = (n + kCopies - 1) / kCopies;
+    if (want) {
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < kCopies; i++) tc::mb_init(&full[i], 1);
+            tc::mb_init_fence();
+            for (int i = 0; i < kCopies; i++) {
+                int a = i * per, b = min(n, a + per);
+                if (a < b && !whole(g0 + a)) a++;
+                if (a < b && !whole(g0 + b - 1)) b--;
+                const uint32_t bytes = a < b ? (uint32_t)(b - a) * 16 : 0;
+                tc::mb_expect_tx(&full[i], bytes);
+                if (bytes)
+                    asm volatile(
+                        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                            tc::su32(slice_smem + a)),
+                        "l"(x + ((g0 + a) * N - skew)), "r"(bytes), "r"(tc::su32(&full[i]))
+                        : "memory");
+            }
+        }
+        for (int e = threadIdx.x; e < 2 * N; e += THREADS) {
+            const int64_t g = e < N ? 0 : granules - 1, at = g * N + e % N - skew;
+            if (g >= g0 && g < g1 && !whole(g) && (e < N || granules > 1) && at >= 0 && at < A.vocab)
+                ((T *)(slice_smem + (g - g0)))[e % N] = x[at];
+        }
+    }
+
+    // the teacher's distribution
+    float um = -INFINITY;
+    bool bad = false;
+    if (want)
+        for (int k = threadIdx.x; k < A.top; k += THREADS) {
+            const int64_t i = load_index(A.indices, A.itype, row * A.ldi + k);
+            const bool in = i >= 0 && i < A.vocab;
+            bad |= !in && i != -1;
+            const float u = in ? load_f(A.teacher, A.ttype, row * A.ldt + k) * inv_t : -INFINITY;
+            si[k] = in ? (int)i : -1;
+            sp[k] = u;
+            um = max_nan(um, u);
+        }
+    um = warp_max_nan(um);
+    if (lane == 0) red[0][warp] = um;
+    bad = __syncthreads_or(bad);  // and the barriers are ready, the partial granules in place
+    um = warp_max_nan(red[0][lane % WARPS]);
+    const bool empty = um == -INFINITY && !bad;
+    const bool alone = !want || empty;  // nothing to learn from this row: alike in all its blocks
+    bool ok = true;
+    if (!alone) {
+        float us = 0.0f, ul = 0.0f;
+        for (int k = threadIdx.x; k < A.top; k += THREADS) {
+            const float d = sp[k] - um, e = expf(d);
+            sp[k] = e;
+            us += e;
+            if (e != 0.0f) ul += e * d;
+        }
+        us = warp_sum(us);
+        ul = warp_sum(ul);
+        if (lane == 0) {
+            red[1][warp] = us;
+            if (LOSS) sh.part[0][warp].x = ul;  // until the shares are exchanged
+        }
+        __syncthreads();
+        us = warp_sum(lane < WARPS ? red[1][lane] : 0.0f);
+        if (LOSS) ul = warp_sum(lane < WARPS ? sh.part[0][lane].x : 0.0f);
+        __syncthreads();
+        const float ur = 1.0f / us;
+        float lse = LOSS ? 0.0f : A.lse_in[row];
+        if constexpr (LOSS) {
+            if (size > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this block is there
+            // this warp's maximum, then its sum
+            float m = -INFINITY;
+            int landed = 0, copy = 0;
+            for (int g = threadIdx.x; g < n; g += THREADS) {
+                for (; g >= landed; landed += per, copy++)
+                    if (!tc::mb_wait(&full[copy], 0, &g_distill_error)) ok = false;
+                uint4 q = slice_smem[g];
+                if (!whole(g0 + g)) {
+                    const int64_t at = (g0 + g) * N - skew;
+                    q = keep_elements<T>(q, at < 0 ? (int)-at : 0, A.vocab - at < N ? (int)(A.vocab - at) : N);
+                    slice_smem[g] = q;
+                }
+                float f[N];
+                unpack<T>(q, f);
+#pragma unroll
+                for (int e = 0; e < N; e++) m = fmaxf(m, f[e]);
+            }
+            for (; copy < kCopies; copy++)
+                if (!tc::mb_wait(&full[copy], 0, &g_distill_error)) ok = false;
+            __syncwarp();
+#pragma unroll
+            for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            m = fmaxf(m * inv_t, -3.0e38f);  // a slice of -inf has a sum of 0
+            const Scale<T> sc(inv_t, m);
+            f32x2 s2 = make2(0.0f);
+            for (int g = threadIdx.x; g < n; g += THREADS) {
+                f32x2 f[N / 2];
+                unpack2<T>(slice_smem[g], f);
+#pragma unroll
+                for (int e = 0; e < N / 2; e++) {
+                    const f32x2 t = sc.arg(f[e]);
+                    s2 = add2(s2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t))));
+                }
+            }
+            __syncwarp();
+            const float s = warp_sum(lo2(s2) + hi2(s2));
+            __syncthreads();  // every copy has landed for every warp
+            float pz = 0.0f;
+            for (int k = threadIdx.x; k < A.top; k += THREADS) {
+                const int64_t g = si[k] < 0 ? -1 : ((int64_t)si[k] + skew) / N;
+                if (g >= g0 && g < g1 && sp[k] != 0.0f)
+                    pz += sp[k] * ur * (to_f(((const T *)slice_smem)[(int64_t)si[k] + skew - g0 * N]) * inv_t);
+            }
+            pz = warp_sum(pz);
+            if (lane == 0) red[0][warp] = pz;
+            __syncthreads();
+            pz = warp_sum(lane < WARPS ? red[0][lane] : 0.0f);
+            if (size > 1) {
+                asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others are there
+                if (lane < (int)size) {
+                    uint32_t there;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(tc::su32(&sh.part[rank][warp])), "r"(lane));
+                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(m), "f"(s) : "memory");
+                    if (warp == 0) {
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(tc::su32(&sh.pz[rank])), "r"(lane));
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(pz) : "memory");
+                    }
+                }
+                __syncwarp();
+                asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            } else {
+                if (lane == 0) {
+                    sh.part[0][warp] = make_float2(m, s);
+                    if (warp == 0) sh.pz[0] = pz;
+                }
+                __syncthreads();
+            }
+            float am = -INFINITY, as = 0.0f;
+            for (int i = lane; i < (int)size * WARPS; i += 32) am = fmaxf(am, sh.part[i / WARPS][i % WARPS].x);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, d));
+            for (int i = lane; i < (int)size * WARPS; i += 32) {
+                const float2 p = sh.part[i / WARPS][i % WARPS];
+                as += p.y * expf(p.x - am);
+            }
+            lse = am + logf(warp_sum(as));
+            if (rank == 0 && threadIdx.x == 0) {
+                float all = 0.0f;
+                for (uint32_t r = 0; r < size; r++) all += sh.pz[r];
+                // sum of p log p, less that of p z, plus lse
+                const float l = (ul * ur - logf(us)) - (all - lse);
+                A.loss[row] = bad || !ok ? NAN : w == 0.0f ? 0.0f : w * (A.T * A.T) * l;
+                if (A.lse_out) A.lse_out[row] = w == 0.0f ? 0.0f : lse;
+            }
+        } else {
+            for (int i = 0; i < kCopies; i++)
+                if (!tc::mb_wait(&full[i], 0, &g_distill_error)) ok = false;
+        }
+        if constexpr (GRAD) {
+            const Scale<T> sc(inv_t, lse);
+            const f32x2 c2 = make2(bad || !ok ? NAN : c);
+            const bool same = ((uintptr_t)o & 15) == ((uintptr_t)x & 15);
+            for (int g = threadIdx.x; g < n; g += THREADS) {
+                f32x2 f[N / 2];
+                unpack2<T>(slice_smem[g], f);
+#pragma unroll
+                for (int e = 0; e < N / 2; e++) {
+                    const f32x2 t = sc.arg(f[e]);
+                    f[e] = mul2(c2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t))));
+                }
+                if (!want_grad)
+#pragma unroll
+                    for (int e = 0; e < N / 2; e++) f[e] = make2(0.0f);
+                const uint4 q = pack2<T>(f);
+                const int64_t at = (g0 + g) * N - skew;
+                if (same && whole(g0 + g)) *(uint4 *)(o + at) = q;
+                else store_elements(o + at, q, at < 0 ? (int)-at : 0, A.vocab - at < N ? (int)(A.vocab - at) : N);
+            }
+            if (want_grad && !bad && ok) {
+                __syncthreads();  // the listed entries are written over
+                // an index that is listed again is written by its first entry
+                for (int k = threadIdx.x; k < A.top; k += THREADS) {
+                    const int i = si[k];
+                    const int64_t g = i < 0 ? -1 : ((int64_t)i + skew) / N;
+                    if (g < g0 || g >= g1) continue;
+                    float p = 0.0f;
+                    bool first = true;
+                    for (int j = 0; j < A.top; j++)
+                        if (si[j] == i) {
+                            if (j < k) first = false;
+                            p += sp[j];
+                        }
+                    if (!first) continue;
+                    const float z = to_f(((const T *)slice_smem)[(int64_t)i + skew - g0 * N]);
+                    o[i] = from_f<T>(c * (exp2_fast(lo2(sc.arg(make2(z)))) - p * ur));
+                }
+            }
+        }
+        if (!ok)  // give up only once the copies in flight have landed
+            for (int i = 0; i < kCopies; i++) tc::mb_wait(&full[i], 0, &g_distill_error);
+        return;
+    }
+    if (want)  // the copies are on their way: not before they have landed
+        for (int i = 0; i < kCopies; i++) tc::mb_wait(&full[i], 0, &g_distill_error);
+    if (GRAD) {
+        for (int64_t g = g0 + threadIdx.x; g < g1; g += THREADS) {
+            const int64_t at = g * N - skew;
+            if (whole(g) && ((uintptr_t)(o + at) & 15) == 0) *(uint4 *)(o + at) = make_uint4(0, 0, 0, 0);
+            else store_elements(o + at, make_uint4(0, 0, 0, 0), at < 0 ? (int)-at : 0, A.vocab - at < N ? (int)(A.vocab - at) : N);
+        }
+    }
+    if (LOSS && rank == 0 && threadIdx.x == 0) {
+        A.loss[row] = 0.0f;
+        if (A.lse_out) A.lse_out[row] = 0.0f;
+    }
+}
+
+// Rows that no cluster holds, read three times.
 template <typename T, bool LOSS, bool GRAD>
-__global__ void __launch_bounds__(NT) distill_kernel(const T *logits, int64_t ld, T *out, int64_t ldo, Args A) {
+__global__ void __launch_bounds__(NT) distill_long_kernel(const T *logits, int64_t ld, T *out, int64_t ldo, Args A) {
     __shared__ float sm[NT / 32];
     __shared__ float sp[kMaxTop], sz[kMaxTop];
     __shared__ int si[kMaxTop];
@@ -155,6 +469,48 @@ int check_args(const char *who, int dtype, const void *logits, int64_t ld, const
     return ZPUCUDA_OK;
 }
 
+template <typename T, bool LOSS, bool GRAD, int THREADS>
+int launch_cluster(const T *logits, int64_t ld, T *out, int64_t ldo, const Args &A, int64_t rows, int cluster, cudaStream_t s) {
+    auto f = distill_kernel<T, LOSS, GRAD, THREADS>;
+    static bool attr[64] = {false};
+    const int dev = current_device();
+    if (dev < 0 || dev >= 64 || !attr[dev]) {
+        ZC_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice));
+        if (dev >= 0 && dev < 64) attr[dev] = true;
+    }
+    const int64_t granules = (A.vocab * (int64_t)sizeof(T) + 15) / 16 + 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * cluster));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = (size_t)((granules + cluster - 1) / cluster) * 16;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    ZC_CUDA(cudaLaunchKernelEx(&cfg, f, logits, ld, out, ldo, A));
+    count_launch();
+    return ZPUCUDA_OK;
+}
+
+template <typename T, bool LOSS, bool GRAD>
+int launch_rows(const T *logits, int64_t ld, T *out, int64_t ldo, const Args &A, int64_t rows, cudaStream_t s) {
+    const int64_t bytes = A.vocab * (int64_t)sizeof(T) + 32;
+    // slices of 64 KiB at most while a cluster allows it; smaller ones, of 8 KiB at least, while blocks are few
+    int64_t cluster = 1;
+    while (cluster < kMaxCluster && (bytes > cluster * kSlice || (rows * cluster < 2 * (int64_t)num_sms() && bytes > cluster * 16384)))
+        cluster *= 2;
+    if (bytes > cluster * kMaxSlice || rows * cluster > 0x7fffffff) {
+        distill_long_kernel<T, LOSS, GRAD><<<(unsigned)rows, NT, 0, s>>>(logits, ld, out, ldo, A);
+        ZC_LAUNCHED("distill_long_kernel");
+        return ZPUCUDA_OK;
+    }
+    if (bytes <= cluster * 8192) return launch_cluster<T, LOSS, GRAD, 128>(logits, ld, out, ldo, A, rows, (int)cluster, s);
+    return launch_cluster<T, LOSS, GRAD, 512>(logits, ld, out, ldo, A, rows, (int)cluster, s);
+}
+
 template <bool LOSS, bool GRAD>
 int launch(const char *who, int dtype, const void *logits, int64_t ld, void *out, int64_t ldo, const Args &A,
            int64_t rows, void *stream) {
@@ -165,11 +521,7 @@ int launch(const char *who, int dtype, const void *logits, int64_t ld, void *out
         return head_error(ZPUCUDA_ERR_INVALID_ARGUMENT, who, "lse: null pointer");
     if (rows == 0) return ZPUCUDA_OK;
     cudaStream_t s = resolve_stream(stream);
-    ZC_HEAD_TYPE(dtype, T,
-                 (distill_kernel<T, LOSS, GRAD>
-                  <<<(unsigned)rows, NT, 0, s>>>((const T *)logits, ld, (T *)out, ldo, A)));
-    ZC_LAUNCHED("distill_kernel");
-    return ZPUCUDA_OK;
+    ZC_HEAD_TYPE(dtype, T, return (launch_rows<T, LOSS, GRAD>((const T *)logits, ld, (T *)out, ldo, A, rows, s)));
 }
 
 // top is checked here, before it is narrowed.

@@ -68,7 +68,7 @@
 #include <mutex>
 
 #include "gemm.cuh"
-#include "int8.cuh"
+#include "waits.cuh"
 #include "region.cuh"
 
 namespace zc {
@@ -1757,9 +1757,10 @@ extern "C" int zpucuda_check_device(void) {
     cudaError_t r = cudaMemcpyFromSymbol(&e, zc::g_gemm_error, sizeof e);
     if (r != cudaSuccess) return zc::cuda_fail(r, "cudaMemcpyFromSymbol(device error word)");
     if (!e) {
-        const int st = zc::int8_device_error(&e);
+        int st = zc::int8_device_error(&e);
+        if (!st && !e) st = zc::distill_device_error(&e);
         if (st) return st;
     }
-    if (e) return zc::set_error(ZPUCUDA_ERR_TIMEOUT, "a device-side bounded wait ran out in a GEMM kernel");
+    if (e) return zc::set_error(ZPUCUDA_ERR_TIMEOUT, "a device-side bounded wait ran out in a GEMM or distillation kernel");
     return ZPUCUDA_OK;
 }

@@ -7,8 +7,8 @@
 #include <string.h>
 
 #include "head.cuh"
-#include "int8.cuh"
 #include "tcgen05.cuh"
+#include "waits.cuh"
 
 namespace zc {
 
