@@ -33,7 +33,7 @@ namespace {
 constexpr int NT = 256;
 constexpr int kMaxTop = 1024;
 constexpr int kMaxCluster = 8;
-constexpr int kSlice = 64 * 1024, kMaxSlice = 200 * 1024;  // bytes: wanted, possible
+constexpr int kSlice = 66 * 1024, kMaxSlice = 200 * 1024;  // bytes: wanted (three blocks an SM), possible
 constexpr int kCopies = 4;                                 // of a slice, each waited for by itself
 
 struct Args {
@@ -45,6 +45,7 @@ struct Args {
     float T;
     int64_t vocab;
     int top;
+    int slice_bytes;  // of a block's shared memory
 };
 
 __device__ __forceinline__ int64_t load_index(const void *p, int it, int64_t i) {
@@ -91,6 +92,26 @@ __device__ __forceinline__ uint4 keep_elements(const uint4 &q, int from, int to)
     return pack<T>(f);  // exact: the values come from that type
 }
 
+// The larger of two granules' elements, NaN passed over.
+template <typename T>
+__device__ __forceinline__ uint4 max_elements(const uint4 &a, const uint4 &b) {
+    uint32_t x[4] = {a.x, a.y, a.z, a.w};
+    const uint32_t y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            x[i] = __float_as_uint(fmaxf(__uint_as_float(x[i]), __uint_as_float(y[i])));
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const __half2 m = __hmax2(*(const __half2 *)&x[i], *(const __half2 *)&y[i]);
+            x[i] = *(const uint32_t *)&m;
+        } else {
+            const __nv_bfloat162 m = __hmax2(*(const __nv_bfloat162 *)&x[i], *(const __nv_bfloat162 *)&y[i]);
+            x[i] = *(const uint32_t *)&m;
+        }
+    }
+    return make_uint4(x[0], x[1], x[2], x[3]);
+}
+
 // exp2 arguments of a granule relative to `ref`.  16-bit logits take one
 // multiply-add (k = log2(e) / T, its rounding is far below theirs); 32-bit ones
 // form z - ref first, so that the error stays relative to the distance.
@@ -122,58 +143,64 @@ struct Shares {
 };
 
 template <typename T, bool LOSS, bool GRAD, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 768 / THREADS)
     distill_kernel(const T *logits, int64_t ld, T *out, int64_t ldo, const Args A) {
     constexpr int N = kPiece<T>, WARPS = THREADS / 32;
     extern __shared__ __align__(128) uint4 slice_smem[];
     __shared__ uint64_t full[kCopies];
     __shared__ Shares<WARPS> sh;
-    __shared__ float red[2][WARPS];
-    __shared__ float sp[kMaxTop];
-    __shared__ int si[kMaxTop];
+    __shared__ float red[3][WARPS], lse_smem;
+    // behind the slice, for each listed entry: its probability, its logit, its place in the slice (-1: elsewhere)
+    float *sp = (float *)((uint8_t *)slice_smem + A.slice_bytes), *sz = sp + A.top;
+    int *si = (int *)(sz + A.top);
     uint32_t rank, size;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
     const int64_t row = blockIdx.x / size;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const T *x = logits + row * ld;
-    T *o = GRAD ? out + row * ldo : nullptr;
-    // the row's granules g: elements g * N - skew + e
-    const int skew = (int)(((uintptr_t)x & 15) / sizeof(T));
-    const int64_t granules = (skew + A.vocab + N - 1) / N;
-    const int64_t g0 = granules * rank / size, g1 = granules * (rank + 1) / size;
-    const int n = (int)(g1 - g0);
+    const T *xr = logits + row * ld;
+    // the row's granules: granule g holds elements g * N - skew + e; this block's are g0 .. g0 + n - 1, and element 0 of
+    // the slice is element `base` of the row
+    const int skew = (int)(((uintptr_t)xr & 15) / sizeof(T));
+    const int64_t granules = (skew + A.vocab + N - 1) / N, g0 = granules * rank / size;
+    const int n = (int)(granules * (rank + 1) / size - g0);
+    const int64_t base = g0 * N - skew;
+    const T *x = xr + base;
+    T *o = GRAD ? out + row * ldo + base : nullptr;
+    // the slice's elements that are in the row, and its granules that are whole
+    const int from = base < 0 ? skew : 0, to = A.vocab - base < (int64_t)n * N ? (int)(A.vocab - base) : n * N;
+    const int w0 = from > 0, w1 = to / N;
     const float inv_t = 1.0f / A.T;
 
     const float w = A.weight ? A.weight[row] : 1.0f;
     const float c = GRAD ? A.T * (w * (A.dloss ? A.dloss[row] : 1.0f)) : 0.0f;
     const bool want_loss = LOSS && w != 0.0f, want_grad = GRAD && c != 0.0f, want = want_loss || want_grad;
-    auto whole = [&](int64_t g) { return g * N >= skew && (g + 1) * N <= skew + A.vocab; };
 
-    // the slice's whole granules by bulk copies, the others element by element
+    // the whole granules by bulk copies, the others element by element
     const int per = (n + kCopies - 1) / kCopies;
     if (want) {
         if (threadIdx.x == 0) {
             for (int i = 0; i < kCopies; i++) tc::mb_init(&full[i], 1);
             tc::mb_init_fence();
             for (int i = 0; i < kCopies; i++) {
-                int a = i * per, b = min(n, a + per);
-                if (a < b && !whole(g0 + a)) a++;
-                if (a < b && !whole(g0 + b - 1)) b--;
+                const int a = max(i * per, w0), b = min(i * per + per, w1);
                 const uint32_t bytes = a < b ? (uint32_t)(b - a) * 16 : 0;
                 tc::mb_expect_tx(&full[i], bytes);
                 if (bytes)
                     asm volatile(
                         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                             tc::su32(slice_smem + a)),
-                        "l"(x + ((g0 + a) * N - skew)), "r"(bytes), "r"(tc::su32(&full[i]))
+                        "l"(x + (int64_t)a * N), "r"(bytes), "r"(tc::su32(&full[i]))
                         : "memory");
             }
         }
-        for (int e = threadIdx.x; e < 2 * N; e += THREADS) {
-            const int64_t g = e < N ? 0 : granules - 1, at = g * N + e % N - skew;
-            if (g >= g0 && g < g1 && !whole(g) && (e < N || granules > 1) && at >= 0 && at < A.vocab)
-                ((T *)(slice_smem + (g - g0)))[e % N] = x[at];
+        if (threadIdx.x < N && w0) {
+            const int e = threadIdx.x;
+            ((T *)slice_smem)[e] = e >= from && e < to ? x[e] : from_f<T>(-INFINITY);
+        }
+        if (threadIdx.x >= 32 && threadIdx.x < 32 + N && w1 < n && !(w0 && w1 == 0)) {
+            const int e = w1 * N + threadIdx.x - 32;
+            ((T *)slice_smem)[e] = e < to ? x[e] : from_f<T>(-INFINITY);
         }
     }
 
@@ -186,7 +213,7 @@ __global__ void __launch_bounds__(THREADS)
             const bool in = i >= 0 && i < A.vocab;
             bad |= !in && i != -1;
             const float u = in ? load_f(A.teacher, A.ttype, row * A.ldt + k) * inv_t : -INFINITY;
-            si[k] = in ? (int)i : -1;
+            si[k] = in && i >= base && i - base < (int64_t)n * N ? (int)(i - base) : -1;
             sp[k] = u;
             um = max_nan(um, u);
         }
@@ -194,10 +221,8 @@ __global__ void __launch_bounds__(THREADS)
     if (lane == 0) red[0][warp] = um;
     bad = __syncthreads_or(bad);  // and the barriers are ready, the partial granules in place
     um = warp_max_nan(red[0][lane % WARPS]);
-    const bool empty = um == -INFINITY && !bad;
-    const bool alone = !want || empty;  // nothing to learn from this row: alike in all its blocks
-    bool ok = true;
-    if (!alone) {
+    // with nothing to learn from the row (alike in all its blocks) what follows is left out
+    if (want && (um != -INFINITY || bad)) {
         float us = 0.0f, ul = 0.0f;
         for (int k = threadIdx.x; k < A.top; k += THREADS) {
             const float d = sp[k] - um, e = expf(d);
@@ -206,144 +231,162 @@ __global__ void __launch_bounds__(THREADS)
             if (e != 0.0f) ul += e * d;
         }
         us = warp_sum(us);
-        ul = warp_sum(ul);
+        if (LOSS) ul = warp_sum(ul);
         if (lane == 0) {
             red[1][warp] = us;
-            if (LOSS) sh.part[0][warp].x = ul;  // until the shares are exchanged
+            red[2][warp] = ul;
         }
-        __syncthreads();
-        us = warp_sum(lane < WARPS ? red[1][lane] : 0.0f);
-        if (LOSS) ul = warp_sum(lane < WARPS ? sh.part[0][lane].x : 0.0f);
-        __syncthreads();
+        bool ok = true;
+        uint4 mx = make_uint4(0, 0, 0, 0);
+        if (LOSS && size > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this block is there
+        int landed = 0, copy = 0;
+        bool any = false;
+        for (int g = threadIdx.x; g < n; g += THREADS) {
+            for (; g >= landed; landed += per, copy++)
+                if (!tc::mb_wait(&full[copy], 0, &g_distill_error)) ok = false;
+            if (!LOSS) break;
+            const uint4 q = slice_smem[g];
+            mx = any ? max_elements<T>(mx, q) : q;
+            any = true;
+        }
+        for (; copy < kCopies; copy++)
+            if (!tc::mb_wait(&full[copy], 0, &g_distill_error)) ok = false;
+        __syncthreads();  // every copy has landed for every thread; the teacher's sums are there
+        us = 0.0f;
+        for (int i = 0; i < WARPS; i++) us += red[1][i];
         const float ur = 1.0f / us;
+        // the listed entries in this slice
+        float pz = 0.0f;
+        for (int k = threadIdx.x; k < A.top; k += THREADS) {
+            sp[k] *= ur;
+            if (si[k] < 0) continue;
+            sz[k] = to_f(((const T *)slice_smem)[si[k]]);
+            if (LOSS && sp[k] != 0.0f) pz += sp[k] * (sz[k] * inv_t);
+        }
         float lse = LOSS ? 0.0f : A.lse_in[row];
         if constexpr (LOSS) {
-            if (size > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this block is there
-            // this warp's maximum, then its sum
-            float m = -INFINITY;
-            int landed = 0, copy = 0;
-            for (int g = threadIdx.x; g < n; g += THREADS) {
-                for (; g >= landed; landed += per, copy++)
-                    if (!tc::mb_wait(&full[copy], 0, &g_distill_error)) ok = false;
-                uint4 q = slice_smem[g];
-                if (!whole(g0 + g)) {
-                    const int64_t at = (g0 + g) * N - skew;
-                    q = keep_elements<T>(q, at < 0 ? (int)-at : 0, A.vocab - at < N ? (int)(A.vocab - at) : N);
-                    slice_smem[g] = q;
-                }
-                float f[N];
-                unpack<T>(q, f);
+            float f[N], m = -INFINITY;
+            unpack<T>(mx, f);
+            if (any)
 #pragma unroll
                 for (int e = 0; e < N; e++) m = fmaxf(m, f[e]);
-            }
-            for (; copy < kCopies; copy++)
-                if (!tc::mb_wait(&full[copy], 0, &g_distill_error)) ok = false;
-            __syncwarp();
 #pragma unroll
             for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
             m = fmaxf(m * inv_t, -3.0e38f);  // a slice of -inf has a sum of 0
             const Scale<T> sc(inv_t, m);
             f32x2 s2 = make2(0.0f);
             for (int g = threadIdx.x; g < n; g += THREADS) {
-                f32x2 f[N / 2];
-                unpack2<T>(slice_smem[g], f);
+                f32x2 v[N / 2];
+                unpack2<T>(slice_smem[g], v);
 #pragma unroll
                 for (int e = 0; e < N / 2; e++) {
-                    const f32x2 t = sc.arg(f[e]);
+                    const f32x2 t = sc.arg(v[e]);
                     s2 = add2(s2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t))));
                 }
             }
             __syncwarp();
             const float s = warp_sum(lo2(s2) + hi2(s2));
-            __syncthreads();  // every copy has landed for every warp
-            float pz = 0.0f;
-            for (int k = threadIdx.x; k < A.top; k += THREADS) {
-                const int64_t g = si[k] < 0 ? -1 : ((int64_t)si[k] + skew) / N;
-                if (g >= g0 && g < g1 && sp[k] != 0.0f)
-                    pz += sp[k] * ur * (to_f(((const T *)slice_smem)[(int64_t)si[k] + skew - g0 * N]) * inv_t);
-            }
             pz = warp_sum(pz);
             if (lane == 0) red[0][warp] = pz;
-            __syncthreads();
-            pz = warp_sum(lane < WARPS ? red[0][lane] : 0.0f);
             if (size > 1) {
                 asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others are there
                 if (lane < (int)size) {
                     uint32_t there;
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(tc::su32(&sh.part[rank][warp])), "r"(lane));
                     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(m), "f"(s) : "memory");
-                    if (warp == 0) {
-                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(tc::su32(&sh.pz[rank])), "r"(lane));
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(pz) : "memory");
-                    }
+                }
+                __syncthreads();  // red
+                if (warp == 0 && lane < (int)size) {
+                    pz = 0.0f;
+                    for (int i = 0; i < WARPS; i++) pz += red[0][i];
+                    uint32_t there;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(tc::su32(&sh.pz[rank])), "r"(lane));
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(pz) : "memory");
                 }
                 __syncwarp();
                 asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
             } else {
-                if (lane == 0) {
-                    sh.part[0][warp] = make_float2(m, s);
-                    if (warp == 0) sh.pz[0] = pz;
-                }
+                if (lane == 0) sh.part[0][warp] = make_float2(m, s);
                 __syncthreads();
+                if (threadIdx.x == 0) {
+                    pz = 0.0f;
+                    for (int i = 0; i < WARPS; i++) pz += red[0][i];
+                    sh.pz[0] = pz;
+                }
             }
-            float am = -INFINITY, as = 0.0f;
-            for (int i = lane; i < (int)size * WARPS; i += 32) am = fmaxf(am, sh.part[i / WARPS][i % WARPS].x);
+            if (warp == 0) {  // the row's normaliser and loss
+                __syncwarp();
+                float am = -INFINITY, as = 0.0f;
+                for (int i = lane; i < (int)size * WARPS; i += 32) am = fmaxf(am, sh.part[i / WARPS][i % WARPS].x);
 #pragma unroll
-            for (int d = 16; d; d >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, d));
-            for (int i = lane; i < (int)size * WARPS; i += 32) {
-                const float2 p = sh.part[i / WARPS][i % WARPS];
-                as += p.y * expf(p.x - am);
+                for (int d = 16; d; d >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, d));
+                for (int i = lane; i < (int)size * WARPS; i += 32) {
+                    const float2 p = sh.part[i / WARPS][i % WARPS];
+                    as += p.y * expf(p.x - am);
+                }
+                lse = am + logf(warp_sum(as));
+                if (lane == 0) {
+                    lse_smem = lse;
+                    if (rank == 0) {
+                        float all = 0.0f;
+                        ul = 0.0f;
+                        for (uint32_t r = 0; r < size; r++) all += sh.pz[r];
+                        for (int i = 0; i < WARPS; i++) ul += red[2][i];
+                        // sum of p log p, less that of p z, plus lse
+                        const float l = (ul * ur - logf(us)) - (all - lse);
+                        A.loss[row] = bad || !ok ? NAN : w == 0.0f ? 0.0f : w * (A.T * A.T) * l;
+                        if (A.lse_out) A.lse_out[row] = w == 0.0f ? 0.0f : lse;
+                    }
+                }
             }
-            lse = am + logf(warp_sum(as));
-            if (rank == 0 && threadIdx.x == 0) {
-                float all = 0.0f;
-                for (uint32_t r = 0; r < size; r++) all += sh.pz[r];
-                // sum of p log p, less that of p z, plus lse
-                const float l = (ul * ur - logf(us)) - (all - lse);
-                A.loss[row] = bad || !ok ? NAN : w == 0.0f ? 0.0f : w * (A.T * A.T) * l;
-                if (A.lse_out) A.lse_out[row] = w == 0.0f ? 0.0f : lse;
+            if (GRAD) {
+                __syncthreads();
+                lse = lse_smem;
             }
-        } else {
-            for (int i = 0; i < kCopies; i++)
-                if (!tc::mb_wait(&full[i], 0, &g_distill_error)) ok = false;
         }
         if constexpr (GRAD) {
             const Scale<T> sc(inv_t, lse);
             const f32x2 c2 = make2(bad || !ok ? NAN : c);
-            const bool same = ((uintptr_t)o & 15) == ((uintptr_t)x & 15);
+            const bool same = ((uintptr_t)o & 15) == 0;  // x is on a granule: o, too?
             for (int g = threadIdx.x; g < n; g += THREADS) {
                 f32x2 f[N / 2];
                 unpack2<T>(slice_smem[g], f);
 #pragma unroll
                 for (int e = 0; e < N / 2; e++) {
                     const f32x2 t = sc.arg(f[e]);
-                    f[e] = mul2(c2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t))));
+                    f[e] = want_grad ? mul2(c2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t)))) : make2(0.0f);
                 }
-                if (!want_grad)
-#pragma unroll
-                    for (int e = 0; e < N / 2; e++) f[e] = make2(0.0f);
                 const uint4 q = pack2<T>(f);
-                const int64_t at = (g0 + g) * N - skew;
-                if (same && whole(g0 + g)) *(uint4 *)(o + at) = q;
-                else store_elements(o + at, q, at < 0 ? (int)-at : 0, A.vocab - at < N ? (int)(A.vocab - at) : N);
+                if (same && g >= w0 && g < w1) *(uint4 *)(o + g * N) = q;
+                else store_elements(o + g * N, q, max(from - g * N, 0), min(to - g * N, N));
             }
             if (want_grad && !bad && ok) {
-                __syncthreads();  // the listed entries are written over
-                // an index that is listed again is written by its first entry
+                // The listed entries are written over, an index that is listed again by one of its entries: each
+                // leaves its number in the logit's place, and is alone if it finds it there.
+                __syncthreads();
+                using Mark = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+                Mark *mark = (Mark *)slice_smem;
+                for (int k = threadIdx.x; k < A.top; k += THREADS)
+                    if (si[k] >= 0) mark[si[k]] = (Mark)k;
+                __syncthreads();
+                bool again = false;
+                for (int k = threadIdx.x; k < A.top; k += THREADS) again |= si[k] >= 0 && mark[si[k]] != (Mark)k;
+                again = __syncthreads_or(again);
                 for (int k = threadIdx.x; k < A.top; k += THREADS) {
                     const int i = si[k];
-                    const int64_t g = i < 0 ? -1 : ((int64_t)i + skew) / N;
-                    if (g < g0 || g >= g1) continue;
-                    float p = 0.0f;
-                    bool first = true;
-                    for (int j = 0; j < A.top; j++)
-                        if (si[j] == i) {
-                            if (j < k) first = false;
-                            p += sp[j];
-                        }
-                    if (!first) continue;
-                    const float z = to_f(((const T *)slice_smem)[(int64_t)i + skew - g0 * N]);
-                    o[i] = from_f<T>(c * (exp2_fast(lo2(sc.arg(make2(z)))) - p * ur));
+                    if (i < 0) continue;
+                    float p = sp[k];
+                    if (again) {  // in the entries' order; the first one writes
+                        bool first = true;
+                        p = 0.0f;
+                        for (int j = 0; j < A.top; j++)
+                            if (si[j] == i) {
+                                first &= j >= k;
+                                p += sp[j];
+                            }
+                        if (!first) continue;
+                    }
+                    o[i] = from_f<T>(c * (exp2_fast(lo2(sc.arg(make2(sz[k])))) - p));
                 }
             }
         }
@@ -353,13 +396,11 @@ __global__ void __launch_bounds__(THREADS)
     }
     if (want)  // the copies are on their way: not before they have landed
         for (int i = 0; i < kCopies; i++) tc::mb_wait(&full[i], 0, &g_distill_error);
-    if (GRAD) {
-        for (int64_t g = g0 + threadIdx.x; g < g1; g += THREADS) {
-            const int64_t at = g * N - skew;
-            if (whole(g) && ((uintptr_t)(o + at) & 15) == 0) *(uint4 *)(o + at) = make_uint4(0, 0, 0, 0);
-            else store_elements(o + at, make_uint4(0, 0, 0, 0), at < 0 ? (int)-at : 0, A.vocab - at < N ? (int)(A.vocab - at) : N);
+    if (GRAD)
+        for (int g = threadIdx.x; g < n; g += THREADS) {
+            if (((uintptr_t)o & 15) == 0 && g >= w0 && g < w1) *(uint4 *)(o + g * N) = make_uint4(0, 0, 0, 0);
+            else store_elements(o + g * N, make_uint4(0, 0, 0, 0), max(from - g * N, 0), min(to - g * N, N));
         }
-    }
     if (LOSS && rank == 0 && threadIdx.x == 0) {
         A.loss[row] = 0.0f;
         if (A.lse_out) A.lse_out[row] = 0.0f;
@@ -470,19 +511,20 @@ int check_args(const char *who, int dtype, const void *logits, int64_t ld, const
 }
 
 template <typename T, bool LOSS, bool GRAD, int THREADS>
-int launch_cluster(const T *logits, int64_t ld, T *out, int64_t ldo, const Args &A, int64_t rows, int cluster, cudaStream_t s) {
+int launch_cluster(const T *logits, int64_t ld, T *out, int64_t ldo, Args A, int64_t rows, int cluster, cudaStream_t s) {
     auto f = distill_kernel<T, LOSS, GRAD, THREADS>;
     static bool attr[64] = {false};
     const int dev = current_device();
     if (dev < 0 || dev >= 64 || !attr[dev]) {
-        ZC_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice));
+        ZC_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice + 16 + 12 * kMaxTop));
         if (dev >= 0 && dev < 64) attr[dev] = true;
     }
     const int64_t granules = (A.vocab * (int64_t)sizeof(T) + 15) / 16 + 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * cluster));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = (size_t)((granules + cluster - 1) / cluster) * 16;
+    A.slice_bytes = (int)((granules + cluster - 1) / cluster) * 16;
+    cfg.dynamicSmemBytes = (size_t)A.slice_bytes + 12 * (size_t)A.top;
     cfg.stream = s;
     cudaLaunchAttribute at[1] = {};
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -508,7 +550,7 @@ int launch_rows(const T *logits, int64_t ld, T *out, int64_t ldo, const Args &A,
         return ZPUCUDA_OK;
     }
     if (bytes <= cluster * 8192) return launch_cluster<T, LOSS, GRAD, 128>(logits, ld, out, ldo, A, rows, (int)cluster, s);
-    return launch_cluster<T, LOSS, GRAD, 512>(logits, ld, out, ldo, A, rows, (int)cluster, s);
+    return launch_cluster<T, LOSS, GRAD, 256>(logits, ld, out, ldo, A, rows, (int)cluster, s);
 }
 
 template <bool LOSS, bool GRAD>
