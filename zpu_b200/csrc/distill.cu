@@ -45,6 +45,7 @@ struct Args {
     float T;
     int64_t vocab;
     int top;
+    int64_t rows;
     int slice_bytes;  // of a block's shared memory
 };
 
@@ -79,17 +80,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
-}
-
-// The elements of a granule outside [from, to) replaced by -inf.
-template <typename T>
-__device__ __forceinline__ uint4 keep_elements(const uint4 &q, int from, int to) {
-    float f[kPiece<T>];
-    unpack<T>(q, f);
-#pragma unroll
-    for (int e = 0; e < kPiece<T>; e++)
-        if (e < from || e >= to) f[e] = -INFINITY;
-    return pack<T>(f);  // exact: the values come from that type
 }
 
 // The larger of two granules' elements, NaN passed over.
@@ -135,53 +125,64 @@ struct Scale {
     }
 };
 
-// What the blocks of a row tell one another.
-template <int WARPS>
-struct Shares {
-    float2 part[kMaxCluster][WARPS];  // each warp's maximum of z and its sum of e^(z - maximum)
-    float pz[kMaxCluster];            // each block's sum of p z over the listed entries in its slice
-};
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
 
+// The first waits of a block must not be the last: several blocks share an SM,
+// and what one waits for another's arithmetic hides, but each byte of shared
+// memory is held from its copy to its gradient, so HBM's bandwidth needs a short
+// way from one to the other.  Hence: the listed entries are fetched while the
+// copies are on their way, every warp works out the teacher's sums for itself, and
+// the warps of a row's blocks exchange their maxima and sums directly, by stores
+// to one another's shared memory and one arrival, without a barrier of all.
 template <typename T, bool LOSS, bool GRAD, int THREADS>
 __global__ void __launch_bounds__(THREADS, 768 / THREADS)
     distill_kernel(const T *logits, int64_t ld, T *out, int64_t ldo, const Args A) {
-    constexpr int N = kPiece<T>, WARPS = THREADS / 32;
+    constexpr int N = kPiece<T>, WARPS = THREADS / 32, MARKS = 2048;
     extern __shared__ __align__(128) uint4 slice_smem[];
-    __shared__ uint64_t full[kCopies];
-    __shared__ Shares<WARPS> sh;
-    __shared__ float red[3][WARPS], lse_smem;
+    __shared__ uint64_t full[kCopies], told;
+    __shared__ float4 part[kMaxCluster * WARPS];  // each warp's maximum of z, sum of e^(z - maximum), sum of p z
+    __shared__ uint16_t mark[MARKS];              // an entry's number, by its place: to find indices listed twice
+    __shared__ int again;
     // behind the slice, for each listed entry: its probability, its logit, its place in the slice (-1: elsewhere)
     float *sp = (float *)((uint8_t *)slice_smem + A.slice_bytes), *sz = sp + A.top;
     int *si = (int *)(sz + A.top);
     uint32_t rank, size;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
-    const int64_t row = blockIdx.x / size;
+    const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+    if (row >= A.rows) return;  // the whole cluster
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float w = A.weight ? A.weight[row] : 1.0f, dl = GRAD && A.dloss ? A.dloss[row] : 1.0f;
     const T *xr = logits + row * ld;
     // the row's granules: granule g holds elements g * N - skew + e; this block's are g0 .. g0 + n - 1, and element 0 of
     // the slice is element `base` of the row
     const int skew = (int)(((uintptr_t)xr & 15) / sizeof(T));
-    const int64_t granules = (skew + A.vocab + N - 1) / N, g0 = granules * rank / size;
-    const int n = (int)(granules * (rank + 1) / size - g0);
+    const int64_t granules = (skew + A.vocab + N - 1) / N, g0 = (int64_t)rank * (A.slice_bytes / 16);
+    const int n = (int)max((int64_t)0, min((int64_t)(A.slice_bytes / 16), granules - g0));
     const int64_t base = g0 * N - skew;
     const T *x = xr + base;
     T *o = GRAD ? out + row * ldo + base : nullptr;
     // the slice's elements that are in the row, and its granules that are whole
-    const int from = base < 0 ? skew : 0, to = A.vocab - base < (int64_t)n * N ? (int)(A.vocab - base) : n * N;
+    const int from = base < 0 ? skew : 0, to = (int)max((int64_t)0, min((int64_t)n * N, A.vocab - base));
     const int w0 = from > 0, w1 = to / N;
     const float inv_t = 1.0f / A.T;
-
-    const float w = A.weight ? A.weight[row] : 1.0f;
-    const float c = GRAD ? A.T * (w * (A.dloss ? A.dloss[row] : 1.0f)) : 0.0f;
+    const int per = (n + kCopies - 1) / kCopies;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kCopies; i++) tc::mb_init(&full[i], 1);
+        tc::mb_init(&told, size * WARPS);
+        tc::mb_init_fence();
+        again = 0;
+    }
+    const float c = GRAD ? A.T * (w * dl) : 0.0f;
     const bool want_loss = LOSS && w != 0.0f, want_grad = GRAD && c != 0.0f, want = want_loss || want_grad;
 
     // the whole granules by bulk copies, the others element by element
-    const int per = (n + kCopies - 1) / kCopies;
     if (want) {
-        if (threadIdx.x == 0) {
-            for (int i = 0; i < kCopies; i++) tc::mb_init(&full[i], 1);
-            tc::mb_init_fence();
+        if (threadIdx.x == 0)
             for (int i = 0; i < kCopies; i++) {
                 const int a = max(i * per, w0), b = min(i * per + per, w1);
                 const uint32_t bytes = a < b ? (uint32_t)(b - a) * 16 : 0;
@@ -193,7 +194,6 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS)
                         "l"(x + (int64_t)a * N), "r"(bytes), "r"(tc::su32(&full[i]))
                         : "memory");
             }
-        }
         if (threadIdx.x < N && w0) {
             const int e = threadIdx.x;
             ((T *)slice_smem)[e] = e >= from && e < to ? x[e] : from_f<T>(-INFINITY);
@@ -203,190 +203,166 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS)
             ((T *)slice_smem)[e] = e < to ? x[e] : from_f<T>(-INFINITY);
         }
     }
-
-    // the teacher's distribution
-    float um = -INFINITY;
+    // the listed entries
     bool bad = false;
     if (want)
         for (int k = threadIdx.x; k < A.top; k += THREADS) {
             const int64_t i = load_index(A.indices, A.itype, row * A.ldi + k);
+            const float u = load_f(A.teacher, A.ttype, row * A.ldt + k) * inv_t;
             const bool in = i >= 0 && i < A.vocab;
             bad |= !in && i != -1;
-            const float u = in ? load_f(A.teacher, A.ttype, row * A.ldt + k) * inv_t : -INFINITY;
-            si[k] = in && i >= base && i - base < (int64_t)n * N ? (int)(i - base) : -1;
-            sp[k] = u;
-            um = max_nan(um, u);
+            si[k] = in && i >= base && i - base < to ? (int)(i - base) : -1;
+            sp[k] = in ? u : -INFINITY;
         }
+    bad = __syncthreads_or(bad);  // the entries, the barriers and the partial granules are in place
+    float um = -INFINITY, us = 0.0f, ul = 0.0f;
+    if (want)
+        for (int k = lane; k < A.top; k += 32) um = max_nan(um, sp[k]);
     um = warp_max_nan(um);
-    if (lane == 0) red[0][warp] = um;
-    bad = __syncthreads_or(bad);  // and the barriers are ready, the partial granules in place
-    um = warp_max_nan(red[0][lane % WARPS]);
     // with nothing to learn from the row (alike in all its blocks) what follows is left out
     if (want && (um != -INFINITY || bad)) {
-        float us = 0.0f, ul = 0.0f;
-        for (int k = threadIdx.x; k < A.top; k += THREADS) {
+        if (LOSS && size > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // `told` is ready
+        for (int k = lane; k < A.top; k += 32) {
             const float d = sp[k] - um, e = expf(d);
-            sp[k] = e;
             us += e;
             if (e != 0.0f) ul += e * d;
         }
         us = warp_sum(us);
         if (LOSS) ul = warp_sum(ul);
-        if (lane == 0) {
-            red[1][warp] = us;
-            red[2][warp] = ul;
-        }
-        bool ok = true;
+        const float ur = 1.0f / us;
+        bool ok = true, any = false;
         uint4 mx = make_uint4(0, 0, 0, 0);
-        if (LOSS && size > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this block is there
         int landed = 0, copy = 0;
-        bool any = false;
-        for (int g = threadIdx.x; g < n; g += THREADS) {
-            for (; g >= landed; landed += per, copy++)
-                if (!tc::mb_wait(&full[copy], 0, &g_distill_error)) ok = false;
-            if (!LOSS) break;
-            const uint4 q = slice_smem[g];
-            mx = any ? max_elements<T>(mx, q) : q;
-            any = true;
-        }
+        if (LOSS)
+            for (int g = threadIdx.x; g < n; g += THREADS) {
+                for (; g >= landed; landed += per, copy++)
+                    if (!tc::mb_wait(&full[copy], 0, &g_distill_error)) ok = false;
+                const uint4 q = slice_smem[g];
+                mx = any ? max_elements<T>(mx, q) : q;
+                any = true;
+            }
         for (; copy < kCopies; copy++)
             if (!tc::mb_wait(&full[copy], 0, &g_distill_error)) ok = false;
-        __syncthreads();  // every copy has landed for every thread; the teacher's sums are there
-        us = 0.0f;
-        for (int i = 0; i < WARPS; i++) us += red[1][i];
-        const float ur = 1.0f / us;
-        // the listed entries in this slice
-        float pz = 0.0f;
-        for (int k = threadIdx.x; k < A.top; k += THREADS) {
-            sp[k] *= ur;
-            if (si[k] < 0) continue;
-            sz[k] = to_f(((const T *)slice_smem)[si[k]]);
-            if (LOSS && sp[k] != 0.0f) pz += sp[k] * (sz[k] * inv_t);
-        }
+        __syncwarp();
         float lse = LOSS ? 0.0f : A.lse_in[row];
+        float4 mine;
         if constexpr (LOSS) {
             float f[N], m = -INFINITY;
             unpack<T>(mx, f);
             if (any)
 #pragma unroll
                 for (int e = 0; e < N; e++) m = fmaxf(m, f[e]);
-#pragma unroll
-            for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            m = fmaxf(m * inv_t, -3.0e38f);  // a slice of -inf has a sum of 0
-            const Scale<T> sc(inv_t, m);
-            f32x2 s2 = make2(0.0f);
+            mine.x = fmaxf(warp_max(m) * inv_t, -3.0e38f);  // a slice of -inf has a sum of 0
+            const Scale<T> sc(inv_t, mine.x);
+            f32x2 s2 = make2(0.0f), s3 = s2;
+#pragma unroll 4
             for (int g = threadIdx.x; g < n; g += THREADS) {
                 f32x2 v[N / 2];
                 unpack2<T>(slice_smem[g], v);
 #pragma unroll
                 for (int e = 0; e < N / 2; e++) {
-                    const f32x2 t = sc.arg(v[e]);
-                    s2 = add2(s2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t))));
+                    const f32x2 t = sc.arg(v[e]), q = make2(exp2_fast(lo2(t)), exp2_fast(hi2(t)));
+                    if (e & 1) s3 = add2(s3, q);
+                    else s2 = add2(s2, q);
                 }
             }
             __syncwarp();
-            const float s = warp_sum(lo2(s2) + hi2(s2));
-            pz = warp_sum(pz);
-            if (lane == 0) red[0][warp] = pz;
-            if (size > 1) {
-                asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others are there
-                if (lane < (int)size) {
-                    uint32_t there;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(tc::su32(&sh.part[rank][warp])), "r"(lane));
-                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(m), "f"(s) : "memory");
-                }
-                __syncthreads();  // red
-                if (warp == 0 && lane < (int)size) {
-                    pz = 0.0f;
-                    for (int i = 0; i < WARPS; i++) pz += red[0][i];
-                    uint32_t there;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(tc::su32(&sh.pz[rank])), "r"(lane));
-                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(pz) : "memory");
-                }
-                __syncwarp();
-                asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-            } else {
-                if (lane == 0) sh.part[0][warp] = make_float2(m, s);
-                __syncthreads();
-                if (threadIdx.x == 0) {
-                    pz = 0.0f;
-                    for (int i = 0; i < WARPS; i++) pz += red[0][i];
-                    sh.pz[0] = pz;
-                }
+            s2 = add2(s2, s3);
+            mine.y = warp_sum(lo2(s2) + hi2(s2));
+        }
+        // the listed entries in this slice
+        float pz = 0.0f;
+        for (int k = threadIdx.x; k < A.top; k += THREADS) {
+            if (si[k] < 0) continue;
+            const float p = expf(sp[k] - um) * ur, z = to_f(((const T *)slice_smem)[si[k]]);
+            sz[k] = z;
+            if (LOSS && p != 0.0f) pz += p * (z * inv_t);
+            if (GRAD) mark[si[k] % MARKS] = (uint16_t)k;
+        }
+        if constexpr (LOSS) {
+            mine.z = warp_sum(pz);
+            mine.w = 0.0f;
+            if (size > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // of all blocks
+            __syncwarp();
+            if (lane < (int)size) {
+                uint32_t there, bar;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(tc::su32(&part[rank * WARPS + warp])), "r"(lane));
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(tc::su32(&told)), "r"(lane));
+                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(mine.x), "f"(mine.y), "f"(mine.z),
+                             "f"(mine.w)
+                             : "memory");
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
             }
-            if (warp == 0) {  // the row's normaliser and loss
-                __syncwarp();
-                float am = -INFINITY, as = 0.0f;
-                for (int i = lane; i < (int)size * WARPS; i += 32) am = fmaxf(am, sh.part[i / WARPS][i % WARPS].x);
-#pragma unroll
-                for (int d = 16; d; d >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, d));
-                for (int i = lane; i < (int)size * WARPS; i += 32) {
-                    const float2 p = sh.part[i / WARPS][i % WARPS];
-                    as += p.y * expf(p.x - am);
-                }
-                lse = am + logf(warp_sum(as));
+            if (!tc::mb_wait_cluster(&told, 0, &g_distill_error)) ok = false;
+            __syncwarp();
+            float am = -INFINITY, as = 0.0f, az = 0.0f;
+            for (int i = lane; i < (int)size * WARPS; i += 32) am = fmaxf(am, part[i].x);
+            am = warp_max(am);
+            for (int i = lane; i < (int)size * WARPS; i += 32) {
+                const float4 q = part[i];
+                as += q.y * expf(q.x - am);
+                az += q.z;
+            }
+            lse = am + logf(warp_sum(as));
+            if (rank == 0 && warp == 0) {
+                az = warp_sum(az);
                 if (lane == 0) {
-                    lse_smem = lse;
-                    if (rank == 0) {
-                        float all = 0.0f;
-                        ul = 0.0f;
-                        for (uint32_t r = 0; r < size; r++) all += sh.pz[r];
-                        for (int i = 0; i < WARPS; i++) ul += red[2][i];
-                        // sum of p log p, less that of p z, plus lse
-                        const float l = (ul * ur - logf(us)) - (all - lse);
-                        A.loss[row] = bad || !ok ? NAN : w == 0.0f ? 0.0f : w * (A.T * A.T) * l;
-                        if (A.lse_out) A.lse_out[row] = w == 0.0f ? 0.0f : lse;
-                    }
+                    // sum of p log p, less that of p z, plus lse
+                    const float l = (ul * ur - logf(us)) - (az - lse);
+                    A.loss[row] = bad || !ok ? NAN : w == 0.0f ? 0.0f : w * (A.T * A.T) * l;
+                    if (A.lse_out) A.lse_out[row] = w == 0.0f ? 0.0f : lse;
                 }
             }
-            if (GRAD) {
-                __syncthreads();
-                lse = lse_smem;
-            }
+        } else {
+            __syncthreads();  // the marks
         }
         if constexpr (GRAD) {
             const Scale<T> sc(inv_t, lse);
             const f32x2 c2 = make2(bad || !ok ? NAN : c);
             const bool same = ((uintptr_t)o & 15) == 0;  // x is on a granule: o, too?
-            for (int g = threadIdx.x; g < n; g += THREADS) {
-                f32x2 f[N / 2];
-                unpack2<T>(slice_smem[g], f);
+            if (want_grad && same) {
+#pragma unroll 2
+                for (int g = threadIdx.x; g < n; g += THREADS) {
+                    f32x2 f[N / 2];
+                    unpack2<T>(slice_smem[g], f);
 #pragma unroll
-                for (int e = 0; e < N / 2; e++) {
-                    const f32x2 t = sc.arg(f[e]);
-                    f[e] = want_grad ? mul2(c2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t)))) : make2(0.0f);
+                    for (int e = 0; e < N / 2; e++) {
+                        const f32x2 t = sc.arg(f[e]);
+                        f[e] = mul2(c2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t))));
+                    }
+                    const uint4 q = pack2<T>(f);
+                    if (g >= w0 && g < w1) *(uint4 *)(o + g * N) = q;
+                    else store_elements(o + g * N, q, max(from - g * N, 0), min(to - g * N, N));
                 }
-                const uint4 q = pack2<T>(f);
-                if (same && g >= w0 && g < w1) *(uint4 *)(o + g * N) = q;
-                else store_elements(o + g * N, q, max(from - g * N, 0), min(to - g * N, N));
+            } else {
+                for (int g = threadIdx.x; g < n; g += THREADS) {
+                    f32x2 f[N / 2];
+                    unpack2<T>(slice_smem[g], f);
+#pragma unroll
+                    for (int e = 0; e < N / 2; e++) {
+                        const f32x2 t = sc.arg(f[e]);
+                        f[e] = want_grad ? mul2(c2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t)))) : make2(0.0f);
+                    }
+                    store_elements(o + g * N, pack2<T>(f), max(from - g * N, 0), min(to - g * N, N));
+                }
             }
-            if (want_grad && !bad && ok) {
-                // The listed entries are written over, an index that is listed again by one of its entries: each
-                // leaves its number in the logit's place, and is alone if it finds it there.
-                __syncthreads();
-                using Mark = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
-                Mark *mark = (Mark *)slice_smem;
+            if (want_grad && !bad) {
+                // The listed entries are written over, an index that is listed again by its first entry.
                 for (int k = threadIdx.x; k < A.top; k += THREADS)
-                    if (si[k] >= 0) mark[si[k]] = (Mark)k;
+                    if (si[k] >= 0 && mark[si[k] % MARKS] != (uint16_t)k) again = 1;
                 __syncthreads();
-                bool again = false;
-                for (int k = threadIdx.x; k < A.top; k += THREADS) again |= si[k] >= 0 && mark[si[k]] != (Mark)k;
-                again = __syncthreads_or(again);
+                const bool twice = again;  // perhaps: two places may share a mark
                 for (int k = threadIdx.x; k < A.top; k += THREADS) {
                     const int i = si[k];
                     if (i < 0) continue;
-                    float p = sp[k];
-                    if (again) {  // in the entries' order; the first one writes
-                        bool first = true;
-                        p = 0.0f;
-                        for (int j = 0; j < A.top; j++)
-                            if (si[j] == i) {
-                                first &= j >= k;
-                                p += sp[j];
-                            }
-                        if (!first) continue;
-                    }
-                    o[i] = from_f<T>(c * (exp2_fast(lo2(sc.arg(make2(sz[k])))) - p));
+                    float p = 0.0f;
+                    bool first = true;
+                    for (int j = twice ? 0 : k; j < (twice ? A.top : k + 1); j++)  // in the entries' order
+                        if (si[j] == i) {
+                            first &= j >= k;
+                            p += expf(sp[j] - um) * ur;
+                        }
+                    if (first) o[i] = from_f<T>(ok ? c * (exp2_fast(lo2(sc.arg(make2(sz[k])))) - p) : NAN);
                 }
             }
         }
@@ -511,7 +487,7 @@ int check_args(const char *who, int dtype, const void *logits, int64_t ld, const
 }
 
 template <typename T, bool LOSS, bool GRAD, int THREADS>
-int launch_cluster(const T *logits, int64_t ld, T *out, int64_t ldo, Args A, int64_t rows, int cluster, cudaStream_t s) {
+int launch_cluster(const T *logits, int64_t ld, T *out, int64_t ldo, const Args &A, int cluster, cudaStream_t s) {
     auto f = distill_kernel<T, LOSS, GRAD, THREADS>;
     static bool attr[64] = {false};
     const int dev = current_device();
@@ -519,11 +495,10 @@ int launch_cluster(const T *logits, int64_t ld, T *out, int64_t ldo, Args A, int
         ZC_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice + 16 + 12 * kMaxTop));
         if (dev >= 0 && dev < 64) attr[dev] = true;
     }
-    const int64_t granules = (A.vocab * (int64_t)sizeof(T) + 15) / 16 + 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * cluster));
+    const int64_t y = A.rows < 32768 ? A.rows : 32768;
+    cfg.gridDim = dim3((unsigned)cluster, (unsigned)y, (unsigned)((A.rows + y - 1) / y));
     cfg.blockDim = dim3(THREADS);
-    A.slice_bytes = (int)((granules + cluster - 1) / cluster) * 16;
     cfg.dynamicSmemBytes = (size_t)A.slice_bytes + 12 * (size_t)A.top;
     cfg.stream = s;
     cudaLaunchAttribute at[1] = {};
@@ -538,19 +513,22 @@ int launch_cluster(const T *logits, int64_t ld, T *out, int64_t ldo, Args A, int
 }
 
 template <typename T, bool LOSS, bool GRAD>
-int launch_rows(const T *logits, int64_t ld, T *out, int64_t ldo, const Args &A, int64_t rows, cudaStream_t s) {
-    const int64_t bytes = A.vocab * (int64_t)sizeof(T) + 32;
-    // slices of 64 KiB at most while a cluster allows it; smaller ones, of 8 KiB at least, while blocks are few
-    int64_t cluster = 1;
-    while (cluster < kMaxCluster && (bytes > cluster * kSlice || (rows * cluster < 2 * (int64_t)num_sms() && bytes > cluster * 16384)))
-        cluster *= 2;
-    if (bytes > cluster * kMaxSlice || rows * cluster > 0x7fffffff) {
+int launch_rows(const T *logits, int64_t ld, T *out, int64_t ldo, Args A, int64_t rows, cudaStream_t s) {
+    // slices of kSlice bytes at most while a cluster allows it; smaller ones while blocks are few
+    const int64_t granules = (A.vocab * (int64_t)sizeof(T) + 15) / 16 + 1;
+    int64_t cluster = (granules * 16 + kSlice - 1) / kSlice;
+    while (cluster < kMaxCluster && rows * cluster < 2 * (int64_t)num_sms() && granules * 16 > cluster * 16384) cluster++;
+    if (cluster > kMaxCluster) cluster = kMaxCluster;
+    const int64_t slice = (granules + cluster - 1) / cluster * 16;
+    if (slice > kMaxSlice) {
         distill_long_kernel<T, LOSS, GRAD><<<(unsigned)rows, NT, 0, s>>>(logits, ld, out, ldo, A);
         ZC_LAUNCHED("distill_long_kernel");
         return ZPUCUDA_OK;
     }
-    if (bytes <= cluster * 8192) return launch_cluster<T, LOSS, GRAD, 128>(logits, ld, out, ldo, A, rows, (int)cluster, s);
-    return launch_cluster<T, LOSS, GRAD, 256>(logits, ld, out, ldo, A, rows, (int)cluster, s);
+    A.rows = rows;
+    A.slice_bytes = (int)slice;
+    if (slice <= 8192) return launch_cluster<T, LOSS, GRAD, 128>(logits, ld, out, ldo, A, (int)cluster, s);
+    return launch_cluster<T, LOSS, GRAD, 256>(logits, ld, out, ldo, A, (int)cluster, s);
 }
 
 template <bool LOSS, bool GRAD>

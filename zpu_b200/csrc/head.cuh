@@ -319,6 +319,20 @@ inline int check_matrix(const char *who, const char *name, const void *p, int dt
     return ZPUCUDA_OK;
 }
 inline int head_error(int st, const char *who, const char *what) { return set_error(st, std::string(who) + ": " + what); }
+// Blocks of f that an SM holds at once with `smem` bytes each (looked up once a
+// device, for the first size asked for), after allowing it `allow`.
+template <typename F>
+int blocks_per_sm(F f, int block, size_t smem, size_t allow, int *cache) {
+    const int dev = current_device();
+    if (dev >= 0 && dev < 64 && cache[dev]) return cache[dev];
+    int n = 0;
+    if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)allow) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, f, block, smem) != cudaSuccess || n < 1)
+        return 0;
+    if (dev >= 0 && dev < 64) cache[dev] = n;
+    return n;
+}
+
 #define ZC_TRY(call)                  \
     do {                              \
         const int st_ = (call);       \

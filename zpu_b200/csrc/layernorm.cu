@@ -231,19 +231,6 @@ __global__ void __launch_bounds__(1024)
     }
 }
 
-// Blocks of f that an SM holds at once (looked up once a device), after allowing it `smem`.
-template <typename F>
-int blocks_per_sm(F f, int block, size_t smem, int *cache) {
-    const int dev = current_device();
-    if (dev >= 0 && dev < 64 && cache[dev]) return cache[dev];
-    int n = 0;
-    if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, f, block, smem) != cudaSuccess || n < 1)
-        return 0;
-    if (dev >= 0 && dev < 64) cache[dev] = n;
-    return n;
-}
-
 // Whether rows of cols elements at pitches of ld start on 16-byte boundaries and hold whole pieces.
 template <typename T>
 bool even_rows(const void *p, int64_t ld, int64_t rows, int64_t cols) {
@@ -257,7 +244,7 @@ int launch_ln_ring(const T *x, int64_t ldx, int wt, const void *gamma, const voi
     auto f = ln_kernel<T, TPR, NV, D, EVEN>;
     const size_t smem = (size_t)(BLOCK / 32) * RowRing<T, TPR, NV, 1, D, EVEN>::kWarp * 16;
     static int cache[64] = {0};
-    const int per = blocks_per_sm(f, BLOCK, smem, cache);
+    const int per = blocks_per_sm(f, BLOCK, smem, smem, cache);
     if (!per) return cuda_fail(cudaGetLastError(), "layer_norm: occupancy");
     const int64_t want = (rows + GROUPS - 1) / GROUPS, most = (int64_t)per * num_sms();
     f<<<(unsigned)(want < most ? want : most), BLOCK, smem, s>>>(x, ldx, wt, gamma, beta, y, ldy, mean, rstd, rows, cols, eps);
@@ -549,7 +536,7 @@ int launch_grad(const GradShape &g, const T *dy, int64_t lddy, const T *x, int64
     constexpr size_t smem = ring > sums ? ring : sums;
     static_assert(smem <= 226 * 1024, "shared memory");
     static int cache[64] = {0};
-    if (!blocks_per_sm(f, BLOCK, smem, cache)) return cuda_fail(cudaGetLastError(), "layer_norm_grad: occupancy");
+    if (!blocks_per_sm(f, BLOCK, smem, smem, cache)) return cuda_fail(cudaGetLastError(), "layer_norm_grad: occupancy");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(g.parts * g.cluster));
     cfg.blockDim = dim3(BLOCK);

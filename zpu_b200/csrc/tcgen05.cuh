@@ -37,6 +37,21 @@ __device__ __forceinline__ bool mb_wait(uint64_t *b, uint32_t parity, unsigned *
     return false;
 }
 
+// The same where other blocks of the cluster arrive: their writes before it are seen after it.
+__device__ __forceinline__ bool mb_wait_cluster(uint64_t *b, uint32_t parity, unsigned *err) {
+    for (uint32_t i = 0; i < kSpin; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(ok)
+            : "r"(su32(b)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+    }
+    atomicOr(err, 1u);
+    return false;
+}
+
 // A box of a 2-D tensor map at element column x (x times the element size a
 // multiple of 16 bytes) and row y; out-of-range elements are 0.
 __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
