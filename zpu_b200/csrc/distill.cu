@@ -9,12 +9,15 @@
 // and its logits are not read.  Any other index outside [0, vocab) makes its
 // row NaN.
 // HBM bounds it, with the exponential unit close behind (two exponentials an
-// element where both loss and gradient are wanted): a row is copied once into
-// the shared memory of a cluster of blocks, a slice each, where its maximum, sum
-// and gradient are computed; slices are small enough (64 KiB) that several
-// blocks of an SM overlap one another's copies and arithmetic.  A slice is
-// counted in aligned 16-byte granules of memory, so an odd vocabulary costs two
-// partial granules a row and nothing else.
+// element where both loss and gradient are wanted).  A row is split over the
+// blocks of a cluster: each reads its slice once for maximum and sum, the blocks
+// exchange those, and the gradient reads the slice again, from L2, where it has
+// stayed (slices are at most 64 KiB, so all that is in flight is a third of L2).
+// Holding slices in shared memory instead was slower: every byte then occupies
+// its place from the copy to the gradient, 13.7 us, and 192 KiB an SM do not
+// cover that time at HBM's rate (2048 x 131072 bf16: @SMEM@ us, @L2@ us now).
+// A slice is counted in aligned 16-byte granules of memory, so an odd vocabulary
+// costs two partial granules a row and nothing else.
 #include "head.cuh"
 #include "tcgen05.cuh"
 #include "waits.cuh"
@@ -30,11 +33,10 @@ int distill_device_error(unsigned int *e) {
 
 namespace {
 
-constexpr int NT = 256;
 constexpr int kMaxTop = 1024;
 constexpr int kMaxCluster = 8;
-constexpr int kSlice = 66 * 1024, kMaxSlice = 200 * 1024;  // bytes: wanted (three blocks an SM), possible
-constexpr int kCopies = 4;                                 // of a slice, each waited for by itself
+constexpr int kThreads = 1536, kGradThreads = 1024;  // an SM's, at 40 and 64 registers each (the latter without the loss)
+constexpr int kSlice = 64 * 1024 + 64;  // bytes of a block's slice at most, where a cluster of kMaxCluster allows it
 
 struct Args {
     const void *teacher, *indices;
@@ -46,33 +48,11 @@ struct Args {
     int64_t vocab;
     int top;
     int64_t rows;
-    int slice_bytes;  // of a block's shared memory
+    int slice;  // granules of a block
 };
 
 __device__ __forceinline__ int64_t load_index(const void *p, int it, int64_t i) {
     return it == ZPUCUDA_I64 ? ((const int64_t *)p)[i] : (int64_t)((const int32_t *)p)[i];
-}
-
-__device__ __forceinline__ float block_max(float v, float *sm) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = sm[0];
-#pragma unroll
-    for (int w = 1; w < NT / 32; w++) v = fmaxf(v, sm[w]);
-    return v;
-}
-__device__ __forceinline__ float block_sum(float v, float *sm) {
-    v = warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NT / 32; w++) v += sm[w];
-    return v;
 }
 
 // 2^x (error 2^-22 of the result; -inf gives 0).
@@ -82,7 +62,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return r;
 }
 
-// The larger of two granules' elements, NaN passed over.
+// The larger of two granules' elements; a NaN among them stays.
 template <typename T>
 __device__ __forceinline__ uint4 max_elements(const uint4 &a, const uint4 &b) {
     uint32_t x[4] = {a.x, a.y, a.z, a.w};
@@ -90,40 +70,17 @@ __device__ __forceinline__ uint4 max_elements(const uint4 &a, const uint4 &b) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if constexpr (sizeof(T) == 4) {
-            x[i] = __float_as_uint(fmaxf(__uint_as_float(x[i]), __uint_as_float(y[i])));
+            x[i] = __float_as_uint(max_nan(__uint_as_float(x[i]), __uint_as_float(y[i])));
         } else if constexpr (std::is_same<T, __half>::value) {
-            const __half2 m = __hmax2(*(const __half2 *)&x[i], *(const __half2 *)&y[i]);
+            const __half2 m = __hmax2_nan(*(const __half2 *)&x[i], *(const __half2 *)&y[i]);
             x[i] = *(const uint32_t *)&m;
         } else {
-            const __nv_bfloat162 m = __hmax2(*(const __nv_bfloat162 *)&x[i], *(const __nv_bfloat162 *)&y[i]);
+            const __nv_bfloat162 m = __hmax2_nan(*(const __nv_bfloat162 *)&x[i], *(const __nv_bfloat162 *)&y[i]);
             x[i] = *(const uint32_t *)&m;
         }
     }
     return make_uint4(x[0], x[1], x[2], x[3]);
 }
-
-// exp2 arguments of a granule relative to `ref`.  16-bit logits take one
-// multiply-add (k = log2(e) / T, its rounding is far below theirs); 32-bit ones
-// form z - ref first, so that the error stays relative to the distance.
-template <typename T>
-struct Scale {
-    f32x2 k, off, log2e;
-    __device__ __forceinline__ Scale(float inv_t, float ref) {
-        if constexpr (sizeof(T) == 4) {
-            k = make2(inv_t);
-            off = make2(-ref);
-            log2e = make2(1.4426950408889634f);
-        } else {
-            k = make2(inv_t * 1.4426950408889634f);
-            off = make2(-ref * 1.4426950408889634f);
-        }
-    }
-    __device__ __forceinline__ f32x2 arg(f32x2 x) const {
-        const f32x2 d = fma2(x, k, off);
-        if constexpr (sizeof(T) == 4) return mul2(d, log2e);
-        else return d;
-    }
-};
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -131,24 +88,26 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-// The first waits of a block must not be the last: several blocks share an SM,
-// and what one waits for another's arithmetic hides, but each byte of shared
-// memory is held from its copy to its gradient, so HBM's bandwidth needs a short
-// way from one to the other.  Hence: the listed entries are fetched while the
-// copies are on their way, every warp works out the teacher's sums for itself, and
-// the warps of a row's blocks exchange their maxima and sums directly, by stores
-// to one another's shared memory and one arrival, without a barrier of all.
+// A granule at a row's end, -inf in the place of elements outside [from, to) (counted from the granule's first).
+template <typename T>
+__device__ __noinline__ uint4 load_edge(const T *p, int from, int to) {
+    float f[kPiece<T>];
+#pragma unroll
+    for (int e = 0; e < kPiece<T>; e++) f[e] = e >= from && e < to ? to_f(p[e]) : -INFINITY;
+    return pack<T>(f);  // exact: the values come from that type
+}
+
 template <typename T, bool LOSS, bool GRAD, int THREADS>
-__global__ void __launch_bounds__(THREADS, 768 / THREADS)
+__global__ void __launch_bounds__(THREADS, (LOSS ? kThreads : kGradThreads) / THREADS)
     distill_kernel(const T *logits, int64_t ld, T *out, int64_t ldo, const Args A) {
-    constexpr int N = kPiece<T>, WARPS = THREADS / 32, MARKS = 2048;
-    extern __shared__ __align__(128) uint4 slice_smem[];
-    __shared__ uint64_t full[kCopies], told;
-    __shared__ float4 part[kMaxCluster * WARPS];  // each warp's maximum of z, sum of e^(z - maximum), sum of p z
+    constexpr int N = kPiece<T>, H = N / 2, WARPS = THREADS / 32, MARKS = 2048, U = 4;
+    extern __shared__ __align__(16) float entries[];
+    __shared__ uint64_t told;
+    __shared__ float4 part[kMaxCluster * WARPS];  // each warp's largest logit, its sum of e^z relative to that, its sum of p z
     __shared__ uint16_t mark[MARKS];              // an entry's number, by its place: to find indices listed twice
     __shared__ int again;
-    // behind the slice, for each listed entry: its probability, its logit, its place in the slice (-1: elsewhere)
-    float *sp = (float *)((uint8_t *)slice_smem + A.slice_bytes), *sz = sp + A.top;
+    // for each listed entry: its teacher logit / T, its logit, its place in the slice (-1: elsewhere)
+    float *sp = entries, *sz = sp + A.top;
     int *si = (int *)(sz + A.top);
     uint32_t rank, size;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -161,49 +120,42 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS)
     // the row's granules: granule g holds elements g * N - skew + e; this block's are g0 .. g0 + n - 1, and element 0 of
     // the slice is element `base` of the row
     const int skew = (int)(((uintptr_t)xr & 15) / sizeof(T));
-    const int64_t granules = (skew + A.vocab + N - 1) / N, g0 = (int64_t)rank * (A.slice_bytes / 16);
-    const int n = (int)max((int64_t)0, min((int64_t)(A.slice_bytes / 16), granules - g0));
+    const int64_t granules = (skew + A.vocab + N - 1) / N, g0 = (int64_t)rank * A.slice;
+    const int n = (int)max((int64_t)0, min((int64_t)A.slice, granules - g0));
     const int64_t base = g0 * N - skew;
     const T *x = xr + base;
     T *o = GRAD ? out + row * ldo + base : nullptr;
-    // the slice's elements that are in the row, and its granules that are whole
+    // the slice's elements that are in the row, its whole granules, and the partial one that this thread has
     const int from = base < 0 ? skew : 0, to = (int)max((int64_t)0, min((int64_t)n * N, A.vocab - base));
     const int w0 = from > 0, w1 = to / N;
+    const int edge = threadIdx.x == 0 && w0 && n ? 0 : threadIdx.x == 32 && w1 < n && !(w0 && w1 == 0) ? w1 : -1;
+    const bool same = ((uintptr_t)o & 15) == 0;  // x is on a granule: o, too?
+    auto zero = [&]() {
+        for (int g = w0 + threadIdx.x; g < w1; g += THREADS) {
+            if (same) __stcs((uint4 *)(o + g * N), make_uint4(0, 0, 0, 0));
+            else store_elements(o + g * N, make_uint4(0, 0, 0, 0), 0, N);
+        }
+        if (edge >= 0) store_elements(o + edge * N, make_uint4(0, 0, 0, 0), max(from - edge * N, 0), min(to - edge * N, N));
+    };
     const float inv_t = 1.0f / A.T;
-    const int per = (n + kCopies - 1) / kCopies;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < kCopies; i++) tc::mb_init(&full[i], 1);
+    if (LOSS && threadIdx.x == 0) {
         tc::mb_init(&told, size * WARPS);
         tc::mb_init_fence();
-        again = 0;
     }
+    if (threadIdx.x == 0) again = 0;
     const float c = GRAD ? A.T * (w * dl) : 0.0f;
     const bool want_loss = LOSS && w != 0.0f, want_grad = GRAD && c != 0.0f, want = want_loss || want_grad;
-
-    // the whole granules by bulk copies, the others element by element
-    if (want) {
-        if (threadIdx.x == 0)
-            for (int i = 0; i < kCopies; i++) {
-                const int a = max(i * per, w0), b = min(i * per + per, w1);
-                const uint32_t bytes = a < b ? (uint32_t)(b - a) * 16 : 0;
-                tc::mb_expect_tx(&full[i], bytes);
-                if (bytes)
-                    asm volatile(
-                        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                            tc::su32(slice_smem + a)),
-                        "l"(x + (int64_t)a * N), "r"(bytes), "r"(tc::su32(&full[i]))
-                        : "memory");
-            }
-        if (threadIdx.x < N && w0) {
-            const int e = threadIdx.x;
-            ((T *)slice_smem)[e] = e >= from && e < to ? x[e] : from_f<T>(-INFINITY);
-        }
-        if (threadIdx.x >= 32 && threadIdx.x < 32 + N && w1 < n && !(w0 && w1 == 0)) {
-            const int e = w1 * N + threadIdx.x - 32;
-            ((T *)slice_smem)[e] = e < to ? x[e] : from_f<T>(-INFINITY);
-        }
-    }
-    // the listed entries
+    // the first of the row's bytes are sent for (with the loss there are no registers to spare for them), then the listed entries
+    uint4 q[U];
+    int g = w0 + threadIdx.x;
+    auto load = [&]() {  // this thread's next U granules, -inf past its last
+        constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            q[u] = g + u * THREADS < w1 ? __ldcg((const uint4 *)(x + g * N) + u * THREADS) : make_uint4(none, none, none, none);
+        return g < w1;
+    };
+    bool more = !LOSS && want && load();
     bool bad = false;
     if (want)
         for (int k = threadIdx.x; k < A.top; k += THREADS) {
@@ -211,10 +163,12 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS)
             const float u = load_f(A.teacher, A.ttype, row * A.ldt + k) * inv_t;
             const bool in = i >= 0 && i < A.vocab;
             bad |= !in && i != -1;
-            si[k] = in && i >= base && i - base < to ? (int)(i - base) : -1;
+            const bool here = in && i >= base && i - base < to;
+            if (here) sz[k] = to_f(x[i - base]);
+            si[k] = here ? (int)(i - base) : -1;
             sp[k] = in ? u : -INFINITY;
         }
-    bad = __syncthreads_or(bad);  // the entries, the barriers and the partial granules are in place
+    bad = __syncthreads_or(bad);  // and the barrier is ready
     float um = -INFINITY, us = 0.0f, ul = 0.0f;
     if (want)
         for (int k = lane; k < A.top; k += 32) um = max_nan(um, sp[k]);
@@ -222,6 +176,58 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS)
     // with nothing to learn from the row (alike in all its blocks) what follows is left out
     if (want && (um != -INFINITY || bad)) {
         if (LOSS && size > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // `told` is ready
+        const f32x2 k2 = make2(inv_t * 1.4426950408889634f);
+        float lse = LOSS ? 0.0f : A.lse_in[row], high = 0.0f, bits = 0.0f;  // largest logit, log2 of the sum relative to it
+        float4 mine;
+        if constexpr (LOSS) {
+            // A thread's sum is relative to its largest logit so far; a larger one scales it down first.  The distance of
+            // two logits comes before 1 / T: it is exact where it counts, and does not overflow for masks of the type's
+            // lowest value.
+            float m = -INFINITY;
+            f32x2 s2 = make2(0.0f), s3 = s2;
+            auto raise = [&](const uint4 &mx) {
+                float f[N], top = -INFINITY;
+                unpack<T>(mx, f);
+#pragma unroll
+                for (int e = 0; e < N; e++) top = max_nan(top, f[e]);
+                if (!(top <= m)) {
+                    const float down = m == -INFINITY ? 0.0f : expf((m - top) * inv_t);
+                    s2 = mul2(add2(s2, s3), make2(down));
+                    s3 = make2(0.0f);
+                    m = top;
+                }
+            };
+            auto sum = [&](const uint4 &q) {
+                const f32x2 neg = make2(m == -INFINITY ? 0.0f : -m);  // all -inf so far: exponentials of -inf
+                f32x2 v[H];
+                unpack2<T>(q, v);
+#pragma unroll
+                for (int e = 0; e < H; e++) {
+                    const f32x2 t = mul2(add2(v[e], neg), k2), p = make2(exp2_fast(lo2(t)), exp2_fast(hi2(t)));
+                    if (e & 1) s3 = add2(s3, p);
+                    else s2 = add2(s2, p);
+                }
+            };
+            more = load();
+            if (edge >= 0) {
+                const uint4 r = load_edge(x + edge * N, from - edge * N, to - edge * N);
+                raise(r);
+                sum(r);
+            }
+            for (; more; g += U * THREADS, more = load()) {
+                uint4 mx = q[0];
+#pragma unroll
+                for (int u = 1; u < U; u++) mx = max_elements<T>(mx, q[u]);
+                raise(mx);
+#pragma unroll
+                for (int u = 0; u < U; u++) sum(q[u]);
+            }
+            g = w0 + threadIdx.x;
+            __syncwarp();
+            s2 = add2(s2, s3);
+            mine.x = warp_max(m);
+            mine.y = warp_sum((lo2(s2) + hi2(s2)) * (m == mine.x ? 1.0f : expf((m - mine.x) * inv_t)));
+        }
         for (int k = lane; k < A.top; k += 32) {
             const float d = sp[k] - um, e = expf(d);
             us += e;
@@ -230,56 +236,18 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS)
         us = warp_sum(us);
         if (LOSS) ul = warp_sum(ul);
         const float ur = 1.0f / us;
-        bool ok = true, any = false;
-        uint4 mx = make_uint4(0, 0, 0, 0);
-        int landed = 0, copy = 0;
-        if (LOSS)
-            for (int g = threadIdx.x; g < n; g += THREADS) {
-                for (; g >= landed; landed += per, copy++)
-                    if (!tc::mb_wait(&full[copy], 0, &g_distill_error)) ok = false;
-                const uint4 q = slice_smem[g];
-                mx = any ? max_elements<T>(mx, q) : q;
-                any = true;
-            }
-        for (; copy < kCopies; copy++)
-            if (!tc::mb_wait(&full[copy], 0, &g_distill_error)) ok = false;
-        __syncwarp();
-        float lse = LOSS ? 0.0f : A.lse_in[row];
-        float4 mine;
-        if constexpr (LOSS) {
-            float f[N], m = -INFINITY;
-            unpack<T>(mx, f);
-            if (any)
-#pragma unroll
-                for (int e = 0; e < N; e++) m = fmaxf(m, f[e]);
-            mine.x = fmaxf(warp_max(m) * inv_t, -3.0e38f);  // a slice of -inf has a sum of 0
-            const Scale<T> sc(inv_t, mine.x);
-            f32x2 s2 = make2(0.0f), s3 = s2;
-#pragma unroll 4
-            for (int g = threadIdx.x; g < n; g += THREADS) {
-                f32x2 v[N / 2];
-                unpack2<T>(slice_smem[g], v);
-#pragma unroll
-                for (int e = 0; e < N / 2; e++) {
-                    const f32x2 t = sc.arg(v[e]), q = make2(exp2_fast(lo2(t)), exp2_fast(hi2(t)));
-                    if (e & 1) s3 = add2(s3, q);
-                    else s2 = add2(s2, q);
-                }
-            }
-            __syncwarp();
-            s2 = add2(s2, s3);
-            mine.y = warp_sum(lo2(s2) + hi2(s2));
-        }
         // the listed entries in this slice
         float pz = 0.0f;
         for (int k = threadIdx.x; k < A.top; k += THREADS) {
             if (si[k] < 0) continue;
-            const float p = expf(sp[k] - um) * ur, z = to_f(((const T *)slice_smem)[si[k]]);
-            sz[k] = z;
-            if (LOSS && p != 0.0f) pz += p * (z * inv_t);
+            const float p = expf(sp[k] - um) * ur;
+            if (LOSS && p != 0.0f) pz += p * (sz[k] * inv_t);
             if (GRAD) mark[si[k] % MARKS] = (uint16_t)k;
         }
+        bool ok = true;
         if constexpr (LOSS) {
+            // Each warp tells all blocks of the row, by stores into their shared memory and one arrival, and goes on
+            // when all warps of the row have: sooner than by a barrier of the whole cluster.
             mine.z = warp_sum(pz);
             mine.w = 0.0f;
             if (size > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // of all blocks
@@ -293,17 +261,19 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS)
                              : "memory");
                 asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
             }
-            if (!tc::mb_wait_cluster(&told, 0, &g_distill_error)) ok = false;
-            __syncwarp();
-            float am = -INFINITY, as = 0.0f, az = 0.0f;
-            for (int i = lane; i < (int)size * WARPS; i += 32) am = fmaxf(am, part[i].x);
-            am = warp_max(am);
+            ok = __all_sync(0xffffffffu, tc::mb_wait_cluster(&told, 0, &g_distill_error));
+            float as = 0.0f, az = 0.0f;
+            high = -INFINITY;
+            for (int i = lane; i < (int)size * WARPS; i += 32) high = fmaxf(high, part[i].x);
+            high = warp_max(high);
             for (int i = lane; i < (int)size * WARPS; i += 32) {
                 const float4 q = part[i];
-                as += q.y * expf(q.x - am);
+                as += q.x == high ? q.y : q.y * expf((q.x - high) * inv_t);
                 az += q.z;
             }
-            lse = am + logf(warp_sum(as));
+            as = warp_sum(as);
+            bits = log2f(as);
+            lse = high * inv_t + logf(as);
             if (rank == 0 && warp == 0) {
                 az = warp_sum(az);
                 if (lane == 0) {
@@ -314,37 +284,40 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS)
                 }
             }
         } else {
-            __syncthreads();  // the marks
+            __syncthreads();  // the marks, and the entries' logits are read
         }
         if constexpr (GRAD) {
-            const Scale<T> sc(inv_t, lse);
+            // log2 of q: from the largest logit and the sum, or (without them) from lse, whose z is rounded like it
+            auto log2q = [&](f32x2 v) {
+                return LOSS ? fma2(add2(v, make2(-high)), k2, make2(-bits))
+                            : mul2(add2(mul2(v, make2(inv_t)), make2(-lse)), make2(1.4426950408889634f));
+            };
             const f32x2 c2 = make2(bad || !ok ? NAN : c);
-            const bool same = ((uintptr_t)o & 15) == 0;  // x is on a granule: o, too?
-            if (want_grad && same) {
-#pragma unroll 2
-                for (int g = threadIdx.x; g < n; g += THREADS) {
-                    f32x2 f[N / 2];
-                    unpack2<T>(slice_smem[g], f);
+            auto grad = [&](const uint4 &q) {
+                f32x2 f[H];
+                unpack2<T>(q, f);
 #pragma unroll
-                    for (int e = 0; e < N / 2; e++) {
-                        const f32x2 t = sc.arg(f[e]);
-                        f[e] = mul2(c2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t))));
-                    }
-                    const uint4 q = pack2<T>(f);
-                    if (g >= w0 && g < w1) *(uint4 *)(o + g * N) = q;
-                    else store_elements(o + g * N, q, max(from - g * N, 0), min(to - g * N, N));
+                for (int e = 0; e < H; e++) {
+                    const f32x2 t = log2q(f[e]);
+                    f[e] = mul2(c2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t))));
                 }
+                return pack2<T>(f);
+            };
+            if (!want_grad) {
+                zero();
             } else {
-                for (int g = threadIdx.x; g < n; g += THREADS) {
-                    f32x2 f[N / 2];
-                    unpack2<T>(slice_smem[g], f);
+                if (LOSS) more = load();
+                if (edge >= 0)
+                    store_elements(o + edge * N, grad(load_edge(x + edge * N, from - edge * N, to - edge * N)),
+                                   max(from - edge * N, 0), min(to - edge * N, N));
+                for (; more; g += U * THREADS, more = load())
 #pragma unroll
-                    for (int e = 0; e < N / 2; e++) {
-                        const f32x2 t = sc.arg(f[e]);
-                        f[e] = want_grad ? mul2(c2, make2(exp2_fast(lo2(t)), exp2_fast(hi2(t)))) : make2(0.0f);
+                    for (int u = 0; u < U; u++) {
+                        const uint4 d = grad(q[u]);
+                        if (g + u * THREADS >= w1) break;
+                        if (same) __stcs((uint4 *)(o + g * N) + u * THREADS, d);
+                        else store_elements(o + (g + u * THREADS) * N, d, 0, N);
                     }
-                    store_elements(o + g * N, pack2<T>(f), max(from - g * N, 0), min(to - g * N, N));
-                }
             }
             if (want_grad && !bad) {
                 // The listed entries are written over, an index that is listed again by its first entry.
@@ -362,112 +335,16 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS)
                             first &= j >= k;
                             p += expf(sp[j] - um) * ur;
                         }
-                    if (first) o[i] = from_f<T>(ok ? c * (exp2_fast(lo2(sc.arg(make2(sz[k])))) - p) : NAN);
+                    if (first) o[i] = from_f<T>(ok ? c * (exp2_fast(lo2(log2q(make2(sz[k])))) - p) : NAN);
                 }
             }
         }
-        if (!ok)  // give up only once the copies in flight have landed
-            for (int i = 0; i < kCopies; i++) tc::mb_wait(&full[i], 0, &g_distill_error);
         return;
     }
-    if (want)  // the copies are on their way: not before they have landed
-        for (int i = 0; i < kCopies; i++) tc::mb_wait(&full[i], 0, &g_distill_error);
-    if (GRAD)
-        for (int g = threadIdx.x; g < n; g += THREADS) {
-            if (((uintptr_t)o & 15) == 0 && g >= w0 && g < w1) *(uint4 *)(o + g * N) = make_uint4(0, 0, 0, 0);
-            else store_elements(o + g * N, make_uint4(0, 0, 0, 0), max(from - g * N, 0), min(to - g * N, N));
-        }
+    if (GRAD) zero();
     if (LOSS && rank == 0 && threadIdx.x == 0) {
         A.loss[row] = 0.0f;
         if (A.lse_out) A.lse_out[row] = 0.0f;
-    }
-}
-
-// Rows that no cluster holds, read three times.
-template <typename T, bool LOSS, bool GRAD>
-__global__ void __launch_bounds__(NT) distill_long_kernel(const T *logits, int64_t ld, T *out, int64_t ldo, Args A) {
-    __shared__ float sm[NT / 32];
-    __shared__ float sp[kMaxTop], sz[kMaxTop];
-    __shared__ int si[kMaxTop];
-    const int64_t row = blockIdx.x;
-    const T *x = logits + row * ld;
-    T *o = GRAD ? out + row * ldo : nullptr;
-    const float w = A.weight ? A.weight[row] : 1.0f;
-    const float c = GRAD ? A.T * (w * (A.dloss ? A.dloss[row] : 1.0f)) : 0.0f;
-    const bool want_loss = LOSS && w != 0.0f, want_grad = GRAD && c != 0.0f;
-
-    // the teacher's distribution
-    float um = -INFINITY;
-    bool bad = false;
-    if (want_loss || want_grad)
-        for (int k = threadIdx.x; k < A.top; k += NT) {
-            const int64_t i = load_index(A.indices, A.itype, row * A.ldi + k);
-            const bool in = i >= 0 && i < A.vocab;
-            bad |= !in && i != -1;
-            const float u = in ? load_f(A.teacher, A.ttype, row * A.ldt + k) / A.T : -INFINITY;
-            si[k] = in ? (int)i : -1;
-            sp[k] = u;
-            sz[k] = in ? to_f(x[i]) / A.T : 0.0f;
-            um = max_nan(um, u);
-        }
-    bad = __syncthreads_or(bad);
-    const bool un = __syncthreads_or(um != um);
-    um = un ? NAN : block_max(um, sm);
-    if (!(want_loss || want_grad) || (um == -INFINITY && !bad)) {
-        if (GRAD)
-            for (int64_t v = threadIdx.x; v < A.vocab; v += NT) o[v] = from_f<T>(0.0f);
-        if (LOSS && threadIdx.x == 0) {
-            A.loss[row] = 0.0f;
-            if (A.lse_out) A.lse_out[row] = 0.0f;
-        }
-        return;
-    }
-    float us = 0.0f;
-    for (int k = threadIdx.x; k < A.top; k += NT) us += expf(sp[k] - um);
-    us = block_sum(us, sm);
-    const float lus = logf(us);
-
-    // the student's normaliser
-    float lse;
-    if (LOSS) {
-        float m = -INFINITY, s = 0.0f;
-        for (int64_t v = threadIdx.x; v < A.vocab; v += NT) m = fmaxf(m, to_f(x[v]) / A.T);
-        m = block_max(m, sm);
-        for (int64_t v = threadIdx.x; v < A.vocab; v += NT) s += expf(to_f(x[v]) / A.T - m);
-        lse = m + logf(block_sum(s, sm));
-    } else {
-        lse = A.lse_in[row];
-    }
-    if (LOSS) {
-        float l = 0.0f;
-        for (int k = threadIdx.x; k < A.top; k += NT) {
-            const float lp = (sp[k] - um) - lus, p = expf(sp[k] - um) / us;
-            if (p != 0.0f) l += p * (lp - (sz[k] - lse));
-        }
-        l = block_sum(l, sm);
-        if (threadIdx.x == 0) {
-            A.loss[row] = bad ? NAN : w == 0.0f ? 0.0f : w * (A.T * A.T) * l;
-            if (A.lse_out) A.lse_out[row] = lse;
-        }
-    }
-    if (!GRAD) return;
-    for (int64_t v = threadIdx.x; v < A.vocab; v += NT)
-        o[v] = from_f<T>(bad ? NAN : c == 0.0f ? 0.0f : c * expf(to_f(x[v]) / A.T - lse));
-    if (bad || c == 0.0f) return;
-    for (int k = threadIdx.x; k < A.top; k += NT) sp[k] = expf(sp[k] - um) / us;
-    __syncthreads();
-    // the listed entries; an index that is listed again is written by its first entry
-    for (int k = threadIdx.x; k < A.top; k += NT) {
-        const int i = si[k];
-        if (i < 0) continue;
-        float p = 0.0f;
-        bool first = true;
-        for (int j = 0; j < A.top; j++)
-            if (si[j] == i) {
-                if (j < k) first = false;
-                p += sp[j];
-            }
-        if (first) o[i] = from_f<T>(c * (expf(sz[k] - lse) - p));
     }
 }
 
@@ -489,17 +366,11 @@ int check_args(const char *who, int dtype, const void *logits, int64_t ld, const
 template <typename T, bool LOSS, bool GRAD, int THREADS>
 int launch_cluster(const T *logits, int64_t ld, T *out, int64_t ldo, const Args &A, int cluster, cudaStream_t s) {
     auto f = distill_kernel<T, LOSS, GRAD, THREADS>;
-    static bool attr[64] = {false};
-    const int dev = current_device();
-    if (dev < 0 || dev >= 64 || !attr[dev]) {
-        ZC_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice + 16 + 12 * kMaxTop));
-        if (dev >= 0 && dev < 64) attr[dev] = true;
-    }
     cudaLaunchConfig_t cfg = {};
     const int64_t y = A.rows < 32768 ? A.rows : 32768;
     cfg.gridDim = dim3((unsigned)cluster, (unsigned)y, (unsigned)((A.rows + y - 1) / y));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = (size_t)A.slice_bytes + 12 * (size_t)A.top;
+    cfg.dynamicSmemBytes = 12 * (size_t)A.top;
     cfg.stream = s;
     cudaLaunchAttribute at[1] = {};
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -514,20 +385,24 @@ int launch_cluster(const T *logits, int64_t ld, T *out, int64_t ldo, const Args 
 
 template <typename T, bool LOSS, bool GRAD>
 int launch_rows(const T *logits, int64_t ld, T *out, int64_t ldo, Args A, int64_t rows, cudaStream_t s) {
-    // slices of kSlice bytes at most while a cluster allows it; smaller ones while blocks are few
-    const int64_t granules = (A.vocab * (int64_t)sizeof(T) + 15) / 16 + 1;
-    int64_t cluster = (granules * 16 + kSlice - 1) / kSlice;
-    while (cluster < kMaxCluster && rows * cluster < 2 * (int64_t)num_sms() && granules * 16 > cluster * 16384) cluster++;
+    // The blocks of a row: as few as keep slices to kSlice (what is read again has to stay in L2), or more where that
+    // fills the SMs' last wave better.  A block takes about 3 us and 7 us for each 64 KiB.
+    const int64_t granules = (A.vocab * (int64_t)sizeof(T) + 15) / 16 + 1, resident = (int64_t)num_sms() * ((LOSS ? kThreads : kGradThreads) / 256);
+    int64_t cluster = LOSS ? (granules * 16 + kSlice - 1) / kSlice : 1;
     if (cluster > kMaxCluster) cluster = kMaxCluster;
-    const int64_t slice = (granules + cluster - 1) / cluster * 16;
-    if (slice > kMaxSlice) {
-        distill_long_kernel<T, LOSS, GRAD><<<(unsigned)rows, NT, 0, s>>>(logits, ld, out, ldo, A);
-        ZC_LAUNCHED("distill_long_kernel");
-        return ZPUCUDA_OK;
+    double best = 0.0;
+    for (int64_t n = cluster; n <= kMaxCluster; n++) {
+        const double t = (double)((rows * n + resident - 1) / resident) * (3.0 + 7.0 * (double)(granules * 16) / (double)(n << 16));
+        if (n == cluster) best = t;
+        if (n > cluster && granules * 16 < n * 8192) break;
+        if (t < 0.97 * best) {
+            best = t;
+            cluster = n;
+        }
     }
     A.rows = rows;
-    A.slice_bytes = (int)slice;
-    if (slice <= 8192) return launch_cluster<T, LOSS, GRAD, 128>(logits, ld, out, ldo, A, (int)cluster, s);
+    A.slice = (int)((granules + cluster - 1) / cluster);
+    if (A.slice <= 512) return launch_cluster<T, LOSS, GRAD, 128>(logits, ld, out, ldo, A, (int)cluster, s);
     return launch_cluster<T, LOSS, GRAD, 256>(logits, ld, out, ldo, A, (int)cluster, s);
 }
 
