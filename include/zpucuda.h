@@ -534,7 +534,7 @@ int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d
                         const float *d_bias, void *d_y, int64_t ldy, int64_t rows, int64_t cols, int64_t inner,
                         void *d_work, int64_t work_bytes, void *stream);
 int64_t zpucuda_int8_linear_work(int64_t rows, int64_t inner);
-/* Chooses a token of each row of logits [rows, vocab] (vocab <= 2^22) from one
+/* Chooses a token of each row of logits [rows, vocab] (vocab < 2^22) from one
  * given uniform number in [0, 1) a row (utype F32 or F64).  Tokens are ranked by
  * falling logit, equal ones by rising index; a token's weight is the whole number
  * floor(2^40 exp((x - max x) / temperature)).  Kept are the top_k first ranks (<= 0:

@@ -15,20 +15,29 @@
 // or -inf logit has no weight; a row without any gives token -1 and log
 // probability -inf.
 //
-// The ranks are never sorted: a set of first ranks is described by the key
-// (the logit's bits in rising order) of its last member and how many of the
-// tokens with that key belong to it, both found by histograms over ever
-// narrower key ranges.
+// A set of first ranks is described by the key (the logit's bits in rising order)
+// of its last member and how many of the tokens with that key belong to it.  The
+// vocabulary is never sorted.  One block takes a row, which stays in L2 between
+// its passes, read 16 bytes at a time:
+//   - Few first ranks (top_k up to kQuick): the k-th largest of the threads' own
+//     maxima is a bound that at least k tokens reach and few more do; those are
+//     listed and sorted, and the rest of the row is not looked at again.
+//   - Otherwise a histogram of exact weights (or counts) over the logits' distance
+//     from the largest finds the bin in which the set ends, and that bin's tokens are
+//     listed and sorted.  What weighs too little to reach into the set is left out.
+// Instructions bound it, not HBM: an exponential for each token that may count.
 #include "head.cuh"
 
 namespace zc {
 namespace {
 
-constexpr int NT = 1024, NW = NT / 32;
+constexpr int NT = 512, NW = NT / 32;
 constexpr int NB = 2048;                 // histogram bins
+constexpr int kList = 4096;              // tokens listed at most
+constexpr int kQuick = 400;              // first ranks that the threads' maxima bound well
 constexpr uint64_t kOne = 1ull << 40;
 constexpr float kSpan = 28.0f;           // w = 0 beyond (max - x) / T = 40 ln 2 = 27.73
-constexpr int64_t kMaxVocab = 1 << 22;   // sums of weights stay below 2^62
+constexpr int64_t kMaxVocab = (1 << 22) - 1;  // sums of weights stay below 2^62, of their 10-bit digits below 2^32
 
 struct Args {
     const void *uniform;
@@ -51,146 +60,389 @@ __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float((key >> 31) ? (key & 0x7fffffffu) : ~key);
 }
 
-struct Row {
-    float m, inv;  // max, 1 / T
-    __device__ __forceinline__ float dist(float x) const { return x == m ? 0.0f : (x - m) * inv; }
-    __device__ __forceinline__ uint64_t weight(float x) const {
-        if (!(x > -INFINITY)) return 0;
-        if (x == m) return kOne;
-        return __float2ull_rz(expf((x - m) * inv) * (float)kOne);
-    }
-    // Histogram bin of a logit: falling logits, rising bins; -1: no weight.
-    __device__ __forceinline__ int bin(float x) const {
-        const float d = -dist(x);
-        return d < kSpan && x > -INFINITY ? min(NB - 1, (int)(d * ((float)NB / kSpan))) : -1;
-    }
-};
-
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-
-struct Shared {
-    unsigned long long mass[NB];
-    unsigned long long part[NW];
-    uint32_t ties[NW];
-    float fmax_[NW];
-    unsigned long long before, total;
-    uint32_t kmin, kmax;
-    int bin;
-};
-
-__device__ void clear(Shared &S) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < NB; i += NT) S.mass[i] = 0;
-    __syncthreads();
-}
-
-// The sum of the histogram.
-__device__ uint64_t hist_total(Shared &S) {
-    __syncthreads();
-    uint64_t v = 0;
-    for (int i = threadIdx.x; i < NB; i += NT) v += S.mass[i];
-    v = warp_sum64(v);
-    if ((threadIdx.x & 31) == 0) S.part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0;
-    for (int i = 0; i < NW; i++) v += S.part[i];
-    __syncthreads();
+// The sum of the values of this lane and those below it.
+__device__ __forceinline__ uint64_t warp_scan64(uint64_t v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+    }
     return v;
 }
 
-// The first bin whose running sum reaches target (<= the total); *before: the
-// sum of the bins before it.
-__device__ int hist_find(Shared &S, uint64_t target, uint64_t *before) {
+struct Shared {
+    union {
+        uint32_t digit[4][NB];            // a histogram: 10 bits of the weights each (a count: the first)
+        unsigned long long list[kList];   // key << 32 | ~index: sorted falling, ranks
+    };
+    unsigned long long w[NT];
+    unsigned long long part[NW];
+    uint32_t ties[NW];
+    float fmax_[NW];
+    unsigned long long before;
+    uint32_t kmin, kmax;
+    int bin, count;
+};
+
+// A row in granules of 16 aligned bytes, warp w's from w * seg on; and its weights.
+template <typename T>
+struct Row {
+    static constexpr int N = kPiece<T>, U = 4;
+    const T *x;   // granule 0 (which may begin before the row)
+    int skew, n;  // elements of granule 0 before the row, granules
+    int64_t vocab;
+    int seg, g0, g1, lane;  // granules of a warp, this warp's
+    float m, inv;           // the largest logit, 1 / T
+
+    __device__ __forceinline__ uint4 load(int g) const {
+        const int64_t at = (int64_t)g * N - skew;
+        if (at >= 0 && at + N <= vocab) return __ldcg((const uint4 *)(x + (int64_t)g * N));
+        float f[N];
+#pragma unroll
+        for (int e = 0; e < N; e++) f[e] = at + e >= 0 && at + e < vocab ? to_f(x[(int64_t)g * N + e]) : -INFINITY;
+        return pack<T>(f);  // exact: the values come from that type
+    }
+    // f(granule's bytes, its number) for each of this lane's granules from a to b, U loads in flight; lanes past the end
+    // are left out.
+    template <typename F>
+    __device__ __forceinline__ void each(int a, int b, F f) const {
+        for (int g = a + lane; g < b; g += 32 * U) {
+            uint4 q[U];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (g + 32 * u < b) q[u] = load(g + 32 * u);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (g + 32 * u < b) f(q[u], g + 32 * u);
+        }
+        __syncwarp();
+    }
+    static __device__ __forceinline__ float largest(const uint4 &q) {  // passes NaN over
+        float f[N], t = -INFINITY;
+        unpack<T>(q, f);
+#pragma unroll
+        for (int e = 0; e < N; e++) t = fmaxf(t, f[e]);
+        return t;
+    }
+    __device__ __forceinline__ float dist(float f) const { return f == m ? 0.0f : (f - m) * inv; }
+    __device__ __forceinline__ uint64_t weight(float f) const {
+        if (!(f > -INFINITY)) return 0;
+        if (f == m) return kOne;
+        return __float2ull_rz(expf((f - m) * inv) * (float)kOne);
+    }
+    __device__ __forceinline__ int64_t index(int g, int e) const { return (int64_t)g * N + e - skew; }
+};
+
+__device__ __forceinline__ unsigned long long entry_of(uint32_t key, int64_t index) {
+    return (unsigned long long)key << 32 | (uint32_t)~(uint32_t)index;
+}
+__device__ __forceinline__ uint32_t entry_key(unsigned long long e) { return (uint32_t)(e >> 32); }
+__device__ __forceinline__ uint32_t entry_index(unsigned long long e) { return ~(uint32_t)e; }
+
+// The list's n entries in falling order.
+__device__ void sort_list(Shared &S, int n) {
+    int size = 32;
+    while (size < n) size <<= 1;
+    for (int i = n + (int)threadIdx.x; i < size; i += NT) S.list[i] = 0;
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j; j >>= 1) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < size / 2; i += NT) {
+                const int lo = (i / j) * 2 * j + i % j, hi = lo + j;
+                const unsigned long long a = S.list[lo], b = S.list[hi];
+                if ((a < b) == ((lo & k) == 0)) {
+                    S.list[lo] = b;
+                    S.list[hi] = a;
+                }
+            }
+        }
     __syncthreads();
-    if (threadIdx.x < 32) {
-        constexpr int PER = NB / 32;
-        uint64_t v = 0;
-        for (int i = 0; i < PER; i++) v += S.mass[threadIdx.x * PER + i];
-        uint64_t inc = v;
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t t = __shfl_up_sync(0xffffffffu, inc, o);
-            if (threadIdx.x >= o) inc += t;
-        }
-        if (inc >= target && inc - v < target) {
-            uint64_t c = inc - v;
-            int b = threadIdx.x * PER;
-            while (c + S.mass[b] < target) c += S.mass[b++];
-            S.bin = b;
-            S.before = c;
-        }
+}
+
+__device__ void clear(Shared &S) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 4 * NB; i += NT) S.digit[0][i] = 0;
+    __syncthreads();
+}
+__device__ __forceinline__ uint64_t bin_value(const Shared &S, int b) {
+    return (uint64_t)S.digit[0][b] + ((uint64_t)S.digit[1][b] << 10) + ((uint64_t)S.digit[2][b] << 20) + ((uint64_t)S.digit[3][b] << 30);
+}
+// MASS: the weight; otherwise one.
+template <bool MASS>
+__device__ __forceinline__ void bin_add(Shared &S, int b, uint64_t w) {
+    if (!MASS) {
+        atomicAdd(&S.digit[0][b], 1u);
+        return;
+    }
+    atomicAdd(&S.digit[0][b], (uint32_t)w & 1023);
+    atomicAdd(&S.digit[1][b], (uint32_t)(w >> 10) & 1023);
+    atomicAdd(&S.digit[2][b], (uint32_t)(w >> 20) & 1023);
+    atomicAdd(&S.digit[3][b], (uint32_t)(w >> 30));
+}
+
+// The first bin whose running sum reaches target, and (*before) the sum of the bins before it; -1 if none does.
+__device__ int hist_find(Shared &S, uint64_t target, uint64_t *before) {
+    if (threadIdx.x == 0) S.bin = -1;
+    __syncthreads();
+    constexpr int PER = NB / NT;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint64_t v[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) sum += v[i] = bin_value(S, threadIdx.x * PER + i);
+    uint64_t upto = warp_scan64(sum, lane);
+    if (lane == 31) S.part[warp] = upto;
+    __syncthreads();
+    for (int i = 0; i < warp; i++) upto += S.part[i];
+    uint64_t c = upto - sum;
+    if (upto >= target && c < target) {
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (c < target) {
+                if (c + v[i] >= target) {
+                    S.bin = threadIdx.x * PER + i;
+                    S.before = c;
+                }
+                c += v[i];
+            }
     }
     __syncthreads();
     *before = S.before;
     return S.bin;
 }
 
-// After a histogram over bin(): the key at which the running measure (tokens,
-// or MASS: their weights) of the tokens above `floor_key` reaches target, and
-// in *rem what of the measure its own tokens have to give.
+// The last of the first ranks at which the running measure (tokens, or MASS:
+// their weights) of the tokens with keys above `floor_key` and distances up to
+// `span` reaches target: its key, and how many of that key's tokens belong to the
+// ranks (0: the measure does not reach target).  Not for tokens without weight.
 template <typename T, bool MASS>
-__device__ uint32_t select_key(Shared &S, const T *x, int64_t V, const Row &R, uint32_t floor_key, uint64_t target,
-                               uint64_t *rem) {
+__device__ uint32_t select_ranks(Shared &S, const Row<T> &R, uint32_t floor_key, float span, uint64_t target, uint64_t *ties) {
+    constexpr int N = Row<T>::N;
+    const float scale = (float)NB / span;
+    auto bin = [&](float f) { return min(NB - 1, (int)(-R.dist(f) * scale)); };
+    auto counts = [&](float f) { return f > -INFINITY && -R.dist(f) < span && key_of(f) > floor_key; };
+    clear(S);
+    R.each(R.g0, R.g1, [&](const uint4 &q, int) {
+        float f[N];
+        unpack<T>(q, f);
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (counts(f[e])) bin_add<MASS>(S, bin(f[e]), MASS ? R.weight(f[e]) : 1);
+    });
+    __syncthreads();
     uint64_t before;
     const int b = hist_find(S, target, &before);
+    *ties = 0;
+    if (b < 0) return 0;
     target -= before;
-    if (threadIdx.x == 0) {
-        S.kmin = 0xffffffffu;
-        S.kmax = 0;
-    }
-    __syncthreads();
-    uint32_t lo = 0xffffffffu, hi = 0;
-    for (int64_t v = threadIdx.x; v < V; v += NT) {
-        const float f = to_f(x[v]);
-        const uint32_t k = key_of(f);
-        if (k > floor_key && R.bin(f) == b) {
-            lo = min(lo, k);
-            hi = max(hi, k);
+    // the bin's tokens: their keys' range, and the list of them if it holds them
+    uint32_t lo = 0, hi = 0xffffffffu;
+    for (int level = 0; level < 5; level++) {  // a range of 32 bits is down to one key after three
+        const bool first = level == 0;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            S.count = 0;
+            S.kmin = 0xffffffffu;
+            S.kmax = 0;
         }
-    }
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    if ((threadIdx.x & 31) == 0) {
-        atomicMin(&S.kmin, lo);
-        atomicMax(&S.kmax, hi);
-    }
-    __syncthreads();
-    lo = S.kmin;
-    hi = S.kmax;
-    while (lo < hi) {
+        __syncthreads();
+        uint32_t kmin = 0xffffffffu, kmax = 0;
+        R.each(R.g0, R.g1, [&](const uint4 &q, int g) {
+            float f[N];
+            unpack<T>(q, f);
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const uint32_t k = key_of(f[e]);
+                if (first ? !(counts(f[e]) && bin(f[e]) == b) : k < lo || k > hi) continue;
+                kmin = min(kmin, k);
+                kmax = max(kmax, k);
+                const int i = atomicAdd(&S.count, 1);
+                if (i < kList) S.list[i] = entry_of(k, R.index(g, e));
+            }
+        });
+        kmin = __reduce_min_sync(0xffffffffu, kmin);
+        kmax = __reduce_max_sync(0xffffffffu, kmax);
+        if (R.lane == 0) {
+            atomicMin(&S.kmin, kmin);
+            atomicMax(&S.kmax, kmax);
+        }
+        __syncthreads();
+        lo = S.kmin;
+        hi = S.kmax;
+        const int n = S.count;
+        if (n <= kList || lo == hi) {
+            if (lo != hi) {
+                sort_list(S, n);
+                // the entry at which the measure reaches target, and how many up to it have its key
+                uint64_t below = 0;
+                for (int i0 = 0; i0 < n; i0 += NT) {
+                    const int i = i0 + (int)threadIdx.x, warp = threadIdx.x >> 5;
+                    const uint64_t w = i >= n ? 0 : MASS ? R.weight(value_of(entry_key(S.list[i]))) : 1;
+                    uint64_t upto = below + warp_scan64(w, R.lane);
+                    if (R.lane == 31) S.part[warp] = upto - below;
+                    __syncthreads();
+                    for (int v = 0; v < NW; v++) {
+                        if (v < warp) upto += S.part[v];
+                        below += S.part[v];
+                    }
+                    if (upto >= target && upto - w < target) {
+                        S.kmin = entry_key(S.list[i]);
+                        S.count = i;
+                    }
+                    __syncthreads();
+                    if (below >= target) break;
+                }
+                int same = 0;
+                for (int i = threadIdx.x; i <= S.count; i += NT) same += entry_key(S.list[i]) == S.kmin;
+                if (threadIdx.x == 0) S.before = 0;
+                __syncthreads();
+                if (same) atomicAdd(&S.before, (unsigned long long)same);
+                __syncthreads();
+                *ties = S.before;
+                return S.kmin;
+            }
+            const uint64_t w = MASS ? R.weight(value_of(hi)) : 1;
+            *ties = (target + w - 1) / w;
+            return hi;
+        }
+        // too many: a histogram of their keys, and again for the part that counts
         int shift = 0;
         while (((hi - lo) >> shift) >= NB) shift++;
         clear(S);
-        for (int64_t v = threadIdx.x; v < V; v += NT) {
-            const float f = to_f(x[v]);
-            const uint32_t k = key_of(f);
-            if (k >= lo && k <= hi) atomicAdd(&S.mass[(hi - k) >> shift], MASS ? (unsigned long long)R.weight(f) : 1ull);
-        }
-        const int s = hist_find(S, target, &before);
+        R.each(R.g0, R.g1, [&](const uint4 &q, int) {
+            float f[N];
+            unpack<T>(q, f);
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const uint32_t k = key_of(f[e]);
+                if (k >= lo && k <= hi) bin_add<MASS>(S, (hi - k) >> shift, MASS ? R.weight(f[e]) : 1);
+            }
+        });
+        __syncthreads();
+        const int part = hist_find(S, target, &before);
+        if (part < 0) break;
         target -= before;
-        hi -= (uint32_t)s << shift;
+        hi -= (uint32_t)part << shift;
         const uint32_t width = (1u << shift) - 1;
         lo = hi - lo > width ? hi - width : lo;
     }
-    *rem = target;
-    return hi;
+    return 0;
+}
+
+// floor(u * total), below total.
+__device__ __forceinline__ uint64_t place(const Args &A, int64_t row, uint64_t total) {
+    const double u = A.utype == ZPUCUDA_F64 ? ((const double *)A.uniform)[row] : (double)((const float *)A.uniform)[row];
+    if (!(u > 0.0)) return 0;
+    const double r = floor(u * (double)(int64_t)total);
+    const uint64_t at = r < (double)(int64_t)total ? (uint64_t)r : total;
+    return at < total ? at : total - 1;
+}
+__device__ __forceinline__ uint64_t top_p_edge(float p, uint64_t total) {
+    const double edge = ceil((double)p * (double)(int64_t)total);
+    return edge >= 1.0 ? (uint64_t)edge : 1;
+}
+template <typename T>
+__device__ __forceinline__ void choose(const Args &A, int64_t row, const Row<T> &R, int64_t token, float f, uint64_t total) {
+    A.token[row] = token;
+    if (A.logprob) A.logprob[row] = R.dist(f) - logf((float)(int64_t)total / (float)kOne);
+}
+
+// The choice among the k first ranks (k <= kQuick); false if there are too many tokens to list.
+template <typename T>
+__device__ bool sample_quick(Shared &S, const Row<T> &R, const Args &A, int64_t row, float mine, int k, float p, uint64_t least) {
+    constexpr int N = Row<T>::N;
+    const int lane = R.lane, warp = threadIdx.x >> 5;
+    // the k-th largest of the threads' maxima, bit by bit; -inf is not listed
+    const uint32_t key = key_of(mine);
+    uint32_t bound = 0;
+    for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t t = bound | (1u << bit);
+        if (__syncthreads_count(key >= t) >= k) bound = t;
+    }
+    bound = max(bound, 0x00800000u);  // the lowest finite value
+    if (threadIdx.x == 0) S.count = 0;
+    __syncthreads();
+    const float low = value_of(bound);
+    R.each(R.g0, R.g1, [&](const uint4 &q, int g) {
+        if (Row<T>::largest(q) < low) return;
+        float f[N];
+        unpack<T>(q, f);
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (f[e] >= low) {
+                const int i = atomicAdd(&S.count, 1);
+                if (i < kList) S.list[i] = entry_of(key_of(f[e]), R.index(g, e));
+            }
+    });
+    __syncthreads();
+    const int n = S.count;
+    if (n > kList) return false;
+    sort_list(S, n);
+    // a thread a rank
+    const bool in = (int)threadIdx.x < min(k, n);
+    const unsigned long long e = in ? S.list[threadIdx.x] : 0;
+    const float f = value_of(entry_key(e));
+    const uint32_t index = entry_index(e);
+    uint64_t w = in ? R.weight(f) : 0;
+    auto block_scan = [&](uint64_t v, uint64_t *total) {
+        const uint64_t upto = warp_scan64(v, lane);
+        __syncthreads();
+        if (lane == 31) S.part[warp] = upto;
+        __syncthreads();
+        uint64_t below = 0, all = 0;
+        for (int i = 0; i < NW; i++) {
+            if (i < warp) below += S.part[i];
+            all += S.part[i];
+        }
+        *total = all;
+        return below + upto;
+    };
+    uint64_t total;
+    if (p < 1.0f) {
+        const uint64_t upto = block_scan(w, &total);
+        if (upto - w >= top_p_edge(p, total)) w = 0;
+    }
+    if (w < least) w = 0;
+    block_scan(w, &total);
+    const uint64_t at = place(A, row, total);
+    // the running sum by index, up to this one
+    S.w[threadIdx.x] = w;
+    __syncthreads();
+    uint64_t upto = 0;
+    if (w)
+        for (int j = 0; j < min(k, n); j++)
+            if (entry_index(S.list[j]) <= index) upto += S.w[j];
+    if (w && upto > at && upto - w <= at) choose(A, row, R, (int64_t)index, f, total);
+    return true;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT) sample_kernel(const T *logits, int64_t ld, Args A) {
+__global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t ld, Args A) {
+    constexpr int N = Row<T>::N;
     __shared__ Shared S;
     const int64_t row = blockIdx.x, V = A.vocab;
+    const int warp = threadIdx.x >> 5;
+    Row<T> R;
+    R.vocab = V;
+    R.lane = threadIdx.x & 31;
     const T *x = logits + row * ld;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    R.skew = (int)(((uintptr_t)x & 15) / sizeof(T));
+    R.x = x - R.skew;
+    R.n = (int)((R.skew + V + N - 1) / N);
+    R.seg = (R.n + NW - 1) / NW;
+    R.g0 = min(R.n, warp * R.seg);
+    R.g1 = min(R.n, R.g0 + R.seg);
 
-    float m = -INFINITY;
-    for (int64_t v = threadIdx.x; v < V; v += NT) m = fmaxf(m, to_f(x[v]));  // passes NaN over
+    float mine = -INFINITY;
+    R.each(R.g0, R.g1, [&](const uint4 &q, int) { mine = fmaxf(mine, Row<T>::largest(q)); });
+    float m = mine;
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) S.fmax_[warp] = m;
+    if (R.lane == 0) S.fmax_[warp] = m;
     __syncthreads();
     for (int w = 0; w < NW; w++) m = fmaxf(m, S.fmax_[w]);
     if (m == -INFINITY) {
@@ -201,7 +453,11 @@ __global__ void __launch_bounds__(NT) sample_kernel(const T *logits, int64_t ld,
         return;
     }
     const float temp = A.temperature ? A.temperature[row] : 1.0f;
-    const Row R = {m, temp > 0.0f ? 1.0f / temp : 0.0f};
+    R.m = m;
+    R.inv = temp > 0.0f ? 1.0f / temp : 0.0f;
+    const float p = A.top_p ? A.top_p[row] : 1.0f, mp = A.min_p ? A.min_p[row] : 0.0f;
+    uint64_t least = 0;
+    if (mp > 0.0f) least = mp < 1.0f ? (uint64_t)ceil((double)mp * (double)kOne) : kOne;
 
     // The kept ranks: keys above `key`, and the first `ties` tokens of that key.
     uint32_t key = 0;
@@ -211,109 +467,150 @@ __global__ void __launch_bounds__(NT) sample_kernel(const T *logits, int64_t ld,
         ties = 1;
     } else {
         const int64_t k = A.top_k ? A.top_k[row] : 0;
-        if (k > 0 && k < V) {
-            clear(S);
-            for (int64_t v = threadIdx.x; v < V; v += NT) {
-                const int b = R.bin(to_f(x[v]));
-                if (b >= 0) atomicAdd(&S.mass[b], 1ull);
-            }
-            if (hist_total(S) > (uint64_t)k) key = select_key<T, false>(S, x, V, R, 0, (uint64_t)k, &ties);
-        }
-        const float p = A.top_p ? A.top_p[row] : 1.0f;
+        if (k > 0 && k <= kQuick && k < V && sample_quick(S, R, A, row, mine, (int)k, p, least)) return;
+        if (k > 0 && k < V) key = select_ranks<T, false>(S, R, 0, kSpan, (uint64_t)k, &ties);
         if (p < 1.0f) {
-            clear(S);
-            for (int64_t v = threadIdx.x; v < V; v += NT) {
-                const float f = to_f(x[v]);
-                const int b = R.bin(f);
-                if (b >= 0 && key_of(f) > key) atomicAdd(&S.mass[b], (unsigned long long)R.weight(f));
-            }
-            const uint64_t above = hist_total(S), wk = key ? R.weight(value_of(key)) : 0;
-            const double edge = ceil((double)p * (double)(int64_t)(above + ties * wk));
-            const uint64_t target = edge >= 1.0 ? (uint64_t)edge : 1;
+            // all the weight above the key
+            uint64_t sum = 0;
+            R.each(R.g0, R.g1, [&](const uint4 &q, int) {
+                float f[N];
+                unpack<T>(q, f);
+#pragma unroll
+                for (int e = 0; e < N; e++)
+                    if (key_of(f[e]) > key) sum += R.weight(f[e]);
+            });
+            sum = warp_sum64(sum);
+            __syncthreads();
+            if (R.lane == 0) S.part[warp] = sum;
+            __syncthreads();
+            uint64_t above = 0;
+            for (int i = 0; i < NW; i++) above += S.part[i];
+            const uint64_t wk = key ? R.weight(value_of(key)) : 0, target = top_p_edge(p, above + ties * wk);
             if (above >= target) {
-                uint64_t rem;
-                key = select_key<T, true>(S, x, V, R, key, target, &rem);
-                const uint64_t w = R.weight(value_of(key));
-                ties = (rem + w - 1) / w;
+                // Tokens lighter than (above - target) / vocab weigh less than what the set leaves out, all together:
+                // they are not in it (a distance a little larger stands for that weight).
+                const float light = (float)((above - target) / (uint64_t)V) / (float)kOne;
+                const float span = light > 0.0f ? fminf(kSpan, 1e-3f - logf(light)) : kSpan;
+                key = select_ranks<T, true>(S, R, key, span, target, &ties);
             } else {
                 const uint64_t need = (target - above + wk - 1) / wk;  // wk > 0: the total is above `above`
                 ties = need < ties ? need : ties;
             }
         }
     }
-    uint64_t least = 0;
-    const float mp = A.min_p ? A.min_p[row] : 0.0f;
-    if (mp > 0.0f) least = mp < 1.0f ? (uint64_t)ceil((double)mp * (double)kOne) : kOne;
 
-    // Running sums by index: a segment for each warp.
+    // Running sums by index, of each warp's granules first, then of 32 parts of the ones that hold the place.
     uint64_t wk = key ? R.weight(value_of(key)) : 0;
     if (wk < least) wk = 0;
-    const int64_t seg = (V + NT - 1) / NT * 32, v0 = warp * seg, v1 = v0 + seg < V ? v0 + seg : V;
+    const float low = key ? value_of(key) : -INFINITY;
     auto kept = [&](float f) -> uint64_t {
         if (key_of(f) <= key) return 0;
         const uint64_t w = R.weight(f);
         return w >= least ? w : 0;
     };
-    uint64_t sum = 0;
-    uint32_t same = 0;
-    for (int64_t v = v0 + lane; v < v1; v += 32) {
-        const float f = to_f(x[v]);
-        sum += kept(f);
-        same += key && key_of(f) == key;
-    }
-    sum = warp_sum64(sum);
-    same = __reduce_add_sync(0xffffffffu, same);
+    // of granules a to b: the kept weight above the key, and how many tokens have it
+    auto sums = [&](int a, int b, uint64_t *sum, uint32_t *same) {
+        uint64_t s = 0;
+        uint32_t t = 0;
+        R.each(a, b, [&](const uint4 &q, int) {
+            if (Row<T>::largest(q) < low) return;
+            float f[N];
+            unpack<T>(q, f);
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                s += kept(f[e]);
+                t += key && key_of(f[e]) == key;
+            }
+        });
+        *sum = warp_sum64(s);
+        *same = __reduce_add_sync(0xffffffffu, t);
+    };
+    // the part of NW parts that holds `at` once `before` and `left` ties lie before them; those are moved on
+    auto find = [&](uint64_t at, uint64_t *before, uint64_t *left, uint64_t *total) {
+        int found = NW - 1;
+        uint64_t b = *before, l = *left, fb = b, fl = l;
+        bool open = true;
+        for (int i = 0; i < NW; i++) {
+            const uint64_t t = S.ties[i] < l ? S.ties[i] : l, w = S.part[i] + t * wk;
+            if (open && b + w > at) {
+                open = false;
+                found = i;
+                fb = b;
+                fl = l;
+            }
+            b += w;
+            l -= t;
+        }
+        *total = b - *before;
+        *before = fb;
+        *left = fl;
+        return found;
+    };
+    uint64_t sum;
+    uint32_t same;
+    sums(R.g0, R.g1, &sum, &same);
     __syncthreads();
-    if (lane == 0) {
+    if (R.lane == 0) {
         S.part[warp] = sum;
         S.ties[warp] = same;
     }
     __syncthreads();
-    uint64_t total = 0, left = ties;
-    for (int w = 0; w < NW; w++) {
-        const uint64_t t = S.ties[w] < left ? S.ties[w] : left;
-        left -= t;
-        total += S.part[w] + t * wk;
-    }
-    const double u = A.utype == ZPUCUDA_F64 ? ((const double *)A.uniform)[row] : (double)((const float *)A.uniform)[row];
-    uint64_t at = 0;
-    if (u > 0.0) {
-        const double r = floor(u * (double)(int64_t)total);
-        at = r < (double)(int64_t)total ? (uint64_t)r : total;
-        if (at >= total) at = total - 1;
-    }
-    uint64_t before = 0;
+    uint64_t before = 0, left = ties, total, unused;
+    find(~0ull, &before, &left, &total);
+    const uint64_t at = place(A, row, total);
+    before = 0;
     left = ties;
-    for (int w = 0; w < warp; w++) {
-        const uint64_t t = S.ties[w] < left ? S.ties[w] : left;
-        left -= t;
-        before += S.part[w] + t * wk;
+    const int w0 = find(at, &before, &left, &unused);
+    // that warp's granules, in NW parts
+    const int a = min(R.n, w0 * R.seg), b = min(R.n, a + R.seg), sub = (b - a + NW - 1) / NW;
+    sums(min(b, a + warp * sub), min(b, a + (warp + 1) * sub), &sum, &same);
+    __syncthreads();
+    if (R.lane == 0) {
+        S.part[warp] = sum;
+        S.ties[warp] = same;
     }
-    const uint64_t mine = S.part[warp] + (S.ties[warp] < left ? S.ties[warp] : left) * wk;
-    if (at < before || at >= before + mine) return;
-    for (int64_t v = v0; v < v1; v += 32) {
-        const float f = v + lane < v1 ? to_f(x[v + lane]) : -INFINITY;
-        const bool eq = key && key_of(f) == key;
-        const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
-        uint64_t w = kept(f);
-        if (eq && __popc(eqs & ((1u << lane) - 1)) < left) w = wk;
-        uint64_t inc = w;
+    __syncthreads();
+    const int w1 = find(at, &before, &left, &unused);
+    if (warp != w1) return;
+    // one granule a lane
+    for (int g = min(b, a + w1 * sub), end = min(b, g + sub); g < end; g += 32) {
+        float f[N];
+        unpack<T>(g + R.lane < end ? R.load(g + R.lane) : make_uint4(0, 0, 0, 0), f);
+        uint64_t s[N], mine_ = 0;
+        uint32_t t = 0;
+#pragma unroll
+        for (int e = 0; e < N; e++) t += g + R.lane < end && key && key_of(f[e]) == key;
+        uint32_t upto = t;  // ties up to this lane's last
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t t = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += t;
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (R.lane >= o) upto += v;
         }
-        const uint32_t over = __ballot_sync(0xffffffffu, before + inc > at);
+        uint64_t rank = upto - t;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            uint64_t w = g + R.lane < end ? kept(f[e]) : 0;
+            if (g + R.lane < end && key && key_of(f[e]) == key && rank++ < left) w = wk;
+            mine_ += w;
+            s[e] = mine_;
+        }
+        const uint64_t incl = warp_scan64(mine_, R.lane), excl = before + incl - mine_;
+        const uint32_t over = __ballot_sync(0xffffffffu, before + incl > at);
         if (over) {
-            if (lane == __ffs(over) - 1) {
-                A.token[row] = v + lane;
-                if (A.logprob) A.logprob[row] = R.dist(f) - logf((float)(int64_t)total / (float)kOne);
+            if (R.lane == __ffs(over) - 1) {
+                bool open = true;
+#pragma unroll
+                for (int e = 0; e < N; e++)
+                    if (open && excl + s[e] > at) {
+                        open = false;
+                        choose(A, row, R, R.index(g + R.lane, e), f[e], total);
+                    }
             }
             return;
         }
-        before += __shfl_sync(0xffffffffu, inc, 31);
-        const uint64_t n = __popc(eqs);
-        left -= n < left ? n : left;
+        before += __shfl_sync(0xffffffffu, incl, 31);
+        const uint64_t seen = __shfl_sync(0xffffffffu, upto, 31);
+        left -= seen < left ? seen : left;
     }
 }
 
@@ -327,7 +624,7 @@ extern "C" int zpucuda_sample(int dtype, const void *d_logits, int64_t ld, int u
                               const float *d_min_p, int64_t *d_token, float *d_logprob, int64_t rows, int64_t vocab,
                               void *stream) {
     if (rows < 0 || vocab < 1) return set_error(ZPUCUDA_ERR_INVALID_SHAPE, "sample: rows >= 0 and vocab >= 1 are wanted");
-    if (vocab > kMaxVocab) return set_error(ZPUCUDA_ERR_NOT_SUPPORTED, "sample: more than 2^22 tokens");
+    if (vocab > kMaxVocab) return set_error(ZPUCUDA_ERR_NOT_SUPPORTED, "sample: 2^22 tokens or more");
     if (rows > 0x7fffffff) return set_error(ZPUCUDA_ERR_NOT_SUPPORTED, "sample: more than 2^31 - 1 rows");
     ZC_TRY(check_matrix("sample", "logits", d_logits, dtype, ld, rows, vocab));
     if (utype != ZPUCUDA_F32 && utype != ZPUCUDA_F64) return set_error(ZPUCUDA_ERR_NOT_SUPPORTED, "sample: uniform is not f32 or f64");
