@@ -97,7 +97,7 @@ struct Row {
     int skew, n;  // elements of granule 0 before the row, granules
     int64_t vocab;
     int seg, g0, g1, lane;  // granules of a warp, this warp's
-    float m, inv;           // the largest logit, 1 / T
+    float m, inv;           // the largest logit, 1 / T (0: the largest alone)
 
     __device__ __forceinline__ uint4 load(int g) const {
         const int64_t at = (int64_t)g * N - skew;
@@ -130,10 +130,16 @@ struct Row {
         return t;
     }
     __device__ __forceinline__ float dist(float f) const { return f == m ? 0.0f : (f - m) * inv; }
+    // The weight of a token at a distance: floor(2^40 e^d), the significand shifted into place (0 <= e^d <= 1).
+    static __device__ __forceinline__ uint64_t weigh(float d) {
+        const uint32_t u = __float_as_uint(expf(d));
+        return ((uint64_t)((u & 0x7fffffu) | 0x800000u) << 17) >> (127 - (u >> 23));
+    }
+    bool spike;  // only the largest logit has weight: it is infinite, or 1 / T is
     __device__ __forceinline__ uint64_t weight(float f) const {
-        if (!(f > -INFINITY)) return 0;
-        if (f == m) return kOne;
-        return __float2ull_rz(expf((f - m) * inv) * (float)kOne);
+        if (spike) return f == m ? kOne : 0;
+        const float d = (f - m) * inv;
+        return d > -kSpan + 0.2f ? weigh(d) : 0;  // NaN: 0
     }
     __device__ __forceinline__ int64_t index(int g, int e) const { return (int64_t)g * N + e - skew; }
 };
@@ -215,24 +221,22 @@ __device__ int hist_find(Shared &S, uint64_t target, uint64_t *before) {
     return S.bin;
 }
 
+// A histogram of the tokens above `low` at distances below `span`, by distance.
+template <typename T>
+struct Bins {
+    float span, scale, low;
+    __device__ __forceinline__ Bins(float span_, float low_) : span(span_), scale((float)NB / span_), low(low_) {}
+    // The bin of a token, -1: it is not counted.  d: its distance.
+    __device__ __forceinline__ int at(float f, float d) const { return f > low && -d < span ? min(NB - 1, (int)(-d * scale)) : -1; }
+};
+
 // The last of the first ranks at which the running measure (tokens, or MASS:
-// their weights) of the tokens with keys above `floor_key` and distances up to
-// `span` reaches target: its key, and how many of that key's tokens belong to the
-// ranks (0: the measure does not reach target).  Not for tokens without weight.
+// their weights) of the tokens in the histogram reaches target: its key, and how
+// many of that key's tokens belong to the ranks (0: the measure does not reach
+// target).  Not for tokens without weight.
 template <typename T, bool MASS>
-__device__ uint32_t select_ranks(Shared &S, const Row<T> &R, uint32_t floor_key, float span, uint64_t target, uint64_t *ties) {
+__device__ uint32_t select_ranks(Shared &S, const Row<T> &R, const Bins<T> &H, uint64_t target, uint64_t *ties) {
     constexpr int N = Row<T>::N;
-    const float scale = (float)NB / span;
-    auto bin = [&](float f) { return min(NB - 1, (int)(-R.dist(f) * scale)); };
-    auto counts = [&](float f) { return f > -INFINITY && -R.dist(f) < span && key_of(f) > floor_key; };
-    clear(S);
-    R.each(R.g0, R.g1, [&](const uint4 &q, int) {
-        float f[N];
-        unpack<T>(q, f);
-#pragma unroll
-        for (int e = 0; e < N; e++)
-            if (counts(f[e])) bin_add<MASS>(S, bin(f[e]), MASS ? R.weight(f[e]) : 1);
-    });
     __syncthreads();
     uint64_t before;
     const int b = hist_find(S, target, &before);
@@ -257,7 +261,7 @@ __device__ uint32_t select_ranks(Shared &S, const Row<T> &R, uint32_t floor_key,
 #pragma unroll
             for (int e = 0; e < N; e++) {
                 const uint32_t k = key_of(f[e]);
-                if (first ? !(counts(f[e]) && bin(f[e]) == b) : k < lo || k > hi) continue;
+                if (first ? H.at(f[e], R.dist(f[e])) != b : k < lo || k > hi) continue;
                 kmin = min(kmin, k);
                 kmax = max(kmax, k);
                 const int i = atomicAdd(&S.count, 1);
@@ -455,6 +459,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
     const float temp = A.temperature ? A.temperature[row] : 1.0f;
     R.m = m;
     R.inv = temp > 0.0f ? 1.0f / temp : 0.0f;
+    R.spike = isinf(m) || isinf(R.inv);
     const float p = A.top_p ? A.top_p[row] : 1.0f, mp = A.min_p ? A.min_p[row] : 0.0f;
     uint64_t least = 0;
     if (mp > 0.0f) least = mp < 1.0f ? (uint64_t)ceil((double)mp * (double)kOne) : kOne;
@@ -468,16 +473,48 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
     } else {
         const int64_t k = A.top_k ? A.top_k[row] : 0;
         if (k > 0 && k <= kQuick && k < V && sample_quick(S, R, A, row, mine, (int)k, p, least)) return;
-        if (k > 0 && k < V) key = select_ranks<T, false>(S, R, 0, kSpan, (uint64_t)k, &ties);
+        if (k > 0 && k < V) {
+            const Bins<T> H(kSpan, -INFINITY);
+            clear(S);
+            R.each(R.g0, R.g1, [&](const uint4 &q, int) {
+                float f[N];
+                unpack<T>(q, f);
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const int b = H.at(f[e], R.dist(f[e]));
+                    if (b >= 0) bin_add<false>(S, b, 1);
+                }
+            });
+            key = select_ranks<T, false>(S, R, H, (uint64_t)k, &ties);
+        }
         if (p < 1.0f) {
-            // all the weight above the key
+            // Tokens that, all together, weigh less than what the set leaves out are not in it: with the whole weight at
+            // least `sure` (of the threads' largest tokens; with a top_k set, of the largest token), those lighter than
+            // (1 - p) sure / vocab are left out of the histogram (a distance a little larger stands for that weight).
+            const float low = key ? value_of(key) : -INFINITY;
+            uint64_t sure = mine > -INFINITY && !key ? R.weight(mine) : 0;
+            sure = warp_sum64(sure);
+            __syncthreads();
+            if (R.lane == 0) S.part[warp] = sure;
+            clear(S);
+            sure = 0;
+            for (int i = 0; i < NW; i++) sure += S.part[i];
+            if (sure < kOne) sure = kOne;
+            const float light = (1.0f - p) * (float)sure / (float)kOne / (float)V;
+            const float span = p > 0.0f && light > 0.0f ? fminf(kSpan, fmaxf(1e-3f, 1e-3f - logf(light))) : kSpan;
+            const Bins<T> H(span, low);
             uint64_t sum = 0;
             R.each(R.g0, R.g1, [&](const uint4 &q, int) {
                 float f[N];
                 unpack<T>(q, f);
 #pragma unroll
-                for (int e = 0; e < N; e++)
-                    if (key_of(f[e]) > key) sum += R.weight(f[e]);
+                for (int e = 0; e < N; e++) {
+                    const float d = R.dist(f[e]);
+                    const uint64_t w = f[e] > low ? R.weight(f[e]) : 0;
+                    sum += w;
+                    const int b = H.at(f[e], d);
+                    if (b >= 0) bin_add<true>(S, b, w);
+                }
             });
             sum = warp_sum64(sum);
             __syncthreads();
@@ -485,13 +522,10 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
             __syncthreads();
             uint64_t above = 0;
             for (int i = 0; i < NW; i++) above += S.part[i];
+            __syncthreads();
             const uint64_t wk = key ? R.weight(value_of(key)) : 0, target = top_p_edge(p, above + ties * wk);
             if (above >= target) {
-                // Tokens lighter than (above - target) / vocab weigh less than what the set leaves out, all together:
-                // they are not in it (a distance a little larger stands for that weight).
-                const float light = (float)((above - target) / (uint64_t)V) / (float)kOne;
-                const float span = light > 0.0f ? fminf(kSpan, 1e-3f - logf(light)) : kSpan;
-                key = select_ranks<T, true>(S, R, key, span, target, &ties);
+                key = select_ranks<T, true>(S, R, H, target, &ties);
             } else {
                 const uint64_t need = (target - above + wk - 1) / wk;  // wk > 0: the total is above `above`
                 ties = need < ties ? need : ties;
@@ -504,7 +538,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
     if (wk < least) wk = 0;
     const float low = key ? value_of(key) : -INFINITY;
     auto kept = [&](float f) -> uint64_t {
-        if (key_of(f) <= key) return 0;
+        if (!(f > low)) return 0;
         const uint64_t w = R.weight(f);
         return w >= least ? w : 0;
     };
@@ -519,7 +553,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
 #pragma unroll
             for (int e = 0; e < N; e++) {
                 s += kept(f[e]);
-                t += key && key_of(f[e]) == key;
+                t += key && f[e] == low;
             }
         });
         *sum = warp_sum64(s);
@@ -579,7 +613,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
         uint64_t s[N], mine_ = 0;
         uint32_t t = 0;
 #pragma unroll
-        for (int e = 0; e < N; e++) t += g + R.lane < end && key && key_of(f[e]) == key;
+        for (int e = 0; e < N; e++) t += g + R.lane < end && key && f[e] == low;
         uint32_t upto = t;  // ties up to this lane's last
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -590,7 +624,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
 #pragma unroll
         for (int e = 0; e < N; e++) {
             uint64_t w = g + R.lane < end ? kept(f[e]) : 0;
-            if (g + R.lane < end && key && key_of(f[e]) == key && rank++ < left) w = wk;
+            if (g + R.lane < end && key && f[e] == low && rank++ < left) w = wk;
             mine_ += w;
             s[e] = mine_;
         }
