@@ -25,17 +25,22 @@
 //   - Otherwise a histogram of exact weights (or counts) over the logits' distance
 //     from the largest finds the bin in which the set ends, and that bin's tokens are
 //     listed and sorted.  What weighs too little to reach into the set is left out.
-// Instructions bound it, not HBM: an exponential for each token that may count.
+//   - 16-bit logits have few values: a histogram of the values themselves takes the
+//     place of both the distances and the list, and a table of their exponentials
+//     that of computing one for every token.
+// Instructions bound it, not HBM: a few for each token in each pass, an exponential
+// among them for 32-bit logits.
 #include "head.cuh"
 
 namespace zc {
 namespace {
 
-constexpr int NT = 512, NW = NT / 32;
+constexpr int NT = 1024, NW = NT / 32;
 constexpr int NB = 2048;                 // histogram bins
 constexpr int kList = 4096;              // tokens listed at most
 constexpr int kQuick = 400;              // first ranks that the threads' maxima bound well
 constexpr uint64_t kOne = 1ull << 40;
+constexpr int kPlaces = 44 * 1024;       // values of 16-bit logits in the table (176 KiB)
 constexpr float kSpan = 28.0f;           // w = 0 beyond (max - x) / T = 40 ln 2 = 27.73
 constexpr int64_t kMaxVocab = (1 << 22) - 1;  // sums of weights stay below 2^62, of their 10-bit digits below 2^32
 
@@ -48,6 +53,7 @@ struct Args {
     int64_t *token;
     float *logprob;
     int64_t vocab;
+    int places;  // of the table of values
 };
 
 // The logit's bits as a number that rises with it; NaN is 0, below all others.
@@ -92,7 +98,7 @@ struct Shared {
 // A row in granules of 16 aligned bytes, warp w's from w * seg on; and its weights.
 template <typename T>
 struct Row {
-    static constexpr int N = kPiece<T>, U = 4;
+    static constexpr int N = kPiece<T>;
     const T *x;   // granule 0 (which may begin before the row)
     int skew, n;  // elements of granule 0 before the row, granules
     int64_t vocab;
@@ -109,7 +115,7 @@ struct Row {
     }
     // f(granule's bytes, its number) for each of this lane's granules from a to b, U loads in flight; lanes past the end
     // are left out.
-    template <typename F>
+    template <int U = 2, typename F>
     __device__ __forceinline__ void each(int a, int b, F f) const {
         for (int g = a + lane; g < b; g += 32 * U) {
             uint4 q[U];
@@ -355,6 +361,114 @@ __device__ __forceinline__ void choose(const Args &A, int64_t row, const Row<T> 
     if (A.logprob) A.logprob[row] = R.dist(f) - logf((float)(int64_t)total / (float)kOne);
 }
 
+// The token whose running sum by index exceeds the place: kept(granule, element, &same) is a token's kept weight, or 0 and
+// same = true for a token of the last kept key, of which the first `ties` weigh wk each.  Sums of each warp's granules first,
+// then of NW parts of the ones that hold the place, then of those.
+template <typename T, typename K>
+__device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t row, uint64_t ties, uint64_t wk, K kept) {
+    constexpr int N = Row<T>::N;
+    const int warp = threadIdx.x >> 5;
+    auto sums = [&](int a, int b) {  // of granules a to b, to S
+        uint64_t s = 0;
+        uint32_t t = 0;
+        R.each(a, b, [&](const uint4 &q, int) {
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                bool same;
+                s += kept(q, e, &same);
+                t += same;
+            }
+        });
+        s = warp_sum64(s);
+        t = __reduce_add_sync(0xffffffffu, t);
+        __syncthreads();
+        if (R.lane == 0) {
+            S.part[warp] = s;
+            S.ties[warp] = t;
+        }
+        __syncthreads();
+    };
+    // the part of NW parts that holds `at` once `before` and `left` ties lie before them; those are moved on
+    auto find = [&](uint64_t at, uint64_t *before, uint64_t *left, uint64_t *total) {
+        int found = NW - 1;
+        uint64_t b = *before, l = *left, fb = b, fl = l;
+        bool open = true;
+        for (int i = 0; i < NW; i++) {
+            const uint64_t t = S.ties[i] < l ? S.ties[i] : l, w = S.part[i] + t * wk;
+            if (open && b + w > at) {
+                open = false;
+                found = i;
+                fb = b;
+                fl = l;
+            }
+            b += w;
+            l -= t;
+        }
+        *total = b - *before;
+        *before = fb;
+        *left = fl;
+        return found;
+    };
+    sums(R.g0, R.g1);
+    uint64_t before = 0, left = ties, total, unused;
+    find(~0ull, &before, &left, &total);
+    const uint64_t at = place(A, row, total);
+    before = 0;
+    left = ties;
+    const int w0 = find(at, &before, &left, &unused);
+    const int a = min(R.n, w0 * R.seg), b = min(R.n, a + R.seg), sub = (b - a + NW - 1) / NW;
+    sums(min(b, a + warp * sub), min(b, a + (warp + 1) * sub));
+    const int w1 = find(at, &before, &left, &unused);
+    if (warp != w1) return;
+    // one granule a lane
+    for (int g = min(b, a + w1 * sub), end = min(b, g + sub); g < end; g += 32) {
+        const bool in = g + R.lane < end;
+        const uint4 q = in ? R.load(g + R.lane) : make_uint4(0, 0, 0, 0);
+        float f[N];
+        unpack<T>(q, f);
+        uint64_t s[N], sum = 0;
+        uint32_t t = 0;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            bool same;
+            s[e] = kept(q, e, &same);
+            t += in && same;
+        }
+        uint32_t upto = t;  // ties up to this lane's last
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (R.lane >= o) upto += v;
+        }
+        uint64_t rank = upto - t;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            bool same;
+            kept(q, e, &same);
+            if (in && same && rank++ < left) s[e] = wk;
+            sum += in ? s[e] : 0;
+            s[e] = sum;
+        }
+        const uint64_t incl = warp_scan64(sum, R.lane), excl = before + incl - sum;
+        const uint32_t over = __ballot_sync(0xffffffffu, before + incl > at);
+        if (over) {
+            if (R.lane == __ffs(over) - 1) {
+                bool open = true;
+#pragma unroll
+                for (int e = 0; e < N; e++)
+                    if (open && excl + s[e] > at) {
+                        open = false;
+                        choose(A, row, R, R.index(g + R.lane, e), f[e], total);
+                    }
+            }
+            return;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+        const uint64_t seen = __shfl_sync(0xffffffffu, upto, 31);
+        left -= seen < left ? seen : left;
+    }
+}
+
 // The choice among the k first ranks (k <= kQuick); false if there are too many tokens to list.
 template <typename T>
 __device__ bool sample_quick(Shared &S, const Row<T> &R, const Args &A, int64_t row, float mine, int k, float p, uint64_t least) {
@@ -371,7 +485,7 @@ __device__ bool sample_quick(Shared &S, const Row<T> &R, const Args &A, int64_t 
     if (threadIdx.x == 0) S.count = 0;
     __syncthreads();
     const float low = value_of(bound);
-    R.each(R.g0, R.g1, [&](const uint4 &q, int g) {
+    R.template each<4>(R.g0, R.g1, [&](const uint4 &q, int g) {
         if (Row<T>::largest(q) < low) return;
         float f[N];
         unpack<T>(q, f);
@@ -424,9 +538,133 @@ __device__ bool sample_quick(Shared &S, const Row<T> &R, const Args &A, int64_t 
     return true;
 }
 
+// 16-bit logits as whole numbers: falling logits, rising places from the largest (0) on.  NaN has none (its place is
+// past all others).
 template <typename T>
-__global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t ld, Args A) {
+struct Values {
+    uint32_t top;  // the order of the largest
+    static __device__ __forceinline__ uint32_t order(uint32_t raw) {  // rises with the value; -0 is 0
+        raw = raw == 0x8000u ? 0 : raw;
+        return raw & 0x8000u ? 0x7fffu - (raw & 0x7fffu) : raw + 0x7fffu;  // NaN: above +inf, or below -inf
+    }
+    __device__ __forceinline__ uint32_t place(uint32_t raw) const { return top - order(raw); }  // NaN above: wraps to far past all
+    __device__ __forceinline__ float value(uint32_t place_) const {
+        const uint32_t o = top - place_, raw = o >= 0x7fffu ? o - 0x7fffu : 0x8000u | (0x7fffu - o);
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(raw << 16);
+        else return __half2float(__ushort_as_half((unsigned short)raw));
+    }
+};
+
+// The same choice for 16-bit logits by their values: counts of each value at `n` places from the largest on (what lies past
+// them has no weight), then in their place e^((x - max) / T) of those that are kept (0: not kept).
+template <typename T>
+__device__ void sample_values(Shared &S, uint32_t *table, const Row<T> &R, const Args &A, int64_t row, int n, int64_t k, float p,
+                              uint64_t least) {
+    static_assert(sizeof(T) == 2, "16-bit logits");
+    const int lane = R.lane, warp = threadIdx.x >> 5;
+    const Values<T> O = {Values<T>::order(raw_bits(from_f<T>(R.m)))};
+    auto block_scan = [&](uint64_t v, uint64_t *total) {
+        const uint64_t upto = warp_scan64(v, lane);
+        __syncthreads();
+        if (lane == 31) S.part[warp] = upto;
+        __syncthreads();
+        uint64_t below = 0, all = 0;
+        for (int i = 0; i < NW; i++) {
+            if (i < warp) below += S.part[i];
+            all += S.part[i];
+        }
+        *total = all;
+        return below + upto;
+    };
+    const int per = (n + NT - 1) / NT, b0 = min(n, (int)threadIdx.x * per), b1 = min(n, b0 + per);  // a thread's places
+    // The kept ranks: places below `last`, and the first `ties` tokens at it.
+    uint32_t last = (uint32_t)n;
+    uint64_t ties = 0;
+    if (k > 0 || p < 1.0f) {
+        for (int i = threadIdx.x; i < n; i += NT) table[i] = 0;
+        __syncthreads();
+        R.template each<4>(R.g0, R.g1, [&](const uint4 &q, int) {
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint32_t at = O.place(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu);
+                if (at < (uint32_t)n) atomicAdd(&table[at], 1u);
+            }
+        });
+        __syncthreads();
+        uint64_t total;
+        if (k > 0) {
+            uint64_t c = 0;
+            for (int i = b0; i < b1; i++) c += table[i];
+            uint64_t upto = block_scan(c, &total);
+            if (threadIdx.x == 0) S.bin = -1;
+            __syncthreads();
+            if (upto >= (uint64_t)k && upto - c < (uint64_t)k) {
+                uint64_t s = upto - c;
+                int i = b0;
+                while (s + table[i] < (uint64_t)k) s += table[i++];
+                S.bin = i;
+                S.before = (uint64_t)k - s;
+            }
+            __syncthreads();
+            if (S.bin >= 0) {
+                last = (uint32_t)S.bin;
+                ties = S.before;
+            }
+        }
+        if (p < 1.0f) {
+            // of a value's tokens, those that top_k leaves
+            auto count = [&](int i) -> uint64_t { return (uint32_t)i < last ? table[i] : (uint32_t)i == last ? ties : 0; };
+            uint64_t c = 0;
+            for (int i = b0; i < b1; i++) {
+                const uint64_t m = count(i);
+                if (m) c += m * R.weight(O.value(i));
+            }
+            const uint64_t upto = block_scan(c, &total), edge = top_p_edge(p, total);
+            if (upto >= edge && upto - c < edge) {
+                uint64_t s = upto - c, w = 0, m = 0;
+                int i = b0;
+                for (;; i++) {
+                    m = count(i);
+                    w = m ? R.weight(O.value(i)) : 0;
+                    if (s + m * w >= edge) break;
+                    s += m * w;
+                }
+                S.bin = i;
+                S.before = (edge - s + w - 1) / w;
+            }
+            __syncthreads();
+            last = (uint32_t)S.bin;
+            ties = S.before;
+        }
+        __syncthreads();
+    }
+    uint64_t wk = last < (uint32_t)n ? R.weight(O.value(last)) : 0;
+    if (wk < least) wk = 0;
+    for (int i = threadIdx.x; i < n; i += NT) {
+        const float f = O.value(i);
+        const uint64_t w = (uint32_t)i < last ? R.weight(f) : 0;
+        table[i] = w == 0 || w < least ? 0 : R.spike ? 0x3f800000u : __float_as_uint(expf((f - R.m) * R.inv));
+    }
+    __syncthreads();
+    auto kept = [&](uint32_t at) -> uint64_t {
+        if (at >= last) return 0;
+        const uint32_t u = table[at];
+        // the shift is past 63 only for 0
+        return u ? ((uint64_t)((u & 0x7fffffu) | 0x800000u) << 17) >> (127 - (u >> 23)) : 0;
+    };
+    finish_row(S, R, A, row, ties, wk, [&](const uint4 &q, int e, bool *same) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        const uint32_t at = O.place(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu);
+        *same = at == last && ties > 0;
+        return kept(at);
+    });
+}
+
+template <typename T>
+__global__ void __launch_bounds__(NT, 1) sample_kernel(const T *logits, int64_t ld, const Args A) {
     constexpr int N = Row<T>::N;
+    extern __shared__ uint32_t table[];
     __shared__ Shared S;
     const int64_t row = blockIdx.x, V = A.vocab;
     const int warp = threadIdx.x >> 5;
@@ -442,7 +680,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
     R.g1 = min(R.n, R.g0 + R.seg);
 
     float mine = -INFINITY;
-    R.each(R.g0, R.g1, [&](const uint4 &q, int) { mine = fmaxf(mine, Row<T>::largest(q)); });
+    R.template each<4>(R.g0, R.g1, [&](const uint4 &q, int) { mine = fmaxf(mine, Row<T>::largest(q)); });
     float m = mine;
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -473,6 +711,14 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
     } else {
         const int64_t k = A.top_k ? A.top_k[row] : 0;
         if (k > 0 && k <= kQuick && k < V && sample_quick(S, R, A, row, mine, (int)k, p, least)) return;
+        if constexpr (sizeof(T) == 2) {
+            // places down to the last value with weight (a little lower does no harm), if the table holds them
+            const float lowest = R.spike ? m : fmaxf(m - kSpan / R.inv, -3.0e38f);
+            const uint32_t top = Values<T>::order(raw_bits(from_f<T>(m)));
+            const uint32_t end = Values<T>::order(raw_bits(from_f<T>(lowest)));  // rounded to nearest: kSpan has room for it
+            const int n = (int)(top - end) + 2;
+            if (n <= A.places) return sample_values(S, table, R, A, row, n, k < V ? k : 0, p, least);
+        }
         if (k > 0 && k < V) {
             const Bins<T> H(kSpan, -INFINITY);
             clear(S);
@@ -533,119 +779,28 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
         }
     }
 
-    // Running sums by index, of each warp's granules first, then of 32 parts of the ones that hold the place.
     uint64_t wk = key ? R.weight(value_of(key)) : 0;
     if (wk < least) wk = 0;
     const float low = key ? value_of(key) : -INFINITY;
-    auto kept = [&](float f) -> uint64_t {
-        if (!(f > low)) return 0;
-        const uint64_t w = R.weight(f);
-        return w >= least ? w : 0;
-    };
-    // of granules a to b: the kept weight above the key, and how many tokens have it
-    auto sums = [&](int a, int b, uint64_t *sum, uint32_t *same) {
-        uint64_t s = 0;
-        uint32_t t = 0;
-        R.each(a, b, [&](const uint4 &q, int) {
-            if (Row<T>::largest(q) < low) return;
-            float f[N];
-            unpack<T>(q, f);
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                s += kept(f[e]);
-                t += key && f[e] == low;
-            }
-        });
-        *sum = warp_sum64(s);
-        *same = __reduce_add_sync(0xffffffffu, t);
-    };
-    // the part of NW parts that holds `at` once `before` and `left` ties lie before them; those are moved on
-    auto find = [&](uint64_t at, uint64_t *before, uint64_t *left, uint64_t *total) {
-        int found = NW - 1;
-        uint64_t b = *before, l = *left, fb = b, fl = l;
-        bool open = true;
-        for (int i = 0; i < NW; i++) {
-            const uint64_t t = S.ties[i] < l ? S.ties[i] : l, w = S.part[i] + t * wk;
-            if (open && b + w > at) {
-                open = false;
-                found = i;
-                fb = b;
-                fl = l;
-            }
-            b += w;
-            l -= t;
-        }
-        *total = b - *before;
-        *before = fb;
-        *left = fl;
-        return found;
-    };
-    uint64_t sum;
-    uint32_t same;
-    sums(R.g0, R.g1, &sum, &same);
-    __syncthreads();
-    if (R.lane == 0) {
-        S.part[warp] = sum;
-        S.ties[warp] = same;
-    }
-    __syncthreads();
-    uint64_t before = 0, left = ties, total, unused;
-    find(~0ull, &before, &left, &total);
-    const uint64_t at = place(A, row, total);
-    before = 0;
-    left = ties;
-    const int w0 = find(at, &before, &left, &unused);
-    // that warp's granules, in NW parts
-    const int a = min(R.n, w0 * R.seg), b = min(R.n, a + R.seg), sub = (b - a + NW - 1) / NW;
-    sums(min(b, a + warp * sub), min(b, a + (warp + 1) * sub), &sum, &same);
-    __syncthreads();
-    if (R.lane == 0) {
-        S.part[warp] = sum;
-        S.ties[warp] = same;
-    }
-    __syncthreads();
-    const int w1 = find(at, &before, &left, &unused);
-    if (warp != w1) return;
-    // one granule a lane
-    for (int g = min(b, a + w1 * sub), end = min(b, g + sub); g < end; g += 32) {
+    finish_row(S, R, A, row, ties, wk, [&](const uint4 &q, int e, bool *same) -> uint64_t {
         float f[N];
-        unpack<T>(g + R.lane < end ? R.load(g + R.lane) : make_uint4(0, 0, 0, 0), f);
-        uint64_t s[N], mine_ = 0;
-        uint32_t t = 0;
-#pragma unroll
-        for (int e = 0; e < N; e++) t += g + R.lane < end && key && f[e] == low;
-        uint32_t upto = t;  // ties up to this lane's last
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (R.lane >= o) upto += v;
-        }
-        uint64_t rank = upto - t;
-#pragma unroll
-        for (int e = 0; e < N; e++) {
-            uint64_t w = g + R.lane < end ? kept(f[e]) : 0;
-            if (g + R.lane < end && key && f[e] == low && rank++ < left) w = wk;
-            mine_ += w;
-            s[e] = mine_;
-        }
-        const uint64_t incl = warp_scan64(mine_, R.lane), excl = before + incl - mine_;
-        const uint32_t over = __ballot_sync(0xffffffffu, before + incl > at);
-        if (over) {
-            if (R.lane == __ffs(over) - 1) {
-                bool open = true;
-#pragma unroll
-                for (int e = 0; e < N; e++)
-                    if (open && excl + s[e] > at) {
-                        open = false;
-                        choose(A, row, R, R.index(g + R.lane, e), f[e], total);
-                    }
-            }
-            return;
-        }
-        before += __shfl_sync(0xffffffffu, incl, 31);
-        const uint64_t seen = __shfl_sync(0xffffffffu, upto, 31);
-        left -= seen < left ? seen : left;
-    }
+        unpack<T>(q, f);
+        *same = key && f[e] == low;
+        if (!(f[e] > low)) return 0;
+        const uint64_t w = R.weight(f[e]);
+        return w >= least ? w : 0;
+    });
+}
+
+template <typename T>
+int launch_sample(const T *logits, int64_t ld, const Args &A, int64_t rows, cudaStream_t s) {
+    auto f = sample_kernel<T>;
+    const size_t smem = sizeof(T) == 2 ? kPlaces * sizeof(uint32_t) : 0;
+    static int cache[64] = {0};
+    if (!blocks_per_sm(f, NT, smem, smem, cache)) return cuda_fail(cudaGetLastError(), "sample: occupancy");
+    f<<<(unsigned)rows, NT, smem, s>>>(logits, ld, A);
+    ZC_LAUNCHED("sample_kernel");
+    return ZPUCUDA_OK;
 }
 
 }  // namespace
@@ -664,9 +819,7 @@ extern "C" int zpucuda_sample(int dtype, const void *d_logits, int64_t ld, int u
     if (utype != ZPUCUDA_F32 && utype != ZPUCUDA_F64) return set_error(ZPUCUDA_ERR_NOT_SUPPORTED, "sample: uniform is not f32 or f64");
     if (rows == 0) return ZPUCUDA_OK;
     if (!d_uniform || !d_token) return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "sample: uniform or token: null pointer");
-    const Args A = {d_uniform, utype, d_temperature, d_top_k, d_top_p, d_min_p, d_token, d_logprob, vocab};
+    const Args A = {d_uniform, utype, d_temperature, d_top_k, d_top_p, d_min_p, d_token, d_logprob, vocab, kPlaces};
     cudaStream_t s = resolve_stream(stream);
-    ZC_HEAD_TYPE(dtype, T, sample_kernel<T><<<(unsigned)rows, NT, 0, s>>>((const T *)d_logits, ld, A));
-    ZC_LAUNCHED("sample_kernel");
-    return ZPUCUDA_OK;
+    ZC_HEAD_TYPE(dtype, T, return launch_sample((const T *)d_logits, ld, A, rows, s));
 }
