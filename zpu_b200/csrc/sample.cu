@@ -35,12 +35,12 @@
 namespace zc {
 namespace {
 
-constexpr int NT = 1024, NW = NT / 32;
+constexpr int NT = 512, NW = NT / 32;  // two blocks an SM
 constexpr int NB = 2048;                 // histogram bins
 constexpr int kList = 4096;              // tokens listed at most
 constexpr int kQuick = 400;              // first ranks that the threads' maxima bound well
 constexpr uint64_t kOne = 1ull << 40;
-constexpr int kPlaces = 44 * 1024;       // values of 16-bit logits in the table (176 KiB)
+constexpr int kPlaces = 20 * 1024;       // values of 16-bit logits in the table
 constexpr float kSpan = 28.0f;           // w = 0 beyond (max - x) / T = 40 ln 2 = 27.73
 constexpr int64_t kMaxVocab = (1 << 22) - 1;  // sums of weights stay below 2^62, of their 10-bit digits below 2^32
 
@@ -81,11 +81,16 @@ __device__ __forceinline__ uint64_t warp_scan64(uint64_t v, int lane) {
     return v;
 }
 
+// Dynamic shared memory: one of the three at a time.
+extern __shared__ __align__(16) uint32_t sample_smem[];
+constexpr size_t kSmem = 4 * NB * sizeof(uint32_t);
+static_assert(kSmem >= kList * sizeof(unsigned long long) && kPlaces * sizeof(uint32_t) >= kSmem, "shared memory");
+// a histogram: 10 bits of the weights each (a count: the first)
+__device__ __forceinline__ uint32_t &digit(int i, int b) { return sample_smem[i * NB + b]; }
+// tokens as key << 32 | ~index: sorted falling, ranks
+__device__ __forceinline__ unsigned long long &list(int i) { return ((unsigned long long *)sample_smem)[i]; }
+
 struct Shared {
-    union {
-        uint32_t digit[4][NB];            // a histogram: 10 bits of the weights each (a count: the first)
-        unsigned long long list[kList];   // key << 32 | ~index: sorted falling, ranks
-    };
     unsigned long long w[NT];
     unsigned long long part[NW];
     uint32_t ties[NW];
@@ -137,15 +142,14 @@ struct Row {
     }
     __device__ __forceinline__ float dist(float f) const { return f == m ? 0.0f : (f - m) * inv; }
     // The weight of a token at a distance: floor(2^40 e^d), the significand shifted into place (0 <= e^d <= 1).
-    static __device__ __forceinline__ uint64_t weigh(float d) {
-        const uint32_t u = __float_as_uint(expf(d));
+    static __device__ __forceinline__ uint64_t weigh_bits(uint32_t u) {
         return ((uint64_t)((u & 0x7fffffu) | 0x800000u) << 17) >> (127 - (u >> 23));
     }
     bool spike;  // only the largest logit has weight: it is infinite, or 1 / T is
     __device__ __forceinline__ uint64_t weight(float f) const {
         if (spike) return f == m ? kOne : 0;
         const float d = (f - m) * inv;
-        return d > -kSpan + 0.2f ? weigh(d) : 0;  // NaN: 0
+        return d > -kSpan + 0.2f ? weigh_bits(__float_as_uint(expf(d))) : 0;  // NaN: 0
     }
     __device__ __forceinline__ int64_t index(int g, int e) const { return (int64_t)g * N + e - skew; }
 };
@@ -157,44 +161,67 @@ __device__ __forceinline__ uint32_t entry_key(unsigned long long e) { return (ui
 __device__ __forceinline__ uint32_t entry_index(unsigned long long e) { return ~(uint32_t)e; }
 
 // The list's n entries in falling order.
-__device__ void sort_list(Shared &S, int n) {
-    int size = 32;
+__device__ void sort_list(int n) {
+    if (n <= 2 * NT) {  // each to the place of its rank
+        __syncthreads();
+        const int i = threadIdx.x, j = i + NT;
+        const unsigned long long a = i < n ? list(i) : 0, b = j < n ? list(j) : 0;
+        int ra = 0, rb = 0;
+        if (n <= NT) {
+            if (i < n)
+#pragma unroll 4
+                for (int k = 0; k < n; k++) ra += list(k) > a;
+        } else {
+#pragma unroll 4
+            for (int k = 0; k < n; k++) {
+                const unsigned long long e = list(k);
+                ra += e > a;
+                rb += e > b;
+            }
+        }
+        __syncthreads();
+        if (i < n) list(ra) = a;
+        if (j < n) list(rb) = b;
+        __syncthreads();
+        return;
+    }
+    int size = 4 * NT;
     while (size < n) size <<= 1;
-    for (int i = n + (int)threadIdx.x; i < size; i += NT) S.list[i] = 0;
+    for (int i = n + (int)threadIdx.x; i < size; i += NT) list(i) = 0;
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j; j >>= 1) {
             __syncthreads();
             for (int i = threadIdx.x; i < size / 2; i += NT) {
                 const int lo = (i / j) * 2 * j + i % j, hi = lo + j;
-                const unsigned long long a = S.list[lo], b = S.list[hi];
+                const unsigned long long a = list(lo), b = list(hi);
                 if ((a < b) == ((lo & k) == 0)) {
-                    S.list[lo] = b;
-                    S.list[hi] = a;
+                    list(lo) = b;
+                    list(hi) = a;
                 }
             }
         }
     __syncthreads();
 }
 
-__device__ void clear(Shared &S) {
+__device__ void clear() {
     __syncthreads();
-    for (int i = threadIdx.x; i < 4 * NB; i += NT) S.digit[0][i] = 0;
+    for (int i = threadIdx.x; i < 4 * NB; i += NT) digit(0, i) = 0;
     __syncthreads();
 }
-__device__ __forceinline__ uint64_t bin_value(const Shared &S, int b) {
-    return (uint64_t)S.digit[0][b] + ((uint64_t)S.digit[1][b] << 10) + ((uint64_t)S.digit[2][b] << 20) + ((uint64_t)S.digit[3][b] << 30);
+__device__ __forceinline__ uint64_t bin_value(int b) {
+    return (uint64_t)digit(0, b) + ((uint64_t)digit(1, b) << 10) + ((uint64_t)digit(2, b) << 20) + ((uint64_t)digit(3, b) << 30);
 }
 // MASS: the weight; otherwise one.
 template <bool MASS>
-__device__ __forceinline__ void bin_add(Shared &S, int b, uint64_t w) {
+__device__ __forceinline__ void bin_add(int b, uint64_t w) {
     if (!MASS) {
-        atomicAdd(&S.digit[0][b], 1u);
+        atomicAdd(&digit(0, b), 1u);
         return;
     }
-    atomicAdd(&S.digit[0][b], (uint32_t)w & 1023);
-    atomicAdd(&S.digit[1][b], (uint32_t)(w >> 10) & 1023);
-    atomicAdd(&S.digit[2][b], (uint32_t)(w >> 20) & 1023);
-    atomicAdd(&S.digit[3][b], (uint32_t)(w >> 30));
+    atomicAdd(&digit(0, b), (uint32_t)w & 1023);
+    atomicAdd(&digit(1, b), (uint32_t)(w >> 10) & 1023);
+    atomicAdd(&digit(2, b), (uint32_t)(w >> 20) & 1023);
+    atomicAdd(&digit(3, b), (uint32_t)(w >> 30));
 }
 
 // The first bin whose running sum reaches target, and (*before) the sum of the bins before it; -1 if none does.
@@ -205,7 +232,7 @@ __device__ int hist_find(Shared &S, uint64_t target, uint64_t *before) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint64_t v[PER], sum = 0;
 #pragma unroll
-    for (int i = 0; i < PER; i++) sum += v[i] = bin_value(S, threadIdx.x * PER + i);
+    for (int i = 0; i < PER; i++) sum += v[i] = bin_value(threadIdx.x * PER + i);
     uint64_t upto = warp_scan64(sum, lane);
     if (lane == 31) S.part[warp] = upto;
     __syncthreads();
@@ -271,7 +298,7 @@ __device__ uint32_t select_ranks(Shared &S, const Row<T> &R, const Bins<T> &H, u
                 kmin = min(kmin, k);
                 kmax = max(kmax, k);
                 const int i = atomicAdd(&S.count, 1);
-                if (i < kList) S.list[i] = entry_of(k, R.index(g, e));
+                if (i < kList) list(i) = entry_of(k, R.index(g, e));
             }
         });
         kmin = __reduce_min_sync(0xffffffffu, kmin);
@@ -286,12 +313,12 @@ __device__ uint32_t select_ranks(Shared &S, const Row<T> &R, const Bins<T> &H, u
         const int n = S.count;
         if (n <= kList || lo == hi) {
             if (lo != hi) {
-                sort_list(S, n);
+                sort_list(n);
                 // the entry at which the measure reaches target, and how many up to it have its key
                 uint64_t below = 0;
                 for (int i0 = 0; i0 < n; i0 += NT) {
                     const int i = i0 + (int)threadIdx.x, warp = threadIdx.x >> 5;
-                    const uint64_t w = i >= n ? 0 : MASS ? R.weight(value_of(entry_key(S.list[i]))) : 1;
+                    const uint64_t w = i >= n ? 0 : MASS ? R.weight(value_of(entry_key(list(i)))) : 1;
                     uint64_t upto = below + warp_scan64(w, R.lane);
                     if (R.lane == 31) S.part[warp] = upto - below;
                     __syncthreads();
@@ -300,14 +327,14 @@ __device__ uint32_t select_ranks(Shared &S, const Row<T> &R, const Bins<T> &H, u
                         below += S.part[v];
                     }
                     if (upto >= target && upto - w < target) {
-                        S.kmin = entry_key(S.list[i]);
+                        S.kmin = entry_key(list(i));
                         S.count = i;
                     }
                     __syncthreads();
                     if (below >= target) break;
                 }
                 int same = 0;
-                for (int i = threadIdx.x; i <= S.count; i += NT) same += entry_key(S.list[i]) == S.kmin;
+                for (int i = threadIdx.x; i <= S.count; i += NT) same += entry_key(list(i)) == S.kmin;
                 if (threadIdx.x == 0) S.before = 0;
                 __syncthreads();
                 if (same) atomicAdd(&S.before, (unsigned long long)same);
@@ -322,14 +349,14 @@ __device__ uint32_t select_ranks(Shared &S, const Row<T> &R, const Bins<T> &H, u
         // too many: a histogram of their keys, and again for the part that counts
         int shift = 0;
         while (((hi - lo) >> shift) >= NB) shift++;
-        clear(S);
+        clear();
         R.each(R.g0, R.g1, [&](const uint4 &q, int) {
             float f[N];
             unpack<T>(q, f);
 #pragma unroll
             for (int e = 0; e < N; e++) {
                 const uint32_t k = key_of(f[e]);
-                if (k >= lo && k <= hi) bin_add<MASS>(S, (hi - k) >> shift, MASS ? R.weight(f[e]) : 1);
+                if (k >= lo && k <= hi) bin_add<MASS>((hi - k) >> shift, MASS ? R.weight(f[e]) : 1);
             }
         });
         __syncthreads();
@@ -388,25 +415,17 @@ __device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t ro
         }
         __syncthreads();
     };
-    // the part of NW parts that holds `at` once `before` and `left` ties lie before them; those are moved on
+    // the part of NW parts that holds `at` once `before` and `left` ties lie before them; those are moved on.  A lane a part.
     auto find = [&](uint64_t at, uint64_t *before, uint64_t *left, uint64_t *total) {
-        int found = NW - 1;
-        uint64_t b = *before, l = *left, fb = b, fl = l;
-        bool open = true;
-        for (int i = 0; i < NW; i++) {
-            const uint64_t t = S.ties[i] < l ? S.ties[i] : l, w = S.part[i] + t * wk;
-            if (open && b + w > at) {
-                open = false;
-                found = i;
-                fb = b;
-                fl = l;
-            }
-            b += w;
-            l -= t;
-        }
-        *total = b - *before;
-        *before = fb;
-        *left = fl;
+        const uint32_t t = R.lane < NW ? S.ties[R.lane] : 0;
+        const uint64_t ties_before = warp_scan64(t, R.lane) - t, mine = *left > ties_before ? min(*left - ties_before, (uint64_t)t) : 0;
+        const uint64_t w = R.lane < NW ? S.part[R.lane] + mine * wk : 0, upto = warp_scan64(w, R.lane);
+        const uint32_t over = __ballot_sync(0xffffffffu, *before + upto > at);
+        const int found = over ? min(__ffs(over) - 1, NW - 1) : NW - 1;
+        *total = __shfl_sync(0xffffffffu, upto, 31);
+        *before += __shfl_sync(0xffffffffu, upto - w, found);
+        const uint64_t gone = __shfl_sync(0xffffffffu, ties_before, found);
+        *left -= min(*left, gone);
         return found;
     };
     sums(R.g0, R.g1);
@@ -479,7 +498,9 @@ __device__ bool sample_quick(Shared &S, const Row<T> &R, const Args &A, int64_t 
     uint32_t bound = 0;
     for (int bit = 31; bit >= 0; bit--) {
         const uint32_t t = bound | (1u << bit);
-        if (__syncthreads_count(key >= t) >= k) bound = t;
+        const int c = __syncthreads_count(key >= t);
+        if (c >= k) bound = t;
+        if (c == k) break;
     }
     bound = max(bound, 0x00800000u);  // the lowest finite value
     if (threadIdx.x == 0) S.count = 0;
@@ -493,16 +514,16 @@ __device__ bool sample_quick(Shared &S, const Row<T> &R, const Args &A, int64_t 
         for (int e = 0; e < N; e++)
             if (f[e] >= low) {
                 const int i = atomicAdd(&S.count, 1);
-                if (i < kList) S.list[i] = entry_of(key_of(f[e]), R.index(g, e));
+                if (i < kList) list(i) = entry_of(key_of(f[e]), R.index(g, e));
             }
     });
     __syncthreads();
     const int n = S.count;
     if (n > kList) return false;
-    sort_list(S, n);
+    sort_list(n);
     // a thread a rank
     const bool in = (int)threadIdx.x < min(k, n);
-    const unsigned long long e = in ? S.list[threadIdx.x] : 0;
+    const unsigned long long e = in ? list(threadIdx.x) : 0;
     const float f = value_of(entry_key(e));
     const uint32_t index = entry_index(e);
     uint64_t w = in ? R.weight(f) : 0;
@@ -533,138 +554,154 @@ __device__ bool sample_quick(Shared &S, const Row<T> &R, const Args &A, int64_t 
     uint64_t upto = 0;
     if (w)
         for (int j = 0; j < min(k, n); j++)
-            if (entry_index(S.list[j]) <= index) upto += S.w[j];
+            if (entry_index(list(j)) <= index) upto += S.w[j];
     if (w && upto > at && upto - w <= at) choose(A, row, R, (int64_t)index, f, total);
     return true;
 }
 
-// 16-bit logits as whole numbers: falling logits, rising places from the largest (0) on.  NaN has none (its place is
-// past all others).
+// 16-bit logits as whole numbers: falling logits, rising places from the largest's (0) on.  NaN has none (its place is
+// past all others).  Half of all values lie within 2^-6 of zero, and few logits: those share one place, `zero`, and are
+// treated one by one.
 template <typename T>
 struct Values {
-    uint32_t top;  // the order of the largest
-    static __device__ __forceinline__ uint32_t order(uint32_t raw) {  // rises with the value; -0 is 0
-        raw = raw == 0x8000u ? 0 : raw;
-        return raw & 0x8000u ? 0x7fffu - (raw & 0x7fffu) : raw + 0x7fffu;  // NaN: above +inf, or below -inf
+    static constexpr uint32_t kSmall = std::is_same<T, __half>::value ? 0x2400 : 0x3c80, kMiddle = 0x8000;  // 2^-6
+    uint32_t top, zero;  // the largest's order, the place of the values about zero
+    static __device__ __forceinline__ uint32_t order(uint32_t raw) {  // rises with the value
+        const uint32_t far = max(raw & 0x7fffu, kSmall) - kSmall;
+        return raw & 0x8000u ? kMiddle - far : kMiddle + far;
     }
-    __device__ __forceinline__ uint32_t place(uint32_t raw) const { return top - order(raw); }  // NaN above: wraps to far past all
+    __device__ __forceinline__ explicit Values(float m) {
+        top = order(raw_bits(from_f<T>(m)));
+        zero = top - kMiddle;
+    }
+    __device__ __forceinline__ uint32_t place(uint32_t raw) const { return top - order(raw); }
     __device__ __forceinline__ float value(uint32_t place_) const {
-        const uint32_t o = top - place_, raw = o >= 0x7fffu ? o - 0x7fffu : 0x8000u | (0x7fffu - o);
+        const uint32_t o = top - place_, raw = o >= kMiddle ? o - kMiddle + kSmall : 0x8000u | (kMiddle - o + kSmall);
         if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(raw << 16);
         else return __half2float(__ushort_as_half((unsigned short)raw));
     }
 };
 
 // The same choice for 16-bit logits by their values: counts of each value at `n` places from the largest on (what lies past
-// them has no weight), then in their place e^((x - max) / T) of those that are kept (0: not kept).
+// them has no weight), then in their place e^((x - max) / T) of those that are kept (0: not kept).  False: the ranks end
+// among the values about zero.
 template <typename T>
-__device__ void sample_values(Shared &S, uint32_t *table, const Row<T> &R, const Args &A, int64_t row, int n, int64_t k, float p,
-                              uint64_t least) {
+__device__ bool sample_values(Shared &S, const Row<T> &R, const Args &A, int64_t row, int n, int64_t k, float p, uint64_t least) {
     static_assert(sizeof(T) == 2, "16-bit logits");
+    uint32_t *table = sample_smem;
     const int lane = R.lane, warp = threadIdx.x >> 5;
-    const Values<T> O = {Values<T>::order(raw_bits(from_f<T>(R.m)))};
-    auto block_scan = [&](uint64_t v, uint64_t *total) {
-        const uint64_t upto = warp_scan64(v, lane);
-        __syncthreads();
-        if (lane == 31) S.part[warp] = upto;
-        __syncthreads();
-        uint64_t below = 0, all = 0;
-        for (int i = 0; i < NW; i++) {
-            if (i < warp) below += S.part[i];
-            all += S.part[i];
-        }
-        *total = all;
-        return below + upto;
+    const Values<T> O(R.m);
+    auto raw_of = [](const uint4 &q, int e) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        return e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
     };
-    const int per = (n + NT - 1) / NT, b0 = min(n, (int)threadIdx.x * per), b1 = min(n, b0 + per);  // a thread's places
+    auto float_of = [](uint32_t raw) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(raw << 16);
+        else return __half2float(__ushort_as_half((unsigned short)raw));
+    };
     // The kept ranks: places below `last`, and the first `ties` tokens at it.
     uint32_t last = (uint32_t)n;
     uint64_t ties = 0;
     if (k > 0 || p < 1.0f) {
         for (int i = threadIdx.x; i < n; i += NT) table[i] = 0;
         __syncthreads();
+        uint64_t about = 0;  // the weight of the values about zero
         R.template each<4>(R.g0, R.g1, [&](const uint4 &q, int) {
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const uint32_t at = O.place(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu);
+                const uint32_t raw = raw_of(q, e), at = O.place(raw);
                 if (at < (uint32_t)n) atomicAdd(&table[at], 1u);
+                if (at == O.zero && p < 1.0f) about += R.weight(float_of(raw));
             }
         });
+        about = warp_sum64(about);
+        if (lane == 0) S.w[warp] = about;
         __syncthreads();
-        uint64_t total;
-        if (k > 0) {
+        about = 0;
+        for (int i = 0; i < NW; i++) about += S.w[i];
+        // A warp has a run of places.  What they measure, and the place at which the running measure reaches target, with
+        // what is left of the target there; all threads get both (n: it does not reach target).
+        const int per = (n + NT - 1) / NT * 32, b0 = min(n, warp * per), b1 = min(n, b0 + per);
+        auto reach = [&](auto measure, auto target_of, uint64_t *rest) {
             uint64_t c = 0;
-            for (int i = b0; i < b1; i++) c += table[i];
-            uint64_t upto = block_scan(c, &total);
-            if (threadIdx.x == 0) S.bin = -1;
+            for (int i = b0 + lane; i < b1; i += 32) c += measure(i);
+            c = warp_sum64(c);
             __syncthreads();
-            if (upto >= (uint64_t)k && upto - c < (uint64_t)k) {
-                uint64_t s = upto - c;
-                int i = b0;
-                while (s + table[i] < (uint64_t)k) s += table[i++];
-                S.bin = i;
-                S.before = (uint64_t)k - s;
+            if (lane == 0) S.part[warp] = c;
+            if (threadIdx.x == 0) S.bin = n;
+            __syncthreads();
+            uint64_t before = 0, total = 0;
+            for (int i = 0; i < NW; i++) {
+                before += i < warp ? S.part[i] : 0;
+                total += S.part[i];
+            }
+            const uint64_t target = target_of(total);
+            if (before < target && before + c >= target) {  // this warp's, a run of places a lane
+                const int run = (b1 - b0 + 31) / 32, r0 = min(b1, b0 + lane * run), r1 = min(b1, r0 + run);
+                uint64_t v = 0;
+                for (int i = r0; i < r1; i++) v += measure(i);
+                uint64_t s = before + warp_scan64(v, lane) - v;
+                if (s < target && s + v >= target)
+                    for (int i = r0; i < r1; i++) {
+                        const uint64_t m = measure(i);
+                        if (s + m >= target) {
+                            S.bin = i;
+                            S.before = target - s;
+                            break;
+                        }
+                        s += m;
+                    }
             }
             __syncthreads();
-            if (S.bin >= 0) {
-                last = (uint32_t)S.bin;
-                ties = S.before;
-            }
+            *rest = S.before;
+            return (uint32_t)S.bin;
+        };
+        if (k > 0) {
+            last = reach([&](int i) -> uint64_t { return table[i]; }, [&](uint64_t) { return (uint64_t)k; }, &ties);
+            if (last == (uint32_t)n) ties = 0;
+            if (last == O.zero) return false;
         }
         if (p < 1.0f) {
-            // of a value's tokens, those that top_k leaves
-            auto count = [&](int i) -> uint64_t { return (uint32_t)i < last ? table[i] : (uint32_t)i == last ? ties : 0; };
-            uint64_t c = 0;
-            for (int i = b0; i < b1; i++) {
-                const uint64_t m = count(i);
-                if (m) c += m * R.weight(O.value(i));
-            }
-            const uint64_t upto = block_scan(c, &total), edge = top_p_edge(p, total);
-            if (upto >= edge && upto - c < edge) {
-                uint64_t s = upto - c, w = 0, m = 0;
-                int i = b0;
-                for (;; i++) {
-                    m = count(i);
-                    w = m ? R.weight(O.value(i)) : 0;
-                    if (s + m * w >= edge) break;
-                    s += m * w;
-                }
-                S.bin = i;
-                S.before = (edge - s + w - 1) / w;
-            }
-            __syncthreads();
-            last = (uint32_t)S.bin;
-            ties = S.before;
+            const uint32_t end = last;
+            const uint64_t some = ties;  // of the end's tokens, those that top_k leaves
+            uint64_t rest;
+            last = reach(
+                [&](int i) -> uint64_t {
+                    const uint64_t m = (uint32_t)i < end ? table[i] : (uint32_t)i == end ? some : 0;
+                    return (uint32_t)i == O.zero ? (m ? about : 0) : m ? m * R.weight(O.value(i)) : 0;
+                },
+                [&](uint64_t total) { return top_p_edge(p, total); }, &rest);
+            if (last == O.zero || last == (uint32_t)n) return false;
+            const uint64_t w = R.weight(O.value(last));
+            ties = (rest + w - 1) / w;
         }
         __syncthreads();
     }
     uint64_t wk = last < (uint32_t)n ? R.weight(O.value(last)) : 0;
     if (wk < least) wk = 0;
     for (int i = threadIdx.x; i < n; i += NT) {
-        const float f = O.value(i);
-        const uint64_t w = (uint32_t)i < last ? R.weight(f) : 0;
-        table[i] = w == 0 || w < least ? 0 : R.spike ? 0x3f800000u : __float_as_uint(expf((f - R.m) * R.inv));
+        const float f = O.value(i), d = R.spike ? 0.0f : (f - R.m) * R.inv, e = expf(d);
+        const uint64_t w = R.spike ? (f == R.m ? kOne : 0) : d > -kSpan + 0.2f ? Row<T>::weigh_bits(__float_as_uint(e)) : 0;
+        table[i] = (uint32_t)i >= last || w == 0 || w < least ? 0 : __float_as_uint(e);
     }
     __syncthreads();
-    auto kept = [&](uint32_t at) -> uint64_t {
-        if (at >= last) return 0;
-        const uint32_t u = table[at];
-        // the shift is past 63 only for 0
-        return u ? ((uint64_t)((u & 0x7fffffu) | 0x800000u) << 17) >> (127 - (u >> 23)) : 0;
-    };
-    finish_row(S, R, A, row, ties, wk, [&](const uint4 &q, int e, bool *same) {
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        const uint32_t at = O.place(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu);
+    finish_row(S, R, A, row, ties, wk, [&](const uint4 &q, int e, bool *same) -> uint64_t {
+        const uint32_t raw = raw_of(q, e), at = O.place(raw);
         *same = at == last && ties > 0;
-        return kept(at);
+        if (at >= last) return 0;
+        if (at == O.zero) {
+            const uint64_t w = R.weight(float_of(raw));
+            return w >= least ? w : 0;
+        }
+        const uint32_t u = table[at];
+        return u ? Row<T>::weigh_bits(u) : 0;
     });
+    return true;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT, 1) sample_kernel(const T *logits, int64_t ld, const Args A) {
+__global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t ld, const Args A) {
     constexpr int N = Row<T>::N;
-    extern __shared__ uint32_t table[];
     __shared__ Shared S;
     const int64_t row = blockIdx.x, V = A.vocab;
     const int warp = threadIdx.x >> 5;
@@ -714,21 +751,19 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const T *logits, int64_t 
         if constexpr (sizeof(T) == 2) {
             // places down to the last value with weight (a little lower does no harm), if the table holds them
             const float lowest = R.spike ? m : fmaxf(m - kSpan / R.inv, -3.0e38f);
-            const uint32_t top = Values<T>::order(raw_bits(from_f<T>(m)));
-            const uint32_t end = Values<T>::order(raw_bits(from_f<T>(lowest)));  // rounded to nearest: kSpan has room for it
-            const int n = (int)(top - end) + 2;
-            if (n <= A.places) return sample_values(S, table, R, A, row, n, k < V ? k : 0, p, least);
+            const int n = (int)Values<T>(m).place(raw_bits(from_f<T>(lowest))) + 2;  // lowest is rounded to nearest: kSpan has room
+            if (n <= A.places && sample_values(S, R, A, row, n, k < V ? k : 0, p, least)) return;
         }
         if (k > 0 && k < V) {
             const Bins<T> H(kSpan, -INFINITY);
-            clear(S);
+            clear();
             R.each(R.g0, R.g1, [&](const uint4 &q, int) {
                 float f[N];
                 unpack<T>(q, f);
 #pragma unroll
                 for (int e = 0; e < N; e++) {
                     const int b = H.at(f[e], R.dist(f[e]));
-                    if (b >= 0) bin_add<false>(S, b, 1);
+                    if (b >= 0) bin_add<false>(b, 1);
                 }
             });
             key = select_ranks<T, false>(S, R, H, (uint64_t)k, &ties);
@@ -742,7 +777,7 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const T *logits, int64_t 
             sure = warp_sum64(sure);
             __syncthreads();
             if (R.lane == 0) S.part[warp] = sure;
-            clear(S);
+            clear();
             sure = 0;
             for (int i = 0; i < NW; i++) sure += S.part[i];
             if (sure < kOne) sure = kOne;
@@ -759,7 +794,7 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const T *logits, int64_t 
                     const uint64_t w = f[e] > low ? R.weight(f[e]) : 0;
                     sum += w;
                     const int b = H.at(f[e], d);
-                    if (b >= 0) bin_add<true>(S, b, w);
+                    if (b >= 0) bin_add<true>(b, w);
                 }
             });
             sum = warp_sum64(sum);
@@ -795,7 +830,7 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const T *logits, int64_t 
 template <typename T>
 int launch_sample(const T *logits, int64_t ld, const Args &A, int64_t rows, cudaStream_t s) {
     auto f = sample_kernel<T>;
-    const size_t smem = sizeof(T) == 2 ? kPlaces * sizeof(uint32_t) : 0;
+    const size_t smem = sizeof(T) == 2 ? kPlaces * sizeof(uint32_t) : kSmem;
     static int cache[64] = {0};
     if (!blocks_per_sm(f, NT, smem, smem, cache)) return cuda_fail(cudaGetLastError(), "sample: occupancy");
     f<<<(unsigned)rows, NT, smem, s>>>(logits, ld, A);
