@@ -9,18 +9,36 @@ along the row and with any row pitch (a slice of a wider tensor is read in
 place); results are new tensors unless `out` names one.  With `stream`, the
 call runs on that torch stream and its new tensors belong to it.
 """
-from . import _capi
+import functools
+
+from . import CUDA_STREAM_LEGACY, _capi
 from ._capi import check, lib
 
 
+@functools.cache
 def _torch():
     import torch
     return torch
 
 
-def _stream(stream):
-    from . import stream_of
-    return stream_of(stream)
+@functools.cache
+def _codes():
+    torch = _torch()
+    return {torch.float32: _capi.F32, torch.float16: 2, torch.bfloat16: _capi.DT_BF16}
+
+
+def _stream(stream, x):
+    """The cudaStream_t that a call on x runs on.  A launch goes to the current
+    device, so x has to be there.  (The current stream's handle without a
+    Stream object around it: a call on one token is the shorter by 2 us.)"""
+    torch = _torch()
+    dev = x.get_device()
+    if dev != torch._C._cuda_getDevice():
+        _refuse(12, "the tensors are on %s, the current device is cuda:%d" % (x.device, torch._C._cuda_getDevice()))
+    h = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    # torch's default stream is the legacy NULL stream; NULL means the thread's
+    # own stream to the C ABI, so it is named as cudaStreamLegacy.
+    return h if h else CUDA_STREAM_LEGACY
 
 
 def _refuse(status, text):
@@ -28,34 +46,33 @@ def _refuse(status, text):
 
 
 def _code(name, t):
-    torch = _torch()
-    if t.dtype == torch.float32:
-        return _capi.F32
-    if t.dtype == torch.float16:
-        return 2
-    if t.dtype == torch.bfloat16:
-        return _capi.DT_BF16
-    _refuse(9, "%s: dtype %s is not float32, float16 or bfloat16" % (name, t.dtype))
+    code = _codes().get(t.dtype)
+    if code is None:
+        _refuse(9, "%s: dtype %s is not float32, float16 or bfloat16" % (name, t.dtype))
+    return code
 
 
 def _matrix(name, t, like=None, shape=None):
     """Checks a [rows, n] argument; its row pitch in elements."""
-    if t.dim() != 2:
-        _refuse(5, "%s: %d axes, [rows, n] is wanted" % (name, t.dim()))
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        _refuse(2, "%s: shape %s, %s is wanted" % (name, tuple(t.shape), tuple(shape)))
+    size = t.shape
+    if len(size) != 2:
+        _refuse(5, "%s: %d axes, [rows, n] is wanted" % (name, len(size)))
+    if shape is not None and size != shape:
+        _refuse(2, "%s: shape %s, %s is wanted" % (name, tuple(size), tuple(shape)))
     _device(name, t, like)
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    ld, step = t.stride()
+    rows, n = size
+    if step != 1 and n > 1:
         _refuse(7, "%s: its rows are not contiguous" % name)
-    # torch leaves the stride of an axis of one (or no) row arbitrary
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if ld < t.shape[1]:
+    if rows <= 1:  # torch leaves the stride of an axis of one (or no) row arbitrary
+        return n
+    if ld < n:
         _refuse(7, "%s: its rows overlap" % name)
     return ld
 
 
 def _device(name, t, like=None):
-    if not t.is_cuda or (like is not None and t.device != like.device):
+    if not t.is_cuda or (like is not None and t.get_device() != like.get_device()):
         _refuse(12, "%s is on %s" % (name, t.device if like is None or not t.is_cuda
                                      else "%s, not %s" % (t.device, like.device)))
 
@@ -64,7 +81,7 @@ def _vector(name, t, n, like, dtype=None):
     """Checks an optional [n] argument; its address."""
     if t is None:
         return None
-    if tuple(t.shape) != (n,):
+    if t.shape != (n,):
         _refuse(2, "%s: shape %s, (%d,) is wanted" % (name, tuple(t.shape), n))
     if dtype is not None and t.dtype != dtype:
         _refuse(3, "%s: dtype %s, %s is wanted" % (name, t.dtype, dtype))
@@ -76,21 +93,31 @@ def _vector(name, t, n, like, dtype=None):
 
 def _output(name, out, like, shape=None, dtype=None):
     """`out`, checked, or a new tensor; and its row pitch."""
-    shape = tuple(like.shape) if shape is None else shape
-    dtype = like.dtype if dtype is None else dtype
+    if shape is None:
+        shape = like.shape
+    if dtype is None:
+        dtype = like.dtype
     if out is None:
-        return _torch().empty(shape, dtype=dtype, device=like.device), shape[1]
+        return like.new_empty(shape, dtype=dtype), shape[1]
     if out.dtype != dtype:
         _refuse(3, "%s: dtype %s, %s is wanted" % (name, out.dtype, dtype))
     return out, _matrix(name, out, like, shape)
 
 
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *_):
+        pass
+
+
+_here = _Here()
+
+
 def _on(stream):
     """New tensors of the block belong to the stream that the call runs on."""
-    if stream is None:
-        import contextlib
-        return contextlib.nullcontext()
-    return _torch().cuda.stream(stream)
+    return _here if stream is None else _torch().cuda.stream(stream)
 
 
 # ------------------------------------------------------------- layer norm
@@ -113,11 +140,11 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, out=None, stats=False, stream
     rows, cols = x.shape
     with _on(stream):
         y, ldy = _output("out", out, x)
-        mean = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
-        rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
+        if stats:
+            mean, rstd = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
     check(lib().zpucuda_layer_norm(code, x.data_ptr(), ldx, wt, g, b, y.data_ptr(), ldy,
                                    mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None,
-                                   rows, cols, eps, _stream(stream)))
+                                   rows, cols, eps, _stream(stream, x)))
     return (y, mean, rstd) if stats else y
 
 
@@ -141,7 +168,7 @@ def layer_norm_grad(dy, x, mean, rstd, gamma=None, out=None, stream=None):
         work = torch.empty(lib().zpucuda_layer_norm_grad_work(rows, cols), dtype=torch.uint8, device=x.device)
     check(lib().zpucuda_layer_norm_grad(code, dy.data_ptr(), lddy, x.data_ptr(), ldx, m, r, wt, g, dx.data_ptr(), lddx,
                                         dgamma.data_ptr(), dbeta.data_ptr(), rows, cols, work.data_ptr(), work.numel(),
-                                        _stream(stream)))
+                                        _stream(stream, x)))
     return dx, dgamma, dbeta
 
 
@@ -172,7 +199,8 @@ def distill_loss(logits, teacher, indices, temperature=1.0, weight=None, stream=
     with _on(stream):
         loss = torch.empty(dims[0], dtype=torch.float32, device=logits.device)
         lse = torch.empty_like(loss)
-    check(lib().zpucuda_distill_loss(*head, temperature, loss.data_ptr(), lse.data_ptr(), *dims, _stream(stream)))
+    check(lib().zpucuda_distill_loss(*head, temperature, loss.data_ptr(), lse.data_ptr(), *dims,
+                                     _stream(stream, logits)))
     return loss, lse
 
 
@@ -185,7 +213,8 @@ def distill_grad(logits, teacher, indices, lse, dloss=None, temperature=1.0, wei
     d = _vector("dloss", dloss, dims[0], logits, torch.float32)
     with _on(stream):
         g, ldg = _output("out", out, logits)
-    check(lib().zpucuda_distill_grad(*head, temperature, l, d, g.data_ptr(), ldg, *dims, _stream(stream)))
+    check(lib().zpucuda_distill_grad(*head, temperature, l, d, g.data_ptr(), ldg, *dims,
+                                     _stream(stream, logits)))
     return g
 
 
@@ -199,7 +228,7 @@ def distill_value_and_grad(logits, teacher, indices, dloss=None, temperature=1.0
         loss = torch.empty(dims[0], dtype=torch.float32, device=logits.device)
         g, ldg = _output("out", out, logits)
     check(lib().zpucuda_distill_value_and_grad(*head, temperature, d, loss.data_ptr(), g.data_ptr(), ldg, *dims,
-                                               _stream(stream)))
+                                               _stream(stream, logits)))
     return loss, g
 
 
@@ -214,7 +243,7 @@ def quantize_rows(x, stream=None):
         q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :cols]
         scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     check(lib().zpucuda_int8_quantize(code, x.data_ptr(), ldx, q.data_ptr(), _matrix("q", q), scale.data_ptr(),
-                                      rows, cols, _stream(stream)))
+                                      rows, cols, _stream(stream, x)))
     return q, scale
 
 
@@ -242,7 +271,7 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=None, out=None, stream=
     with _on(stream):
         y, ldy = _output("out", out, a, (m, n), dtype)
     check(lib().zpucuda_int8_matmul(a.data_ptr(), lda, sa, b.data_ptr(), ldb, sb, bi, _code("out", y), y.data_ptr(),
-                                    ldy, m, n, k, _stream(stream)))
+                                    ldy, m, n, k, _stream(stream, a)))
     return y
 
 
@@ -280,11 +309,11 @@ class Int8Linear:
             _refuse(2, "x is %s, the weight %s" % (tuple(x.shape), tuple(self.weight.shape)))
         with _on(stream):
             y, ldy = _output("out", out, x, (rows, cols))
-            work = torch.empty(lib().zpucuda_int8_linear_work(rows, inner), dtype=torch.uint8, device=x.device)
+            work = x.new_empty(lib().zpucuda_int8_linear_work(rows, inner), dtype=torch.uint8)
         check(lib().zpucuda_int8_linear(code, x.data_ptr(), ldx, self.weight.data_ptr(), self._ld,
                                         self.scale.data_ptr(), None if self.bias is None else self.bias.data_ptr(),
                                         y.data_ptr(), ldy, rows, cols, inner, work.data_ptr(), work.numel(),
-                                        _stream(stream)))
+                                        _stream(stream, x)))
         return y
 
 
@@ -318,5 +347,5 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
         token = torch.empty(rows, dtype=torch.int64, device=logits.device)
         logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
     check(lib().zpucuda_sample(code, logits.data_ptr(), ld, 0 if uniform.dtype == torch.float64 else 1, u, *rules,
-                               token.data_ptr(), logprob.data_ptr(), rows, vocab, _stream(stream)))
+                               token.data_ptr(), logprob.data_ptr(), rows, vocab, _stream(stream, logits)))
     return token, logprob
