@@ -30,6 +30,8 @@
 //     that of computing one for every token.
 // Instructions bound it, not HBM: a few for each token in each pass, an exponential
 // among them for 32-bit logits.
+#include <cstring>
+
 #include "head.cuh"
 
 namespace zc {
@@ -118,22 +120,33 @@ struct Row {
         for (int e = 0; e < N; e++) f[e] = at + e >= 0 && at + e < vocab ? to_f(x[(int64_t)g * N + e]) : -INFINITY;
         return pack<T>(f);  // exact: the values come from that type
     }
-    // f(granule's bytes, its number) for each of this lane's granules from a to b, U loads in flight; lanes past the end
-    // are left out.
+    // f(granule's bytes, its number) for each of this lane's granules from a to b, U loads in flight: the whole ones, then
+    // the first and the last of the row; lanes past the end are left out.
     template <int U = 2, typename F>
     __device__ __forceinline__ void each(int a, int b, F f) const {
-        for (int g = a + lane; g < b; g += 32 * U) {
+        const int first = skew ? 1 : 0, last = (skew + vocab) % N ? n - 1 : n;  // the whole granules of the row
+        const int b1 = min(b, last);
+        for (int g = max(a, first) + lane; g < b1; g += 32 * U) {
             uint4 q[U];
 #pragma unroll
             for (int u = 0; u < U; u++)
-                if (g + 32 * u < b) q[u] = load(g + 32 * u);
+                if (g + 32 * u < b1) q[u] = __ldcg((const uint4 *)(x + (int64_t)(g + 32 * u) * N));
 #pragma unroll
             for (int u = 0; u < U; u++)
-                if (g + 32 * u < b) f(q[u], g + 32 * u);
+                if (g + 32 * u < b1) f(q[u], g + 32 * u);
         }
+        const int g = lane == 0 ? 0 : n - 1;
+        if (lane < 2 && g >= a && g < b && (lane == 0 ? first == 1 : last < n && (n > 1 || first == 0))) f(load(g), g);
         __syncwarp();
     }
     static __device__ __forceinline__ float largest(const uint4 &q) {  // passes NaN over
+        if constexpr (sizeof(T) == 2) {
+            using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+            T2 h[4];
+            memcpy(h, &q, 16);
+            const T2 t = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            return fmaxf(fmaxf(-INFINITY, to_f(t.x)), to_f(t.y));
+        }
         float f[N], t = -INFINITY;
         unpack<T>(q, f);
 #pragma unroll
@@ -388,25 +401,48 @@ __device__ __forceinline__ void choose(const Args &A, int64_t row, const Row<T> 
     if (A.logprob) A.logprob[row] = R.dist(f) - logf((float)(int64_t)total / (float)kOne);
 }
 
-// The token whose running sum by index exceeds the place: kept(granule, element, &same) is a token's kept weight, or 0 and
-// same = true for a token of the last kept key, of which the first `ties` weigh wk each.  Sums of each warp's granules first,
-// then of NW parts of the ones that hold the place, then of those.
-template <typename T, typename K>
-__device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t row, uint64_t ties, uint64_t wk, K kept) {
+// What is kept: tokens above `low` whose e^((x - max) / T) is at least `least`, and the first `ties` equal to `low`, which
+// weigh wk each.
+struct Kept {
+    float low, least;
+    uint64_t ties, wk;
+    template <typename T>
+    __device__ __forceinline__ float power(const Row<T> &R, float f) const {  // e^..., 0: not kept
+        const float e = expf((f - R.m) * R.inv);
+        return f > low && e >= least ? e : 0.0f;
+    }
+};
+
+// The token whose running sum of kept weights by index exceeds the place.  Sums of each warp's granules first, then of NW
+// parts of the ones that hold the place, then of those.
+//
+// A weight is summed as two whole numbers of 20 bits, floor(2^20 e) and floor(2^40 (e - the first / 2^20)): adding 8 = 2^3
+// to e with rounding towards zero leaves the first in the last bits of the sum, adding 2^-17 to the exact rest the second.
+template <typename T>
+__device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t row, const Kept K) {
     constexpr int N = Row<T>::N;
+    const uint64_t ties = K.ties, wk = K.wk;
     const int warp = threadIdx.x >> 5;
-    auto sums = [&](int a, int b) {  // of granules a to b, to S
-        uint64_t s = 0;
+    auto add = [&](int a, int b, auto tied) {  // of granules a to b, to S
+        constexpr uint32_t k3 = 0x41000000u, k17 = 0x37000000u;  // 2^3, 2^-17
+        uint64_t high = 0, low = 0;
         uint32_t t = 0;
-        R.each(a, b, [&](const uint4 &q, int) {
+        R.template each<2>(a, b, [&](const uint4 &q, int) {
+            float f[N];
+            unpack<T>(q, f);
+            uint32_t h = -N * k3, l = -N * k17;
 #pragma unroll
             for (int e = 0; e < N; e++) {
-                bool same;
-                s += kept(q, e, &same);
-                t += same;
+                const float p = K.power(R, f[e]);
+                const float hi = __fadd_rz(p, __uint_as_float(k3)), rest = p - (hi - __uint_as_float(k3));
+                h += __float_as_uint(hi);
+                l += __float_as_uint(__fadd_rz(rest, __uint_as_float(k17)));
+                if (decltype(tied)::value) t += f[e] == K.low;
             }
+            high += h;
+            low += l;
         });
-        s = warp_sum64(s);
+        const uint64_t s = warp_sum64((high << 20) + low);
         t = __reduce_add_sync(0xffffffffu, t);
         __syncthreads();
         if (R.lane == 0) {
@@ -414,6 +450,10 @@ __device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t ro
             S.ties[warp] = t;
         }
         __syncthreads();
+    };
+    auto sums = [&](int a, int b) {
+        if (ties) add(a, b, std::true_type());
+        else add(a, b, std::false_type());
     };
     // the part of NW parts that holds `at` once `before` and `left` ties lie before them; those are moved on.  A lane a part.
     auto find = [&](uint64_t at, uint64_t *before, uint64_t *left, uint64_t *total) {
@@ -449,9 +489,8 @@ __device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t ro
         uint32_t t = 0;
 #pragma unroll
         for (int e = 0; e < N; e++) {
-            bool same;
-            s[e] = kept(q, e, &same);
-            t += in && same;
+            s[e] = Row<T>::weigh_bits(__float_as_uint(K.power(R, f[e])));
+            t += in && f[e] == K.low;
         }
         uint32_t upto = t;  // ties up to this lane's last
 #pragma unroll
@@ -462,9 +501,7 @@ __device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t ro
         uint64_t rank = upto - t;
 #pragma unroll
         for (int e = 0; e < N; e++) {
-            bool same;
-            kept(q, e, &same);
-            if (in && same && rank++ < left) s[e] = wk;
+            if (in && f[e] == K.low && rank++ < left) s[e] = wk;
             sum += in ? s[e] : 0;
             s[e] = sum;
         }
@@ -582,11 +619,11 @@ struct Values {
     }
 };
 
-// The same choice for 16-bit logits by their values: counts of each value at `n` places from the largest on (what lies past
-// them has no weight), then in their place e^((x - max) / T) of those that are kept (0: not kept).  False: the ranks end
-// among the values about zero.
+// The kept ranks of 16-bit logits (k > 0 or p < 1) from counts of each value at `n` places from the largest on (what lies
+// past them has no weight): the key of the last, 0: all, and in *ties how many of that key.  False: the ranks end among the
+// values about zero.
 template <typename T>
-__device__ bool sample_values(Shared &S, const Row<T> &R, const Args &A, int64_t row, int n, int64_t k, float p, uint64_t least) {
+__device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, float p, uint32_t *key, uint64_t *ties_) {
     static_assert(sizeof(T) == 2, "16-bit logits");
     uint32_t *table = sample_smem;
     const int lane = R.lane, warp = threadIdx.x >> 5;
@@ -602,100 +639,81 @@ __device__ bool sample_values(Shared &S, const Row<T> &R, const Args &A, int64_t
     // The kept ranks: places below `last`, and the first `ties` tokens at it.
     uint32_t last = (uint32_t)n;
     uint64_t ties = 0;
-    if (k > 0 || p < 1.0f) {
-        for (int i = threadIdx.x; i < n; i += NT) table[i] = 0;
-        __syncthreads();
-        uint64_t about = 0;  // the weight of the values about zero
-        R.template each<4>(R.g0, R.g1, [&](const uint4 &q, int) {
+    for (int i = threadIdx.x; i < n; i += NT) table[i] = 0;
+    __syncthreads();
+    uint64_t about = 0;  // the weight of the values about zero
+    R.template each<4>(R.g0, R.g1, [&](const uint4 &q, int) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint32_t raw = raw_of(q, e), at = O.place(raw);
-                if (at < (uint32_t)n) atomicAdd(&table[at], 1u);
-                if (at == O.zero && p < 1.0f) about += R.weight(float_of(raw));
-            }
-        });
-        about = warp_sum64(about);
-        if (lane == 0) S.w[warp] = about;
+        for (int e = 0; e < 8; e++) {
+            const uint32_t raw = raw_of(q, e), at = O.place(raw);
+            if (at < (uint32_t)n) atomicAdd(&table[at], 1u);
+            if (at == O.zero && p < 1.0f) about += R.weight(float_of(raw));
+        }
+    });
+    about = warp_sum64(about);
+    if (lane == 0) S.w[warp] = about;
+    __syncthreads();
+    about = 0;
+    for (int i = 0; i < NW; i++) about += S.w[i];
+    // A warp has a run of places.  What they measure, and the place at which the running measure reaches target, with
+    // what is left of the target there; all threads get both (n: it does not reach target).
+    const int per = (n + NT - 1) / NT * 32, b0 = min(n, warp * per), b1 = min(n, b0 + per);
+    auto reach = [&](auto measure, auto target_of, uint64_t *rest) {
+        uint64_t c = 0;
+        for (int i = b0 + lane; i < b1; i += 32) c += measure(i);
+        c = warp_sum64(c);
         __syncthreads();
-        about = 0;
-        for (int i = 0; i < NW; i++) about += S.w[i];
-        // A warp has a run of places.  What they measure, and the place at which the running measure reaches target, with
-        // what is left of the target there; all threads get both (n: it does not reach target).
-        const int per = (n + NT - 1) / NT * 32, b0 = min(n, warp * per), b1 = min(n, b0 + per);
-        auto reach = [&](auto measure, auto target_of, uint64_t *rest) {
-            uint64_t c = 0;
-            for (int i = b0 + lane; i < b1; i += 32) c += measure(i);
-            c = warp_sum64(c);
-            __syncthreads();
-            if (lane == 0) S.part[warp] = c;
-            if (threadIdx.x == 0) S.bin = n;
-            __syncthreads();
-            uint64_t before = 0, total = 0;
-            for (int i = 0; i < NW; i++) {
-                before += i < warp ? S.part[i] : 0;
-                total += S.part[i];
-            }
-            const uint64_t target = target_of(total);
-            if (before < target && before + c >= target) {  // this warp's, a run of places a lane
-                const int run = (b1 - b0 + 31) / 32, r0 = min(b1, b0 + lane * run), r1 = min(b1, r0 + run);
-                uint64_t v = 0;
-                for (int i = r0; i < r1; i++) v += measure(i);
-                uint64_t s = before + warp_scan64(v, lane) - v;
-                if (s < target && s + v >= target)
-                    for (int i = r0; i < r1; i++) {
-                        const uint64_t m = measure(i);
-                        if (s + m >= target) {
-                            S.bin = i;
-                            S.before = target - s;
-                            break;
-                        }
-                        s += m;
+        if (lane == 0) S.part[warp] = c;
+        if (threadIdx.x == 0) S.bin = n;
+        __syncthreads();
+        uint64_t before = 0, total = 0;
+        for (int i = 0; i < NW; i++) {
+            before += i < warp ? S.part[i] : 0;
+            total += S.part[i];
+        }
+        const uint64_t target = target_of(total);
+        if (before < target && before + c >= target) {  // this warp's, a run of places a lane
+            const int run = (b1 - b0 + 31) / 32, r0 = min(b1, b0 + lane * run), r1 = min(b1, r0 + run);
+            uint64_t v = 0;
+            for (int i = r0; i < r1; i++) v += measure(i);
+            uint64_t s = before + warp_scan64(v, lane) - v;
+            if (s < target && s + v >= target)
+                for (int i = r0; i < r1; i++) {
+                    const uint64_t m = measure(i);
+                    if (s + m >= target) {
+                        S.bin = i;
+                        S.before = target - s;
+                        break;
                     }
-            }
-            __syncthreads();
-            *rest = S.before;
-            return (uint32_t)S.bin;
-        };
-        if (k > 0) {
-            last = reach([&](int i) -> uint64_t { return table[i]; }, [&](uint64_t) { return (uint64_t)k; }, &ties);
-            if (last == (uint32_t)n) ties = 0;
-            if (last == O.zero) return false;
-        }
-        if (p < 1.0f) {
-            const uint32_t end = last;
-            const uint64_t some = ties;  // of the end's tokens, those that top_k leaves
-            uint64_t rest;
-            last = reach(
-                [&](int i) -> uint64_t {
-                    const uint64_t m = (uint32_t)i < end ? table[i] : (uint32_t)i == end ? some : 0;
-                    return (uint32_t)i == O.zero ? (m ? about : 0) : m ? m * R.weight(O.value(i)) : 0;
-                },
-                [&](uint64_t total) { return top_p_edge(p, total); }, &rest);
-            if (last == O.zero || last == (uint32_t)n) return false;
-            const uint64_t w = R.weight(O.value(last));
-            ties = (rest + w - 1) / w;
+                    s += m;
+                }
         }
         __syncthreads();
+        *rest = S.before;
+        return (uint32_t)S.bin;
+    };
+    if (k > 0) {
+        last = reach([&](int i) -> uint64_t { return table[i]; }, [&](uint64_t) { return (uint64_t)k; }, &ties);
+        if (last == (uint32_t)n) ties = 0;
+        if (last == O.zero) return false;
     }
-    uint64_t wk = last < (uint32_t)n ? R.weight(O.value(last)) : 0;
-    if (wk < least) wk = 0;
-    for (int i = threadIdx.x; i < n; i += NT) {
-        const float f = O.value(i), d = R.spike ? 0.0f : (f - R.m) * R.inv, e = expf(d);
-        const uint64_t w = R.spike ? (f == R.m ? kOne : 0) : d > -kSpan + 0.2f ? Row<T>::weigh_bits(__float_as_uint(e)) : 0;
-        table[i] = (uint32_t)i >= last || w == 0 || w < least ? 0 : __float_as_uint(e);
+    if (p < 1.0f) {
+        const uint32_t end = last;
+        const uint64_t some = ties;  // of the end's tokens, those that top_k leaves
+        uint64_t rest;
+        last = reach(
+            [&](int i) -> uint64_t {
+                const uint64_t m = (uint32_t)i < end ? table[i] : (uint32_t)i == end ? some : 0;
+                return (uint32_t)i == O.zero ? (m ? about : 0) : m ? m * R.weight(O.value(i)) : 0;
+            },
+            [&](uint64_t total) { return top_p_edge(p, total); }, &rest);
+        if (last == O.zero || last == (uint32_t)n) return false;
+        const uint64_t w = R.weight(O.value(last));
+        ties = (rest + w - 1) / w;
     }
     __syncthreads();
-    finish_row(S, R, A, row, ties, wk, [&](const uint4 &q, int e, bool *same) -> uint64_t {
-        const uint32_t raw = raw_of(q, e), at = O.place(raw);
-        *same = at == last && ties > 0;
-        if (at >= last) return 0;
-        if (at == O.zero) {
-            const uint64_t w = R.weight(float_of(raw));
-            return w >= least ? w : 0;
-        }
-        const uint32_t u = table[at];
-        return u ? Row<T>::weigh_bits(u) : 0;
-    });
+    *key = last < (uint32_t)n ? key_of(O.value(last)) : 0;
+    *ties_ = *key ? ties : 0;
     return true;
 }
 
@@ -717,7 +735,14 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
     R.g1 = min(R.n, R.g0 + R.seg);
 
     float mine = -INFINITY;
-    R.template each<4>(R.g0, R.g1, [&](const uint4 &q, int) { mine = fmaxf(mine, Row<T>::largest(q)); });
+    int at = 0;  // the first granule that has it
+    R.template each<4>(R.g0, R.g1, [&](const uint4 &q, int g) {
+        const float t = Row<T>::largest(q);
+        if (t > mine || (t == mine && g < at)) {
+            mine = t;
+            at = g;
+        }
+    });
     float m = mine;
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -742,19 +767,36 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
     // The kept ranks: keys above `key`, and the first `ties` tokens of that key.
     uint32_t key = 0;
     uint64_t ties = 0;
-    if (!(temp > 0.0f)) {
-        key = key_of(m);
-        ties = 1;
-    } else {
+    if (!(temp > 0.0f)) {  // the first of the largest
+        if (threadIdx.x == 0) S.count = R.n;
+        __syncthreads();
+        if (mine == m) atomicMin(&S.count, at);
+        __syncthreads();
+        if (mine == m && at == S.count) {
+            float f[N];
+            unpack<T>(R.load(at), f);
+            bool open = true;
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (open && f[e] == m) {
+                    open = false;
+                    choose(A, row, R, R.index(at, e), f[e], kOne);
+                }
+        }
+        return;
+    }
+    bool known = false;
+    {
         const int64_t k = A.top_k ? A.top_k[row] : 0;
         if (k > 0 && k <= kQuick && k < V && sample_quick(S, R, A, row, mine, (int)k, p, least)) return;
         if constexpr (sizeof(T) == 2) {
             // places down to the last value with weight (a little lower does no harm), if the table holds them
             const float lowest = R.spike ? m : fmaxf(m - kSpan / R.inv, -3.0e38f);
             const int n = (int)Values<T>(m).place(raw_bits(from_f<T>(lowest))) + 2;  // lowest is rounded to nearest: kSpan has room
-            if (n <= A.places && sample_values(S, R, A, row, n, k < V ? k : 0, p, least)) return;
+            if ((p < 1.0f || (k > 0 && k < V)) && n <= A.places)
+                known = select_values(S, R, n, k < V ? k : 0, p, &key, &ties);
         }
-        if (k > 0 && k < V) {
+        if (!known && k > 0 && k < V) {
             const Bins<T> H(kSpan, -INFINITY);
             clear();
             R.each(R.g0, R.g1, [&](const uint4 &q, int) {
@@ -768,7 +810,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
             });
             key = select_ranks<T, false>(S, R, H, (uint64_t)k, &ties);
         }
-        if (p < 1.0f) {
+        if (!known && p < 1.0f) {
             // Tokens that, all together, weigh less than what the set leaves out are not in it: with the whole weight at
             // least `sure` (of the threads' largest tokens; with a top_k set, of the largest token), those lighter than
             // (1 - p) sure / vocab are left out of the histogram (a distance a little larger stands for that weight).
@@ -814,17 +856,13 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
         }
     }
 
-    uint64_t wk = key ? R.weight(value_of(key)) : 0;
-    if (wk < least) wk = 0;
-    const float low = key ? value_of(key) : -INFINITY;
-    finish_row(S, R, A, row, ties, wk, [&](const uint4 &q, int e, bool *same) -> uint64_t {
-        float f[N];
-        unpack<T>(q, f);
-        *same = key && f[e] == low;
-        if (!(f[e] > low)) return 0;
-        const uint64_t w = R.weight(f[e]);
-        return w >= least ? w : 0;
-    });
+    if (R.spike && key != key_of(m)) {  // the largest alone have weight
+        key = key_of(m);
+        ties = (uint64_t)V;
+    }
+    Kept K = {key ? value_of(key) : -INFINITY, __ull2float_ru(least) / (float)kOne, key ? ties : 0, key ? R.weight(value_of(key)) : 0};
+    if (K.wk < least) K.wk = 0;
+    finish_row(S, R, A, row, K);
 }
 
 template <typename T>
