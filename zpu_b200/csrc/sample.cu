@@ -43,6 +43,7 @@ constexpr int kList = 4096;              // tokens listed at most
 constexpr int kQuick = 400;              // first ranks that the threads' maxima bound well
 constexpr uint64_t kOne = 1ull << 40;
 constexpr int kPlaces = 20 * 1024;       // values of 16-bit logits in the table
+constexpr int kNear = 2048;              // logits about zero listed at most
 constexpr float kSpan = 28.0f;           // w = 0 beyond (max - x) / T = 40 ln 2 = 27.73
 constexpr int64_t kMaxVocab = (1 << 22) - 1;  // sums of weights stay below 2^62, of their 10-bit digits below 2^32
 
@@ -100,6 +101,7 @@ struct Shared {
     unsigned long long before;
     uint32_t kmin, kmax;
     int bin, count;
+    uint4 edge[2];  // the row's first and last granule, if they reach past it
 };
 
 // A row in granules of 16 aligned bytes, warp w's from w * seg on; and its weights.
@@ -110,33 +112,33 @@ struct Row {
     int skew, n;  // elements of granule 0 before the row, granules
     int64_t vocab;
     int seg, g0, g1, lane;  // granules of a warp, this warp's
+    int first, last;        // the granules that lie in the row as a whole
+    const uint4 *edge;      // the others, -inf outside the row
     float m, inv;           // the largest logit, 1 / T (0: the largest alone)
 
-    __device__ __forceinline__ uint4 load(int g) const {
+    __device__ __forceinline__ uint4 load_edge(int g) const {
         const int64_t at = (int64_t)g * N - skew;
-        if (at >= 0 && at + N <= vocab) return __ldcg((const uint4 *)(x + (int64_t)g * N));
         float f[N];
 #pragma unroll
         for (int e = 0; e < N; e++) f[e] = at + e >= 0 && at + e < vocab ? to_f(x[(int64_t)g * N + e]) : -INFINITY;
         return pack<T>(f);  // exact: the values come from that type
     }
-    // f(granule's bytes, its number) for each of this lane's granules from a to b, U loads in flight: the whole ones, then
-    // the first and the last of the row; lanes past the end are left out.
+    __device__ __forceinline__ uint4 load(int g) const {
+        return g >= first && g < last ? __ldcg((const uint4 *)(x + (int64_t)g * N)) : edge[g >= first];
+    }
+    // f(granule's bytes, its number) for each of this lane's granules from a to b, U loads in flight; lanes past the end
+    // are left out.
     template <int U = 2, typename F>
     __device__ __forceinline__ void each(int a, int b, F f) const {
-        const int first = skew ? 1 : 0, last = (skew + vocab) % N ? n - 1 : n;  // the whole granules of the row
-        const int b1 = min(b, last);
-        for (int g = max(a, first) + lane; g < b1; g += 32 * U) {
+        for (int g = a + lane; g < b; g += 32 * U) {
             uint4 q[U];
 #pragma unroll
             for (int u = 0; u < U; u++)
-                if (g + 32 * u < b1) q[u] = __ldcg((const uint4 *)(x + (int64_t)(g + 32 * u) * N));
+                if (g + 32 * u < b) q[u] = load(g + 32 * u);
 #pragma unroll
             for (int u = 0; u < U; u++)
-                if (g + 32 * u < b1) f(q[u], g + 32 * u);
+                if (g + 32 * u < b) f(q[u], g + 32 * u);
         }
-        const int g = lane == 0 ? 0 : n - 1;
-        if (lane < 2 && g >= a && g < b && (lane == 0 ? first == 1 : last < n && (n > 1 || first == 0))) f(load(g), g);
         __syncwarp();
     }
     static __device__ __forceinline__ float largest(const uint4 &q) {  // passes NaN over
@@ -276,6 +278,37 @@ struct Bins {
     __device__ __forceinline__ int at(float f, float d) const { return f > low && -d < span ? min(NB - 1, (int)(-d * scale)) : -1; }
 };
 
+// The key of the entry of a sorted list at which the running measure reaches target, and how many up to it have that key.
+template <typename T, bool MASS>
+__device__ uint32_t list_find(Shared &S, const Row<T> &R, int n, uint64_t target, uint64_t *ties) {
+    uint64_t below = 0;
+    for (int i0 = 0; i0 < n; i0 += NT) {
+        const int i = i0 + (int)threadIdx.x, warp = threadIdx.x >> 5;
+        const uint64_t w = i >= n ? 0 : MASS ? R.weight(value_of(entry_key(list(i)))) : 1;
+        uint64_t upto = below + warp_scan64(w, R.lane);
+        if (R.lane == 31) S.part[warp] = upto - below;
+        __syncthreads();
+        for (int v = 0; v < NW; v++) {
+            if (v < warp) upto += S.part[v];
+            below += S.part[v];
+        }
+        if (upto >= target && upto - w < target) {
+            S.kmin = entry_key(list(i));
+            S.count = i;
+        }
+        __syncthreads();
+        if (below >= target) break;
+    }
+    int same = 0;
+    for (int i = threadIdx.x; i <= S.count; i += NT) same += entry_key(list(i)) == S.kmin;
+    if (threadIdx.x == 0) S.before = 0;
+    __syncthreads();
+    if (same) atomicAdd(&S.before, (unsigned long long)same);
+    __syncthreads();
+    *ties = S.before;
+    return S.kmin;
+}
+
 // The last of the first ranks at which the running measure (tokens, or MASS:
 // their weights) of the tokens in the histogram reaches target: its key, and how
 // many of that key's tokens belong to the ranks (0: the measure does not reach
@@ -327,33 +360,7 @@ __device__ uint32_t select_ranks(Shared &S, const Row<T> &R, const Bins<T> &H, u
         if (n <= kList || lo == hi) {
             if (lo != hi) {
                 sort_list(n);
-                // the entry at which the measure reaches target, and how many up to it have its key
-                uint64_t below = 0;
-                for (int i0 = 0; i0 < n; i0 += NT) {
-                    const int i = i0 + (int)threadIdx.x, warp = threadIdx.x >> 5;
-                    const uint64_t w = i >= n ? 0 : MASS ? R.weight(value_of(entry_key(list(i)))) : 1;
-                    uint64_t upto = below + warp_scan64(w, R.lane);
-                    if (R.lane == 31) S.part[warp] = upto - below;
-                    __syncthreads();
-                    for (int v = 0; v < NW; v++) {
-                        if (v < warp) upto += S.part[v];
-                        below += S.part[v];
-                    }
-                    if (upto >= target && upto - w < target) {
-                        S.kmin = entry_key(list(i));
-                        S.count = i;
-                    }
-                    __syncthreads();
-                    if (below >= target) break;
-                }
-                int same = 0;
-                for (int i = threadIdx.x; i <= S.count; i += NT) same += entry_key(list(i)) == S.kmin;
-                if (threadIdx.x == 0) S.before = 0;
-                __syncthreads();
-                if (same) atomicAdd(&S.before, (unsigned long long)same);
-                __syncthreads();
-                *ties = S.before;
-                return S.kmin;
+                return list_find<T, MASS>(S, R, n, target, ties);
             }
             const uint64_t w = MASS ? R.weight(value_of(hi)) : 1;
             *ties = (target + w - 1) / w;
@@ -406,11 +413,7 @@ __device__ __forceinline__ void choose(const Args &A, int64_t row, const Row<T> 
 struct Kept {
     float low, least;
     uint64_t ties, wk;
-    template <typename T>
-    __device__ __forceinline__ float power(const Row<T> &R, float f) const {  // e^..., 0: not kept
-        const float e = expf((f - R.m) * R.inv);
-        return f > low && e >= least ? e : 0.0f;
-    }
+    __device__ __forceinline__ float keep(float f, float e) const { return f > low && e >= least ? e : 0.0f; }
 };
 
 // The token whose running sum of kept weights by index exceeds the place.  Sums of each warp's granules first, then of NW
@@ -425,6 +428,8 @@ __device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t ro
     const int warp = threadIdx.x >> 5;
     auto add = [&](int a, int b, auto tied) {  // of granules a to b, to S
         constexpr uint32_t k3 = 0x41000000u, k17 = 0x37000000u;  // 2^3, 2^-17
+        const f32x2 c3 = make2(__uint_as_float(k3)), c17 = make2(__uint_as_float(k17));
+        auto sub2 = [](f32x2 x, f32x2 y) { return fma2(y, make2(-1.0f), x); };
         uint64_t high = 0, low = 0;
         uint32_t t = 0;
         R.template each<2>(a, b, [&](const uint4 &q, int) {
@@ -432,12 +437,14 @@ __device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t ro
             unpack<T>(q, f);
             uint32_t h = -N * k3, l = -N * k17;
 #pragma unroll
-            for (int e = 0; e < N; e++) {
-                const float p = K.power(R, f[e]);
-                const float hi = __fadd_rz(p, __uint_as_float(k3)), rest = p - (hi - __uint_as_float(k3));
-                h += __float_as_uint(hi);
-                l += __float_as_uint(__fadd_rz(rest, __uint_as_float(k17)));
-                if (decltype(tied)::value) t += f[e] == K.low;
+            for (int e = 0; e < N; e += 2) {
+                const f32x2 d = mul2(add2(make2(f[e], f[e + 1]), make2(-R.m)), make2(R.inv));
+                const float e0 = expf(lo2(d)), e1 = expf(hi2(d));
+                const f32x2 w = make2(K.keep(f[e], e0), K.keep(f[e + 1], e1));
+                const f32x2 hi = add2_rz(w, c3), rest = sub2(w, sub2(hi, c3)), lo = add2_rz(rest, c17);
+                h += __float_as_uint(lo2(hi)) + __float_as_uint(hi2(hi));
+                l += __float_as_uint(lo2(lo)) + __float_as_uint(hi2(lo));
+                if (decltype(tied)::value) t += (f[e] == K.low) + (f[e + 1] == K.low);
             }
             high += h;
             low += l;
@@ -489,7 +496,7 @@ __device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t ro
         uint32_t t = 0;
 #pragma unroll
         for (int e = 0; e < N; e++) {
-            s[e] = Row<T>::weigh_bits(__float_as_uint(K.power(R, f[e])));
+            s[e] = Row<T>::weigh_bits(__float_as_uint(K.keep(f[e], expf((f[e] - R.m) * R.inv))));
             t += in && f[e] == K.low;
         }
         uint32_t upto = t;  // ties up to this lane's last
@@ -612,6 +619,17 @@ struct Values {
         zero = top - kMiddle;
     }
     __device__ __forceinline__ uint32_t place(uint32_t raw) const { return top - order(raw); }
+    // The places of a word's two values: each one's bits in rising order, then (middle - them), and of that what the small
+    // ones span is taken off.
+    __device__ __forceinline__ void places(uint32_t word, uint32_t (&at)[2]) const {
+        const uint32_t sign = word & 0x80008000u, rising = word ^ (0x80008000u | (sign - (sign >> 15)));
+        const int z = (int)zero, middle = z + (int)(0x8000u + kSmall), small = (int)(2 * kSmall + 1);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int t = middle - (int)(i ? rising >> 16 : rising & 0xffffu);
+            at[i] = (uint32_t)min(max(t - small, z), t);
+        }
+    }
     __device__ __forceinline__ float value(uint32_t place_) const {
         const uint32_t o = top - place_, raw = o >= kMiddle ? o - kMiddle + kSmall : 0x8000u | (kMiddle - o + kSmall);
         if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(raw << 16);
@@ -620,8 +638,8 @@ struct Values {
 };
 
 // The kept ranks of 16-bit logits (k > 0 or p < 1) from counts of each value at `n` places from the largest on (what lies
-// past them has no weight): the key of the last, 0: all, and in *ties how many of that key.  False: the ranks end among the
-// values about zero.
+// past them has no weight): the key of the last, 0: all, and in *ties how many of that key.  False: the ranks end among
+// more values about zero than are listed, or top_k's do and top_p follows.
 template <typename T>
 __device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, float p, uint32_t *key, uint64_t *ties_) {
     static_assert(sizeof(T) == 2, "16-bit logits");
@@ -641,15 +659,41 @@ __device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, floa
     uint64_t ties = 0;
     for (int i = threadIdx.x; i < n; i += NT) table[i] = 0;
     __syncthreads();
-    uint64_t about = 0;  // the weight of the values about zero
-    R.template each<4>(R.g0, R.g1, [&](const uint4 &q, int) {
+    unsigned short *near_ = (unsigned short *)(sample_smem + kPlaces);
+    if (threadIdx.x == 0) S.count = 0;
+    __syncthreads();
+    const uint32_t zero = O.zero < (uint32_t)n ? O.zero : 0xffffffffu;
+    R.each(R.g0, R.g1, [&](const uint4 &q, int) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const uint32_t raw = raw_of(q, e), at = O.place(raw);
-            if (at < (uint32_t)n) atomicAdd(&table[at], 1u);
-            if (at == O.zero && p < 1.0f) about += R.weight(float_of(raw));
+        for (int e = 0; e < 4; e++) {
+            uint32_t at[2];
+            O.places(w[e], at);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (at[i] >= (uint32_t)n) continue;
+                atomicAdd(&table[at[i]], 1u);
+                if (at[i] == zero) {
+                    const int to = atomicAdd(&S.count, 1);
+                    if (to < kNear) near_[to] = (unsigned short)(i ? w[e] >> 16 : w[e]);
+                }
+            }
         }
     });
+    __syncthreads();
+    uint64_t about = 0;  // the weight of the values about zero
+    const int nears = S.count;
+    if (p >= 1.0f) {
+    } else if (nears <= kNear) {
+        for (int i = threadIdx.x; i < nears; i += NT) about += R.weight(float_of(near_[i]));
+    } else {
+        R.each(R.g0, R.g1, [&](const uint4 &q, int) {
+            for (int e = 0; e < 8; e++) {
+                const uint32_t raw = raw_of(q, e);
+                if (O.place(raw) == zero) about += R.weight(float_of(raw));
+            }
+        });
+    }
     about = warp_sum64(about);
     if (lane == 0) S.w[warp] = about;
     __syncthreads();
@@ -695,7 +739,7 @@ __device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, floa
     if (k > 0) {
         last = reach([&](int i) -> uint64_t { return table[i]; }, [&](uint64_t) { return (uint64_t)k; }, &ties);
         if (last == (uint32_t)n) ties = 0;
-        if (last == O.zero) return false;
+        if (last == O.zero && p < 1.0f) return false;
     }
     if (p < 1.0f) {
         const uint32_t end = last;
@@ -707,9 +751,19 @@ __device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, floa
                 return (uint32_t)i == O.zero ? (m ? about : 0) : m ? m * R.weight(O.value(i)) : 0;
             },
             [&](uint64_t total) { return top_p_edge(p, total); }, &rest);
-        if (last == O.zero || last == (uint32_t)n) return false;
-        const uint64_t w = R.weight(O.value(last));
-        ties = (rest + w - 1) / w;
+        if (last == (uint32_t)n) return false;
+        if (last != O.zero) {
+            const uint64_t w = R.weight(O.value(last));
+            rest = (rest + w - 1) / w;
+        }
+        ties = rest;
+    }
+    if (last == zero) {  // its tokens in order, up to the rest of the target
+        if (nears > kNear) return false;
+        for (int i = threadIdx.x; i < nears; i += NT) list(i) = entry_of(key_of(float_of(near_[i])), i);
+        sort_list(nears);
+        *key = p < 1.0f ? list_find<T, true>(S, R, nears, ties, ties_) : list_find<T, false>(S, R, nears, ties, ties_);
+        return true;
     }
     __syncthreads();
     *key = last < (uint32_t)n ? key_of(O.value(last)) : 0;
@@ -733,6 +787,13 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
     R.seg = (R.n + NW - 1) / NW;
     R.g0 = min(R.n, warp * R.seg);
     R.g1 = min(R.n, R.g0 + R.seg);
+
+    R.first = R.skew ? 1 : 0;
+    R.last = (R.skew + V) % N ? R.n - 1 : R.n;
+    R.edge = S.edge;
+    if (threadIdx.x == 0 && R.first) S.edge[0] = R.load_edge(0);
+    if (threadIdx.x == 1 && R.last < R.n && R.n > R.first) S.edge[1] = R.load_edge(R.n - 1);
+    __syncthreads();
 
     float mine = -INFINITY;
     int at = 0;  // the first granule that has it
@@ -868,7 +929,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
 template <typename T>
 int launch_sample(const T *logits, int64_t ld, const Args &A, int64_t rows, cudaStream_t s) {
     auto f = sample_kernel<T>;
-    const size_t smem = sizeof(T) == 2 ? kPlaces * sizeof(uint32_t) : kSmem;
+    const size_t smem = sizeof(T) == 2 ? kPlaces * sizeof(uint32_t) + kNear * sizeof(short) : kSmem;
     static int cache[64] = {0};
     if (!blocks_per_sm(f, NT, smem, smem, cache)) return cuda_fail(cudaGetLastError(), "sample: occupancy");
     f<<<(unsigned)rows, NT, smem, s>>>(logits, ld, A);
