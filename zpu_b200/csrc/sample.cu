@@ -37,7 +37,7 @@
 namespace zc {
 namespace {
 
-constexpr int NT = 512, NW = NT / 32;  // two blocks an SM
+constexpr int kThreads = 1024, kWarps = kThreads / 32;  // of a block at most
 constexpr int NB = 2048;                 // histogram bins
 constexpr int kList = 4096;              // tokens listed at most
 constexpr int kQuick = 400;              // first ranks that the threads' maxima bound well
@@ -58,6 +58,9 @@ struct Args {
     int64_t vocab;
     int places;  // of the table of values
 };
+
+__device__ __forceinline__ int NT() { return (int)blockDim.x; }
+__device__ __forceinline__ int NW() { return (int)blockDim.x >> 5; }
 
 // The logit's bits as a number that rises with it; NaN is 0, below all others.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -94,10 +97,10 @@ __device__ __forceinline__ uint32_t &digit(int i, int b) { return sample_smem[i 
 __device__ __forceinline__ unsigned long long &list(int i) { return ((unsigned long long *)sample_smem)[i]; }
 
 struct Shared {
-    unsigned long long w[NT];
-    unsigned long long part[NW];
-    uint32_t ties[NW];
-    float fmax_[NW];
+    unsigned long long w[kThreads];
+    unsigned long long part[kWarps];
+    uint32_t ties[kWarps];
+    float fmax_[kWarps];
     unsigned long long before;
     uint32_t kmin, kmax;
     int bin, count;
@@ -177,12 +180,12 @@ __device__ __forceinline__ uint32_t entry_index(unsigned long long e) { return ~
 
 // The list's n entries in falling order.
 __device__ void sort_list(int n) {
-    if (n <= 2 * NT) {  // each to the place of its rank
+    if (n <= 2 * NT()) {  // each to the place of its rank
         __syncthreads();
-        const int i = threadIdx.x, j = i + NT;
+        const int i = threadIdx.x, j = i + NT();
         const unsigned long long a = i < n ? list(i) : 0, b = j < n ? list(j) : 0;
         int ra = 0, rb = 0;
-        if (n <= NT) {
+        if (n <= NT()) {
             if (i < n)
 #pragma unroll 4
                 for (int k = 0; k < n; k++) ra += list(k) > a;
@@ -200,13 +203,13 @@ __device__ void sort_list(int n) {
         __syncthreads();
         return;
     }
-    int size = 4 * NT;
+    int size = 4 * NT();
     while (size < n) size <<= 1;
-    for (int i = n + (int)threadIdx.x; i < size; i += NT) list(i) = 0;
+    for (int i = n + (int)threadIdx.x; i < size; i += NT()) list(i) = 0;
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j; j >>= 1) {
             __syncthreads();
-            for (int i = threadIdx.x; i < size / 2; i += NT) {
+            for (int i = threadIdx.x; i < size / 2; i += NT()) {
                 const int lo = (i / j) * 2 * j + i % j, hi = lo + j;
                 const unsigned long long a = list(lo), b = list(hi);
                 if ((a < b) == ((lo & k) == 0)) {
@@ -220,7 +223,7 @@ __device__ void sort_list(int n) {
 
 __device__ void clear() {
     __syncthreads();
-    for (int i = threadIdx.x; i < 4 * NB; i += NT) digit(0, i) = 0;
+    for (int i = threadIdx.x; i < 4 * NB; i += NT()) digit(0, i) = 0;
     __syncthreads();
 }
 __device__ __forceinline__ uint64_t bin_value(int b) {
@@ -243,26 +246,25 @@ __device__ __forceinline__ void bin_add(int b, uint64_t w) {
 __device__ int hist_find(Shared &S, uint64_t target, uint64_t *before) {
     if (threadIdx.x == 0) S.bin = -1;
     __syncthreads();
-    constexpr int PER = NB / NT;
+    const int per = NB / NT();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint64_t v[PER], sum = 0;
-#pragma unroll
-    for (int i = 0; i < PER; i++) sum += v[i] = bin_value(threadIdx.x * PER + i);
+    uint64_t sum = 0;
+    for (int i = 0; i < per; i++) sum += bin_value(threadIdx.x * per + i);
     uint64_t upto = warp_scan64(sum, lane);
     if (lane == 31) S.part[warp] = upto;
     __syncthreads();
     for (int i = 0; i < warp; i++) upto += S.part[i];
     uint64_t c = upto - sum;
     if (upto >= target && c < target) {
-#pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (c < target) {
-                if (c + v[i] >= target) {
-                    S.bin = threadIdx.x * PER + i;
-                    S.before = c;
-                }
-                c += v[i];
+        for (int i = threadIdx.x * per;; i++) {
+            const uint64_t v = bin_value(i);
+            if (c + v >= target) {
+                S.bin = i;
+                S.before = c;
+                break;
             }
+            c += v;
+        }
     }
     __syncthreads();
     *before = S.before;
@@ -282,13 +284,13 @@ struct Bins {
 template <typename T, bool MASS>
 __device__ uint32_t list_find(Shared &S, const Row<T> &R, int n, uint64_t target, uint64_t *ties) {
     uint64_t below = 0;
-    for (int i0 = 0; i0 < n; i0 += NT) {
+    for (int i0 = 0; i0 < n; i0 += NT()) {
         const int i = i0 + (int)threadIdx.x, warp = threadIdx.x >> 5;
         const uint64_t w = i >= n ? 0 : MASS ? R.weight(value_of(entry_key(list(i)))) : 1;
         uint64_t upto = below + warp_scan64(w, R.lane);
         if (R.lane == 31) S.part[warp] = upto - below;
         __syncthreads();
-        for (int v = 0; v < NW; v++) {
+        for (int v = 0; v < NW(); v++) {
             if (v < warp) upto += S.part[v];
             below += S.part[v];
         }
@@ -300,7 +302,7 @@ __device__ uint32_t list_find(Shared &S, const Row<T> &R, int n, uint64_t target
         if (below >= target) break;
     }
     int same = 0;
-    for (int i = threadIdx.x; i <= S.count; i += NT) same += entry_key(list(i)) == S.kmin;
+    for (int i = threadIdx.x; i <= S.count; i += NT()) same += entry_key(list(i)) == S.kmin;
     if (threadIdx.x == 0) S.before = 0;
     __syncthreads();
     if (same) atomicAdd(&S.before, (unsigned long long)same);
@@ -416,7 +418,7 @@ struct Kept {
     __device__ __forceinline__ float keep(float f, float e) const { return f > low && e >= least ? e : 0.0f; }
 };
 
-// The token whose running sum of kept weights by index exceeds the place.  Sums of each warp's granules first, then of NW
+// The token whose running sum of kept weights by index exceeds the place.  Sums of each warp's granules first, then of
 // parts of the ones that hold the place, then of those.
 //
 // A weight is summed as two whole numbers of 20 bits, floor(2^20 e) and floor(2^40 (e - the first / 2^20)): adding 8 = 2^3
@@ -462,13 +464,13 @@ __device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t ro
         if (ties) add(a, b, std::true_type());
         else add(a, b, std::false_type());
     };
-    // the part of NW parts that holds `at` once `before` and `left` ties lie before them; those are moved on.  A lane a part.
+    // the part that holds `at` once `before` and `left` ties lie before them; those are moved on.  A lane a part.
     auto find = [&](uint64_t at, uint64_t *before, uint64_t *left, uint64_t *total) {
-        const uint32_t t = R.lane < NW ? S.ties[R.lane] : 0;
+        const uint32_t t = R.lane < NW() ? S.ties[R.lane] : 0;
         const uint64_t ties_before = warp_scan64(t, R.lane) - t, mine = *left > ties_before ? min(*left - ties_before, (uint64_t)t) : 0;
-        const uint64_t w = R.lane < NW ? S.part[R.lane] + mine * wk : 0, upto = warp_scan64(w, R.lane);
+        const uint64_t w = R.lane < NW() ? S.part[R.lane] + mine * wk : 0, upto = warp_scan64(w, R.lane);
         const uint32_t over = __ballot_sync(0xffffffffu, *before + upto > at);
-        const int found = over ? min(__ffs(over) - 1, NW - 1) : NW - 1;
+        const int found = over ? min(__ffs(over) - 1, NW() - 1) : NW() - 1;
         *total = __shfl_sync(0xffffffffu, upto, 31);
         *before += __shfl_sync(0xffffffffu, upto - w, found);
         const uint64_t gone = __shfl_sync(0xffffffffu, ties_before, found);
@@ -482,7 +484,7 @@ __device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t ro
     before = 0;
     left = ties;
     const int w0 = find(at, &before, &left, &unused);
-    const int a = min(R.n, w0 * R.seg), b = min(R.n, a + R.seg), sub = (b - a + NW - 1) / NW;
+    const int a = min(R.n, w0 * R.seg), b = min(R.n, a + R.seg), sub = (b - a + NW() - 1) / NW();
     sums(min(b, a + warp * sub), min(b, a + (warp + 1) * sub));
     const int w1 = find(at, &before, &left, &unused);
     if (warp != w1) return;
@@ -577,7 +579,7 @@ __device__ bool sample_quick(Shared &S, const Row<T> &R, const Args &A, int64_t 
         if (lane == 31) S.part[warp] = upto;
         __syncthreads();
         uint64_t below = 0, all = 0;
-        for (int i = 0; i < NW; i++) {
+        for (int i = 0; i < NW(); i++) {
             if (i < warp) below += S.part[i];
             all += S.part[i];
         }
@@ -657,7 +659,7 @@ __device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, floa
     // The kept ranks: places below `last`, and the first `ties` tokens at it.
     uint32_t last = (uint32_t)n;
     uint64_t ties = 0;
-    for (int i = threadIdx.x; i < n; i += NT) table[i] = 0;
+    for (int i = threadIdx.x; i < n; i += NT()) table[i] = 0;
     __syncthreads();
     unsigned short *near_ = (unsigned short *)(sample_smem + kPlaces);
     if (threadIdx.x == 0) S.count = 0;
@@ -685,7 +687,7 @@ __device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, floa
     const int nears = S.count;
     if (p >= 1.0f) {
     } else if (nears <= kNear) {
-        for (int i = threadIdx.x; i < nears; i += NT) about += R.weight(float_of(near_[i]));
+        for (int i = threadIdx.x; i < nears; i += NT()) about += R.weight(float_of(near_[i]));
     } else {
         R.each(R.g0, R.g1, [&](const uint4 &q, int) {
             for (int e = 0; e < 8; e++) {
@@ -698,10 +700,10 @@ __device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, floa
     if (lane == 0) S.w[warp] = about;
     __syncthreads();
     about = 0;
-    for (int i = 0; i < NW; i++) about += S.w[i];
+    for (int i = 0; i < NW(); i++) about += S.w[i];
     // A warp has a run of places.  What they measure, and the place at which the running measure reaches target, with
     // what is left of the target there; all threads get both (n: it does not reach target).
-    const int per = (n + NT - 1) / NT * 32, b0 = min(n, warp * per), b1 = min(n, b0 + per);
+    const int per = (n + NT() - 1) / NT() * 32, b0 = min(n, warp * per), b1 = min(n, b0 + per);
     auto reach = [&](auto measure, auto target_of, uint64_t *rest) {
         uint64_t c = 0;
         for (int i = b0 + lane; i < b1; i += 32) c += measure(i);
@@ -711,7 +713,7 @@ __device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, floa
         if (threadIdx.x == 0) S.bin = n;
         __syncthreads();
         uint64_t before = 0, total = 0;
-        for (int i = 0; i < NW; i++) {
+        for (int i = 0; i < NW(); i++) {
             before += i < warp ? S.part[i] : 0;
             total += S.part[i];
         }
@@ -760,7 +762,7 @@ __device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, floa
     }
     if (last == zero) {  // its tokens in order, up to the rest of the target
         if (nears > kNear) return false;
-        for (int i = threadIdx.x; i < nears; i += NT) list(i) = entry_of(key_of(float_of(near_[i])), i);
+        for (int i = threadIdx.x; i < nears; i += NT()) list(i) = entry_of(key_of(float_of(near_[i])), i);
         sort_list(nears);
         *key = p < 1.0f ? list_find<T, true>(S, R, nears, ties, ties_) : list_find<T, false>(S, R, nears, ties, ties_);
         return true;
@@ -772,7 +774,7 @@ __device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, floa
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t ld, const Args A) {
+__global__ void __launch_bounds__(kThreads) sample_kernel(const T *logits, int64_t ld, const Args A) {
     constexpr int N = Row<T>::N;
     __shared__ Shared S;
     const int64_t row = blockIdx.x, V = A.vocab;
@@ -784,7 +786,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
     R.skew = (int)(((uintptr_t)x & 15) / sizeof(T));
     R.x = x - R.skew;
     R.n = (int)((R.skew + V + N - 1) / N);
-    R.seg = (R.n + NW - 1) / NW;
+    R.seg = (R.n + NW() - 1) / NW();
     R.g0 = min(R.n, warp * R.seg);
     R.g1 = min(R.n, R.g0 + R.seg);
 
@@ -809,7 +811,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (R.lane == 0) S.fmax_[warp] = m;
     __syncthreads();
-    for (int w = 0; w < NW; w++) m = fmaxf(m, S.fmax_[w]);
+    for (int w = 0; w < NW(); w++) m = fmaxf(m, S.fmax_[w]);
     if (m == -INFINITY) {
         if (threadIdx.x == 0) {
             A.token[row] = -1;
@@ -882,7 +884,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
             if (R.lane == 0) S.part[warp] = sure;
             clear();
             sure = 0;
-            for (int i = 0; i < NW; i++) sure += S.part[i];
+            for (int i = 0; i < NW(); i++) sure += S.part[i];
             if (sure < kOne) sure = kOne;
             const float light = (1.0f - p) * (float)sure / (float)kOne / (float)V;
             const float span = p > 0.0f && light > 0.0f ? fminf(kSpan, fmaxf(1e-3f, 1e-3f - logf(light))) : kSpan;
@@ -905,7 +907,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const T *logits, int64_t 
             if (R.lane == 0) S.part[warp] = sum;
             __syncthreads();
             uint64_t above = 0;
-            for (int i = 0; i < NW; i++) above += S.part[i];
+            for (int i = 0; i < NW(); i++) above += S.part[i];
             __syncthreads();
             const uint64_t wk = key ? R.weight(value_of(key)) : 0, target = top_p_edge(p, above + ties * wk);
             if (above >= target) {
@@ -931,8 +933,9 @@ int launch_sample(const T *logits, int64_t ld, const Args &A, int64_t rows, cuda
     auto f = sample_kernel<T>;
     const size_t smem = sizeof(T) == 2 ? kPlaces * sizeof(uint32_t) + kNear * sizeof(short) : kSmem;
     static int cache[64] = {0};
-    if (!blocks_per_sm(f, NT, smem, smem, cache)) return cuda_fail(cudaGetLastError(), "sample: occupancy");
-    f<<<(unsigned)rows, NT, smem, s>>>(logits, ld, A);
+    if (!blocks_per_sm(f, kThreads, smem, smem, cache)) return cuda_fail(cudaGetLastError(), "sample: occupancy");
+    const int threads = rows <= num_sms() ? kThreads : kThreads / 2;
+    f<<<(unsigned)rows, threads, smem, s>>>(logits, ld, A);
     ZC_LAUNCHED("sample_kernel");
     return ZPUCUDA_OK;
 }
