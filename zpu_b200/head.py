@@ -93,12 +93,14 @@ def _vector(name, t, n, like, dtype=None):
 
 def _output(name, out, like, shape=None, dtype=None):
     """`out`, checked, or a new tensor; and its row pitch."""
+    if out is None and shape is None and dtype is None and like.is_contiguous():
+        return _torch().empty_like(like), like.shape[1]
     if shape is None:
         shape = like.shape
     if dtype is None:
         dtype = like.dtype
     if out is None:
-        return like.new_empty(shape, dtype=dtype), shape[1]
+        return _torch().empty(shape, dtype=dtype, device=like.device), shape[1]
     if out.dtype != dtype:
         _refuse(3, "%s: dtype %s, %s is wanted" % (name, out.dtype, dtype))
     return out, _matrix(name, out, like, shape)
@@ -141,7 +143,8 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, out=None, stats=False, stream
     with _on(stream):
         y, ldy = _output("out", out, x)
         if stats:
-            mean, rstd = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+            mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+            rstd = torch.empty_like(mean)
     check(lib().zpucuda_layer_norm(code, x.data_ptr(), ldx, wt, g, b, y.data_ptr(), ldy,
                                    mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None,
                                    rows, cols, eps, _stream(stream, x)))
@@ -309,7 +312,7 @@ class Int8Linear:
             _refuse(2, "x is %s, the weight %s" % (tuple(x.shape), tuple(self.weight.shape)))
         with _on(stream):
             y, ldy = _output("out", out, x, (rows, cols))
-            work = x.new_empty(lib().zpucuda_int8_linear_work(rows, inner), dtype=torch.uint8)
+            work = torch.empty(lib().zpucuda_int8_linear_work(rows, inner), dtype=torch.uint8, device=x.device)
         check(lib().zpucuda_int8_linear(code, x.data_ptr(), ldx, self.weight.data_ptr(), self._ld,
                                         self.scale.data_ptr(), None if self.bias is None else self.bias.data_ptr(),
                                         y.data_ptr(), ldy, rows, cols, inner, work.data_ptr(), work.numel(),
