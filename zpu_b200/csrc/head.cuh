@@ -238,19 +238,56 @@ __device__ __forceinline__ void store_piece(T *row, int64_t i, int64_t n, const 
     if (lane == 31) store_elements(p, v, head, have);
 }
 
-// A ring of D rows' pieces in shared memory, filled by asynchronous copies: a warp
-// has its lanes' pieces t + j * TPR (j < NV) of ROWS rows (tensors) a slot, and no
-// other warp reads them.  Bytes in flight cost no registers this way.  EVEN: rows
-// start on 16-byte boundaries and hold whole pieces.
-template <typename T, int TPR, int NV, int ROWS, int D, bool EVEN>
-struct RowRing {
-    static constexpr int kWarp = D * ROWS * NV * 33;  // uint4 a warp: 32 lanes' 16 bytes, and the next 16
-    uint4 *base;
-    int lane, t;
+// Stores a warp's run of pieces: lane l has pieces i = i0 + l, i + 32 and so on.  As
+// above, but single elements are stored at the run's ends and the row's alone.
+template <typename T, int NV>
+__device__ __forceinline__ void store_run(T *row, int i, int n, const uint4 (&v)[NV]) {
+    constexpr int N = kPiece<T>;
+    const uint32_t s = (uint32_t)(uintptr_t)row & 15;
+    const int lane = threadIdx.x & 31, head = (int)(16 - s) / (int)sizeof(T);  // elements up to the boundary
+    uint4 carry = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        T *p = row + (i + 32 * j) * N;
+        const int rest = n - (i + 32 * j) * N, have = rest >= N ? N : rest > 0 ? rest : 0;
+        if (s == 0) {
+            if (have == N) *(uint4 *)p = v[j];
+            else if (have) store_elements(p, v[j], 0, have);
+            continue;
+        }
+        uint4 turn;  // lane 0: what goes before its next piece
+        turn.x = __shfl_sync(0xffffffffu, v[j].x, (lane + 31) & 31);
+        turn.y = __shfl_sync(0xffffffffu, v[j].y, (lane + 31) & 31);
+        turn.z = __shfl_sync(0xffffffffu, v[j].z, (lane + 31) & 31);
+        turn.w = __shfl_sync(0xffffffffu, v[j].w, (lane + 31) & 31);
+        const uint4 before = lane ? turn : carry;
+        carry = turn;
+        const bool joined = lane > 0 || j > 0;
+        if (joined && have >= head) {
+            *(uint4 *)((uintptr_t)p & ~(uintptr_t)15) = bytes_from(before, v[j], 16 - s);
+        } else if (joined ? rest + N > head : have > 0) {
+            if (joined) store_elements(p - N, before, head, rest + N < N ? rest + N : N);
+            store_elements(p, v[j], 0, have < head ? have : head);
+        }
+        if (j == NV - 1 && lane == 31 && have > head) store_elements(p, v[j], head, have);
+        __syncwarp();
+    }
+}
 
-    __device__ __forceinline__ RowRing(uint4 *smem, int t_)
-        : base(smem + (threadIdx.x >> 5) * kWarp), lane(threadIdx.x & 31), t(t_) {}
-    __device__ __forceinline__ uint4 *at(int slot, int r, int j) const { return base + ((slot * ROWS + r) * NV + j) * 33; }
+// A ring of D rows' pieces in shared memory, filled by asynchronous copies: a warp
+// has a run of 32 * NV pieces of ROWS rows (tensors) a slot, lane l the pieces
+// p = p0 + l, p + 32 and so on, and no other warp reads them.  Bytes in flight cost
+// no registers this way.  EVEN: rows start on 16-byte boundaries and hold whole
+// pieces.
+template <typename T, int NV, int ROWS, int D, bool EVEN>
+struct RowRing {
+    static constexpr int kWarp = D * ROWS * (NV * 32 + 1);  // uint4 a warp: the run's, and the next 16 bytes
+    uint4 *base;
+    int lane, p;
+
+    __device__ __forceinline__ RowRing(uint4 *smem, int p_)
+        : base(smem + (threadIdx.x >> 5) * kWarp), lane(threadIdx.x & 31), p(p_) {}
+    __device__ __forceinline__ uint4 *at(int slot, int r, int j) const { return base + (slot * ROWS + r) * (NV * 32 + 1) + j * 32; }
 
     static __device__ __forceinline__ void copy(uint4 *dst, const uint8_t *src, int size) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)),
@@ -262,10 +299,10 @@ struct RowRing {
     __device__ __forceinline__ void issue(int slot, int r, const T *row, int64_t n, bool first) const {
         const uint32_t s = EVEN ? 0 : (uint32_t)(uintptr_t)row & 15;
         const uint8_t *from = (const uint8_t *)row - s;
-        const int64_t end = s + n * (int64_t)sizeof(T);
+        const int end = (int)s + (int)n * (int)sizeof(T);
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            const int64_t b = (int64_t)(t + j * TPR) * 16;
+            const int b = (p + j * 32) * 16;
             if (b >= end) continue;
             uint4 *dst = at(slot, r, j);
             if constexpr (EVEN) {
@@ -276,9 +313,9 @@ struct RowRing {
                 T *e = (T *)(dst + lane);
                 for (int i = (int)(s / sizeof(T)); i < kPiece<T> && i * (int)sizeof(T) < end; i++) e[i] = row[i - (int)(s / sizeof(T))];
             } else {
-                copy(dst + lane, from + b, end - b < 16 ? (int)(end - b) : 16);
+                copy(dst + lane, from + b, end - b < 16 ? end - b : 16);
             }
-            if (s && lane == 31 && b + 16 < end) copy(dst + 32, from + b + 16, end - b < 32 ? (int)(end - b) - 16 : 16);
+            if (j == NV - 1 && s && lane == 31 && b + 16 < end) copy(dst + 32, from + b + 16, end - b < 32 ? end - b - 16 : 16);
         }
     }
     static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -290,7 +327,7 @@ struct RowRing {
     // Piece t + j * TPR, 0 past the row's end.
     __device__ __forceinline__ uint4 read(int slot, int r, int j, const T *row, int64_t n) const {
         const uint32_t s = EVEN ? 0 : (uint32_t)(uintptr_t)row & 15;
-        const int64_t b = (int64_t)(t + j * TPR) * 16, end = s + n * (int64_t)sizeof(T);
+        const int b = (p + j * 32) * 16, end = (int)s + (int)n * (int)sizeof(T);
         const uint4 *src = at(slot, r, j) + lane, none = make_uint4(0, 0, 0, 0);
         const uint4 lo = b < end ? src[0] : none;
         if (EVEN || s == 0) return lo;

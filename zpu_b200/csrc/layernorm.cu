@@ -110,7 +110,7 @@ struct Fwd {
 #pragma unroll
         for (int e = 0; e < H; e++) {
             a[e] = add2(a[e], make2(-mu));
-            if (2 * e + 1 >= have) a[e] = make2(2 * e < have ? lo2(a[e]) : 0.0f, 0.0f);
+            if (have < N && 2 * e + 1 >= have) a[e] = make2(2 * e < have ? lo2(a[e]) : 0.0f, 0.0f);
             d1 = add2(d1, a[e]);
             d2 = fma2(a[e], a[e], d2);
         }
@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(TPR < NT ? NT : TPR)
     extern __shared__ uint4 ring_smem[];
     __shared__ float sm[2][2][BLOCK / 16];
     const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, bar = 1 + (TPR > 32 ? group : 0);
-    const RowRing<T, TPR, NV, 1, D, EVEN> ring(ring_smem, t);
+    const int p0 = (t >> 5) * (32 * NV) + (t & 31);  // its first piece
+    const RowRing<T, NV, 1, D, EVEN> ring(ring_smem, p0);
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     int64_t row = (int64_t)blockIdx.x * GROUPS + group;
     const float inv = 1.0f / (float)cols;
@@ -153,9 +154,9 @@ __global__ void __launch_bounds__(TPR < NT ? NT : TPR)
     int have[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        have[j] = EVEN ? ((int64_t)(t + j * TPR) * N < cols ? N : 0) : in_row<N>(t + j * TPR, cols);
-        load_w2<N>(gamma, wt, t + j * TPR, have[j], 1.0f, g[j]);
-        load_w2<N>(beta, wt, t + j * TPR, have[j], 0.0f, b[j]);
+        have[j] = EVEN ? ((int64_t)(p0 + j * 32) * N < cols ? N : 0) : in_row<N>(p0 + j * 32, cols);
+        load_w2<N>(gamma, wt, p0 + j * 32, have[j], 1.0f, g[j]);
+        load_w2<N>(beta, wt, p0 + j * 32, have[j], 0.0f, b[j]);
     }
     int slot = 0;
     for (int odd = 0; row < rows; row += step, odd ^= 1) {
@@ -175,16 +176,16 @@ __global__ void __launch_bounds__(TPR < NT ? NT : TPR)
         for (int j = 0; j < NV; j++)
             if (!EVEN || have[j]) Fwd<T>::spread(v[j], EVEN ? N : have[j], mu, d1, d2);
         const float2 f = Fwd<T>::finish(row_sum2<TPR>(lo2(d1) + hi2(d1), lo2(d2) + hi2(d2), sm[odd][1] + group * (TPR / 16), bar), inv, eps);
+        T *yr = y + row * ldy;
+        uint4 o[NV];
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            T *yr = y + row * ldy;
-            if constexpr (EVEN) {
-                if (have[j]) *(uint4 *)(yr + (t + j * TPR) * N) = Fwd<T>::out(v[j], f, g[j], b[j]);
-            } else {
-                const uint4 o = Fwd<T>::out(v[j], f, g[j], b[j]);
-                __syncwarp();
-                store_piece(yr, t + j * TPR, cols, o);
-            }
+            o[j] = Fwd<T>::out(v[j], f, g[j], b[j]);
+            if (EVEN && have[j]) *(uint4 *)(yr + (p0 + j * 32) * N) = o[j];
+        }
+        if constexpr (!EVEN) {
+            __syncwarp();
+            store_run<T, NV>(yr, p0, (int)cols, o);
         }
         if (t == 0) {
             if (mean) mean[row] = mu + f.x;
@@ -242,7 +243,7 @@ int launch_ln_ring(const T *x, int64_t ldx, int wt, const void *gamma, const voi
                    float *rstd, int64_t rows, int64_t cols, float eps, cudaStream_t s) {
     constexpr int BLOCK = TPR < NT ? NT : TPR, GROUPS = BLOCK / TPR;
     auto f = ln_kernel<T, TPR, NV, D, EVEN>;
-    const size_t smem = (size_t)(BLOCK / 32) * RowRing<T, TPR, NV, 1, D, EVEN>::kWarp * 16;
+    const size_t smem = (size_t)(BLOCK / 32) * RowRing<T, NV, 1, D, EVEN>::kWarp * 16;
     static int cache[64] = {0};
     const int per = blocks_per_sm(f, BLOCK, smem, smem, cache);
     if (!per) return cuda_fail(cudaGetLastError(), "layer_norm: occupancy");
@@ -260,15 +261,17 @@ int launch_ln(const T *x, int64_t ldx, int wt, const void *gamma, const void *be
 #define LN(...)                                                                                                              \
     return even ? launch_ln_ring<T, __VA_ARGS__, true>(x, ldx, wt, gamma, beta, y, ldy, mean, rstd, rows, cols, eps, s)      \
                 : launch_ln_ring<T, __VA_ARGS__, false>(x, ldx, wt, gamma, beta, y, ldy, mean, rstd, rows, cols, eps, s)
-    // sixteen columns a thread at most (32-bit: four pieces; 16-bit: two)
-    constexpr int NV = kPerThread / kPiece<T>;
-    if (n <= 32 * NV / 2) LN(32, NV / 2, 4);
-    if (n <= 32 * NV) LN(32, NV, 4);
-    if (n <= 128 * NV / 2) LN(128, NV / 2, 4);
-    if (n <= 128 * NV) LN(128, NV, 4);
-    if (n <= 512 * NV / 2) LN(512, NV / 2, 4);
-    if (n <= 512 * NV) LN(512, NV, 3);
-    if (n <= 1024 * NV) LN(1024, NV, 2);
+    // Four pieces a thread, and as few threads a row as hold it: sums over few warps cost the least.  (16384 x 1024 f16:
+    // 14.6 us with 32 threads, 16.9 with 64, 20.2 with 128; 4096 x 4096 bf16 15.7 with 128, 20.6 with 512.)  Fewer pieces
+    // for rows that would leave most lanes without: 16384 x 102 bf16 10.2 us with one, 15.9 with two.
+    if (n <= 32) LN(32, 1, 4);
+    if (n <= 64) LN(32, 2, 3);
+    if (n <= 128) LN(32, 4, 2);
+    if (n <= 256) LN(64, 4, 2);
+    if (n <= 512) LN(128, 4, 2);
+    if (n <= 1024) LN(256, 4, 2);
+    if (n <= 2048) LN(512, 4, 2);
+    if (n <= 4096) LN(1024, 4, 2);
 #undef LN
     ln_long_kernel<T><<<(unsigned)rows, 1024, 0, s>>>(x, ldx, wt, gamma, beta, y, ldy, mean, rstd, cols, eps);
     ZC_LAUNCHED("ln_long_kernel");
@@ -296,17 +299,18 @@ __global__ void __launch_bounds__(BLOCK)
         asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
     }
     const int group = threadIdx.x / TPR, bar = 1 + (TPR > 32 ? group : 0);
-    const int t = threadIdx.x % TPR, p0 = t + (int)rank * TPR * NV;  // in the block's part of a row, in the row
+    const int t = threadIdx.x % TPR, t0 = (t >> 5) * (32 * NV) + (t & 31);
+    const int p0 = t0 + (int)rank * TPR * NV;  // its first piece, of the block's part of a row (t0) and of the row
     const int64_t n = (cols + N - 1) / N;
     const float inv = 1.0f / (float)cols;
     f32x2 g[NV][N / 2], ag[NV][N / 2], ab[NV][N / 2];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        load_w2<N>(gamma, wt, p0 + j * TPR, in_row<N>(p0 + j * TPR, cols), 1.0f, g[j]);
+        load_w2<N>(gamma, wt, p0 + j * 32, in_row<N>(p0 + j * 32, cols), 1.0f, g[j]);
 #pragma unroll
         for (int e = 0; e < N / 2; e++) ag[j][e] = ab[j][e] = make2(0.0f);
     }
-    const RowRing<T, TPR, NV, 2, D, EVEN> ring(grad_smem, p0);
+    const RowRing<T, NV, 2, D, EVEN> ring(grad_smem, p0);
     const int64_t step = (int64_t)(gridDim.x / size) * GROUPS;
     int64_t row = (int64_t)(blockIdx.x / size) * GROUPS + group;
     auto issue = [&](int slot, int64_t r) {
@@ -371,17 +375,18 @@ __global__ void __launch_bounds__(BLOCK)
             }
         }
         const f32x2 m = make2(-rs * (q.x * inv)), k = make2(-rs * (q.y * inv)), r2 = make2(rs);
+        T *out = dx + row * lddx;
+        uint4 o[NV];
 #pragma unroll
         for (int j = 0; j < NV; j++) {
 #pragma unroll
             for (int e = 0; e < N / 2; e++) xh[j][e] = fma2(xh[j][e], k, fma2(gd[j][e], r2, m));
-            T *o = dx + row * lddx;
-            if constexpr (EVEN) {
-                if (p0 + j * TPR < n) *(uint4 *)(o + (int64_t)(p0 + j * TPR) * N) = pack2<T>(xh[j]);
-            } else {
-                __syncwarp();
-                store_piece(o, p0 + j * TPR, cols, pack2<T>(xh[j]));
-            }
+            o[j] = pack2<T>(xh[j]);
+            if (EVEN && p0 + j * 32 < n) *(uint4 *)(out + (p0 + j * 32) * N) = o[j];
+        }
+        if constexpr (!EVEN) {
+            __syncwarp();
+            store_run<T, NV>(out, p0, (int)cols, o);
         }
     }
     // no block ends while another may still write to its shared memory
@@ -398,7 +403,7 @@ __global__ void __launch_bounds__(BLOCK)
         if (group == k)
 #pragma unroll
             for (int j = 0; j < NV; j++) {
-                float *sg = comb + (t + j * TPR) * N, *sb = sg + PITCH;
+                float *sg = comb + (t0 + j * 32) * N, *sb = sg + PITCH;
 #pragma unroll
                 for (int e = 0; e < N; e++) {
                     const float u = e & 1 ? hi2(ag[j][e / 2]) : lo2(ag[j][e / 2]), v = e & 1 ? hi2(ab[j][e / 2]) : lo2(ab[j][e / 2]);
@@ -518,7 +523,8 @@ struct GradShape {
 };
 GradShape grad_shape(int64_t rows, int64_t cols) {
     GradShape g;
-    g.tpr = cols <= 32 * kPerThread ? 32 : cols <= 256 * kPerThread ? 256 : 512;
+    g.tpr = 32;
+    while (g.tpr < 512 && cols > (int64_t)g.tpr * kPerThread) g.tpr *= 2;
     g.groups = (g.tpr == 32 ? 256 : 512) / g.tpr;
     g.cluster = (int)((cols + (int64_t)g.tpr * kPerThread - 1) / ((int64_t)g.tpr * kPerThread));
     const int64_t want = (rows + g.groups - 1) / g.groups, most = (int64_t)num_sms() * (g.tpr == 32 ? 2 : 1) / g.cluster;
@@ -532,7 +538,7 @@ int launch_grad(const GradShape &g, const T *dy, int64_t lddy, const T *x, int64
                 int64_t cols, cudaStream_t s) {
     auto f = ln_grad_kernel<T, TPR, NV, BLOCK, D, CLUSTER, EVEN>;
     // the ring, in whose place the sums are added up at the end
-    constexpr size_t ring = (size_t)(BLOCK / 32) * RowRing<T, TPR, NV, 2, D, EVEN>::kWarp * 16, sums = (size_t)TPR * NV * kPiece<T> * 8;
+    constexpr size_t ring = (size_t)(BLOCK / 32) * RowRing<T, NV, 2, D, EVEN>::kWarp * 16, sums = (size_t)TPR * NV * kPiece<T> * 8;
     constexpr size_t smem = ring > sums ? ring : sums;
     static_assert(smem <= 226 * 1024, "shared memory");
     static int cache[64] = {0};
@@ -558,19 +564,15 @@ int launch_grad_for(const GradShape &g, const T *dy, int64_t lddy, const T *x, i
                     const float *rstd, int wt, const void *gamma, T *dx, int64_t lddx, float *parts, int64_t rows,
                     int64_t cols, cudaStream_t s) {
     constexpr int NV = kPerThread / kPiece<T>, D = NV > 2 ? 2 : 4;
-    const bool half = cols * 2 <= (int64_t)g.tpr * kPerThread;  // half of the columns a thread
     const bool even = even_rows<T>(x, ldx, rows, cols) && even_rows<T>(dy, lddy, rows, cols) && even_rows<T>(dx, lddx, rows, cols);
 #define GRAD(...)                                                                                                                     \
     return even ? launch_grad<T, __VA_ARGS__, true>(g, dy, lddy, x, ldx, mean, rstd, wt, gamma, dx, lddx, parts, rows, cols, s)       \
                 : launch_grad<T, __VA_ARGS__, false>(g, dy, lddy, x, ldx, mean, rstd, wt, gamma, dx, lddx, parts, rows, cols, s)
-    if (g.tpr == 32) {
-        if (half) GRAD(32, NV / 2, 256, 4, false);
-        GRAD(32, NV, 256, 4, false);
-    }
-    if (g.tpr == 256) {
-        if (half) GRAD(256, NV / 2, 512, 4, false);
-        GRAD(256, NV, 512, D, false);
-    }
+    if (cols <= 16 * kPerThread) GRAD(32, NV / 2, 256, 4, false);
+    if (g.tpr == 32) GRAD(32, NV, 256, 4, false);
+    if (g.tpr == 64) GRAD(64, NV, 512, D, false);
+    if (g.tpr == 128) GRAD(128, NV, 512, D, false);
+    if (g.tpr == 256) GRAD(256, NV, 512, D, false);
     if (g.cluster == 1) GRAD(512, NV, 512, D, false);
     GRAD(512, NV, 512, D, true);
 #undef GRAD
