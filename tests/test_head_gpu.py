@@ -866,3 +866,117 @@ def test_example_gradients_against_torch(zc):
     assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
     for got, leaf in zip(grads, leaves):
         assert float((got.double() - leaf.grad).norm() / leaf.grad.norm()) <= 2e-5
+
+
+# ------------------------------------------------------------- sizes at which the split of a row changes
+def row_splits(piece):
+    """Columns about the sizes at which a row gets another number of threads, for pieces of `piece` elements."""
+    return [c for n in (32, 64, 128, 256, 512, 1024, 2048, 4096) for c in (n * piece - 1, n * piece, n * piece + 3)]
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_layer_norm_by_the_threads_of_a_row(zc, t):
+    for cols in row_splits(4 if t == "f32" else 8):
+        for rows, pitch, shift in ((3, 0, 0), (310, 1, 1)):
+            if rows * cols > 4 << 20:
+                rows = 4
+            x, gamma, beta, _ = norm_inputs(rows, cols, t, "f32", seed=cols, pitch=pitch, shift=shift)
+            y = check_norm(zc, x, gamma, beta)
+            # a row's result depends neither on the rows beside it nor on where it lies
+            assert torch.equal(y[2:3], zc.layer_norm(x[2:3].contiguous(), gamma, beta))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("cols", [255, 256, 257, 511, 512, 513, 1023, 1025, 2047, 2049, 4095, 4097, 8191, 8193, 16385])
+def test_layer_norm_grad_by_the_threads_of_a_row(zc, cols, t):
+    check_norm_grad(zc, 11, cols, t, "f32", pitch=1, shift=1)
+    check_norm_grad(zc, 330 if cols < 5000 else 80, cols, t, "f32")
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+def test_quantize_by_the_threads_of_a_row(zc, t):
+    g = gen(21)
+    for cols in row_splits(4 if t == "f32" else 8):
+        x = (normal(g, 5, cols) * torch.exp(normal(g, 5, 1))).to(TYPES[t])
+        # values about halfway between two whole numbers of scales
+        x[:, 1:cols // 2] = ((torch.randint(0, 127, (5, cols // 2 - 1), generator=g, device="cuda") + 0.5)
+                             * (x.float().abs().amax(1, keepdim=True) / 127)).to(x.dtype)
+        x[3, cols - 1] = float("nan")
+        x[4, cols // 2] = float("-inf")
+        wq, ws = ref_quantize(x)
+        for v in (x, strided(x, 16, 8), strided(x, 1, 1)):
+            q, s = zc.quantize_rows(v)
+            assert torch.equal(q.cpu(), wq) and torch.equal(s.cpu().nan_to_num(-1), ws.nan_to_num(-1))
+
+
+# ------------------------------------------------------------- sampling: edges in odd places
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,vocab,spread", [(12, 3000, 0.02), (12, 9001, 0.02), (170, 3000, 0.004), (8, 40000, 0.3), (8, 30000, 1.0)])
+def test_sample_sets_that_end_about_zero(zc, rows, vocab, spread, t):
+    """Sets of ranks that end among many small logits, with and without many larger ones above them."""
+    g = gen(22)
+    x = (spread * normal(g, rows, vocab)).to(TYPES[t])
+    x[:, 7:400:3] += 3.0
+    u = torch.rand(rows, generator=g, device="cuda")
+    full = lambda v, d=torch.float32: torch.full((rows,), v, dtype=d, device="cuda")
+    for k, p in ((1200, 1.0), (0, 0.6), (0, 0.95), (2000, 0.8), (vocab // 2, 1.0), (vocab // 2, 0.97), (vocab - 1, 0.999)):
+        token, logprob = check_sample(zc, x[:12], u[:12], None, full(k, torch.int32)[:12], full(p)[:12], None)
+        many = zc.sample(x, u, top_k=full(k, torch.int32), top_p=full(p))  # more rows: other threads a row
+        assert torch.equal(many[0][:12], token) and torch.equal(many[1][:12], logprob)
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+def test_sample_ranges_wider_than_a_table(zc, t):
+    """Temperatures at which every value from the largest finite one down has weight, and logits out to both its ends."""
+    g = gen(23)
+    x = normal(g, 10, 20000).to(TYPES[t])
+    big = torch.finfo(TYPES[t]).max
+    x[:, ::7] *= 100.0
+    x[1, 5], x[1, 6], x[2, 9] = big, -big, -big
+    x[3] = x[3].abs() * 1e-3
+    x[4] = -x[4].abs() - 1.0
+    x[5, 30:40] = -math.inf
+    x[6, 50:60] = float("nan")
+    u = torch.rand(10, generator=g, device="cuda")
+    for T in (0.01, 30.0, 1e4, 3e37):
+        temp = torch.full((10,), T, device="cuda")
+        for k, p in ((0, 1.0), (900, 1.0), (0, 0.7), (15000, 0.9)):
+            check_sample(zc, x, u, temp, torch.full((10,), k, dtype=torch.int32, device="cuda"), torch.full((10,), p, device="cuda"), None)
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("vocab", [1, 3, 9, 300, 5001])
+def test_sample_the_first_of_the_largest(zc, vocab, t):
+    """The likeliest token at every place of short rows and the ends of long ones, at every alignment, with equals after it."""
+    g = gen(24)
+    for shift in range(9):
+        places = sorted({c for c in (0, 1, 2, 3, 6, 7, 8, 9, vocab // 2, vocab - 9, vocab - 2, vocab - 1) if 0 <= c < vocab})
+        x = strided(normal(g, len(places), vocab).to(TYPES[t]), 2, shift)
+        for i, c in enumerate(places):
+            x[i, c] = 50.0
+            x[i, c + 1::5] = 50.0
+        u = torch.rand(len(places), generator=g, device="cuda")
+        for kw in ({"temperature": 0.0}, {"top_k": 1}, {"top_p": 0.0}, {"top_k": 450, "top_p": 1e-6}):
+            assert zc.sample(x, u, **kw)[0].tolist() == places, (shift, kw)
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+def test_sample_infinite_logits_in_large_sets(zc, t):
+    """Infinite logits alone have weight, whatever the set."""
+    g = gen(25)
+    x = normal(g, 4, 12000).to(TYPES[t])
+    x[:, 700] = x[:, 11000] = math.inf
+    for kw in ({}, {"top_k": 2000}, {"top_p": 0.9}, {"min_p": 0.1}, {"top_k": 2000, "top_p": 0.999}):
+        for u, want in ((0.3, 700), (0.7, 11000)):
+            token, logprob = zc.sample(x, torch.full((4,), u, device="cuda"), **kw)
+            assert token.tolist() == [want] * 4
+            assert float((logprob + math.log(2)).abs().amax()) < 1e-6
+
+
+def test_sample_refuses_long_rows(zc):
+    x = torch.zeros(1, 1 << 22, device="cuda", dtype=torch.float16)
+    with pytest.raises(zc.ZpuCudaError) as e:
+        zc.sample(x, torch.zeros(1, device="cuda"))
+    assert e.value.name == "NotSupported"
+    token, logprob = zc.sample(x[:, 1:], torch.full((1,), 0.5, device="cuda", dtype=torch.float64), top_k=1 << 20)
+    assert int(token) == 1 << 19 and abs(float(logprob) + 20 * math.log(2)) < 1e-5
