@@ -462,9 +462,11 @@ int zpucuda_debug_peer_reduce(const float *d_inbox, int world, int64_t n, float 
  *    along the row and any row pitch (ld*, in elements, >= the row's length)
  *    and any alignment that fits their elements; rows may be 0.  Sums are held
  *    in f32 or wider and each result is rounded to its type once.
- *  - Calls are asynchronous on `stream` and, with no wait in them, may be
- *    captured in a CUDA graph.  Results do not depend on the run: the same
- *    inputs give the same bits.
+ *  - Calls are asynchronous on `stream`, allocate nothing and may be captured
+ *    in a CUDA graph.  Waits inside a kernel (of the distillation's clusters
+ *    and the tensor cores' product) are bounded; one that runs out is an error
+ *    that zpucuda_check_device reports.  Results do not depend on the run: the
+ *    same call on the same inputs gives the same bits.
  *
  * layer_norm: y = (x - mean) * rstd * gamma + beta over each row, rstd =
  *   1 / sqrt(mean((x - mean)^2) + eps).  gamma / beta: [cols] of type wtype, or

@@ -15,7 +15,7 @@
 // stayed (slices are at most 64 KiB, so all that is in flight is a third of L2).
 // Holding slices in shared memory instead was slower: every byte then occupies
 // its place from the copy to the gradient, 13.7 us, and 192 KiB an SM do not
-// cover that time at HBM's rate (2048 x 131072 bf16: @SMEM@ us, @L2@ us now).
+// cover that time at HBM's rate (2048 x 131072 bf16: 270 us, 230 us now, 4.7 TB/s).
 // A slice is counted in aligned 16-byte granules of memory, so an odd vocabulary
 // costs two partial granules a row and nothing else.
 #include "head.cuh"

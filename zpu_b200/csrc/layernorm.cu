@@ -6,7 +6,12 @@
 //   dx = rstd * (g - mean(g) - xhat * mean(g * xhat))
 //   dgamma = sum over rows of dy * xhat,  dbeta = sum over rows of dy.
 // HBM bounds both: a row is read once into registers, reduced there, and
-// written.  The gradient's blocks walk rows and keep their columns' sums of
+// written.  What keeps them from its rate are the two sums of a row that
+// everything waits for: rows are on their way to shared memory meanwhile, and a
+// row is held by few threads.  Forward 16384 x 1024 f16 takes 14.0 us (4.8 TB/s),
+// 4096 x 4096 bf16 15.0 us, 4 x 4096 2.8 us; backward 8192 x 4096 bf16 45 us
+// (4.5 TB/s), 1021 x 5003 f32 27.5 us (2.2 TB/s: pieces off the 16-byte grid are
+// shifted into place on both ways).  The gradient's blocks walk rows and keep their columns' sums of
 // dgamma and dbeta in registers; one row of sums a block goes to the caller's
 // workspace, and a second kernel adds those up in the blocks' order, so a
 // result does not depend on the run.
@@ -422,24 +427,24 @@ __global__ void __launch_bounds__(BLOCK)
 }
 
 // dgamma and dbeta from the blocks' sums: 32 columns a block, 16 rows of parts
-// at a time.
+// at a time.  It may be launched while the kernel that makes the sums still runs,
+// and waits for its end.
 __global__ void __launch_bounds__(512) ln_parts_kernel(const float *parts, int nparts, int wt, void *dgamma, void *dbeta,
                                                        int64_t cols) {
     __shared__ float sm[16][33];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;  // of 2 * cols
     float s = 0.0f;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (c < 2 * cols) {
         const float *p = parts + c;
-        int i = w;
-        for (; i + 64 < nparts; i += 80) {  // five loads in flight
-            float v[5];
+        for (int i = w; i < nparts; i += 160) {  // ten loads in flight
+            float v[10];
 #pragma unroll
-            for (int u = 0; u < 5; u++) v[u] = p[(int64_t)(i + 16 * u) * 2 * cols];
+            for (int u = 0; u < 10; u++) v[u] = i + 16 * u < nparts ? p[(int64_t)(i + 16 * u) * 2 * cols] : 0.0f;
 #pragma unroll
-            for (int u = 0; u < 5; u++) s += v[u];
+            for (int u = 0; u < 10; u++) s += v[u];
         }
-        for (; i < nparts; i += 16) s += p[(int64_t)i * 2 * cols];
     }
     sm[w][lane] = s;
     __syncthreads();
@@ -638,9 +643,18 @@ int zpucuda_layer_norm_grad(int dtype, const void *d_dy, int64_t lddy, const voi
                                                d_gamma, (T *)d_dx, lddx, sums ? (float *)d_work : nullptr, rows, cols, s)));
     }
     if (sums) {
-        ln_parts_kernel<<<(unsigned)((2 * cols + 31) / 32), 512, 0, s>>>((const float *)d_work, rows > 0 ? g.parts : 0, wtype,
-                                                                        d_dgamma, d_dbeta, cols);
-        ZC_LAUNCHED("ln_parts_kernel");
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)((2 * cols + 31) / 32));
+        cfg.blockDim = dim3(512);
+        cfg.stream = s;
+        cudaLaunchAttribute at[1] = {};
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = rows > 0 ? 1 : 0;
+        ZC_CUDA(cudaLaunchKernelEx(&cfg, ln_parts_kernel, (const float *)d_work, rows > 0 ? g.parts : 0, wtype, d_dgamma,
+                                   d_dbeta, cols));
+        count_launch();
     }
     return ZPUCUDA_OK;
 }

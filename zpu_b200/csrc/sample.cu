@@ -25,11 +25,16 @@
 //   - Otherwise a histogram of exact weights (or counts) over the logits' distance
 //     from the largest finds the bin in which the set ends, and that bin's tokens are
 //     listed and sorted.  What weighs too little to reach into the set is left out.
-//   - 16-bit logits have few values: a histogram of the values themselves takes the
-//     place of both the distances and the list, and a table of their exponentials
-//     that of computing one for every token.
-// Instructions bound it, not HBM: a few for each token in each pass, an exponential
-// among them for 32-bit logits.
+//   - 16-bit logits have few values: a count of each takes the place of the weights'
+//     histogram, so only the values' weights are computed, not the tokens'.
+// Two blocks of 512 threads share an SM where there are enough rows, otherwise a row
+// has 1024 threads (64 x 32000 f16, top_p: 36 us, with 512 42 us).
+//
+// Instructions bound it, not HBM: one to find the largest, a dozen and an addition in
+// shared memory to count a value, two dozen with an exponential to sum the kept
+// weights.  256 x 131071 bf16 (67 MB) takes 16 us without temperature, 31 with top_k
+// 50, 54 without a rule, 95 with top_p 0.9; 256 x 50000 f32 with top_p 0.9 takes 87
+// (weights in four parts of 10 bits, an addition in shared memory each).
 #include <cstring>
 
 #include "head.cuh"
