@@ -545,6 +545,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         tc::mb_init_fence();
     }
     if (warp == 1) tc::tmem_alloc(&tmem_base, TT::COLS);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // where the quantising kernel may still run
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -756,7 +757,7 @@ bool make_map(CUtensorMap *map, const int8_t *base, int64_t inner, int64_t rows,
 }
 
 template <int BN, bool SWAP, typename T>
-int launch_tc(const CUtensorMap &mp, const CUtensorMap &mq, const TcArgs &A, cudaStream_t s) {
+int launch_tc(const CUtensorMap &mp, const CUtensorMap &mq, const TcArgs &A, bool follows, cudaStream_t s) {
     auto k = int8_tc_kernel<BN, SWAP, T>;
     static bool attr[64] = {false};
     const int dev = current_device();
@@ -770,21 +771,24 @@ int launch_tc(const CUtensorMap &mp, const CUtensorMap &mq, const TcArgs &A, cud
     cfg.blockDim = dim3(TC_THREADS);
     cfg.dynamicSmemBytes = TcTile<BN>::SMEM;
     cfg.stream = s;
-    cudaLaunchAttribute at[1] = {};
+    cudaLaunchAttribute at[2] = {};
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = (unsigned)A.splits;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = follows ? 2 : 1;
     ZC_CUDA(cudaLaunchKernelEx(&cfg, k, mp, mq, A));
     count_launch();
     return ZPUCUDA_OK;
 }
 
-// The tensor-core product of m x n x k: *done says whether its operands allow it.
+// The tensor-core product of m x n x k: *done says whether its operands allow it.  follows: the kernel launched last on the
+// stream made the left operand, and this one's beginning may overlap its end.
 template <typename T>
 int product_tc(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb, const float *sb,
-               const float *bias, T *out, int64_t ldo, int64_t m, int64_t n, int64_t k, cudaStream_t s, bool *done) {
+               const float *bias, T *out, int64_t ldo, int64_t m, int64_t n, int64_t k, bool follows, cudaStream_t s, bool *done) {
     *done = false;
     // a tensor map's rows: at most 2^31, its coordinates 32 bits
     if (!aligned_to(a, 16) || !aligned_to(b, 16) || lda % 16 || ldb % 16 || k == 0) return ZPUCUDA_OK;
@@ -811,11 +815,11 @@ int product_tc(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, i
     if (!make_map(&mp, swap ? b : a, k, P, swap ? ldb : lda, 128) || !make_map(&mq, swap ? a : b, k, Q, swap ? lda : ldb, bn))
         return ZPUCUDA_OK;
     *done = true;
-    if (!swap) return bn == 256 ? launch_tc<256, false, T>(mp, mq, A, s) : launch_tc<128, false, T>(mp, mq, A, s);
-    if (bn == 16) return launch_tc<16, true, T>(mp, mq, A, s);
-    if (bn == 32) return launch_tc<32, true, T>(mp, mq, A, s);
-    if (bn == 64) return launch_tc<64, true, T>(mp, mq, A, s);
-    return launch_tc<128, true, T>(mp, mq, A, s);
+    if (!swap) return bn == 256 ? launch_tc<256, false, T>(mp, mq, A, follows, s) : launch_tc<128, false, T>(mp, mq, A, follows, s);
+    if (bn == 16) return launch_tc<16, true, T>(mp, mq, A, follows, s);
+    if (bn == 32) return launch_tc<32, true, T>(mp, mq, A, follows, s);
+    if (bn == 64) return launch_tc<64, true, T>(mp, mq, A, follows, s);
+    return launch_tc<128, true, T>(mp, mq, A, follows, s);
 }
 
 template <typename T, int V>
@@ -827,10 +831,12 @@ int launch_quantize(const T *x, int64_t ldx, int8_t *q, int64_t ldq, float *scal
         const int block = tpr < NT ? NT : tpr;
         f<<<(unsigned)((rows + block / tpr - 1) / (block / tpr)), block, 0, s>>>(x, ldx, q, ldq, scale, rows, cols);
     };
-    // As few threads a row as hold it in registers: 4096 x 2048 bf16 takes 10.3 us with 64, 13.7 with 256.
+    // As few threads a row as hold it in registers (4096 x 2048 bf16 takes 10.3 us with 64, 13.7 with 256), but 256 where
+    // there are few rows (64 x 4096 bf16: 2.5 us, with 128 3.2; 333 x 1001 3.0, with 64 4.0).
+    const bool few = rows <= 4 * (int64_t)num_sms();
     if (n <= 32 * NV) go(quantize_kernel<T, V, 32, NV>, 32);
-    else if (n <= 64 * NV) go(quantize_kernel<T, V, 64, NV>, 64);
-    else if (n <= 128 * NV) go(quantize_kernel<T, V, 128, NV>, 128);
+    else if (n <= 64 * NV && !few) go(quantize_kernel<T, V, 64, NV>, 64);
+    else if (n <= 128 * NV && !few) go(quantize_kernel<T, V, 128, NV>, 128);
     else if (n <= 256 * NV) go(quantize_kernel<T, V, 256, NV>, 256);
     else if (n <= 512 * NV) go(quantize_kernel<T, V, 512, NV>, 512);
     else if (n <= 1024 * NV) go(quantize_kernel<T, V, 1024, NV>, 1024);
@@ -852,12 +858,12 @@ int quantize(int dtype, const void *x, int64_t ldx, int8_t *q, int64_t ldq, floa
 }
 
 int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb, const float *sb,
-            const float *bias, int dtype, void *out, int64_t ldo, int64_t m, int64_t n, int64_t k, cudaStream_t s) {
+            const float *bias, int dtype, void *out, int64_t ldo, int64_t m, int64_t n, int64_t k, bool follows, cudaStream_t s) {
     if (m == 0 || n == 0) return ZPUCUDA_OK;
     if (takes_vec(b, ldb, m, k))
         ZC_HEAD_TYPE(dtype, T, return (product_vec<int8_t, T>(a, lda, sa, b, ldb, sb, bias, (T *)out, ldo, m, n, k, s)));
     bool done = false;
-    ZC_HEAD_TYPE(dtype, T, ZC_TRY(product_tc<T>(a, lda, sa, b, ldb, sb, bias, (T *)out, ldo, m, n, k, s, &done)));
+    ZC_HEAD_TYPE(dtype, T, ZC_TRY(product_tc<T>(a, lda, sa, b, ldb, sb, bias, (T *)out, ldo, m, n, k, follows, s, &done)));
     if (done) return ZPUCUDA_OK;
     dim3 grid((unsigned)((n + 63) / 64), (unsigned)((m + 63) / 64));
     ZC_HEAD_TYPE(dtype, T,
@@ -903,7 +909,7 @@ int zpucuda_int8_matmul(const int8_t *d_a, int64_t lda, const float *d_sa, const
     if (lda < k) return set_error(ZPUCUDA_ERR_INVALID_SHAPE, "int8_matmul: a: row pitch below the row's length");
     if (m > 0 && ((k > 0 && !d_a) || !d_sa))
         return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "int8_matmul: a or its scales: null pointer");
-    return product(d_a, lda, d_sa, d_b, ldb, d_sb, d_bias, dtype, d_out, ldo, m, n, k, resolve_stream(stream));
+    return product(d_a, lda, d_sa, d_b, ldb, d_sb, d_bias, dtype, d_out, ldo, m, n, k, false, resolve_stream(stream));
 }
 
 int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d_w, int64_t ldw, const float *d_sw,
@@ -922,7 +928,7 @@ int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d
     int8_t *q = (int8_t *)d_work;
     float *scale = (float *)(q + rows * ldq);
     ZC_TRY(quantize(dtype, d_x, ldx, q, ldq, scale, rows, inner, s));
-    return product(q, ldq, scale, d_w, ldw, d_sw, d_bias, dtype, d_y, ldy, rows, cols, inner, s);
+    return product(q, ldq, scale, d_w, ldw, d_sw, d_bias, dtype, d_y, ldy, rows, cols, inner, true, s);
 }
 
 int64_t zpucuda_int8_linear_work(int64_t rows, int64_t inner) {
