@@ -30,11 +30,12 @@
 // Two blocks of 512 threads share an SM where there are enough rows, otherwise a row
 // has 1024 threads (64 x 32000 f16, top_p: 36 us, with 512 42 us).
 //
-// Instructions bound it, not HBM: one to find the largest, a dozen and an addition in
-// shared memory to count a value, two dozen with an exponential to sum the kept
-// weights.  256 x 131071 bf16 (67 MB) takes 16 us without temperature, 31 with top_k
-// 50, 54 without a rule, 95 with top_p 0.9; 256 x 50000 f32 with top_p 0.9 takes 87
-// (weights in four parts of 10 bits, an addition in shared memory each).
+// Instructions bound it, not HBM: one to find the largest; to count a value a dozen
+// and an addition in shared memory, whose banks bound that pass; two dozen with an
+// exponential to sum the kept weights.  256 x 131071 bf16 (67 MB) takes 16 us
+// without temperature, 31 with top_k 50, 52 without a rule, 89 with top_p 0.9; 256 x
+// 50000 f32 with top_p 0.9 takes 87 (weights in four parts of 10 bits, an addition
+// in shared memory each).
 #include <cstring>
 
 #include "head.cuh"
@@ -420,7 +421,7 @@ __device__ __forceinline__ void choose(const Args &A, int64_t row, const Row<T> 
 struct Kept {
     float low, least;
     uint64_t ties, wk;
-    __device__ __forceinline__ float keep(float f, float e) const { return f > low && e >= least ? e : 0.0f; }
+    __device__ __forceinline__ float keep(float f, float e) const { return (f > low) & (e >= least) ? e : 0.0f; }
 };
 
 // The token whose running sum of kept weights by index exceeds the place.  Sums of each warp's granules first, then of
@@ -678,8 +679,7 @@ __device__ bool select_values(Shared &S, const Row<T> &R, int n, int64_t k, floa
             O.places(w[e], at);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                if (at[i] >= (uint32_t)n) continue;
-                atomicAdd(&table[at[i]], 1u);
+                atomicAdd(&table[min(at[i], (uint32_t)(n + lane))], 1u);  // past the places: not looked at
                 if (at[i] == zero) {
                     const int to = atomicAdd(&S.count, 1);
                     if (to < kNear) near_[to] = (unsigned short)(i ? w[e] >> 16 : w[e]);
@@ -861,7 +861,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T *logits, int64
             // places down to the last value with weight (a little lower does no harm), if the table holds them
             const float lowest = R.spike ? m : fmaxf(m - kSpan / R.inv, -3.0e38f);
             const int n = (int)Values<T>(m).place(raw_bits(from_f<T>(lowest))) + 2;  // lowest is rounded to nearest: kSpan has room
-            if ((p < 1.0f || (k > 0 && k < V)) && n <= A.places)
+            if ((p < 1.0f || (k > 0 && k < V)) && n + 32 <= A.places)
                 known = select_values(S, R, n, k < V ? k : 0, p, &key, &ties);
         }
         if (!known && k > 0 && k < V) {
