@@ -980,3 +980,16 @@ def test_sample_refuses_long_rows(zc):
     assert e.value.name == "NotSupported"
     token, logprob = zc.sample(x[:, 1:], torch.full((1,), 0.5, device="cuda", dtype=torch.float64), top_k=1 << 20)
     assert int(token) == 1 << 19 and abs(float(logprob) + 20 * math.log(2)) < 1e-5
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_sample_tiny_temperatures_and_logits(zc, t):
+    """Logits and temperatures at the small end of their type: the same tokens as those of both scaled up."""
+    g = gen(26)
+    x = normal(g, 8, 3000).to(TYPES[t])
+    u = torch.rand(8, generator=g, device="cuda")
+    for scale in (2.0 ** -40, 2.0 ** -100, 2.0 ** -117):
+        for kw in ({}, {"top_p": 0.9}, {"top_k": 1000}, {"top_k": 1000, "top_p": 0.8}):
+            want = zc.sample(x, u, temperature=1.0, **kw)
+            got = zc.sample((x.double() * scale).to(TYPES[t]), u, temperature=scale, **kw)
+            assert torch.equal(got[0], want[0]) and float((got[1] - want[1]).abs().amax()) <= 1e-4

@@ -34,7 +34,7 @@
 // and an addition in shared memory, whose banks bound that pass; two dozen with an
 // exponential to sum the kept weights.  256 x 131071 bf16 (67 MB) takes 16 us
 // without temperature, 31 with top_k 50, 52 without a rule, 89 with top_p 0.9; 256 x
-// 50000 f32 with top_p 0.9 takes 87 (weights in four parts of 10 bits, an addition
+// 50000 f32 with top_p 0.9 takes 72 (weights in four parts of 10 bits, an addition
 // in shared memory each).
 #include <cstring>
 
@@ -235,17 +235,17 @@ __device__ void clear() {
 __device__ __forceinline__ uint64_t bin_value(int b) {
     return (uint64_t)digit(0, b) + ((uint64_t)digit(1, b) << 10) + ((uint64_t)digit(2, b) << 20) + ((uint64_t)digit(3, b) << 30);
 }
-// MASS: the weight; otherwise one.
+// MASS: the weight high * 2^20 + low; otherwise one.
 template <bool MASS>
-__device__ __forceinline__ void bin_add(int b, uint64_t w) {
+__device__ __forceinline__ void bin_add(int b, uint32_t high, uint32_t low) {
     if (!MASS) {
         atomicAdd(&digit(0, b), 1u);
         return;
     }
-    atomicAdd(&digit(0, b), (uint32_t)w & 1023);
-    atomicAdd(&digit(1, b), (uint32_t)(w >> 10) & 1023);
-    atomicAdd(&digit(2, b), (uint32_t)(w >> 20) & 1023);
-    atomicAdd(&digit(3, b), (uint32_t)(w >> 30));
+    atomicAdd(&digit(0, b), low & 1023);
+    atomicAdd(&digit(1, b), low >> 10);
+    atomicAdd(&digit(2, b), high & 1023);
+    atomicAdd(&digit(3, b), high >> 10);
 }
 
 // The first bin whose running sum reaches target, and (*before) the sum of the bins before it; -1 if none does.
@@ -283,7 +283,17 @@ struct Bins {
     float span, scale, low;
     __device__ __forceinline__ Bins(float span_, float low_) : span(span_), scale((float)NB / span_), low(low_) {}
     // The bin of a token, -1: it is not counted.  d: its distance.
-    __device__ __forceinline__ int at(float f, float d) const { return f > low && -d < span ? min(NB - 1, (int)(-d * scale)) : -1; }
+    __device__ __forceinline__ int at(float f, float d) const {
+        // (2^23 added and rounded towards zero leaves a whole number in the last bits, in less time than a conversion.)
+        return f > low && -d < span ? min(NB - 1, (int)(__float_as_uint(__fadd_rz(-d * scale, 8388608.0f)) & 0x7fffffu)) : -1;
+    }
+    // Logits between which bin b's lie, and few others: its ends, moved by more than their rounding.
+    __device__ __forceinline__ float2 about(const Row<T> &R, int b) const {
+        const float unit = 1.0f / (scale * R.inv), far = 1e-6f * fabsf(R.m);
+        if (!(unit > 1e-30f && unit < 1e30f)) return make_float2(-INFINITY, INFINITY);
+        return make_float2(R.m - (float)(b + 1) * 1.00001f * unit - far, R.m - (float)b * 0.99999f * unit + far);
+    }
+
 };
 
 // The key of the entry of a sorted list at which the running measure reaches target, and how many up to it have that key.
@@ -342,11 +352,13 @@ __device__ uint32_t select_ranks(Shared &S, const Row<T> &R, const Bins<T> &H, u
         }
         __syncthreads();
         uint32_t kmin = 0xffffffffu, kmax = 0;
+        const float2 near_ = R.spike ? make_float2(-INFINITY, INFINITY) : first ? H.about(R, b) : make_float2(value_of(lo), value_of(hi));
         R.each(R.g0, R.g1, [&](const uint4 &q, int g) {
             float f[N];
             unpack<T>(q, f);
 #pragma unroll
             for (int e = 0; e < N; e++) {
+                if (!((f[e] >= near_.x) & (f[e] <= near_.y))) continue;
                 const uint32_t k = key_of(f[e]);
                 if (first ? H.at(f[e], R.dist(f[e])) != b : k < lo || k > hi) continue;
                 kmin = min(kmin, k);
@@ -384,7 +396,10 @@ __device__ uint32_t select_ranks(Shared &S, const Row<T> &R, const Bins<T> &H, u
 #pragma unroll
             for (int e = 0; e < N; e++) {
                 const uint32_t k = key_of(f[e]);
-                if (k >= lo && k <= hi) bin_add<MASS>((hi - k) >> shift, MASS ? R.weight(f[e]) : 1);
+                if (k >= lo && k <= hi) {
+                    const uint64_t w = MASS ? R.weight(f[e]) : 0;
+                    bin_add<MASS>((hi - k) >> shift, (uint32_t)(w >> 20), (uint32_t)w & 0xfffffu);
+                }
             }
         });
         __syncthreads();
@@ -416,6 +431,15 @@ __device__ __forceinline__ void choose(const Args &A, int64_t row, const Row<T> 
     if (A.logprob) A.logprob[row] = R.dist(f) - logf((float)(int64_t)total / (float)kOne);
 }
 
+// floor(2^40 e), 0 <= e <= 1, as two whole numbers of 20 bits, floor(2^20 e) and floor(2^40 (e - the first / 2^20)): adding
+// 8 = 2^3 to e with rounding towards zero leaves the first in the last bits of the sum, adding 2^-17 to the exact rest the
+// second.
+constexpr uint32_t k3 = 0x41000000u, k17 = 0x37000000u;  // 2^3, 2^-17
+__device__ __forceinline__ uint2 halves(float e) {
+    const float hi = __fadd_rz(e, __uint_as_float(k3)), rest = e - (hi - __uint_as_float(k3));
+    return make_uint2(__float_as_uint(hi) - k3, __float_as_uint(__fadd_rz(rest, __uint_as_float(k17))) - k17);
+}
+
 // What is kept: tokens above `low` whose e^((x - max) / T) is at least `least`, and the first `ties` equal to `low`, which
 // weigh wk each.
 struct Kept {
@@ -426,16 +450,12 @@ struct Kept {
 
 // The token whose running sum of kept weights by index exceeds the place.  Sums of each warp's granules first, then of
 // parts of the ones that hold the place, then of those.
-//
-// A weight is summed as two whole numbers of 20 bits, floor(2^20 e) and floor(2^40 (e - the first / 2^20)): adding 8 = 2^3
-// to e with rounding towards zero leaves the first in the last bits of the sum, adding 2^-17 to the exact rest the second.
 template <typename T>
 __device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t row, const Kept K) {
     constexpr int N = Row<T>::N;
     const uint64_t ties = K.ties, wk = K.wk;
     const int warp = threadIdx.x >> 5;
     auto add = [&](int a, int b, auto tied) {  // of granules a to b, to S
-        constexpr uint32_t k3 = 0x41000000u, k17 = 0x37000000u;  // 2^3, 2^-17
         const f32x2 c3 = make2(__uint_as_float(k3)), c17 = make2(__uint_as_float(k17));
         auto sub2 = [](f32x2 x, f32x2 y) { return fma2(y, make2(-1.0f), x); };
         uint64_t high = 0, low = 0;
@@ -873,7 +893,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T *logits, int64
 #pragma unroll
                 for (int e = 0; e < N; e++) {
                     const int b = H.at(f[e], R.dist(f[e]));
-                    if (b >= 0) bin_add<false>(b, 1);
+                    if (b >= 0) bin_add<false>(b, 0, 0);
                 }
             });
             key = select_ranks<T, false>(S, R, H, (uint64_t)k, &ties);
@@ -898,14 +918,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T *logits, int64
             R.each(R.g0, R.g1, [&](const uint4 &q, int) {
                 float f[N];
                 unpack<T>(q, f);
+                uint32_t high = 0, rest = 0;  // sums of the weights' two halves
 #pragma unroll
                 for (int e = 0; e < N; e++) {
-                    const float d = R.dist(f[e]);
-                    const uint64_t w = f[e] > low ? R.weight(f[e]) : 0;
-                    sum += w;
+                    const float d = R.dist(f[e]), p = f[e] > low ? R.spike ? (f[e] == m ? 1.0f : 0.0f) : expf(d) : 0.0f;
+                    const uint2 w = halves(p);
+                    high += w.x;
+                    rest += w.y;
                     const int b = H.at(f[e], d);
-                    if (b >= 0) bin_add<true>(b, w);
+                    if (b >= 0) bin_add<true>(b, w.x, w.y);
                 }
+                sum += ((uint64_t)high << 20) + rest;
             });
             sum = warp_sum64(sum);
             __syncthreads();
