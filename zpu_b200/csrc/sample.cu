@@ -318,7 +318,7 @@ __device__ uint32_t list_find(Shared &S, const Row<T> &R, int n, uint64_t target
         if (below >= target) break;
     }
     int same = 0;
-    for (int i = threadIdx.x; i <= S.count; i += NT()) same += entry_key(list(i)) == S.kmin;
+    for (int i = threadIdx.x; i <= min(S.count, n - 1); i += NT()) same += entry_key(list(i)) == S.kmin;
     if (threadIdx.x == 0) S.before = 0;
     __syncthreads();
     if (same) atomicAdd(&S.before, (unsigned long long)same);
