@@ -27,18 +27,17 @@ def _codes():
     return {torch.float32: _capi.F32, torch.float16: 2, torch.bfloat16: _capi.DT_BF16}
 
 
-def _stream(stream, x):
-    """The cudaStream_t that a call on x runs on.  A launch goes to the current
-    device, so x has to be there.  (The current stream's handle without a
-    Stream object around it: a call on one token is the shorter by 2 us.)"""
-    torch = _torch()
+def _stream(x):
+    """The current stream, a cudaStream_t, for a call on x.  A launch goes to
+    the current device, so x has to be there.  (The handle without a Stream
+    object around it: a call on one token is the shorter by 2 us.)"""
+    C = _torch()._C
     dev = x.get_device()
-    if dev != torch._C._cuda_getDevice():
-        _refuse(12, "the tensors are on %s, the current device is cuda:%d" % (x.device, torch._C._cuda_getDevice()))
-    h = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    if dev != C._cuda_getDevice():
+        _refuse(12, "the tensors are on %s, the current device is cuda:%d" % (x.device, C._cuda_getDevice()))
     # torch's default stream is the legacy NULL stream; NULL means the thread's
     # own stream to the C ABI, so it is named as cudaStreamLegacy.
-    return h if h else CUDA_STREAM_LEGACY
+    return C._cuda_getCurrentRawStream(dev) or CUDA_STREAM_LEGACY
 
 
 def _refuse(status, text):
@@ -81,12 +80,13 @@ def _vector(name, t, n, like, dtype=None):
     """Checks an optional [n] argument; its address."""
     if t is None:
         return None
-    if t.shape != (n,):
+    if t.dim() != 1 or t.numel() != n:
         _refuse(2, "%s: shape %s, (%d,) is wanted" % (name, tuple(t.shape), n))
     if dtype is not None and t.dtype != dtype:
         _refuse(3, "%s: dtype %s, %s is wanted" % (name, t.dtype, dtype))
-    _device(name, t, like)
-    if n > 1 and t.stride(0) != 1:
+    if not t.is_cuda or t.get_device() != like.get_device():
+        _device(name, t, like)
+    if n > 1 and not t.is_contiguous():
         _refuse(7, "%s is not contiguous" % name)
     return t.data_ptr()
 
@@ -106,22 +106,6 @@ def _output(name, out, like, shape=None, dtype=None):
     return out, _matrix(name, out, like, shape)
 
 
-class _Here:
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *_):
-        pass
-
-
-_here = _Here()
-
-
-def _on(stream):
-    """New tensors of the block belong to the stream that the call runs on."""
-    return _here if stream is None else _torch().cuda.stream(stream)
-
-
 # ------------------------------------------------------------- layer norm
 def _weights(x, gamma, beta):
     cols = x.shape[1]
@@ -136,18 +120,20 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, out=None, stats=False, stream
     """(x - mean) / sqrt(var + eps) * gamma + beta over each row of x.  With
     `stats` also the rows' mean and 1 / sqrt(var + eps) (float32), which
     layer_norm_grad takes.  `out` may be x."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return layer_norm(x, gamma, beta, eps, out, stats)
     torch = _torch()
     ldx, code = _matrix("x", x), _code("x", x)
     wt, g, b = _weights(x, gamma, beta)
     rows, cols = x.shape
-    with _on(stream):
-        y, ldy = _output("out", out, x)
-        if stats:
-            mean = torch.empty(rows, dtype=torch.float32, device=x.device)
-            rstd = torch.empty_like(mean)
+    y, ldy = _output("out", out, x)
+    if stats:
+        mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
     check(lib().zpucuda_layer_norm(code, x.data_ptr(), ldx, wt, g, b, y.data_ptr(), ldy,
                                    mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None,
-                                   rows, cols, eps, _stream(stream, x)))
+                                   rows, cols, eps, _stream(x)))
     return (y, mean, rstd) if stats else y
 
 
@@ -155,6 +141,9 @@ def layer_norm_grad(dy, x, mean, rstd, gamma=None, out=None, stream=None):
     """(dx, dgamma, dbeta) of layer_norm for the output's gradient dy: dx like
     x (in `out`, which may be dy or x), dgamma and dbeta like gamma (float32
     without one)."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return layer_norm_grad(dy, x, mean, rstd, gamma, out)
     torch = _torch()
     ldx, code = _matrix("x", x), _code("x", x)
     if dy.dtype != x.dtype:
@@ -164,14 +153,13 @@ def layer_norm_grad(dy, x, mean, rstd, gamma=None, out=None, stream=None):
     m = _vector("mean", mean, rows, x, torch.float32)
     r = _vector("rstd", rstd, rows, x, torch.float32)
     wt, g, _ = _weights(x, gamma, None)
-    with _on(stream):
-        dx, lddx = _output("out", out, x)
-        dgamma = torch.empty(cols, dtype=gamma.dtype if gamma is not None else torch.float32, device=x.device)
-        dbeta = torch.empty_like(dgamma)
-        work = torch.empty(lib().zpucuda_layer_norm_grad_work(rows, cols), dtype=torch.uint8, device=x.device)
+    dx, lddx = _output("out", out, x)
+    dgamma = torch.empty(cols, dtype=gamma.dtype if gamma is not None else torch.float32, device=x.device)
+    dbeta = torch.empty_like(dgamma)
+    work = torch.empty(lib().zpucuda_layer_norm_grad_work(rows, cols), dtype=torch.uint8, device=x.device)
     check(lib().zpucuda_layer_norm_grad(code, dy.data_ptr(), lddy, x.data_ptr(), ldx, m, r, wt, g, dx.data_ptr(), lddx,
                                         dgamma.data_ptr(), dbeta.data_ptr(), rows, cols, work.data_ptr(), work.numel(),
-                                        _stream(stream, x)))
+                                        _stream(x)))
     return dx, dgamma, dbeta
 
 
@@ -197,56 +185,64 @@ def distill_loss(logits, teacher, indices, temperature=1.0, weight=None, stream=
     softmax) of each row at temperature T, and log sum exp(logits / T).
     teacher: the teacher's top logits [rows, top] at the vocabulary `indices`
     (int32 / int64; -1: no entry).  A row with weight 0 or no entry gives 0."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return distill_loss(logits, teacher, indices, temperature, weight)
     torch = _torch()
     head, dims = _distill_args(logits, teacher, indices, weight)
-    with _on(stream):
-        loss = torch.empty(dims[0], dtype=torch.float32, device=logits.device)
-        lse = torch.empty_like(loss)
+    loss = torch.empty(dims[0], dtype=torch.float32, device=logits.device)
+    lse = torch.empty_like(loss)
     check(lib().zpucuda_distill_loss(*head, temperature, loss.data_ptr(), lse.data_ptr(), *dims,
-                                     _stream(stream, logits)))
+                                     _stream(logits)))
     return loss, lse
 
 
 def distill_grad(logits, teacher, indices, lse, dloss=None, temperature=1.0, weight=None, out=None, stream=None):
     """The gradient of sum(dloss * loss) with regard to the logits, from
     distill_loss's lse.  `out` may be the logits."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return distill_grad(logits, teacher, indices, lse, dloss, temperature, weight, out)
     torch = _torch()
     head, dims = _distill_args(logits, teacher, indices, weight)
     l = _vector("lse", lse, dims[0], logits, torch.float32)
     d = _vector("dloss", dloss, dims[0], logits, torch.float32)
-    with _on(stream):
-        g, ldg = _output("out", out, logits)
+    g, ldg = _output("out", out, logits)
     check(lib().zpucuda_distill_grad(*head, temperature, l, d, g.data_ptr(), ldg, *dims,
-                                     _stream(stream, logits)))
+                                     _stream(logits)))
     return g
 
 
 def distill_value_and_grad(logits, teacher, indices, dloss=None, temperature=1.0, weight=None, out=None, stream=None):
     """(loss, dlogits): distill_loss and distill_grad from one reading of the
     logits.  `out` may be the logits."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return distill_value_and_grad(logits, teacher, indices, dloss, temperature, weight, out)
     torch = _torch()
     head, dims = _distill_args(logits, teacher, indices, weight)
     d = _vector("dloss", dloss, dims[0], logits, torch.float32)
-    with _on(stream):
-        loss = torch.empty(dims[0], dtype=torch.float32, device=logits.device)
-        g, ldg = _output("out", out, logits)
+    loss = torch.empty(dims[0], dtype=torch.float32, device=logits.device)
+    g, ldg = _output("out", out, logits)
     check(lib().zpucuda_distill_value_and_grad(*head, temperature, d, loss.data_ptr(), g.data_ptr(), ldg, *dims,
-                                               _stream(stream, logits)))
+                                               _stream(logits)))
     return loss, g
 
 
 # ------------------------------------------------------------- 8-bit integers
 def quantize_rows(x, stream=None):
     """(q, scale): int8 rows and their float32 scales, scale = max |row| / 127."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return quantize_rows(x)
     torch = _torch()
     ldx, code = _matrix("x", x), _code("x", x)
     rows, cols = x.shape
-    with _on(stream):
-        # a row pitch of a multiple of 16 bytes, as the product reads best
-        q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :cols]
-        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    # a row pitch of a multiple of 16 bytes, as the product reads best
+    q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :cols]
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     check(lib().zpucuda_int8_quantize(code, x.data_ptr(), ldx, q.data_ptr(), _matrix("q", q), scale.data_ptr(),
-                                      rows, cols, _stream(stream, x)))
+                                      rows, cols, _stream(x)))
     return q, scale
 
 
@@ -260,6 +256,9 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=None, out=None, stream=
     """(a @ b.T) * a_scale[:, None] * b_scale + bias for int8 a [m, k] and b
     [n, k] with float32 scales per row, summed exactly; float32 unless `dtype`
     or `out` says otherwise."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return int8_matmul(a, a_scale, b, b_scale, bias, dtype, out)
     torch = _torch()
     lda, ldb = _int8("a", a), _int8("b", b, a)
     m, k = a.shape
@@ -271,10 +270,9 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=None, out=None, stream=
     bi = _vector("bias", bias, n, a, torch.float32)
     if dtype is None:
         dtype = out.dtype if out is not None else torch.float32
-    with _on(stream):
-        y, ldy = _output("out", out, a, (m, n), dtype)
+    y, ldy = _output("out", out, a, (m, n), dtype)
     check(lib().zpucuda_int8_matmul(a.data_ptr(), lda, sa, b.data_ptr(), ldb, sb, bi, _code("out", y), y.data_ptr(),
-                                    ldy, m, n, k, _stream(stream, a)))
+                                    ldy, m, n, k, _stream(a)))
     return y
 
 
@@ -300,23 +298,27 @@ class Int8Linear:
     @classmethod
     def from_float(cls, weight, bias=None, stream=None):
         """From float32 / float16 / bfloat16 weights [cols, inner]."""
-        with _on(stream):
-            return cls(*quantize_rows(weight, stream), bias)
+        if stream is not None:
+            with _torch().cuda.stream(stream):
+                return cls.from_float(weight, bias)
+        return cls(*quantize_rows(weight), bias)
 
     def __call__(self, x, out=None, stream=None):
+        if stream is not None:
+            with _torch().cuda.stream(stream):
+                return self(x, out)
         torch = _torch()
         ldx, code = _matrix("x", x, self.weight), _code("x", x)
         rows, inner = x.shape
         cols = self.weight.shape[0]
         if inner != self.weight.shape[1]:
             _refuse(2, "x is %s, the weight %s" % (tuple(x.shape), tuple(self.weight.shape)))
-        with _on(stream):
-            y, ldy = _output("out", out, x, (rows, cols))
-            work = torch.empty(lib().zpucuda_int8_linear_work(rows, inner), dtype=torch.uint8, device=x.device)
+        y, ldy = _output("out", out, x, (rows, cols))
+        work = torch.empty(lib().zpucuda_int8_linear_work(rows, inner), dtype=torch.uint8, device=x.device)
         check(lib().zpucuda_int8_linear(code, x.data_ptr(), ldx, self.weight.data_ptr(), self._ld,
                                         self.scale.data_ptr(), None if self.bias is None else self.bias.data_ptr(),
                                         y.data_ptr(), ldy, rows, cols, inner, work.data_ptr(), work.numel(),
-                                        _stream(stream, x)))
+                                        _stream(x)))
         return y
 
 
@@ -328,6 +330,9 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     likeliest token), top_k (int32; <= 0: all), top_p (float32; >= 1: all) and
     min_p (float32; <= 0: all) are [rows] tensors, or plain numbers for every
     row.  NaN and -inf logits are never drawn; a row of nothing else gives -1."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return sample(logits, uniform, temperature, top_k, top_p, min_p)
     torch = _torch()
     ld, code = _matrix("logits", logits), _code("logits", logits)
     rows, vocab = logits.shape
@@ -344,11 +349,10 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
             keep.append(v)
         return _vector(name, v, rows, logits, dtype)
 
-    with _on(stream):
-        rules = (each("temperature", temperature, torch.float32), each("top_k", top_k, torch.int32),
-                 each("top_p", top_p, torch.float32), each("min_p", min_p, torch.float32))
-        token = torch.empty(rows, dtype=torch.int64, device=logits.device)
-        logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    rules = (each("temperature", temperature, torch.float32), each("top_k", top_k, torch.int32),
+             each("top_p", top_p, torch.float32), each("min_p", min_p, torch.float32))
+    token = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
     check(lib().zpucuda_sample(code, logits.data_ptr(), ld, 0 if uniform.dtype == torch.float64 else 1, u, *rules,
-                               token.data_ptr(), logprob.data_ptr(), rows, vocab, _stream(stream, logits)))
+                               token.data_ptr(), logprob.data_ptr(), rows, vocab, _stream(logits)))
     return token, logprob
