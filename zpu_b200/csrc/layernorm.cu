@@ -21,7 +21,7 @@ namespace zc {
 namespace {
 
 constexpr int NT = 256;
-constexpr int kPerThread = 16;  // columns of a row that a thread holds
+constexpr int kPerThread = 16;  // columns of a row that a thread of the gradient holds
 constexpr int kMaxCluster = 8;  // blocks of a cluster of it
 constexpr int64_t kMaxOnePass = 512 * kPerThread * kMaxCluster;
 
@@ -522,7 +522,8 @@ int launch_grad_long(const T *dy, int64_t lddy, const T *x, int64_t ldx, const f
     return ZPUCUDA_OK;
 }
 
-// Threads a row, rows a block, blocks a row and rows of sums of the one-pass gradient.
+// Threads a row, rows a block, blocks a row and rows of sums of the one-pass gradient.  As few threads as hold the row (16384
+// x 1024 f16: 30 us with 64, 54 with 256), and blocks of 512, which fill the registers: more that keep less were slower.
 struct GradShape {
     int tpr, groups, cluster, parts;
 };
