@@ -993,3 +993,25 @@ def test_sample_tiny_temperatures_and_logits(zc, t):
             want = zc.sample(x, u, temperature=1.0, **kw)
             got = zc.sample((x.double() * scale).to(TYPES[t]), u, temperature=scale, **kw)
             assert torch.equal(got[0], want[0]) and float((got[1] - want[1]).abs().amax()) <= 1e-4
+
+
+# ------------------------------------------------------------- rows shorter than 16 bytes
+SHORT = [("f32", 1, 1), ("f32", 2, 1), ("f32", 1, 2), ("f16", 1, 1), ("f16", 2, 3), ("f16", 6, 1), ("bf16", 1, 6), ("bf16", 3, 2)]
+
+
+@pytest.mark.parametrize("t,cols,shift", SHORT)
+def test_layer_norm_of_rows_inside_16_bytes(zc, t, cols, shift):
+    """A first row that begins off the 16-byte grid and ends in the same 16 bytes: nothing that an earlier call left in
+    shared memory (here NaN) is among its sums."""
+    g = gen(27)
+    mess = strided(torch.full((60000, 100), float("nan"), device="cuda", dtype=TYPES[t]), 1, 1)
+    ones = torch.ones(60000, device="cuda")
+    for rows in (1, 5, 700):
+        x, gamma, beta, _ = norm_inputs(rows, cols, t, "f32", seed=cols, pitch=8, shift=shift)
+        dy = strided(normal(g, rows, cols).to(TYPES[t]), 8, shift)
+        want = zc.layer_norm(x.contiguous(), gamma, beta, stats=True)
+        dwant = zc.layer_norm_grad(dy.contiguous(), x.contiguous(), *want[1:], gamma)
+        zc.layer_norm(mess)
+        assert all(torch.equal(a, b) for a, b in zip(zc.layer_norm(x, gamma, beta, stats=True), want))
+        zc.layer_norm_grad(mess, mess, ones, ones)
+        assert all(torch.equal(a, b) for a, b in zip(zc.layer_norm_grad(dy, x, *want[1:], gamma), dwant))

@@ -310,8 +310,8 @@ struct RowRing {
                 continue;
             }
             if (first && s && b == 0) {
-                T *e = (T *)(dst + lane);
-                for (int i = (int)(s / sizeof(T)); i < kPiece<T> && i * (int)sizeof(T) < end; i++) e[i] = row[i - (int)(s / sizeof(T))];
+                T *e = (T *)(dst + lane);  // 0 outside the row, as the copies leave it
+                for (int i = 0, at = -(int)(s / sizeof(T)); i < kPiece<T>; i++, at++) e[i] = at >= 0 && at < n ? row[at] : from_f<T>(0.0f);
             } else {
                 copy(dst + lane, from + b, end - b < 16 ? end - b : 16);
             }
