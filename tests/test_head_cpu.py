@@ -123,3 +123,46 @@ def test_front_end_refuses_host_tensors():
     with pytest.raises(zc.ZpuCudaError) as e:
         zc.layer_norm(torch.zeros(3))
     assert e.value.name == "InvalidShape"
+
+
+# ------------------------------------------------------------- sizes that the kernels go by, walked through on the host
+def host(tmp_path, body, *flags):
+    """The output of a C++ program about csrc/head_rules.h."""
+    import os
+    import subprocess
+    from zpu_b200 import build
+    src, exe = tmp_path / "rules.cpp", tmp_path / "rules"
+    src.write_text('#include <stdio.h>\n#include <algorithm>\n#include "head_rules.h"\nusing namespace zc;\nint main() {\n%s\n}\n' % body)
+    subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-O1", *flags, "-I", build.CSRC, str(src), "-o", str(exe)], check=True)
+    return subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()
+
+
+def test_short_rows_are_read_inside_shared_memory(tmp_path):
+    """The product of one or two tokens: the last byte that the last warp's last slot gives, over all sizes of a row, of a
+    unit and of a block's share, lies inside what the kernel is launched with; and units of several rows do come up.
+    (Four rows read whatever a unit has would end past it: 135168 bytes of 133120 at 2048 values by 8192 channels.)"""
+    out = host(tmp_path, """
+    long bad = 0, over = 0, several = 0, worst = 0;
+    for (int k = 1; k <= 9000; k++)
+        for (int per = 1; per <= 520; per++)
+            for (int m = 1; m <= 2; m++) {
+                const VecUnits U = vec_units(148l * per, k, 148);
+                const long slot = GV_RING - GV_SLOT, smem = vec_smem(m, k);
+                const int size = std::min(U.seg, k), last = (size + 15) / 16 * 16;  // lanes read 16 bytes that begin below size
+                bad += U.rows < 1 || U.rows * U.seg > GV_SLOT || U.per > GV_CHANNELS || (U.segs > 1 && U.rows > 1);
+                several += U.rows > 1;
+                for (int rows = 1; rows <= U.rows; rows++) {  // the last unit of a round may have fewer
+                    long end = 0, wide = 0;
+                    for (int r = 0; r < rows; r += 4)
+                        for (int i = 0; i < (U.rows == 1 ? 1 : 4); i++) {
+                            end = std::max(end, slot + (long)vec_row(r + i, rows) * U.seg + last);
+                            wide = std::max(wide, slot + (long)(r + i) * U.seg + last);
+                        }
+                    bad += end > GV_RING;
+                    over += wide > smem;
+                    if (k == 2048 && per == 56 && m == 1 && rows == 2) worst = wide;
+                }
+            }
+    printf("%ld %d %d %ld", bad, several > 0, over > 0, worst);
+    """)
+    assert out == ["0", "1", "1", "135168"]

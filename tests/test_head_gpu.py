@@ -1015,3 +1015,27 @@ def test_layer_norm_of_rows_inside_16_bytes(zc, t, cols, shift):
         assert all(torch.equal(a, b) for a, b in zip(zc.layer_norm(x, gamma, beta, stats=True), want))
         zc.layer_norm_grad(mess, mess, ones, ones)
         assert all(torch.equal(a, b) for a, b in zip(zc.layer_norm_grad(dy, x, *want[1:], gamma), dwant))
+
+
+# ------------------------------------------------------------- one and two tokens: units of several rows, several rounds
+def check_tokens(zc, m, n, k, t):
+    """Sums of the 8-bit product of m tokens with n channels, to the last bit, and the whole layer."""
+    g = gen(28)
+    a, b = ints(g, m, k), ints(g, n, k)
+    pad = (k + 15) // 16 * 16 - k
+    one = torch.ones(max(m, n), device="cuda")
+    want = (a.double() @ b.double().t()).float()  # whole numbers, rounded once
+    assert torch.equal(zc.int8_matmul(a, one[:m], strided(b, pad), one[:n]), want)
+    layer = zc.Int8Linear(b, torch.rand(n, generator=g, device="cuda") / k, normal(g, n))
+    x = (normal(g, m, k) * torch.exp(normal(g, m, 1))).to(TYPES[t])
+    q, s = ref_quantize(x)
+    for v in (x, strided(x, 3, 1)):
+        check_product(layer(v), q, s, b, layer.scale, layer.bias)
+
+
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("n,k", [(5000, 33), (5000, 100), (16384, 500), (16384, 656), (32000, 784), (32000, 816), (16384, 1001),
+                                 (5000, 1424), (5120, 1536), (4737, 2000), (8192, 2048), (16384, 2047), (80001, 16), (80001, 333),
+                                 (80001, 2048), (50257, 768), (76800, 5000)])
+def test_int8_tokens_by_several_rows(zc, m, n, k):
+    check_tokens(zc, m, n, k, ("f32", "f16", "bf16")[(n + k) % 3])

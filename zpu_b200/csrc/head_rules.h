@@ -1,0 +1,41 @@
+// Sizes that the language-model head's kernels go by, free of CUDA so that a
+// host program can walk through them.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define ZC_RULE __host__ __device__ inline
+#else
+#define ZC_RULE inline
+#endif
+
+namespace zc {
+
+// ---- the 8-bit product of one or two tokens (int8.cu)
+constexpr int GV_WARPS = 16, GV_SLOTS = 2, GV_SLOT = 4096, GV_ROWS = 8, GV_CHANNELS = 512;
+constexpr int GV_RING = GV_WARPS * GV_SLOTS * GV_SLOT, GV_X = 64 * 1024;  // shared memory: weights, tokens
+
+struct VecUnits {
+    int per;        // channels of a block's round
+    int seg, segs;  // bytes of a piece, pieces of a row
+    int rows;       // rows of a unit (1 where a row has several pieces)
+};
+// Bytes of a token's row in shared memory.
+ZC_RULE int vec_pitch(int k) { return (k + 511) / 512 * 512; }
+inline size_t vec_smem(int m, int k) { return GV_RING + (size_t)m * vec_pitch(k); }
+inline VecUnits vec_units(int64_t n, int k, int sms) {
+    VecUnits U;
+    U.seg = k >= GV_SLOT ? GV_SLOT : (k + 15) / 16 * 16;
+    U.segs = (k + U.seg - 1) / U.seg;
+    U.rows = U.segs > 1 ? 1 : GV_SLOT / U.seg < GV_ROWS ? GV_SLOT / U.seg : GV_ROWS;
+    const int64_t per = (n + sms - 1) / sms;
+    U.per = (int)(per > GV_CHANNELS ? GV_CHANNELS : per);
+    // fewer rows a unit while a block has fewer units than warps
+    while (U.rows > 1 && (U.per + U.rows - 1) / U.rows < GV_WARPS) U.rows--;
+    return U;
+}
+// Rows are worked on four at a time; where a unit of `rows` has no such row, its last one is read again.
+ZC_RULE int vec_row(int row, int rows) { return row < rows ? row : rows - 1; }
+
+}  // namespace zc

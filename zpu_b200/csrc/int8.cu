@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include "head.cuh"
+#include "head_rules.h"
 #include "tcgen05.cuh"
 #include "waits.cuh"
 
@@ -219,15 +220,12 @@ __global__ void __launch_bounds__(NT) int8_matmul_kernel(const int8_t *a, int64_
 // for a token's whole linear layer, 15.5 us from bf16 or 4.3 TB/s of weights.  A unit is a slot's worth: several short
 // rows, or a piece of a long one; a block's units are dealt out evenly to its
 // warps, and what a warp has of a channel goes to the block's whole-number sums.
-constexpr int GV_WARPS = 16, GV_SLOTS = 2, GV_SLOT = 4096, GV_ROWS = 8, GV_CHANNELS = 512;
-constexpr int GV_RING = GV_WARPS * GV_SLOTS * GV_SLOT, GV_X = 64 * 1024;  // shared memory: weights, tokens
-
 struct VecArgs {
     const int8_t *w;
     const float *sx, *sw, *bias;
     int64_t ldx, ldw, ldo, n;
-    int m, k, per;       // tokens, values, channels of a block's round
-    int seg, segs, rows; // bytes of a piece, pieces of a row, rows of a unit (1 where a row has several pieces)
+    int m, k;  // tokens, values
+    int per, seg, segs, rows;  // VecUnits
 };
 
 template <int M, typename X, typename T>
@@ -239,7 +237,7 @@ __global__ void __launch_bounds__(GV_WARPS * 32, 1) int8_vec_kernel(const X *x, 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k = A.k;
     uint8_t *ring = vec_smem + warp * (GV_SLOTS * GV_SLOT);
     int8_t *xs = (int8_t *)vec_smem + GV_RING;
-    const int pitch = (k + 511) / 512 * 512;  // of the tokens' rows, zeros past k
+    const int pitch = vec_pitch(k);  // of the tokens' rows, zeros past k
     if (lane == 0) {
         for (int i = 0; i < GV_SLOTS; i++) tc::mb_init(&full[warp][i], 1);
         tc::mb_init_fence();
@@ -391,14 +389,17 @@ __global__ void __launch_bounds__(GV_WARPS * 32, 1) int8_vec_kernel(const X *x, 
                     }
                 __syncwarp();
                 if (piece == A.segs - 1 || u == u1 - 1) flush(acc, ch);  // all that this warp has of the channel
-            } else {  // four short rows at a time (those past `rows` come to nothing)
+            } else {  // four short rows at a time (what the last row gives again is left out)
                 for (int r = 0; r < rows; r += 4) {
                     int sum[4][M] = {};
+                    const uint8_t *from[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) from[i] = src + vec_row(r + i, rows) * A.seg;
                     for (int at = 0; at < size; at += 512)
                         if (at + lane * 16 < size) {
                             token(y, at);
 #pragma unroll
-                            for (int i = 0; i < 4; i++) step(sum[i], src + (r + i) * A.seg + at, y);
+                            for (int i = 0; i < 4; i++) step(sum[i], from[i] + at, y);
                         }
                     __syncwarp();
 #pragma unroll
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(GV_WARPS * 32, 1) int8_vec_kernel(const X *x, 
 // Whether the kernel above takes m tokens of k values: they fit its shared memory.
 // (Four tokens with 16384 x 4096 weights took 25 us, on the tensor cores 18.)
 bool takes_vec(const int8_t *w, int64_t ldw, int64_t m, int64_t k) {
-    return m >= 1 && m <= 2 && k > 0 && aligned_to(w, 16) && ldw % 16 == 0 && m * ((k + 511) / 512 * 512) <= GV_X;
+    return m >= 1 && m <= 2 && k > 0 && aligned_to(w, 16) && ldw % 16 == 0 && m * vec_pitch((int)k) <= GV_X;
 }
 
 template <int M, typename X, typename T>
@@ -439,16 +440,13 @@ int launch_vec(const X *x, T *out, VecArgs A, cudaStream_t s) {
         ZC_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, GV_RING + GV_X));
         if (dev >= 0 && dev < 64) attr[dev] = true;
     }
-    A.seg = A.k >= GV_SLOT ? GV_SLOT : (A.k + 15) / 16 * 16;
-    A.segs = (A.k + A.seg - 1) / A.seg;
-    A.rows = A.segs > 1 ? 1 : GV_SLOT / A.seg < GV_ROWS ? GV_SLOT / A.seg : GV_ROWS;
-    int64_t per = (A.n + num_sms() - 1) / num_sms();
-    if (per > GV_CHANNELS) per = GV_CHANNELS;
-    A.per = (int)per;
-    // fewer rows a unit while a block has fewer units than warps
-    while (A.rows > 1 && (per + A.rows - 1) / A.rows < GV_WARPS) A.rows--;
-    const int64_t blocks = (A.n + per - 1) / per;
-    const size_t smem = GV_RING + (size_t)M * ((A.k + 511) / 512 * 512);
+    const VecUnits U = vec_units(A.n, A.k, num_sms());
+    A.per = U.per;
+    A.seg = U.seg;
+    A.segs = U.segs;
+    A.rows = U.rows;
+    const int64_t blocks = (A.n + U.per - 1) / U.per;
+    const size_t smem = vec_smem(M, A.k);
     f<<<(unsigned)(blocks < num_sms() ? blocks : num_sms()), GV_WARPS * 32, smem, s>>>(x, out, A);
     ZC_LAUNCHED("int8_vec_kernel");
     return ZPUCUDA_OK;
