@@ -1039,3 +1039,20 @@ def check_tokens(zc, m, n, k, t):
                                  (80001, 2048), (50257, 768), (76800, 5000)])
 def test_int8_tokens_by_several_rows(zc, m, n, k):
     check_tokens(zc, m, n, k, ("f32", "f16", "bf16")[(n + k) % 3])
+
+
+# ------------------------------------------------------------- rows over a cluster
+@pytest.mark.parametrize("cols", [8193, 16400, 24576, 32769, 40960, 49000, 57344, 65535, 65536])
+def test_layer_norm_grad_over_clusters_from_the_first_row_on(zc, cols):
+    """Clusters of two to eight blocks whose first exchange is their first or only one: alone, as many as run at a time and
+    more, called in a row, with the same bits each time."""
+    for rows in (1, 2, 75, 160):
+        x, gamma, _, g = norm_inputs(rows, cols, "bf16", "f32", seed=cols)
+        dy = (0.01 * normal(g, rows, cols)).to(x.dtype)
+        _, mean, rstd = zc.layer_norm(x, gamma, stats=True)
+        got = [zc.layer_norm_grad(dy, x, mean, rstd, gamma) for _ in range(8)]
+        assert all(torch.equal(a, b) for other in got[1:] for a, b in zip(other, got[0]))
+        # a row's dx does not depend on the rows beside it
+        one = zc.layer_norm_grad(dy[rows - 1:], x[rows - 1:], mean[rows - 1:], rstd[rows - 1:], gamma)[0]
+        assert torch.equal(one[0], got[0][0][rows - 1])
+    check_norm_grad(zc, 20, cols, "f32", "f32")

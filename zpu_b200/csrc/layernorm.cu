@@ -302,6 +302,7 @@ __global__ void __launch_bounds__(BLOCK)
     if constexpr (CLUSTER) {
         asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
         asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this block runs
     }
     const int group = threadIdx.x / TPR, bar = 1 + (TPR > 32 ? group : 0);
     const int t = threadIdx.x % TPR, t0 = (t >> 5) * (32 * NV) + (t & 31);
@@ -332,6 +333,11 @@ __global__ void __launch_bounds__(BLOCK)
     if (row < rows) {
         next_mu = mean[row];
         next_rs = rstd[row];
+    }
+    // no block writes to another's shared memory before that one runs
+    if constexpr (CLUSTER) {
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     for (int odd = 0; row < rows; row += step, odd ^= 1) {
         const float mu = next_mu, rs = next_rs;
