@@ -536,6 +536,13 @@ int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d
                         const float *d_bias, void *d_y, int64_t ldy, int64_t rows, int64_t cols, int64_t inner,
                         void *d_work, int64_t work_bytes, void *stream);
 int64_t zpucuda_int8_linear_work(int64_t rows, int64_t inner);
+/* Diagnostics: int8_matmul whose warps look for finished sums (one or two rows
+ * of a: for arrived weights) at most spin_limit times and set *d_err where that
+ * runs out (0: at once).  Lets a test make the product's bounded waits run out;
+ * copies and products in flight are waited for all the same. */
+int zpucuda_debug_int8_matmul(const int8_t *d_a, int64_t lda, const float *d_sa, const int8_t *d_b, int64_t ldb,
+                              const float *d_sb, const float *d_bias, int dtype, void *d_out, int64_t ldo, int64_t m,
+                              int64_t n, int64_t k, uint32_t spin_limit, uint32_t *d_err, void *stream);
 /* Chooses a token of each row of logits [rows, vocab] (vocab < 2^22) from one
  * given uniform number in [0, 1) a row (utype F32 or F64).  Tokens are ranked by
  * falling logit, equal ones by rising index; a token's weight is the whole number

@@ -1056,3 +1056,36 @@ def test_layer_norm_grad_over_clusters_from_the_first_row_on(zc, cols):
         one = zc.layer_norm_grad(dy[rows - 1:], x[rows - 1:], mean[rows - 1:], rstd[rows - 1:], gamma)[0]
         assert torch.equal(one[0], got[0][0][rows - 1])
     check_norm_grad(zc, 20, cols, "f32", "f32")
+
+
+# ------------------------------------------------------------- waits of the 8-bit product that run out
+def run_out(zc, m, n, k, t, spin):
+    """The product with `spin` tries for its sums: (result, error word, the usual product)."""
+    g = gen(29)
+    pad = (k + 15) // 16 * 16 - k
+    a, b = strided(ints(g, m, k), pad), strided(ints(g, n, k), pad)
+    sa, sb, bias = torch.rand(m, generator=g, device="cuda"), torch.rand(n, generator=g, device="cuda") / k, normal(g, n)
+    want = zc.int8_matmul(a, sa, b, sb, bias, dtype=TYPES[t])
+    out = torch.full((m, n), 7.0, device="cuda", dtype=TYPES[t])
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    code = {"f32": 1, "f16": 2, "bf16": 9}[t]
+    zc.check(zc.lib().zpucuda_debug_int8_matmul(a.data_ptr(), k + pad, sa.data_ptr(), b.data_ptr(), k + pad, sb.data_ptr(), bias.data_ptr(),
+                                                code, out.data_ptr(), n, m, n, k, spin, err.data_ptr(), zc.stream_of()))
+    torch.cuda.synchronize()
+    # nothing of it stays: the next products are right, and the library's own error word is not set
+    assert torch.equal(zc.int8_matmul(a, sa, b, sb, bias, dtype=TYPES[t]), want)
+    zc.check(zc.lib().zpucuda_check_device())
+    return out, int(err), want
+
+
+ONE_TILE = [(1, 16384, 4096, "bf16"), (2, 300, 100, "f32"), (1, 80001, 333, "f16"), (9, 1000, 784, "f32"), (5, 512, 4096, "bf16"),
+            (40, 129, 8200, "f32"), (333, 4099, 1001, "f16")]
+
+
+@pytest.mark.parametrize("m,n,k,t", ONE_TILE)
+def test_int8_gives_up_and_returns(zc, m, n, k, t):
+    """No try for the sums: the call returns, with its copies landed and its products done, and says so."""
+    out, err, want = run_out(zc, m, n, k, t, 0)
+    assert err == 1
+    out, err, want = run_out(zc, m, n, k, t, 1 << 24)
+    assert err == 0 and torch.equal(out, want)

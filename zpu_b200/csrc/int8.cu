@@ -26,6 +26,14 @@ constexpr int NT = 256;
 // 131071 * 128 * 128 < 2^31: no sum of that many products leaves 32 bits.
 constexpr int64_t kMaxInner = 131071;
 
+// How long the warps that take finished sums (or arrived weights) wait for them, in tries, and where they tell of a wait that
+// ran out (null: the library's own word).  Other waits, of copies and products in flight among them, keep the usual limit.
+struct Patience {
+    uint32_t limit = tc::kSpin;
+    unsigned *err = nullptr;
+    __device__ __forceinline__ unsigned *word() const { return err ? err : &g_int8_error; }
+};
+
 // One result from its sum, rounded alike on every path.
 __device__ __forceinline__ float result(int sum, float sa, float sb, const float *bias, float b) {
     const float v = __fmul_rn(__fmul_rn((float)sum, sa), sb);
@@ -226,6 +234,7 @@ struct VecArgs {
     int64_t ldx, ldw, ldo, n;
     int m, k;  // tokens, values
     int per, seg, segs, rows;  // VecUnits
+    Patience wait;
 };
 
 template <int M, typename X, typename T>
@@ -344,7 +353,7 @@ __global__ void __launch_bounds__(GV_WARPS * 32, 1) int8_vec_kernel(const X *x, 
         int acc[M] = {};
         for (int u = u0; u < u1; u++) {
             const int slot = used % GV_SLOTS, piece = u % A.segs, ch = u / A.segs * A.rows;
-            if (!__all_sync(0xffffffffu, ok && tc::mb_wait(&full[warp][slot], (used / GV_SLOTS) & 1, &g_int8_error))) {
+            if (!__all_sync(0xffffffffu, ok && tc::mb_wait(&full[warp][slot], (used / GV_SLOTS) & 1, A.wait.word(), A.wait.limit))) {
                 ok = false;
                 break;
             }
@@ -422,7 +431,7 @@ __global__ void __launch_bounds__(GV_WARPS * 32, 1) int8_vec_kernel(const X *x, 
         __syncthreads();  // the sums have been read
     }
     if (!ok && lane == 0)  // give up only once the copies in flight have landed
-        for (int i = used; i < issued; i++) tc::mb_wait(&full[warp][i % GV_SLOTS], (i / GV_SLOTS) & 1, &g_int8_error);
+        for (int i = used; i < issued; i++) tc::mb_wait(&full[warp][i % GV_SLOTS], (i / GV_SLOTS) & 1, A.wait.word());
 }
 
 // Whether the kernel above takes m tokens of k values: they fit its shared memory.
@@ -453,8 +462,9 @@ int launch_vec(const X *x, T *out, VecArgs A, cudaStream_t s) {
 }
 template <typename X, typename T>
 int product_vec(const X *x, int64_t ldx, const float *sx, const int8_t *w, int64_t ldw, const float *sw, const float *bias,
-                T *out, int64_t ldo, int64_t m, int64_t n, int64_t k, cudaStream_t s) {
-    const VecArgs A = {w, sx, sw, bias, ldx, ldw, ldo, n, (int)m, (int)k};
+                T *out, int64_t ldo, int64_t m, int64_t n, int64_t k, const Patience &wait, cudaStream_t s) {
+    VecArgs A = {w, sx, sw, bias, ldx, ldw, ldo, n, (int)m, (int)k};
+    A.wait = wait;
     return m == 1 ? launch_vec<1>(x, out, A, s) : launch_vec<2>(x, out, A, s);
 }
 
@@ -494,6 +504,7 @@ struct TcArgs {
     int64_t ldo, tokens, channels;
     int tiles_p, tiles_q, group;  // tiles along P and Q; P tiles per raster group
     int kt, kt_split, splits;     // 128-byte slices, slices of a split
+    Patience wait;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -516,7 +527,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     using TT = TcTile<BN>;
     extern __shared__ uint8_t raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full[TT::STAGES], empty[TT::STAGES], tfull[2], tfree[2];
+    __shared__ uint64_t full[TT::STAGES], empty[TT::STAGES], tfull[2], tfree[2], drained;
     __shared__ uint32_t tmem_base;
     __shared__ float sq[2][BN], bq[2][BN];  // the Q side's scales and biases, of this tile and the next
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -540,6 +551,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             tc::mb_init(&tfull[b], 1);
             tc::mb_init(&tfree[b], 256);
         }
+        tc::mb_init(&drained, 1);
         tc::mb_init_fence();
     }
     if (warp == 1) tc::tmem_alloc(&tmem_base, TT::COLS);
@@ -558,7 +570,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 place(t, &tp, &tq);
                 for (int k = k0; k < k1; k++, j++) {
                     const int s = j % TT::STAGES;
-                    if (j >= TT::STAGES && !tc::mb_wait(&empty[s], ((j / TT::STAGES) - 1) & 1, &g_int8_error)) {
+                    if (j >= TT::STAGES && !tc::mb_wait(&empty[s], ((j / TT::STAGES) - 1) & 1, A.wait.word())) {
                         ok = false;
                         break;
                     }
@@ -568,9 +580,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                     tc::tma_load_2d(st + TC_STAGE_A, &mq, k * 128, tq * BN, &full[s]);
                 }
             }
-            if (!ok)  // give up only once the copies in flight have landed
-                for (int i = max(0, j - TT::STAGES); i < j; i++)
-                    tc::mb_wait(&full[i % TT::STAGES], (i / TT::STAGES) & 1, &g_int8_error);
+            // the block ends only once the copies in flight have landed, also where nobody waits for them any more
+            for (int i = max(0, j - TT::STAGES); i < j; i++)
+                tc::mb_wait(&full[i % TT::STAGES], (i / TT::STAGES) & 1, A.wait.word());
         }
     } else if (warp == 1) {
         if (lane == 0) {
@@ -579,11 +591,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             bool ok = true;
             for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, n++) {
                 const int buf = n & 1;
-                if (n >= 2 && !tc::mb_wait(&tfree[buf], ((n >> 1) - 1) & 1, &g_int8_error)) break;
+                if (n >= 2 && !tc::mb_wait(&tfree[buf], ((n >> 1) - 1) & 1, A.wait.word())) break;
                 tc::fence_after();
                 for (int k = k0; k < k1; k++, j++) {
                     const int s = j % TT::STAGES;
-                    if (!tc::mb_wait(&full[s], (j / TT::STAGES) & 1, &g_int8_error)) {
+                    if (!tc::mb_wait(&full[s], (j / TT::STAGES) & 1, A.wait.word())) {
                         ok = false;
                         break;
                     }
@@ -597,6 +609,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 }
                 if (ok) tc::mma_commit(&tfull[buf]);
             }
+            // nor while products are on their way to TMEM
+            tc::mma_commit(&drained);
+            tc::mb_wait(&drained, 0, A.wait.word());
         }
     } else {
         // warp w reads the quarter w % 4 of the TMEM lanes, and one half of the columns
@@ -625,7 +640,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 if (SWAP && A.bias && p < A.channels) bp = A.bias[p];
                 asm volatile("bar.sync 1, 256;" ::: "memory");
             }
-            const bool ok = tc::mb_wait(&tfull[buf], (n >> 1) & 1, &g_int8_error);
+            const bool ok = tc::mb_wait(&tfull[buf], (n >> 1) & 1, A.wait.word(), A.wait.limit);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc::fence_after();
             if (A.splits > 1) {  // this split's sums, for the whole cluster (one tile per cluster)
@@ -786,7 +801,8 @@ int launch_tc(const CUtensorMap &mp, const CUtensorMap &mq, const TcArgs &A, boo
 // stream made the left operand, and this one's beginning may overlap its end.
 template <typename T>
 int product_tc(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb, const float *sb,
-               const float *bias, T *out, int64_t ldo, int64_t m, int64_t n, int64_t k, bool follows, cudaStream_t s, bool *done) {
+               const float *bias, T *out, int64_t ldo, int64_t m, int64_t n, int64_t k, bool follows,
+               const Patience &wait, cudaStream_t s, bool *done) {
     *done = false;
     // a tensor map's rows: at most 2^31, its coordinates 32 bits
     if (!aligned_to(a, 16) || !aligned_to(b, 16) || lda % 16 || ldb % 16 || k == 0) return ZPUCUDA_OK;
@@ -802,6 +818,7 @@ int product_tc(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, i
     A.tiles_p = (int)((P + 127) / 128);
     A.tiles_q = (int)((Q + bn - 1) / bn);
     A.group = 16;
+    A.wait = wait;
     A.kt = (int)((k + 127) / 128);
     // split the inner axis while the tiles leave most SMs idle, with at least four slices left to each
     int64_t splits = 1;
@@ -856,12 +873,13 @@ int quantize(int dtype, const void *x, int64_t ldx, int8_t *q, int64_t ldq, floa
 }
 
 int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb, const float *sb,
-            const float *bias, int dtype, void *out, int64_t ldo, int64_t m, int64_t n, int64_t k, bool follows, cudaStream_t s) {
+            const float *bias, int dtype, void *out, int64_t ldo, int64_t m, int64_t n, int64_t k, bool follows,
+            cudaStream_t s, const Patience &wait = Patience()) {
     if (m == 0 || n == 0) return ZPUCUDA_OK;
     if (takes_vec(b, ldb, m, k))
-        ZC_HEAD_TYPE(dtype, T, return (product_vec<int8_t, T>(a, lda, sa, b, ldb, sb, bias, (T *)out, ldo, m, n, k, s)));
+        ZC_HEAD_TYPE(dtype, T, return (product_vec<int8_t, T>(a, lda, sa, b, ldb, sb, bias, (T *)out, ldo, m, n, k, wait, s)));
     bool done = false;
-    ZC_HEAD_TYPE(dtype, T, ZC_TRY(product_tc<T>(a, lda, sa, b, ldb, sb, bias, (T *)out, ldo, m, n, k, follows, s, &done)));
+    ZC_HEAD_TYPE(dtype, T, ZC_TRY(product_tc<T>(a, lda, sa, b, ldb, sb, bias, (T *)out, ldo, m, n, k, follows, wait, s, &done)));
     if (done) return ZPUCUDA_OK;
     dim3 grid((unsigned)((n + 63) / 64), (unsigned)((m + 63) / 64));
     ZC_HEAD_TYPE(dtype, T,
@@ -900,14 +918,29 @@ int zpucuda_int8_quantize(int dtype, const void *d_x, int64_t ldx, int8_t *d_q, 
     return quantize(dtype, d_x, ldx, d_q, ldq, d_scale, rows, cols, resolve_stream(stream));
 }
 
+static int int8_matmul(const char *who, const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb,
+                       const float *sb, const float *bias, int dtype, void *out, int64_t ldo, int64_t m, int64_t n,
+                       int64_t k, const Patience &wait, void *stream) {
+    ZC_TRY(check_product(who, sb, b, ldb, bias, dtype, out, ldo, m, n, k));
+    if (lda < k) return head_error(ZPUCUDA_ERR_INVALID_SHAPE, who, "a: row pitch below the row's length");
+    if (m > 0 && ((k > 0 && !a) || !sa)) return head_error(ZPUCUDA_ERR_INVALID_ARGUMENT, who, "a or its scales: null pointer");
+    return product(a, lda, sa, b, ldb, sb, bias, dtype, out, ldo, m, n, k, false, resolve_stream(stream), wait);
+}
+
 int zpucuda_int8_matmul(const int8_t *d_a, int64_t lda, const float *d_sa, const int8_t *d_b, int64_t ldb,
                         const float *d_sb, const float *d_bias, int dtype, void *d_out, int64_t ldo, int64_t m,
                         int64_t n, int64_t k, void *stream) {
-    ZC_TRY(check_product("int8_matmul", d_sb, d_b, ldb, d_bias, dtype, d_out, ldo, m, n, k));
-    if (lda < k) return set_error(ZPUCUDA_ERR_INVALID_SHAPE, "int8_matmul: a: row pitch below the row's length");
-    if (m > 0 && ((k > 0 && !d_a) || !d_sa))
-        return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "int8_matmul: a or its scales: null pointer");
-    return product(d_a, lda, d_sa, d_b, ldb, d_sb, d_bias, dtype, d_out, ldo, m, n, k, false, resolve_stream(stream));
+    return int8_matmul("int8_matmul", d_a, lda, d_sa, d_b, ldb, d_sb, d_bias, dtype, d_out, ldo, m, n, k, Patience(), stream);
+}
+
+int zpucuda_debug_int8_matmul(const int8_t *d_a, int64_t lda, const float *d_sa, const int8_t *d_b, int64_t ldb,
+                              const float *d_sb, const float *d_bias, int dtype, void *d_out, int64_t ldo, int64_t m,
+                              int64_t n, int64_t k, uint32_t spin_limit, uint32_t *d_err, void *stream) {
+    if (!d_err) return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "debug_int8_matmul: err: null pointer");
+    Patience wait;
+    wait.limit = spin_limit;
+    wait.err = d_err;
+    return int8_matmul("debug_int8_matmul", d_a, lda, d_sa, d_b, ldb, d_sb, d_bias, dtype, d_out, ldo, m, n, k, wait, stream);
 }
 
 int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d_w, int64_t ldw, const float *d_sw,
@@ -921,7 +954,7 @@ int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d
     cudaStream_t s = resolve_stream(stream);
     if (takes_vec(d_w, ldw, rows, inner))
         ZC_HEAD_TYPE(dtype, T, return (product_vec<T, T>((const T *)d_x, ldx, nullptr, d_w, ldw, d_sw, d_bias, (T *)d_y,
-                                                         ldy, rows, cols, inner, s)));
+                                                         ldy, rows, cols, inner, Patience(), s)));
     const int64_t ldq = (inner + 15) / 16 * 16;
     int8_t *q = (int8_t *)d_work;
     float *scale = (float *)(q + rows * ldq);

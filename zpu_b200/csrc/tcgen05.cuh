@@ -23,8 +23,8 @@ __device__ __forceinline__ void mb_expect_tx(uint64_t *b, uint32_t bytes) {
 __device__ __forceinline__ void mb_arrive(uint64_t *b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
 }
-__device__ __forceinline__ bool mb_wait(uint64_t *b, uint32_t parity, unsigned *err) {
-    for (uint32_t i = 0; i < kSpin; i++) {
+__device__ __forceinline__ bool mb_wait(uint64_t *b, uint32_t parity, unsigned *err, uint32_t limit = kSpin) {
+    for (uint32_t i = 0; i < limit; i++) {
         uint32_t ok;
         asm volatile(
             "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
