@@ -1089,3 +1089,14 @@ def test_int8_gives_up_and_returns(zc, m, n, k, t):
     assert err == 1
     out, err, want = run_out(zc, m, n, k, t, 1 << 24)
     assert err == 0 and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("m,n,k", [(1100, 5000, 300), (1000, 9000, 130), (64, 80001, 200), (3000, 4100, 1000)])
+def test_int8_gives_up_on_many_tiles(zc, m, n, k, t):
+    """The same where a block has several tiles: a warp that gives up meets the others at the barriers of the tiles to
+    come, whether theirs were in time (a few tries: some warps) or not (none)."""
+    for spin in (0, 1, 2, 3):
+        out, err, want = run_out(zc, m, n, k, t, spin)
+        assert err == 1 or torch.equal(out, want)
+        assert err == 1 or spin > 0

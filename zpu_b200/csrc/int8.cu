@@ -623,6 +623,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         uint8_t *turn = smem + TT::STAGES * TT::STAGE + (warp - 2) * 2048;
         const bool vec = ((uintptr_t)out & 15) == 0 && (A.ldo * (int64_t)sizeof(T)) % 16 == 0;
         int n = 0;
+        bool good = true, coming = true;  // the warp's: no wait has run out; nor one at the usual limit after that
         for (int t = blockIdx.x; t < ntiles; t += gridDim.x, n++) {
             int tp, tq;
             place(t, &tp, &tq);
@@ -640,8 +641,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 if (SWAP && A.bias && p < A.channels) bp = A.bias[p];
                 asm volatile("bar.sync 1, 256;" ::: "memory");
             }
-            const bool ok = tc::mb_wait(&tfull[buf], (n >> 1) & 1, A.wait.word(), A.wait.limit);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            good = __all_sync(0xffffffffu, good && tc::mb_wait(&tfull[buf], (n >> 1) & 1, A.wait.word(), A.wait.limit));
+            if (!good) {
+                // Nothing to store, but the barriers of the tiles to come are met (another warp's wait may have been in time),
+                // at the pace of the sums as long as they come: the issuing warp counts on never being passed.
+                coming = __all_sync(0xffffffffu, coming && tc::mb_wait(&tfull[buf], (n >> 1) & 1, A.wait.word()));
+                tc::mb_arrive(&tfree[buf]);
+                continue;
+            }
             tc::fence_after();
             if (A.splits > 1) {  // this split's sums, for the whole cluster (one tile per cluster)
                 int *part = (int *)smem + q4 * 32 + lane;
