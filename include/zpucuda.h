@@ -464,9 +464,10 @@ int zpucuda_debug_peer_reduce(const float *d_inbox, int world, int64_t n, float 
  *    in f32 or wider and each result is rounded to its type once.
  *  - Calls are asynchronous on `stream`, allocate nothing and may be captured
  *    in a CUDA graph.  Waits inside a kernel (of the distillation's clusters
- *    and the tensor cores' product) are bounded; one that runs out is an error
- *    that zpucuda_check_device reports.  Results do not depend on the run: the
- *    same call on the same inputs gives the same bits.
+ *    and the 8-bit product) are bounded; one that runs out is an error that
+ *    zpucuda_check_device reports, and what depends on it is NaN.  Results do
+ *    not depend on the run: the same call on the same inputs gives the same
+ *    bits.
  *
  * layer_norm: y = (x - mean) * rstd * gamma + beta over each row, rstd =
  *   1 / sqrt(mean((x - mean)^2) + eps).  gamma / beta: [cols] of type wtype, or
@@ -537,9 +538,9 @@ int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d
                         void *d_work, int64_t work_bytes, void *stream);
 int64_t zpucuda_int8_linear_work(int64_t rows, int64_t inner);
 /* Diagnostics: int8_matmul whose warps look for finished sums (one or two rows
- * of a: for arrived weights) at most spin_limit times and set *d_err where that
- * runs out (0: at once).  Lets a test make the product's bounded waits run out;
- * copies and products in flight are waited for all the same. */
+ * of a: for arrived weights) at most spin_limit times and, where that runs out
+ * (0: at once), set *d_err and give NaN.  Lets a test make the product's bounded
+ * waits run out; copies and products in flight are waited for all the same. */
 int zpucuda_debug_int8_matmul(const int8_t *d_a, int64_t lda, const float *d_sa, const int8_t *d_b, int64_t ldb,
                               const float *d_sb, const float *d_bias, int dtype, void *d_out, int64_t ldo, int64_t m,
                               int64_t n, int64_t k, uint32_t spin_limit, uint32_t *d_err, void *stream);

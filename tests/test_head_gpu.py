@@ -1100,3 +1100,12 @@ def test_int8_gives_up_on_many_tiles(zc, m, n, k, t):
         out, err, want = run_out(zc, m, n, k, t, spin)
         assert err == 1 or torch.equal(out, want)
         assert err == 1 or spin > 0
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("m,n,k", [c[:3] for c in ONE_TILE] + [(1100, 5000, 300), (64, 80001, 200)])
+def test_int8_gives_nothing_but_nan_after_a_wait(zc, m, n, k, t):
+    """What was not waited for is NaN, not part of a sum."""
+    assert bool(run_out(zc, m, n, k, t, 0)[0].isnan().all())
+    out, err, want = run_out(zc, m, n, k, t, 1)
+    assert bool((out.isnan() | (out == want)).all()) and bool(out.isnan().any()) <= err

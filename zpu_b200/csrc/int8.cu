@@ -422,11 +422,11 @@ __global__ void __launch_bounds__(GV_WARPS * 32, 1) int8_vec_kernel(const X *x, 
             issued = __shfl_sync(0xffffffffu, issued, 0);
             next = __shfl_sync(0xffffffffu, next, 0);
         }
-        __syncthreads();
+        const bool lost = __syncthreads_or(!ok);  // the sums lack what a warp has given up on: NaN
         for (int i = threadIdx.x; i < nch * A.m; i += GV_WARPS * 32) {
             const int c = i % nch, r = i / nch;
-            out[r * A.ldo + c0 + c] =
-                from_f<T>(result(sums[c * M + r], scale[r], A.sw[c0 + c], A.bias, A.bias ? A.bias[c0 + c] : 0.0f));
+            out[r * A.ldo + c0 + c] = from_f<T>(
+                result(sums[c * M + r], lost ? NAN : scale[r], A.sw[c0 + c], A.bias, A.bias ? A.bias[c0 + c] : 0.0f));
         }
         __syncthreads();  // the sums have been read
     }
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     extern __shared__ uint8_t raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full[TT::STAGES], empty[TT::STAGES], tfull[2], tfree[2], drained;
-    __shared__ uint32_t tmem_base;
+    __shared__ uint32_t tmem_base, gave_up;  // a split's sums are not in place
     __shared__ float sq[2][BN], bq[2][BN];  // the Q side's scales and biases, of this tile and the next
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ntiles = A.tiles_p * A.tiles_q;
@@ -552,6 +552,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             tc::mb_init(&tfree[b], 256);
         }
         tc::mb_init(&drained, 1);
+        gave_up = 0;
         tc::mb_init_fence();
     }
     if (warp == 1) tc::tmem_alloc(&tmem_base, TT::COLS);
@@ -643,18 +644,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             }
             good = __all_sync(0xffffffffu, good && tc::mb_wait(&tfull[buf], (n >> 1) & 1, A.wait.word(), A.wait.limit));
             if (!good) {
-                // Nothing to store, but the barriers of the tiles to come are met (another warp's wait may have been in time),
+                // NaN from here on, but the barriers of the tiles to come are met (another warp's wait may have been in time),
                 // at the pace of the sums as long as they come: the issuing warp counts on never being passed.
                 coming = __all_sync(0xffffffffu, coming && tc::mb_wait(&tfull[buf], (n >> 1) & 1, A.wait.word()));
-                tc::mb_arrive(&tfree[buf]);
-                continue;
+                sp = NAN;
             }
             tc::fence_after();
+            auto sums = [&](int c, int (&v)[16]) {
+                if (good) tc::tmem_ld16(tmem + lanes + (uint32_t)(buf * BN + c), v);
+                else memset(v, 0, sizeof v);
+            };
             if (A.splits > 1) {  // this split's sums, for the whole cluster (one tile per cluster)
+                if (!good) gave_up = 1;
                 int *part = (int *)smem + q4 * 32 + lane;
                 for (int c = half * HALF; !idle && c < half * HALF + HALF; c += 16) {
                     int v[16];
-                    tc::tmem_ld16(tmem + lanes + (uint32_t)(buf * BN + c), v);
+                    sums(c, v);
 #pragma unroll
                     for (int i = 0; i < 16; i++) part[(c + i) * 132] = v[i];
                 }
@@ -664,7 +669,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 for (int c = half * HALF; !idle && c < half * HALF + HALF; c += 16) {
                     int v[16];
                     __syncwarp();
-                    tc::tmem_ld16(tmem + lanes + (uint32_t)(buf * BN + c), v);
+                    sums(c, v);
                     const int64_t q0 = (int64_t)tq * BN + c;
 #pragma unroll
                     for (int i = 0; i < 16; i++)
@@ -681,7 +686,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 #pragma unroll
                     for (int h = 0; h < W; h += 16) {
                         int v[16];
-                        tc::tmem_ld16(tmem + lanes + (uint32_t)(buf * BN + c + h), v);
+                        sums(c + h, v);
                         alignas(16) T w[16];
 #pragma unroll
                         for (int i = 0; i < 16; i++)
@@ -719,6 +724,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     if (A.splits > 1) {
         // all sums are in place (the stages' loads have all been read by then)
         cluster_sync();
+        bool lost = false;
+        for (int r = 0; r < A.splits; r++) lost |= *(const uint32_t *)cluster_map(&gave_up, r) != 0;
         // each CTA adds up its share: four neighbouring channels of a token a thread
         int tp, tq;
         place(blockIdx.x, &tp, &tq);
@@ -738,7 +745,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 sum.w += v.w;
             }
             const int y[4] = {sum.x, sum.y, sum.z, sum.w};
-            const float sa = A.sa[token];
+            const float sa = lost ? NAN : A.sa[token];
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 if (ch + e < A.channels)
