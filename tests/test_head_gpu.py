@@ -1109,3 +1109,32 @@ def test_int8_gives_nothing_but_nan_after_a_wait(zc, m, n, k, t):
     assert bool(run_out(zc, m, n, k, t, 0)[0].isnan().all())
     out, err, want = run_out(zc, m, n, k, t, 1)
     assert bool((out.isnan() | (out == want)).all()) and bool(out.isnan().any()) <= err
+
+
+# ------------------------------------------------------------- the distillation's wait for a row's other blocks
+def loss_run_out(zc, rows, vocab, t, spin):
+    """The loss with `spin` tries for the sums of the row's other blocks: (loss, lse, error word), and the usual ones."""
+    g = gen(30)
+    student, teacher, index = teach(g, rows, vocab, 20, t)
+    want = zc.distill_loss(student, teacher, index, temperature=1.5)
+    loss, lse = torch.full((rows,), 7.0, device="cuda"), torch.full((rows,), 7.0, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    code = {"f32": 1, "f16": 2, "bf16": 9}
+    zc.check(zc.lib().zpucuda_debug_distill_loss(code[t], student.data_ptr(), vocab, zc.head._code("teacher", teacher), teacher.data_ptr(),
+                                                 20, 3 if index.dtype == torch.int64 else 4, index.data_ptr(), 20, None, 1.5,
+                                                 loss.data_ptr(), lse.data_ptr(), rows, vocab, 20, spin, err.data_ptr(), zc.stream_of()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(zc.distill_loss(student, teacher, index, temperature=1.5), want))
+    zc.check(zc.lib().zpucuda_check_device())
+    return loss, lse, int(err), want
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("rows,vocab", [(1, 5000), (3, 70001), (200, 131072), (2000, 40000)])
+def test_distill_gives_up_and_returns(zc, rows, vocab, t):
+    """Blocks that do not wait for one another's sums: none ends before the others have written theirs to it, and the loss
+    is not a number rather than a part of one."""
+    loss, lse, err, want = loss_run_out(zc, rows, vocab, t, 0)
+    assert err == 1 and bool(loss.isnan().all())
+    loss, lse, err, want = loss_run_out(zc, rows, vocab, t, 1 << 24)
+    assert err == 0 and torch.equal(loss, want[0]) and torch.equal(lse, want[1])

@@ -170,6 +170,8 @@ SIGNATURES = {
     "zpucuda_int8_linear": (I32, [I32, P, I64, P, I64, P, P, P, I64, I64, I64, I64, P, I64, P]),
     "zpucuda_int8_linear_work": (I64, [I64, I64]),
     "zpucuda_sample": (I32, [I32, P, I64, I32, P, P, P, P, P, P, P, I64, I64, P]),
+    "zpucuda_debug_distill_loss": (I32, [I32, P, I64, I32, P, I64, I32, P, I64, P, C.c_double, P, P, I64, I64, I64,
+                                         C.c_uint32, P, P]),
     "zpucuda_debug_int8_matmul": (I32, [P, I64, P, P, I64, P, P, I32, P, I64, I64, I64, I64, C.c_uint32, P, P]),
     "zpucuda_debug_peer_reduce": (I32, [P, I32, I64, P, P, U64, C.c_uint32, P, P]),
 }

@@ -38,8 +38,8 @@ __device__ __forceinline__ bool mb_wait(uint64_t *b, uint32_t parity, unsigned *
 }
 
 // The same where other blocks of the cluster arrive: their writes before it are seen after it.
-__device__ __forceinline__ bool mb_wait_cluster(uint64_t *b, uint32_t parity, unsigned *err) {
-    for (uint32_t i = 0; i < kSpin; i++) {
+__device__ __forceinline__ bool mb_wait_cluster(uint64_t *b, uint32_t parity, unsigned *err, uint32_t limit = kSpin) {
+    for (uint32_t i = 0; i < limit; i++) {
         uint32_t ok;
         asm volatile(
             "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
