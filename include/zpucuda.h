@@ -515,8 +515,8 @@ int zpucuda_distill_value_and_grad(int dtype, const void *d_logits, int64_t ld, 
                                    double temperature, const float *d_dloss, float *d_loss, void *d_dlogits,
                                    int64_t ldd, int64_t rows, int64_t vocab, int64_t top, void *stream);
 /* Diagnostics: distill_loss whose blocks look for one another's sums at most
- * spin_limit times (0: not at all) and set *d_err where that runs out.  Lets a
- * test make that bounded wait run out. */
+ * spin_limit times (0: not at all) and, where that runs out, set *d_err and give
+ * NaN.  Lets a test make that bounded wait run out. */
 int zpucuda_debug_distill_loss(int dtype, const void *d_logits, int64_t ld, int ttype, const void *d_teacher, int64_t ldt,
                                int itype, const void *d_indices, int64_t ldi, const float *d_weight, double temperature,
                                float *d_loss, float *d_lse, int64_t rows, int64_t vocab, int64_t top, uint32_t spin_limit,

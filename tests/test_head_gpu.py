@@ -1138,3 +1138,10 @@ def test_distill_gives_up_and_returns(zc, rows, vocab, t):
     assert err == 1 and bool(loss.isnan().all())
     loss, lse, err, want = loss_run_out(zc, rows, vocab, t, 1 << 24)
     assert err == 0 and torch.equal(loss, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 5000), (3, 70001), (200, 131072)])
+def test_distill_gives_no_lse_after_a_wait(zc, rows, vocab):
+    """log sum exp, which the gradient is taken from, is NaN like the loss where some of its parts were not waited for."""
+    loss, lse, err, want = loss_run_out(zc, rows, vocab, "bf16", 0)
+    assert err == 1 and bool(lse.isnan().all())

@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(THREADS, (LOSS ? kThreads : kGradThreads) / TH
                     // sum of p log p, less that of p z, plus lse
                     const float l = (ul * ur - logf(us)) - (az - lse);
                     A.loss[row] = bad || !ok ? NAN : w == 0.0f ? 0.0f : w * (A.T * A.T) * l;
-                    if (A.lse_out) A.lse_out[row] = w == 0.0f ? 0.0f : lse;
+                    if (A.lse_out) A.lse_out[row] = !ok ? NAN : w == 0.0f ? 0.0f : lse;
                 }
             }
         } else {
