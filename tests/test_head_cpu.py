@@ -166,3 +166,19 @@ def test_short_rows_are_read_inside_shared_memory(tmp_path):
     printf("%ld %d %d %ld", bad, several > 0, over > 0, worst);
     """)
     assert out == ["0", "1", "1", "135168"]
+
+
+def test_weights_are_shifted_inside_their_bits(tmp_path):
+    """floor(2^40 e) of every exponent of a 32-bit e in [0, 1] and of many significands, with no shift that C++ leaves open
+    (the compiler's check ends the program at one)."""
+    out = host(tmp_path, """
+    long bad = 0;
+    for (uint32_t u = 0; u <= 0x3f800000u; u += u % 0x800000u < 64 ? 1 : 4099) {
+        const uint32_t exponent = u >> 23, significand = (u & 0x7fffffu) | (exponent ? 0x800000u : 0);
+        const int up = (int)(exponent ? exponent : 1) - 150 + 40;  // e = significand * 2^(up - 40)
+        const uint64_t want = up >= 0 ? (uint64_t)significand << up : up > -32 ? significand >> -up : 0;
+        bad += weigh_bits(u) != want;
+    }
+    printf("%ld", bad);
+    """, "-fsanitize=shift", "-fsanitize-undefined-trap-on-error")
+    assert out == ["0"]

@@ -38,4 +38,12 @@ inline VecUnits vec_units(int64_t n, int k, int sms) {
 // Rows are worked on four at a time; where a unit of `rows` has no such row, its last one is read again.
 ZC_RULE int vec_row(int row, int rows) { return row < rows ? row : rows - 1; }
 
+// ---- the next token (sample.cu)
+// floor(2^40 e) from the bits of e, 0 <= e <= 1: the significand shifted into place.  Below 2^-40 nothing is left of it; how far
+// it would be shifted there passes 64 bits, which C++ does not define.
+ZC_RULE uint64_t weigh_bits(uint32_t u) {
+    const uint32_t down = 127u - (u >> 23);
+    return ((uint64_t)((u & 0x7fffffu) | 0x800000u) << 17) >> (down < 63u ? down : 63u);
+}
+
 }  // namespace zc

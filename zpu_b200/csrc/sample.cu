@@ -39,6 +39,7 @@
 #include <cstring>
 
 #include "head.cuh"
+#include "head_rules.h"
 
 namespace zc {
 namespace {
@@ -165,10 +166,6 @@ struct Row {
         return t;
     }
     __device__ __forceinline__ float dist(float f) const { return f == m ? 0.0f : (f - m) * inv; }
-    // The weight of a token at a distance: floor(2^40 e^d), the significand shifted into place (0 <= e^d <= 1).
-    static __device__ __forceinline__ uint64_t weigh_bits(uint32_t u) {
-        return ((uint64_t)((u & 0x7fffffu) | 0x800000u) << 17) >> (127 - (u >> 23));
-    }
     bool spike;  // only the largest logit has weight: it is infinite, or 1 / T is
     __device__ __forceinline__ uint64_t weight(float f) const {
         if (spike) return f == m ? kOne : 0;
@@ -524,7 +521,7 @@ __device__ void finish_row(Shared &S, const Row<T> &R, const Args &A, int64_t ro
         uint32_t t = 0;
 #pragma unroll
         for (int e = 0; e < N; e++) {
-            s[e] = Row<T>::weigh_bits(__float_as_uint(K.keep(f[e], expf((f[e] - R.m) * R.inv))));
+            s[e] = weigh_bits(__float_as_uint(K.keep(f[e], expf((f[e] - R.m) * R.inv))));
             t += in && f[e] == K.low;
         }
         uint32_t upto = t;  // ties up to this lane's last
