@@ -182,3 +182,22 @@ def test_weights_are_shifted_inside_their_bits(tmp_path):
     printf("%ld", bad);
     """, "-fsanitize=shift", "-fsanitize-undefined-trap-on-error")
     assert out == ["0"]
+
+
+def test_rows_are_copied_from_inside_their_matrix(tmp_path):
+    """Every row whose aligned 16 bytes begin before the matrix is known as such, over short rows, pitches and starts; it is
+    not the first row alone."""
+    out = host(tmp_path, """
+    long bad = 0, others = 0;
+    for (int n : {4, 8})  // elements of 16 bytes
+        for (int base = 0; base < n; base++)
+            for (int ld = 1; ld < 20; ld++)
+                for (int row = 0; row < 40; row++) {
+                    const int start = base + row * ld, skew = start % n;
+                    const bool outside = start - skew < base;
+                    bad += begins_outside((int64_t)row * ld, skew) != outside;
+                    others += outside && row > 0;
+                }
+    printf("%ld %d", bad, others > 0);
+    """)
+    assert out == ["0", "1"]

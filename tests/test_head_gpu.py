@@ -1145,3 +1145,25 @@ def test_distill_gives_no_lse_after_a_wait(zc, rows, vocab):
     """log sum exp, which the gradient is taken from, is NaN like the loss where some of its parts were not waited for."""
     loss, lse, err, want = loss_run_out(zc, rows, vocab, "bf16", 0)
     assert err == 1 and bool(lse.isnan().all())
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("cols", [1, 2, 3, 5])
+def test_layer_norm_of_several_rows_in_16_bytes(zc, cols, t):
+    """Short rows at their own pitch from every start: the bytes before the matrix (NaN here) are no part of any row, and
+    each row comes out as by itself."""
+    g = gen(31)
+    for shift in range(8):
+        for rows in (1, 2, 9, 5000):
+            flat = torch.full((shift + rows * cols + 8,), float("nan"), device="cuda", dtype=TYPES[t])
+            x = flat[shift:shift + rows * cols].view(rows, cols)
+            x.copy_(normal(g, rows, cols))
+            dy = torch.full_like(flat, float("nan"))[shift:shift + rows * cols].view(rows, cols)
+            dy.copy_(normal(g, rows, cols))
+            wide, dwide = strided(x.clone(), 16 - cols), strided(dy.clone(), 16 - cols)  # every row on the grid
+            want = zc.layer_norm(wide, stats=True)
+            assert all(torch.equal(a, b) for a, b in zip(zc.layer_norm(x, stats=True), want))
+            dwant = zc.layer_norm_grad(dwide, wide, *want[1:])
+            got = zc.layer_norm_grad(dy, x, *want[1:])
+            assert all(torch.equal(a, b) for a, b in zip(got, dwant))
+            check_norm(zc, x, None, None)

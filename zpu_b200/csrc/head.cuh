@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "head_rules.h"
 
 namespace zc {
 
@@ -63,7 +64,9 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 // Piece i of a row holds its elements i * N .. i * N + N - 1 (N = 16 / the
 // element's size), wherever the row starts: an address that is no multiple of
 // 16 costs a second load and some shifts, not another order of a sum, so a
-// result does not depend on the alignment.  Nothing outside the row is touched.
+// result does not depend on the alignment.  Nothing outside the row is touched,
+// except that RowRing reads the aligned 16 bytes in which a row begins, as far as
+// they lie in its matrix, and drops what comes before the row.
 
 template <typename T>
 constexpr int kPiece = 16 / (int)sizeof(T);
@@ -294,9 +297,9 @@ struct RowRing {
                      "l"(src), "r"(size)
                      : "memory");
     }
-    // The aligned 16 bytes that hold the row's pieces, clipped at its end.  Before its
-    // beginning lie the bytes of the row before it, except (`first`) at the matrix's.
-    __device__ __forceinline__ void issue(int slot, int r, const T *row, int64_t n, bool first) const {
+    // The aligned 16 bytes that hold the row's pieces, clipped at its end and at the
+    // matrix's beginning (`before`: elements of the matrix before the row).
+    __device__ __forceinline__ void issue(int slot, int r, const T *row, int64_t n, int64_t before) const {
         const uint32_t s = EVEN ? 0 : (uint32_t)(uintptr_t)row & 15;
         const uint8_t *from = (const uint8_t *)row - s;
         const int end = (int)s + (int)n * (int)sizeof(T);
@@ -309,7 +312,7 @@ struct RowRing {
                 copy(dst + lane, from + b, 16);
                 continue;
             }
-            if (first && s && b == 0) {
+            if (b == 0 && begins_outside(before, (int)(s / sizeof(T)))) {
                 T *e = (T *)(dst + lane);  // 0 outside the row, as the copies leave it
                 for (int i = 0, at = -(int)(s / sizeof(T)); i < kPiece<T>; i++, at++) e[i] = at >= 0 && at < n ? row[at] : from_f<T>(0.0f);
             } else {

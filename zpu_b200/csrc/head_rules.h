@@ -38,6 +38,11 @@ inline VecUnits vec_units(int64_t n, int k, int sms) {
 // Rows are worked on four at a time; where a unit of `rows` has no such row, its last one is read again.
 ZC_RULE int vec_row(int row, int rows) { return row < rows ? row : rows - 1; }
 
+// ---- rows on their way to shared memory (head.cuh)
+// Whether the 16 aligned bytes in which a row begins begin before its matrix: the row starts `skew` elements into them, and
+// `before` elements of the matrix (row * pitch) lie before it.  With short rows that is so for more than the first.
+ZC_RULE bool begins_outside(int64_t before, int skew) { return before < skew; }
+
 // ---- the next token (sample.cu)
 // floor(2^40 e) from the bits of e, 0 <= e <= 1: the significand shifted into place.  Below 2^-40 nothing is left of it; how far
 // it would be shifted there passes 64 bits, which C++ does not define.

@@ -7,7 +7,6 @@
 #include <string.h>
 
 #include "head.cuh"
-#include "head_rules.h"
 #include "tcgen05.cuh"
 #include "waits.cuh"
 

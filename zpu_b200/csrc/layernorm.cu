@@ -23,6 +23,9 @@ namespace {
 constexpr int NT = 256;
 constexpr int kPerThread = 16;  // columns of a row that a thread of the gradient holds
 constexpr int kMaxCluster = 8;  // blocks of a cluster of it
+// What lies before a row that is not among a block's first D: more than a granule.  Rows shorter than a granule are taken
+// by blocks of 8 rows with D = 4, so 32 of them lie before it.
+constexpr int64_t kInside = INT64_MAX;
 constexpr int64_t kMaxOnePass = 512 * kPerThread * kMaxCluster;
 
 // The weights of piece i of a row (N from column i * N on, `have` of them), as
@@ -152,7 +155,7 @@ __global__ void __launch_bounds__(TPR < NT ? NT : TPR)
     const float inv = 1.0f / (float)cols;
 #pragma unroll
     for (int d = 0; d < D; d++) {
-        if (row + d * step < rows) ring.issue(d, 0, x + (row + d * step) * ldx, cols, row + d * step == 0);
+        if (row + d * step < rows) ring.issue(d, 0, x + (row + d * step) * ldx, cols, (row + d * step) * ldx);
         ring.commit();
     }
     f32x2 g[NV][N / 2], b[NV][N / 2];
@@ -173,7 +176,7 @@ __global__ void __launch_bounds__(TPR < NT ? NT : TPR)
             Fwd<T>::sum(v[j], s);
         }
         __syncwarp();
-        if (row + D * step < rows) ring.issue(slot, 0, x + (row + D * step) * ldx, cols, false);
+        if (row + D * step < rows) ring.issue(slot, 0, x + (row + D * step) * ldx, cols, kInside);
         ring.commit();
         slot = slot + 1 == D ? 0 : slot + 1;
         const float mu = row_sum2<TPR>(lo2(s) + hi2(s), 0.0f, sm[odd][0] + group * (TPR / 16), bar).x * inv;
@@ -319,15 +322,15 @@ __global__ void __launch_bounds__(BLOCK)
     const RowRing<T, NV, 2, D, EVEN> ring(grad_smem, p0);
     const int64_t step = (int64_t)(gridDim.x / size) * GROUPS;
     int64_t row = (int64_t)(blockIdx.x / size) * GROUPS + group;
-    auto issue = [&](int slot, int64_t r) {
+    auto issue = [&](int slot, int64_t r, auto later) {
         if (r < rows) {
-            ring.issue(slot, 0, x + r * ldx, cols, r == 0);
-            ring.issue(slot, 1, dy + r * lddy, cols, r == 0);
+            ring.issue(slot, 0, x + r * ldx, cols, decltype(later)::value ? kInside : r * ldx);
+            ring.issue(slot, 1, dy + r * lddy, cols, decltype(later)::value ? kInside : r * lddy);
         }
         ring.commit();
     };
 #pragma unroll
-    for (int d = 0; d < D; d++) issue(d, row + d * step);
+    for (int d = 0; d < D; d++) issue(d, row + d * step, std::false_type());
     int slot = 0;
     float next_mu = 0.0f, next_rs = 0.0f;
     if (row < rows) {
@@ -364,7 +367,7 @@ __global__ void __launch_bounds__(BLOCK)
             }
         }
         __syncwarp();
-        issue(slot, row + D * step);
+        issue(slot, row + D * step, std::true_type());
         slot = slot + 1 == D ? 0 : slot + 1;
         if (!dx) continue;
         // two buffers: a thread that is a row ahead does not overwrite what another still reads

@@ -39,7 +39,6 @@
 #include <cstring>
 
 #include "head.cuh"
-#include "head_rules.h"
 
 namespace zc {
 namespace {
