@@ -530,7 +530,8 @@ int zpucuda_debug_distill_loss(int dtype, const void *d_logits, int64_t ld, int 
  *     otherwise NotSupported), out of type dtype.  a: [m, k] with a scale per row
  *     (token), b: [n, k] with a scale per row (output channel).
  *   int8_linear: y = x w^T with x [rows, inner] quantised by row on the way:
- *     int8_quantize and int8_matmul in one call.  work: device memory of
+ *     int8_quantize and int8_matmul in one call.  y may lie over x (one or two
+ *     rows take a launch more then).  work: device memory of
  *     zpucuda_int8_linear_work(rows, inner) bytes, 16-byte aligned, that no other
  *     work in flight uses.
  * The product reads a and b fastest where their addresses and pitches are

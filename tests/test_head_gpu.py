@@ -1167,3 +1167,21 @@ def test_layer_norm_of_several_rows_in_16_bytes(zc, cols, t):
             got = zc.layer_norm_grad(dy, x, *want[1:])
             assert all(torch.equal(a, b) for a, b in zip(got, dwant))
             check_norm(zc, x, None, None)
+
+
+# ------------------------------------------------------------- the linear layer over its own input
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("m", [1, 2, 3, 200])
+def test_int8_linear_over_its_input(zc, m, t):
+    """y over x, whole or in part: x has been read by every block before any stores y (a launch of its own for it)."""
+    g = gen(32)
+    for k, shift in ((512, 0), (4096, 0), (1000, 7), (4096, 40)):
+        layer = zc.Int8Linear.from_float(normal(g, k, k), normal(g, k))
+        x = strided(normal(g, m, k).to(TYPES[t]), 64)
+        start = zc.launch_count()
+        want = layer(x)
+        apart = zc.launch_count()
+        over = layer(x, out=x._base[:, shift:shift + k])
+        assert torch.equal(over, want)
+        if m <= 2:
+            assert apart - start == 1 and zc.launch_count() - apart == 2

@@ -965,7 +965,13 @@ int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d
     if (!d_work || work_bytes < zpucuda_int8_linear_work(rows, inner) || !aligned_to(d_work, 16))
         return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "int8_linear: work: null, too small or not 16-byte aligned");
     cudaStream_t s = resolve_stream(stream);
-    if (takes_vec(d_w, ldw, rows, inner))
+    // The one launch for one or two tokens has every block read x while others store y: where the two share memory, x is
+    // quantised in a launch of its own, as it is for more tokens.
+    const int64_t e = elem_bytes(dtype);
+    const uintptr_t x0 = (uintptr_t)d_x, x1 = x0 + ((rows - 1) * ldx + inner) * e, y0 = (uintptr_t)d_y,
+                    y1 = y0 + ((rows - 1) * ldy + cols) * e;
+    const bool apart = x1 <= y0 || y1 <= x0;
+    if (apart && takes_vec(d_w, ldw, rows, inner))
         ZC_HEAD_TYPE(dtype, T, return (product_vec<T, T>((const T *)d_x, ldx, nullptr, d_w, ldw, d_sw, d_bias, (T *)d_y,
                                                          ldy, rows, cols, inner, Patience(), s)));
     const int64_t ldq = (inner + 15) / 16 * 16;

@@ -280,7 +280,8 @@ class Int8Linear:
     """y = x @ weight.T + bias with int8 weights [cols, inner] and a float32
     scale per output channel, x quantised by row as it comes.  Made from
     quantised weights, or by Int8Linear.from_float.  Weights at a row pitch of
-    a multiple of 16 bytes are kept as they are, others copied to one."""
+    a multiple of 16 bytes are kept as they are, others copied to one.  `out`
+    may be x."""
 
     def __init__(self, weight, scale, bias=None):
         torch = _torch()
