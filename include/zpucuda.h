@@ -460,7 +460,8 @@ int zpucuda_debug_peer_reduce(const float *d_inbox, int world, int64_t n, float 
  * the others have no counterpart in the reference.
  *  - Activations and logits are [rows, n] of F32, F16 or BF16 with unit stride
  *    along the row and any row pitch (ld*, in elements, >= the row's length)
- *    and any alignment that fits their elements; rows may be 0.  Sums are held
+ *    and any alignment that fits their elements (as every vector's, or the call
+ *    is refused with InvalidArgument); rows may be 0.  Sums are held
  *    in f32 or wider and each result is rounded to its type once.
  *  - Calls are asynchronous on `stream`, allocate nothing and may be captured
  *    in a CUDA graph.  Waits inside a kernel (of the distillation's clusters

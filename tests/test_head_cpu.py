@@ -201,3 +201,24 @@ def test_rows_are_copied_from_inside_their_matrix(tmp_path):
     printf("%ld %d", bad, others > 0);
     """)
     assert out == ["0", "1"]
+
+
+VECTORS = [("zpucuda_layer_norm", NORM, NORM_OK, "mean rstd", 4), ("zpucuda_layer_norm_grad", NORM_GRAD, NORM_GRAD_OK, "mean rstd", 4),
+           ("zpucuda_distill_loss", LOSS, TEACH_OK, "weight loss lse", 4), ("zpucuda_distill_loss", LOSS, TEACH_OK, "index", 8),
+           ("zpucuda_distill_loss", LOSS, dict(TEACH_OK, it=I32), "index", 4),
+           ("zpucuda_distill_grad", GRAD, TEACH_OK, "weight lse dloss", 4),
+           ("zpucuda_distill_value_and_grad", BOTH, TEACH_OK, "weight dloss loss", 4),
+           ("zpucuda_int8_quantize", QUANT, QUANT_OK, "scale", 4), ("zpucuda_int8_matmul", MUL, MUL_OK, "sa sb bias", 4),
+           ("zpucuda_int8_linear", LINEAR, LINEAR_OK, "sw bias", 4), ("zpucuda_sample", SAMPLE, SAMPLE_OK, "u temp k p mp logprob", 4),
+           ("zpucuda_sample", SAMPLE, dict(SAMPLE_OK, ut=F64), "u token", 8)]
+
+
+@pytest.mark.parametrize("name,order,good,vectors,size", VECTORS, ids=["%s-%s" % (v[0], v[4]) for v in VECTORS])
+def test_vectors_off_their_elements_are_refused(L, name, order, good, vectors, size):
+    """An address that would fault on the GPU is refused by the call."""
+    for v in vectors.split():
+        for off in (1, size // 2):
+            st, msg = call(L, name, order, good, **{v: A + off})
+            assert st == INVALID and "not aligned" in msg, (v, off, st, msg)
+        if name != "zpucuda_layer_norm_grad":
+            assert call(L, name, order, good, **{v: A + size})[0] == 0

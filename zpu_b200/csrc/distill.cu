@@ -363,6 +363,8 @@ int check_args(const char *who, int dtype, const void *logits, int64_t ld, const
     ZC_TRY(check_matrix(who, "teacher", A.teacher, A.ttype, A.ldt, rows, A.top));
     if (A.itype != ZPUCUDA_I32 && A.itype != ZPUCUDA_I64)
         return head_error(ZPUCUDA_ERR_NOT_SUPPORTED, who, "indices are not i32 or i64");
+    ZC_TRY(check_vectors(who, A.itype == ZPUCUDA_I64 ? 8 : 4, {{"indices", A.indices}}));
+    ZC_TRY(check_vectors(who, 4, {{"weight", A.weight}, {"dloss", A.dloss}, {"lse", A.lse_in}, {"loss", A.loss}, {"lse", A.lse_out}}));
     if (A.ldi < A.top) return head_error(ZPUCUDA_ERR_INVALID_SHAPE, who, "indices: row pitch below the row's length");
     if (rows > 0 && A.top > 0 && !A.indices) return head_error(ZPUCUDA_ERR_INVALID_ARGUMENT, who, "indices: null pointer");
     return ZPUCUDA_OK;

@@ -8,7 +8,9 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <initializer_list>
 #include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 #include "head_rules.h"
@@ -361,6 +363,13 @@ inline int check_matrix(const char *who, const char *name, const void *p, int dt
     if (ld < cols) return fail(ZPUCUDA_ERR_INVALID_SHAPE, "the row pitch is below the row's length");
     if (rows > 0 && cols > 0 && !p) return fail(ZPUCUDA_ERR_INVALID_ARGUMENT, "null pointer");
     if (!aligned_to(p, elem_bytes(dt))) return fail(ZPUCUDA_ERR_INVALID_ARGUMENT, "not aligned to its elements");
+    return ZPUCUDA_OK;
+}
+// Vector arguments `names` of `who`, any of them null, of elements of `bytes` each.
+inline int check_vectors(const char *who, size_t bytes, std::initializer_list<std::pair<const char *, const void *>> vectors) {
+    for (const auto &v : vectors)
+        if (!aligned_to(v.second, bytes))
+            return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, std::string(who) + ": " + v.first + ": not aligned to its elements");
     return ZPUCUDA_OK;
 }
 inline int head_error(int st, const char *who, const char *what) { return set_error(st, std::string(who) + ": " + what); }

@@ -909,8 +909,7 @@ int check_product(const char *who, const float *sb, const int8_t *b, int64_t ldb
     ZC_TRY(check_matrix(who, "out", out, dtype, ldo, m, n));
     if (ldb < k) return head_error(ZPUCUDA_ERR_INVALID_SHAPE, who, "b: row pitch below the row's length");
     if (n > 0 && ((k > 0 && !b) || !sb)) return head_error(ZPUCUDA_ERR_INVALID_ARGUMENT, who, "b or its scales: null pointer");
-    (void)bias;
-    return ZPUCUDA_OK;
+    return check_vectors(who, 4, {{"b's scales", sb}, {"bias", bias}});
 }
 
 }  // namespace
@@ -925,6 +924,7 @@ int zpucuda_int8_quantize(int dtype, const void *d_x, int64_t ldx, int8_t *d_q, 
     if (rows < 0 || cols < 0) return set_error(ZPUCUDA_ERR_INVALID_SHAPE, "int8_quantize: a size is negative");
     if (rows > 0x7fffffff) return set_error(ZPUCUDA_ERR_NOT_SUPPORTED, "int8_quantize: more than 2^31 - 1 rows");
     ZC_TRY(check_matrix("int8_quantize", "x", d_x, dtype, ldx, rows, cols));
+    ZC_TRY(check_vectors("int8_quantize", 4, {{"scale", d_scale}}));
     if (ldq < cols) return set_error(ZPUCUDA_ERR_INVALID_SHAPE, "int8_quantize: q: row pitch below the row's length");
     if (rows > 0 && ((cols > 0 && !d_q) || !d_scale))
         return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "int8_quantize: q or scale: null pointer");
@@ -936,6 +936,7 @@ static int int8_matmul(const char *who, const int8_t *a, int64_t lda, const floa
                        int64_t k, const Patience &wait, void *stream) {
     ZC_TRY(check_product(who, sb, b, ldb, bias, dtype, out, ldo, m, n, k));
     if (lda < k) return head_error(ZPUCUDA_ERR_INVALID_SHAPE, who, "a: row pitch below the row's length");
+    ZC_TRY(check_vectors(who, 4, {{"a's scales", sa}}));
     if (m > 0 && ((k > 0 && !a) || !sa)) return head_error(ZPUCUDA_ERR_INVALID_ARGUMENT, who, "a or its scales: null pointer");
     return product(a, lda, sa, b, ldb, sb, bias, dtype, out, ldo, m, n, k, false, resolve_stream(stream), wait);
 }

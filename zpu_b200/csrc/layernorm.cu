@@ -610,6 +610,7 @@ int zpucuda_layer_norm(int dtype, const void *d_x, int64_t ldx, int wtype, const
     ZC_TRY(check_matrix("layer_norm", "y", d_y, dtype, ldy, rows, cols));
     if (d_gamma) ZC_TRY(check_matrix("layer_norm", "gamma", d_gamma, wtype, cols, 1, cols));
     if (d_beta) ZC_TRY(check_matrix("layer_norm", "beta", d_beta, wtype, cols, 1, cols));
+    ZC_TRY(check_vectors("layer_norm", 4, {{"mean", d_mean}, {"rstd", d_rstd}}));
     if (rows == 0) return ZPUCUDA_OK;
     cudaStream_t s = resolve_stream(stream);
     ZC_HEAD_TYPE(dtype, T,
@@ -635,6 +636,7 @@ int zpucuda_layer_norm_grad(int dtype, const void *d_dy, int64_t lddy, const voi
     if (d_gamma) ZC_TRY(check_matrix("layer_norm_grad", "gamma", d_gamma, wtype, cols, 1, cols));
     if (d_dgamma) ZC_TRY(check_matrix("layer_norm_grad", "dgamma", d_dgamma, wtype, cols, 1, cols));
     if (d_dbeta) ZC_TRY(check_matrix("layer_norm_grad", "dbeta", d_dbeta, wtype, cols, 1, cols));
+    ZC_TRY(check_vectors("layer_norm_grad", 4, {{"mean", d_mean}, {"rstd", d_rstd}}));
     if (rows > 0 && (!d_mean || !d_rstd))
         return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "layer_norm_grad: mean or rstd is null");
     const bool sums = d_dgamma || d_dbeta;

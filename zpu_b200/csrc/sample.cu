@@ -978,6 +978,9 @@ extern "C" int zpucuda_sample(int dtype, const void *d_logits, int64_t ld, int u
     if (rows > 0x7fffffff) return set_error(ZPUCUDA_ERR_NOT_SUPPORTED, "sample: more than 2^31 - 1 rows");
     ZC_TRY(check_matrix("sample", "logits", d_logits, dtype, ld, rows, vocab));
     if (utype != ZPUCUDA_F32 && utype != ZPUCUDA_F64) return set_error(ZPUCUDA_ERR_NOT_SUPPORTED, "sample: uniform is not f32 or f64");
+    ZC_TRY(check_vectors("sample", utype == ZPUCUDA_F64 ? 8 : 4, {{"uniform", d_uniform}}));
+    ZC_TRY(check_vectors("sample", 4, {{"temperature", d_temperature}, {"top_k", d_top_k}, {"top_p", d_top_p}, {"min_p", d_min_p}, {"logprob", d_logprob}}));
+    ZC_TRY(check_vectors("sample", 8, {{"token", d_token}}));
     if (rows == 0) return ZPUCUDA_OK;
     if (!d_uniform || !d_token) return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "sample: uniform or token: null pointer");
     const Args A = {d_uniform, utype, d_temperature, d_top_k, d_top_p, d_min_p, d_token, d_logprob, vocab, kPlaces};
