@@ -1185,3 +1185,17 @@ def test_int8_linear_over_its_input(zc, m, t):
         assert torch.equal(over, want)
         if m <= 2:
             assert apart - start == 1 and zc.launch_count() - apart == 2
+
+
+def test_int8_layer_keeps_the_tensors_it_has_checked(zc):
+    """Sizes, types and the pitch are looked at when a layer is made, so none of its tensors can be put in another's place."""
+    g = gen(33)
+    layer = zc.Int8Linear.from_float(normal(g, 40, 24), normal(g, 40))
+    x = normal(g, 3, 24)
+    want = layer(x)
+    for name in ("weight", "scale", "bias"):
+        with pytest.raises(AttributeError):
+            setattr(layer, name, getattr(layer, name).half())
+    assert torch.equal(layer(x), want)
+    layer.bias.zero_()
+    assert torch.equal(layer(x), zc.Int8Linear(layer.weight, layer.scale)(x))

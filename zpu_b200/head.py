@@ -281,7 +281,12 @@ class Int8Linear:
     scale per output channel, x quantised by row as it comes.  Made from
     quantised weights, or by Int8Linear.from_float.  Weights at a row pitch of
     a multiple of 16 bytes are kept as they are, others copied to one.  `out`
-    may be x."""
+    may be x.  The tensors that a layer has been made with are its own for
+    good (their values may change); others are another layer."""
+
+    weight = property(lambda self: self._weight)
+    scale = property(lambda self: self._scale)
+    bias = property(lambda self: self._bias)
 
     def __init__(self, weight, scale, bias=None):
         torch = _torch()
@@ -294,7 +299,7 @@ class Int8Linear:
             self._ld = (inner + 15) // 16 * 16
             kept = torch.empty((cols, self._ld), dtype=torch.int8, device=weight.device)[:, :inner]
             weight = kept.copy_(weight)
-        self.weight, self.scale, self.bias = weight, scale, bias
+        self._weight, self._scale, self._bias = weight, scale, bias
 
     @classmethod
     def from_float(cls, weight, bias=None, stream=None):
@@ -309,15 +314,16 @@ class Int8Linear:
             with _torch().cuda.stream(stream):
                 return self(x, out)
         torch = _torch()
-        ldx, code = _matrix("x", x, self.weight), _code("x", x)
+        weight, bias = self._weight, self._bias
+        ldx, code = _matrix("x", x, weight), _code("x", x)
         rows, inner = x.shape
-        cols = self.weight.shape[0]
-        if inner != self.weight.shape[1]:
-            _refuse(2, "x is %s, the weight %s" % (tuple(x.shape), tuple(self.weight.shape)))
+        cols = weight.shape[0]
+        if inner != weight.shape[1]:
+            _refuse(2, "x is %s, the weight %s" % (tuple(x.shape), tuple(weight.shape)))
         y, ldy = _output("out", out, x, (rows, cols))
         work = torch.empty(lib().zpucuda_int8_linear_work(rows, inner), dtype=torch.uint8, device=x.device)
-        check(lib().zpucuda_int8_linear(code, x.data_ptr(), ldx, self.weight.data_ptr(), self._ld,
-                                        self.scale.data_ptr(), None if self.bias is None else self.bias.data_ptr(),
+        check(lib().zpucuda_int8_linear(code, x.data_ptr(), ldx, weight.data_ptr(), self._ld,
+                                        self._scale.data_ptr(), None if bias is None else bias.data_ptr(),
                                         y.data_ptr(), ldy, rows, cols, inner, work.data_ptr(), work.numel(),
                                         _stream(x)))
         return y
