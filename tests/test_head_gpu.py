@@ -1199,3 +1199,9 @@ def test_int8_layer_keeps_the_tensors_it_has_checked(zc):
     assert torch.equal(layer(x), want)
     layer.bias.zero_()
     assert torch.equal(layer(x), zc.Int8Linear(layer.weight, layer.scale)(x))
+
+
+def test_int8_layer_without_scales_is_refused(zc):
+    with pytest.raises(zc.ZpuCudaError) as e:
+        zc.Int8Linear(torch.zeros(4, 16, dtype=torch.int8, device="cuda"), None)
+    assert e.value.name == "InvalidArgument"

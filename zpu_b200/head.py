@@ -292,7 +292,8 @@ class Int8Linear:
         torch = _torch()
         _int8("weight", weight)
         cols, inner = weight.shape
-        _vector("scale", scale, cols, weight, torch.float32)
+        if _vector("scale", scale, cols, weight, torch.float32) is None:
+            _refuse(16, "scale: a tensor of (%d,) is wanted" % cols)
         _vector("bias", bias, cols, weight, torch.float32)
         self._ld = weight.stride(0) if cols > 1 else (inner + 15) // 16 * 16
         if self._ld % 16 or weight.data_ptr() % 16:
