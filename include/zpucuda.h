@@ -516,8 +516,8 @@ int zpucuda_distill_value_and_grad(int dtype, const void *d_logits, int64_t ld, 
                                    double temperature, const float *d_dloss, float *d_loss, void *d_dlogits,
                                    int64_t ldd, int64_t rows, int64_t vocab, int64_t top, void *stream);
 /* Diagnostics: distill_loss whose blocks look for one another's sums at most
- * spin_limit times (0: not at all) and, where that runs out, set *d_err and give
- * NaN.  Lets a test make that bounded wait run out. */
+ * spin_limit times (0: not at all) and, where that runs out, set *d_err (NULL: the
+ * word that zpucuda_check_device reads) and give NaN.  Lets a test make that bounded wait run out. */
 int zpucuda_debug_distill_loss(int dtype, const void *d_logits, int64_t ld, int ttype, const void *d_teacher, int64_t ldt,
                                int itype, const void *d_indices, int64_t ldi, const float *d_weight, double temperature,
                                float *d_loss, float *d_lse, int64_t rows, int64_t vocab, int64_t top, uint32_t spin_limit,
@@ -548,7 +548,8 @@ int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d
 int64_t zpucuda_int8_linear_work(int64_t rows, int64_t inner);
 /* Diagnostics: int8_matmul whose warps look for finished sums (one or two rows
  * of a: for arrived weights) at most spin_limit times and, where that runs out
- * (0: at once), set *d_err and give NaN.  Lets a test make the product's bounded
+ * (0: at once), set *d_err (NULL: the word that zpucuda_check_device reads) and
+ * give NaN.  Lets a test make the product's bounded
  * waits run out; copies and products in flight are waited for all the same. */
 int zpucuda_debug_int8_matmul(const int8_t *d_a, int64_t lda, const float *d_sa, const int8_t *d_b, int64_t ldb,
                               const float *d_sb, const float *d_bias, int dtype, void *d_out, int64_t ldo, int64_t m,

@@ -1205,3 +1205,35 @@ def test_int8_layer_without_scales_is_refused(zc):
     with pytest.raises(zc.ZpuCudaError) as e:
         zc.Int8Linear(torch.zeros(4, 16, dtype=torch.int8, device="cuda"), None)
     assert e.value.name == "InvalidArgument"
+
+
+def alone(code):
+    """The output of a program of its own: a wait that runs out there is not reported here."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", "import torch, zpu_b200 as zc\nL = zc.lib()\nzc.check(L.zpucuda_init(0))\n" + code],
+                       cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return r.stdout.split("\n")
+
+
+GIVE_UP = {"8-bit product": """
+a, b, y = torch.ones(64, 64, dtype=torch.int8, device="cuda"), torch.ones(200, 64, dtype=torch.int8, device="cuda"), torch.empty(64, 200, device="cuda")
+s = torch.ones(200, device="cuda")
+zc.check(L.zpucuda_debug_int8_matmul(a.data_ptr(), 64, s.data_ptr(), b.data_ptr(), 64, s.data_ptr(), None, zc.F32, y.data_ptr(), 200, 64, 200, 64, 0,
+                                     None, zc.stream_of()))
+""", "distillation": """
+x, t, i, l = torch.ones(3, 9000, device="cuda"), torch.ones(3, 2, device="cuda"), torch.ones(3, 2, dtype=torch.int64, device="cuda"), torch.empty(3, device="cuda")
+zc.check(L.zpucuda_debug_distill_loss(zc.F32, x.data_ptr(), 9000, zc.F32, t.data_ptr(), 2, 3, i.data_ptr(), 2, None, 1.0, l.data_ptr(), None, 3, 9000, 2, 0,
+                                      None, zc.stream_of()))
+"""}
+
+
+@pytest.mark.parametrize("what", list(GIVE_UP))
+def test_a_wait_that_runs_out_is_reported(zc, what):
+    """By zpucuda_check_device, with the kind of kernel that it ran out in."""
+    before, after, text, *_ = alone("print(L.zpucuda_check_device())" + GIVE_UP[what] + "torch.cuda.synchronize()\nprint(L.zpucuda_check_device())\n"
+                                    "print(L.zpucuda_last_error().decode())")
+    assert before == "0" and after != "0" and what in text, (before, after, text)

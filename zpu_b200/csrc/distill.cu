@@ -469,7 +469,7 @@ int zpucuda_debug_distill_loss(int dtype, const void *d_logits, int64_t ld, int 
                                uint32_t *d_err, void *stream) {
     Args A;
     ZC_TRY(make_args("debug_distill_loss", A, ttype, d_teacher, ldt, itype, d_indices, ldi, d_weight, temperature, vocab, top));
-    if (!d_err) return head_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "debug_distill_loss", "err: null pointer");
+    ZC_TRY(check_vectors("debug_distill_loss", 4, {{"err", d_err}}));
     A.loss = d_loss;
     A.lse_out = d_lse;
     A.limit = spin_limit;

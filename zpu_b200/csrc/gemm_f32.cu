@@ -1761,6 +1761,6 @@ extern "C" int zpucuda_check_device(void) {
         if (!st && !e) st = zc::distill_device_error(&e);
         if (st) return st;
     }
-    if (e) return zc::set_error(ZPUCUDA_ERR_TIMEOUT, "a device-side bounded wait ran out in a GEMM or distillation kernel");
+    if (e) return zc::set_error(ZPUCUDA_ERR_TIMEOUT, "a device-side bounded wait ran out in a GEMM, 8-bit product or distillation kernel");
     return ZPUCUDA_OK;
 }

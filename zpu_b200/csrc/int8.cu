@@ -950,7 +950,7 @@ int zpucuda_int8_matmul(const int8_t *d_a, int64_t lda, const float *d_sa, const
 int zpucuda_debug_int8_matmul(const int8_t *d_a, int64_t lda, const float *d_sa, const int8_t *d_b, int64_t ldb,
                               const float *d_sb, const float *d_bias, int dtype, void *d_out, int64_t ldo, int64_t m,
                               int64_t n, int64_t k, uint32_t spin_limit, uint32_t *d_err, void *stream) {
-    if (!d_err) return set_error(ZPUCUDA_ERR_INVALID_ARGUMENT, "debug_int8_matmul: err: null pointer");
+    ZC_TRY(check_vectors("debug_int8_matmul", 4, {{"err", d_err}}));
     Patience wait;
     wait.limit = spin_limit;
     wait.err = d_err;
