@@ -1237,3 +1237,28 @@ def test_a_wait_that_runs_out_is_reported(zc, what):
     before, after, text, *_ = alone("print(L.zpucuda_check_device())" + GIVE_UP[what] + "torch.cuda.synchronize()\nprint(L.zpucuda_check_device())\n"
                                     "print(L.zpucuda_last_error().decode())")
     assert before == "0" and after != "0" and what in text, (before, after, text)
+
+
+def test_check_device_costs_no_more_without_the_head(zc):
+    """A program that launches none of the head's kernels reads one error word as ever, not three: about a third of the
+    time, and less than two thirds for sure."""
+    few, many, *_ = alone("""
+import time
+def cost():
+    t = []
+    for _ in range(300):
+        a = time.perf_counter()
+        zc.check(L.zpucuda_check_device())
+        t.append(time.perf_counter() - a)
+    return sorted(t)[150]
+cost()
+few = cost()
+x, i = torch.ones(3, 9000, device="cuda"), torch.ones(3, 2, dtype=torch.int64, device="cuda")
+zc.distill_loss(x, x[:, :2].contiguous(), i)
+zc.Int8Linear.from_float(x)(x)
+torch.cuda.synchronize()
+cost()
+print(few * 1e6)
+print(cost() * 1e6)
+""")
+    assert float(few) < 0.67 * float(many), (few, many)

@@ -26,7 +26,10 @@ namespace zc {
 
 static __device__ unsigned int g_distill_error;
 
+static std::atomic<bool> g_distill_waits{false};  // a kernel with waits has been launched
+
 int distill_device_error(unsigned int *e) {
+    if (!g_distill_waits.load(std::memory_order_relaxed)) return ZPUCUDA_OK;
     ZC_CUDA(cudaMemcpyFromSymbol(e, g_distill_error, sizeof *e));
     return ZPUCUDA_OK;
 }
@@ -422,6 +425,7 @@ int launch(const char *who, int dtype, const void *logits, int64_t ld, void *out
     if (rows > 0 && GRAD && !LOSS && !A.lse_in)
         return head_error(ZPUCUDA_ERR_INVALID_ARGUMENT, who, "lse: null pointer");
     if (rows == 0) return ZPUCUDA_OK;
+    if (LOSS) g_distill_waits.store(true, std::memory_order_relaxed);
     cudaStream_t s = resolve_stream(stream);
     ZC_HEAD_TYPE(dtype, T, return (launch_rows<T, LOSS, GRAD>((const T *)logits, ld, (T *)out, ldo, A, rows, s)));
 }

@@ -14,7 +14,10 @@ namespace zc {
 
 static __device__ unsigned int g_int8_error;
 
+static std::atomic<bool> g_int8_waits{false};  // a kernel with waits has been launched
+
 int int8_device_error(unsigned int *e) {
+    if (!g_int8_waits.load(std::memory_order_relaxed)) return ZPUCUDA_OK;
     ZC_CUDA(cudaMemcpyFromSymbol(e, g_int8_error, sizeof *e));
     return ZPUCUDA_OK;
 }
@@ -889,6 +892,7 @@ int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int6
             const float *bias, int dtype, void *out, int64_t ldo, int64_t m, int64_t n, int64_t k, bool follows,
             cudaStream_t s, const Patience &wait = Patience()) {
     if (m == 0 || n == 0) return ZPUCUDA_OK;
+    g_int8_waits.store(true, std::memory_order_relaxed);
     if (takes_vec(b, ldb, m, k))
         ZC_HEAD_TYPE(dtype, T, return (product_vec<int8_t, T>(a, lda, sa, b, ldb, sb, bias, (T *)out, ldo, m, n, k, wait, s)));
     bool done = false;
@@ -972,6 +976,7 @@ int zpucuda_int8_linear(int dtype, const void *d_x, int64_t ldx, const int8_t *d
     const uintptr_t x0 = (uintptr_t)d_x, x1 = x0 + ((rows - 1) * ldx + inner) * e, y0 = (uintptr_t)d_y,
                     y1 = y0 + ((rows - 1) * ldy + cols) * e;
     const bool apart = x1 <= y0 || y1 <= x0;
+    g_int8_waits.store(true, std::memory_order_relaxed);
     if (apart && takes_vec(d_w, ldw, rows, inner))
         ZC_HEAD_TYPE(dtype, T, return (product_vec<T, T>((const T *)d_x, ldx, nullptr, d_w, ldw, d_sw, d_bias, (T *)d_y,
                                                          ldy, rows, cols, inner, Patience(), s)));

@@ -4,7 +4,8 @@
 
 namespace zc {
 
-// Read the word (synchronous); a status.
+// Read the word into *e, left as it is where no kernel that may set it has
+// been launched (a synchronous copy less: 12 us); a status.
 int int8_device_error(unsigned int *e);
 int distill_device_error(unsigned int *e);
 
