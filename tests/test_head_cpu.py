@@ -222,3 +222,17 @@ def test_vectors_off_their_elements_are_refused(L, name, order, good, vectors, s
             assert st == INVALID and "not aligned" in msg, (v, off, st, msg)
         if name != "zpucuda_layer_norm_grad":
             assert call(L, name, order, good, **{v: A + size})[0] == 0
+
+
+def test_any_number_of_rows_has_a_grid(tmp_path):
+    """Up to the 2^31 - 1 rows that the distillation takes."""
+    out = host(tmp_path, """
+    long bad = 0;
+    for (int64_t rows = 1; rows < 1ll << 31; rows += rows < 200000 ? 1 : rows < 2147000000ll ? 99991 : 1) {
+        const RowGrid g = row_grid(rows);
+        const int64_t over = (int64_t)g.y * g.z - rows;
+        bad += g.y < 1 || g.y > 65535 || g.z < 1 || g.z > 65535 || over < 0 || over >= g.z;
+    }
+    printf("%ld", bad);
+    """)
+    assert out == ["0"]

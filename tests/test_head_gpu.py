@@ -1262,3 +1262,14 @@ print(few * 1e6)
 print(cost() * 1e6)
 """)
     assert float(few) < 0.67 * float(many), (few, many)
+
+
+def test_distill_more_rows_than_one_axis_of_a_grid(zc):
+    rows = 70001
+    g = gen(34)
+    student, index = normal(g, rows, 5), torch.randint(0, 5, (rows, 1), generator=g, device="cuda")
+    loss, d = zc.distill_value_and_grad(student, torch.zeros(rows, 1, device="cuda"), index)
+    logq = torch.log_softmax(student.double(), 1)
+    within(loss, -logq.gather(1, index)[:, 0], torch.full((rows,), 16 * E, device="cuda") * (1 + student.double().abs().amax(1)), "loss")
+    want = logq.exp().scatter_add(1, index, torch.full((rows, 1), -1.0, dtype=torch.float64, device="cuda"))
+    within(d, want, 16 * E * (1 + student.double().abs().amax(1, keepdim=True)), "dlogits")

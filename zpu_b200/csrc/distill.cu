@@ -377,8 +377,8 @@ template <typename T, bool LOSS, bool GRAD, int THREADS>
 int launch_cluster(const T *logits, int64_t ld, T *out, int64_t ldo, const Args &A, int cluster, cudaStream_t s) {
     auto f = distill_kernel<T, LOSS, GRAD, THREADS>;
     cudaLaunchConfig_t cfg = {};
-    const int64_t y = A.rows < 32768 ? A.rows : 32768;
-    cfg.gridDim = dim3((unsigned)cluster, (unsigned)y, (unsigned)((A.rows + y - 1) / y));
+    const RowGrid grid = row_grid(A.rows);
+    cfg.gridDim = dim3((unsigned)cluster, grid.y, grid.z);
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = 12 * (size_t)A.top;
     cfg.stream = s;

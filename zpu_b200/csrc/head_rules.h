@@ -38,6 +38,16 @@ inline VecUnits vec_units(int64_t n, int k, int sms) {
 // Rows are worked on four at a time; where a unit of `rows` has no such row, its last one is read again.
 ZC_RULE int vec_row(int row, int rows) { return row < rows ? row : rows - 1; }
 
+// ---- a block (cluster) a row (distill.cu)
+// Rows along y and z of a grid, each at most 65535, with less than z places too many (1 <= rows < 2^31).
+struct RowGrid {
+    unsigned y, z;
+};
+inline RowGrid row_grid(int64_t rows) {
+    const int64_t z = (rows + 65534) / 65535;
+    return {(unsigned)((rows + z - 1) / z), (unsigned)z};
+}
+
 // ---- rows on their way to shared memory (head.cuh)
 // Whether the 16 aligned bytes in which a row begins begin before its matrix: the row starts `skew` elements into them, and
 // `before` elements of the matrix (row * pitch) lie before it.  With short rows that is so for more than the first.
