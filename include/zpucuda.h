@@ -501,7 +501,9 @@ int64_t zpucuda_layer_norm_grad_work(int64_t rows, int64_t cols);
  * twice has the sum of its entries.
  *   distill_loss: the loss, and (unless NULL) lse = log sum exp z, 0 where the
  *     loss is not computed.
- *   distill_grad: the gradient, from that lse.
+ *   distill_grad: the gradient, from that lse.  q is as exact as lse, a 32-bit
+ *     number of the logits' size, leaves it: of logits about the type's lowest
+ *     value throughout a row, not at all.  The other two have no such limit.
  *   distill_value_and_grad: both, from one reading of the logits.
  * dlogits has the logits' type and may be the logits (same pitch). */
 int zpucuda_distill_loss(int dtype, const void *d_logits, int64_t ld, int ttype, const void *d_teacher, int64_t ldt,

@@ -1273,3 +1273,39 @@ def test_distill_more_rows_than_one_axis_of_a_grid(zc):
     within(loss, -logq.gather(1, index)[:, 0], torch.full((rows,), 16 * E, device="cuda") * (1 + student.double().abs().amax(1)), "loss")
     want = logq.exp().scatter_add(1, index, torch.full((rows, 1), -1.0, dtype=torch.float64, device="cuda"))
     within(d, want, 16 * E * (1 + student.double().abs().amax(1, keepdim=True)), "dlogits")
+
+
+# ------------------------------------------------------------- logits far from zero
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("vocab", [33, 5000, 70001])
+def test_distill_of_rows_at_the_lowest_value(zc, vocab, t):
+    """A row of nothing but masks has equal logits: the student's distribution is even, whatever the mask's value."""
+    g = gen(35)
+    _, teacher, index = teach(g, 4, vocab, 7, t, ragged=False)
+    student = torch.full((4, vocab), torch.finfo(TYPES[t]).min, device="cuda", dtype=TYPES[t])
+    student[3] = torch.finfo(TYPES[t]).max
+    for T in (0.5, 1.0, 3.0):
+        lp = torch.log_softmax(teacher.double() / T, 1)
+        want = T * T * (lp.exp() * (lp + math.log(vocab))).sum(1)
+        d = T * torch.full((4, vocab), 1 / vocab, device="cuda", dtype=torch.float64).scatter_add(1, index, -lp.exp())
+        # as for any row: roundings of log V, of each log p and of the teacher's logits, T^2 times
+        size = math.log(vocab) + (lp.exp() * lp.abs()).sum(1) + (teacher.double() / T).abs().amax(1) + 4
+        tol = T * T * 12 * E * size + E * want.abs()
+        loss, got = zc.distill_value_and_grad(student, teacher, index, temperature=T)
+        within(loss, want, tol, "loss")
+        within(zc.distill_loss(student, teacher, index, temperature=T)[0], want, tol, "loss alone")
+        td = T * 12 * E * size[:, None] * (1 / vocab + torch.zeros_like(d).scatter_add(1, index, lp.exp()))
+        within(got, d, td + U[student.dtype] * (d.abs() + td) + S[student.dtype], "grad")
+
+
+def test_distill_far_from_zero(zc):
+    """Logits a long way from zero, exact there: the loss is that of the same logits about zero."""
+    g = gen(36)
+    student, teacher, index = teach(g, 6, 40007, 9, "f32")
+    student = (student * 64).round() / 64
+    want, _ = zc.distill_loss(student, teacher, index, temperature=2.0)
+    for far in (-65536.0, 1024.0, 65536.0):
+        loss, d = zc.distill_value_and_grad(student + far, teacher, index, temperature=2.0)
+        # sums in the same order of the same differences: what is left is the listed entries' reference, a few roundings
+        within(loss, want.double(), 64 * E * (1 + want.double().abs()), "loss")
+        within(zc.distill_loss(student + far, teacher, index, temperature=2.0)[0], want.double(), 64 * E * (1 + want.double().abs()), "loss alone")

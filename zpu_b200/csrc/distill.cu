@@ -108,7 +108,9 @@ __global__ void __launch_bounds__(THREADS, (LOSS ? kThreads : kGradThreads) / TH
     constexpr int N = kPiece<T>, H = N / 2, WARPS = THREADS / 32, MARKS = 2048, U = 4;
     extern __shared__ __align__(16) float entries[];
     __shared__ uint64_t told;
-    __shared__ float4 part[kMaxCluster * WARPS];  // each warp's largest logit, its sum of e^z relative to that, its sum of p z
+    // each warp's largest logit, its sum of e^z relative to that, its sum of p z relative to that (to 0 where it is -inf), and
+    // of p
+    __shared__ float4 part[kMaxCluster * WARPS];
     __shared__ uint16_t mark[MARKS];              // an entry's number, by its place: to find indices listed twice
     __shared__ int again;
     // for each listed entry: its teacher logit / T, its logit, its place in the slice (-1: elsewhere)
@@ -242,11 +244,17 @@ __global__ void __launch_bounds__(THREADS, (LOSS ? kThreads : kGradThreads) / TH
         if (LOSS) ul = warp_sum(ul);
         const float ur = 1.0f / us;
         // the listed entries in this slice
-        float pz = 0.0f;
+        // (Relative to a logit of the row: z itself may be large, or a mask of the type's lowest value, and all that counts of
+        // it lost in a sum with the row's log sum.)
+        float pz = 0.0f, ps = 0.0f;
+        const float ref = LOSS && mine.x != -INFINITY ? mine.x : 0.0f;
         for (int k = threadIdx.x; k < A.top; k += THREADS) {
             if (si[k] < 0) continue;
             const float p = expf(sp[k] - um) * ur;
-            if (LOSS && p != 0.0f) pz += p * (sz[k] * inv_t);
+            if (LOSS && p != 0.0f) {
+                pz += p * ((sz[k] - ref) * inv_t);
+                ps += p;
+            }
             if (GRAD) mark[si[k] % MARKS] = (uint16_t)k;
         }
         bool ok = true;
@@ -254,7 +262,7 @@ __global__ void __launch_bounds__(THREADS, (LOSS ? kThreads : kGradThreads) / TH
             // Each warp tells all blocks of the row, by stores into their shared memory and one arrival, and goes on
             // when all warps of the row have: sooner than by a barrier of the whole cluster.
             mine.z = warp_sum(pz);
-            mine.w = 0.0f;
+            mine.w = warp_sum(ps);
             if (size > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // of all blocks
             __syncwarp();
             if (lane < (int)size) {
@@ -274,7 +282,7 @@ __global__ void __launch_bounds__(THREADS, (LOSS ? kThreads : kGradThreads) / TH
             for (int i = lane; i < (int)size * WARPS; i += 32) {
                 const float4 q = part[i];
                 as += q.x == high ? q.y : q.y * expf((q.x - high) * inv_t);
-                az += q.z;
+                if (q.w != 0.0f) az += q.z + q.w * (((q.x == -INFINITY ? 0.0f : q.x) - high) * inv_t);
             }
             as = warp_sum(as);
             bits = log2f(as);
@@ -282,8 +290,8 @@ __global__ void __launch_bounds__(THREADS, (LOSS ? kThreads : kGradThreads) / TH
             if (rank == 0 && warp == 0) {
                 az = warp_sum(az);
                 if (lane == 0) {
-                    // sum of p log p, less that of p z, plus lse
-                    const float l = (ul * ur - logf(us)) - (az - lse);
+                    // sum of p log p, less that of p z, plus lse, both relative to the largest logit
+                    const float l = (ul * ur - logf(us)) - (az - logf(as));
                     A.loss[row] = bad || !ok ? NAN : w == 0.0f ? 0.0f : w * (A.T * A.T) * l;
                     if (A.lse_out) A.lse_out[row] = !ok ? NAN : w == 0.0f ? 0.0f : lse;
                 }
