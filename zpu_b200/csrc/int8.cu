@@ -594,7 +594,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             bool ok = true;
             for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, n++) {
                 const int buf = n & 1;
-                if (n >= 2 && !tc::mb_wait(&tfree[buf], ((n >> 1) - 1) & 1, A.wait.word())) break;
+                if (n >= 2 && !tc::mb_wait(&tfree[buf], ((n >> 1) - 1) & 1, A.wait.word())) {
+                    ok = false;
+                    break;
+                }
                 tc::fence_after();
                 for (int k = k0; k < k1; k++, j++) {
                     const int s = j % TT::STAGES;
@@ -612,9 +615,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 }
                 if (ok) tc::mma_commit(&tfull[buf]);
             }
-            // nor while products are on their way to TMEM
-            tc::mma_commit(&drained);
-            tc::mb_wait(&drained, 0, A.wait.word());
+            // nor while products are on their way to TMEM (those of finished tiles are waited for by the storing warps, in time or
+            // not)
+            if (!ok) {
+                tc::mma_commit(&drained);
+                tc::mb_wait(&drained, 0, A.wait.word());
+            }
         }
     } else {
         // warp w reads the quarter w % 4 of the TMEM lanes, and one half of the columns
@@ -726,8 +732,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     if (A.splits > 1) {
         // all sums are in place (the stages' loads have all been read by then)
         cluster_sync();
-        bool lost = false;
-        for (int r = 0; r < A.splits; r++) lost |= *(const uint32_t *)cluster_map(&gave_up, r) != 0;
         // each CTA adds up its share: four neighbouring channels of a token a thread
         int tp, tq;
         place(blockIdx.x, &tp, &tq);
@@ -738,6 +742,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             const int64_t token = (int64_t)tq * BN + qc, ch = (int64_t)tp * 128 + (i & 31) * 4;
             if (token >= A.tokens || ch >= A.channels) continue;
             int4 sum = make_int4(0, 0, 0, 0);
+            uint32_t lost = 0;
 #pragma unroll 8
             for (int r = 0; r < A.splits; r++) {
                 const int4 v = *(const int4 *)((const int *)cluster_map(smem, r) + at);
@@ -745,6 +750,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 sum.y += v.y;
                 sum.z += v.z;
                 sum.w += v.w;
+                lost |= *(const uint32_t *)cluster_map(&gave_up, r);
             }
             const int y[4] = {sum.x, sum.y, sum.z, sum.w};
             const float sa = lost ? NAN : A.sa[token];
