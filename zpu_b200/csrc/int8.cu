@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(NT) int8_matmul_kernel(const int8_t *a, int64_
 // on their way before the tokens are even read (loads into registers: 18.5 us
 // where this takes 15.1, 16384 x 4096).  X is int8 (with its scales), or
 // one of the head's types, which each block quantises for itself: one launch
-// for a token's whole linear layer, 15.5 us from bf16 or 4.3 TB/s of weights.  A unit is a slot's worth: several short
+// for a token's whole linear layer, 16.0 us from bf16 or 4.2 TB/s of weights.  A unit is a slot's worth: several short
 // rows, or a piece of a long one; a block's units are dealt out evenly to its
 // warps, and what a warp has of a channel goes to the block's whole-number sums.
 struct VecArgs {
@@ -483,8 +483,8 @@ int product_vec(const X *x, int64_t ldx, const float *sx, const int8_t *w, int64
 // inner axis is split over a cluster, whose CTAs add up each other's sums through
 // shared memory (whole numbers: the split does not change the result).
 //
-// The tensor cores bound a large product: 4096 x 8192 x 8192 takes 188 us, 2.9e15
-// operations a second, at the power limit's clock; 128 x 256 tiles read half as
+// The tensor cores bound a large product: 4096 x 8192 x 8192 takes 171 to 192 us, 2.9e15
+// operations a second or more, at the power limit's clock; 128 x 256 tiles read half as
 // much from L2 a product as 128 x 128 ones.  Small ones are bound by the way from
 // the first load to the last store: 333 x 4099 x 1001 takes 9 us.
 constexpr int TC_THREADS = 320;  // producer, issuer, eight storing warps
@@ -831,7 +831,8 @@ int product_tc(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, i
     // few tokens: weights along the 128 rows, the tokens in the narrowest tile that holds them; so too where
     // the tiles fill less than half of the SMs and the inner axis will be split
     const bool swap = m <= 128 || (m + 127) / 128 * ((n + 127) / 128) * 2 <= num_sms();
-    // wide tiles read half as much per product; narrow ones where they fill the SMs' last wave better
+    // wide tiles read half as much per product (4096 x 8192 by 8192: 192 us, 297 with narrow ones); narrow ones where they fill
+    // the SMs' last wave better by the count of waves, in which a wide one stands for two
     const auto waves = [&](int w) { return ((m + 127) / 128 * ((n + w - 1) / w) + num_sms() - 1) / num_sms(); };
     const int wide = 2 * waves(256) <= waves(128) ? 256 : 128;
     const int bn = !swap ? wide : m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
@@ -842,7 +843,8 @@ int product_tc(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, i
     A.group = 16;
     A.wait = wait;
     A.kt = (int)((k + 127) / 128);
-    // split the inner axis while the tiles leave most SMs idle, with at least four slices left to each
+    // split the inner axis while the tiles leave most SMs idle, with at least four slices left to each (16 x 4096 by 1024: 6.7
+    // us, with eight left 7.9; with two left 8 x 2048 by 512 takes 5.6 instead of 6.4, but 16 x 512 by 2048 6.0 instead of 5.4)
     int64_t splits = 1;
     const int64_t tiles = (int64_t)A.tiles_p * A.tiles_q;
     while (swap && splits < 8 && tiles * splits * 2 <= num_sms() && A.kt / (splits * 2) >= 4) splits *= 2;

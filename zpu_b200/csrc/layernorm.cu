@@ -9,8 +9,8 @@
 // written.  What keeps them from its rate are the two sums of a row that
 // everything waits for: rows are on their way to shared memory meanwhile, and a
 // row is held by few threads.  Forward 16384 x 1024 f16 takes 14.0 us (4.8 TB/s),
-// 4096 x 4096 bf16 15.0 us, 4 x 4096 2.8 us; backward 8192 x 4096 bf16 45 us
-// (4.5 TB/s), 1021 x 5003 f32 27.5 us (2.2 TB/s: pieces off the 16-byte grid are
+// 4096 x 4096 bf16 15.0 us, 4 x 4096 2.8 us; backward 8192 x 4096 bf16 44 us
+// (4.6 TB/s), 1021 x 5003 f32 26.3 us (2.3 TB/s: pieces off the 16-byte grid are
 // shifted into place on both ways).  The gradient's blocks walk rows and keep their columns' sums of
 // dgamma and dbeta in registers; one row of sums a block goes to the caller's
 // workspace, and a second kernel adds those up in the blocks' order, so a
@@ -272,6 +272,8 @@ int launch_ln(const T *x, int64_t ldx, int wt, const void *gamma, const void *be
     // Four pieces a thread, and as few threads a row as hold it: sums over few warps cost the least.  (16384 x 1024 f16:
     // 14.6 us with 32 threads, 16.9 with 64, 20.2 with 128; 4096 x 4096 bf16 15.7 with 128, 20.6 with 512.)  Fewer pieces
     // for rows that would leave most lanes without: 16384 x 102 bf16 10.2 us with one, 15.9 with two.
+    // 16-bit rows above 16384 columns do not fit 1024 threads' registers this way (1.4 to 1.8 KB of spills a thread: 1024 x
+    // 32768 bf16 116 us, 2048 x 16384 28).
     if (n <= 32) LN(32, 1, 4);
     if (n <= 64) LN(32, 2, 3);
     if (n <= 128) LN(32, 4, 2);
